@@ -99,7 +99,7 @@ def draw(rng):
             if c["rows"] * c["cols"] <= 65536 * 1000:
                 return c
     while True:
-        kind = rng.choice(["sigmoid", "sigmoid", "hinge", "ipo"])
+        kind = rng.choice(["sigmoid", "sigmoid", "hinge", "square"])
         c = _preference(None, _log(rng, 1, 262144), _log(rng, 1, 65536), dtype, kind, beta=rng.choice([0.1, 0.5, 1.0]),
                         ref=rng.random() < 0.7, masked=rng.random() < 0.5, temperature=rng.choice([0.0, 0.0, 0.5, 1.0]),
                         smoothing=rng.choice([0.0, 0.1]) if kind == "sigmoid" else 0.0, sign=rng.choice([1.0, -1.0]))
