@@ -86,6 +86,26 @@ class StepBuffers(C.Structure):
                 ("bwd_workspace", C.c_void_p), ("bwd_workspace_bytes", C.c_size_t)]
 
 
+TYPES = {"float32": 0, "bfloat16": 1, "float16": 2}       # kge_type_t by torch's names
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}        # kge_act_t
+PREFERENCES = {"sigmoid": 0, "hinge": 1, "square": 2}      # kge_prefer_t
+
+
+class Linear(C.Structure):
+    _fields_ = [("type", C.c_int32), ("out_type", C.c_int32), ("act", C.c_int32), ("reserved", C.c_int32),
+                ("rows", C.c_int64), ("in_", C.c_int64), ("out", C.c_int64), ("x", C.c_void_p), ("x_stride", C.c_int64),
+                ("weight", C.c_void_p), ("weight_stride", C.c_int64), ("bias", C.c_void_p), ("residual", C.c_void_p),
+                ("residual_stride", C.c_int64), ("p", C.c_double), ("seed", C.c_uint64), ("step", C.c_uint64),
+                ("step_dev", C.c_void_p)]
+
+
+class Preference(C.Structure):
+    _fields_ = [("type", C.c_int32), ("kind", C.c_int32), ("batch", C.c_int64), ("n_neg", C.c_int64), ("pos", C.c_void_p),
+                ("neg", C.c_void_p), ("neg_stride", C.c_int64), ("ref_pos", C.c_void_p), ("ref_neg", C.c_void_p),
+                ("ref_neg_stride", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64), ("beta", C.c_float),
+                ("sign", C.c_float), ("smoothing", C.c_float), ("temperature", C.c_float)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "kge_strerror": (C.c_char_p, [C.c_int]),
@@ -140,6 +160,18 @@ EXPORTS = {
                                 [C.c_int64, C.c_int64, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint32, C.c_void_p]),
     "kge_widen_ids": (C.c_int, [C.POINTER(C.c_void_p), C.POINTER(C.c_void_p), C.POINTER(C.c_int64), C.c_int, C.c_void_p]),
     "kge_publish_counts": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "kge_dropout": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_double,
+                              C.c_uint64, C.c_uint64, C.c_void_p, C.c_void_p]),
+    "kge_linear_saved_bytes": (C.c_size_t, [C.POINTER(Linear)]),
+    "kge_linear_fwd_workspace": (C.c_size_t, [C.POINTER(Linear), C.c_int]),
+    "kge_linear_fwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_int64, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
+                                 C.c_size_t, C.c_void_p]),
+    "kge_linear_bwd_workspace": (C.c_size_t, [C.POINTER(Linear)]),
+    "kge_linear_bwd": (C.c_int, [C.POINTER(Linear), C.c_void_p, C.c_int64, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "kge_preference_workspace": (C.c_size_t, [C.POINTER(Preference)]),
+    "kge_preference_loss": (C.c_int, [C.POINTER(Preference), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                      C.c_void_p]),
     "kge_check_indices": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
 }
 

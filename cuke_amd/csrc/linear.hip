@@ -1,0 +1,363 @@
+// Linear layers with a fused epilogue, y = drop(act(x W^T + b)) + residual, and their gradients (kge_linear_fwd, kge_linear_bwd).
+#include <type_traits>
+
+#include "linear_tile.hpp"
+
+namespace kge {
+
+// ---- operands as the matrix cores take them --------------------------------------------------------
+static int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
+static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+static int planes_of(int type) { return type == KGE_F32 ? 3 : 1; }
+static size_t packed_bytes(int type, int64_t rows, int64_t width) { return up256((size_t)planes_of(type) * rows * up8(width) * 2); }
+
+// Whether an array can be read as it lies: 16 bits, rows that start on 16 bytes and are whole chunks of 8 elements.
+static bool lies_ready(int type, const void *p, int64_t stride, int64_t width) { return type != KGE_F32 && aligned16(p) && stride % 8 == 0 && width % 8 == 0; }
+
+// v = parts[0] + parts[1] + parts[2] exactly (down to 2^-108), also where v is infinite, is NaN or would round to infinity.
+__device__ __forceinline__ void split_value(float v, bf16_t (&part)[3])
+{
+    bf16_t a = (bf16_t)v;
+    if (__builtin_isinf((float)a)) a = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16));
+    const float r = (float)a == v ? 0.0f : v - (float)a;
+    const bf16_t b = (bf16_t)r;
+    part[0] = a, part[1] = b, part[2] = (bf16_t)(r - (float)b);
+}
+
+template <class T>
+using StoredAs = typename std::conditional<sizeof(T) == 4, bf16_t, T>::type;
+
+// four elements of a packed row (8-byte aligned), in one plane or in three
+template <class T>
+__device__ __forceinline__ void store_packed(StoredAs<T> *p, int64_t plane, float4 v)
+{
+    typedef StoredAs<T> quad __attribute__((ext_vector_type(4)));
+    if constexpr (sizeof(T) == 4) {
+        bf16_t x[3], y[3], z[3], w[3];
+        split_value(v.x, x), split_value(v.y, y), split_value(v.z, z), split_value(v.w, w);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) *reinterpret_cast<quad *>(p + k * plane) = quad{x[k], y[k], z[k], w[k]};
+    } else {
+        *reinterpret_cast<quad *>(p) = quad{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
+    }
+}
+
+// Rows copied to whole chunks, zeros behind their end; fp32 as three planes.  One pass at memory speed (fp32: 4 bytes in, 6 out an element).
+template <class T>
+__global__ __launch_bounds__(256) void pack_kernel(const T *src, int64_t stride, int64_t rows, int64_t width, int64_t width8, StoredAs<T> *dst)
+{
+    const int64_t quads = width8 / 4, total = rows * quads;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / quads, col = 4 * (i % quads);
+        const int64_t left = width - col;
+        store_packed<T>(dst + row * width8 + col, rows * width8, load4(src + row * stride + col, (int)(left < 4 ? left : 4)));
+    }
+}
+
+// ---- gradient at the products ----------------------------------------------------------------------
+// dz = drop(dy) act'(z) in the layer's type, and its column sums over a range of rows.  Bound by memory (dy and act' read, dz written); a wave
+// takes 256 columns of a row, four elements a lane, so that the sums stay in registers from row to row.
+struct GradArgs {
+    const void *dy;
+    int64_t dy_stride;
+    const void *slope;  // [rows][4 quads] or NULL
+    int64_t rows, cols, quads, rows_each;
+    Drop drop;
+    void *dz;  // [rows][width8], planes rows * width8 apart; or NULL
+    int64_t width8;
+    float *sums;  // [gridDim.y][4 quads] or NULL
+};
+
+template <class T, class O>
+__global__ __launch_bounds__(256) void linear_dz_kernel(GradArgs g)
+{
+    __shared__ float4 s_sum[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t quad = (int64_t)blockIdx.x * 64 + lane, col = 4 * quad;
+    const int64_t first = (int64_t)blockIdx.y * g.rows_each, last = first + g.rows_each < g.rows ? first + g.rows_each : g.rows;
+    const int64_t left = g.cols - col;
+    const int valid = (int)(left < 4 ? left : 4);
+    const uint64_t base = g.drop.base();
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (col < g.width8) {
+        for (int64_t row = first + wave; row < last; row += 4) {
+            float4 v = load4(static_cast<const O *>(g.dy) + row * g.dy_stride + col, valid);
+            if (g.slope && valid > 0) {
+                const int64_t at = row * 4 * g.quads + col;
+                float4 s;
+                if (sizeof(T) == 4) {
+                    s = *reinterpret_cast<const float4 *>(static_cast<const float *>(g.slope) + at);
+                } else {
+                    const ushort4 q = *reinterpret_cast<const ushort4 *>(static_cast<const uint16_t *>(g.slope) + at);
+                    s = make_float4(slope_from_fixed(q.x), slope_from_fixed(q.y), slope_from_fixed(q.z), slope_from_fixed(q.w));
+                }
+                v.x *= s.x, v.y *= s.y, v.z *= s.z, v.w *= s.w;
+            }
+            if (g.drop.cut && valid > 0) v = g.drop.apply(v, g.drop.word(base, row, quad));  // (last: a dropped element's gradient is zero)
+            if (g.dz) store_packed<T>(static_cast<StoredAs<T> *>(g.dz) + row * g.width8 + col, g.rows * g.width8, v);
+            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+    }
+    if (!g.sums) return;
+    s_sum[wave][lane] = sum;
+    __syncthreads();
+    if (wave || quad >= g.quads) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        const float4 o = s_sum[w][lane];
+        sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
+    }
+    *reinterpret_cast<float4 *>(g.sums + ((int64_t)blockIdx.y * g.quads + quad) * 4) = sum;
+}
+
+// ---- partial sums joined ---------------------------------------------------------------------------
+// out[row][col] = sum over n parts of part[.][row][col], for up to two blocks of partial sums in one launch (a weight's and a bias's gradient).
+struct JoinArgs {
+    const float *part[2];
+    int64_t rows[2], cols[2], quads[2];
+    int n[2];
+    void *out[2];
+    int64_t blocks0;  // workgroups of the first block
+};
+
+template <class T>
+__global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
+{
+    const int which = (int64_t)blockIdx.x < j.blocks0 ? 0 : 1;
+    const int64_t i = ((int64_t)blockIdx.x - (which ? j.blocks0 : 0)) * 256 + threadIdx.x;
+    const int64_t quads = j.quads[which], each = j.rows[which] * quads;
+    if (i >= each) return;
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 *p = reinterpret_cast<const float4 *>(j.part[which]) + i;
+    for (int k = 0; k < j.n[which]; ++k, p += each) {
+        const float4 v = *p;
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const int64_t row = i / quads, col = 4 * (i % quads), left = j.cols[which] - col;
+    store4(static_cast<T *>(j.out[which]) + row * j.cols[which] + col, s, (int)(left < 4 ? left : 4));
+}
+
+// ---- products --------------------------------------------------------------------------------------
+constexpr int kTileX = 128;
+
+template <class E, int PLANES, bool AA, bool BA, EndKind END>
+static void launch_tiles(TileArgs &t, hipStream_t st)
+{
+    t.tiles_a = (int)ceil_div(t.a.extent, kTileX), t.tiles_b = (int)ceil_div(t.b.extent, kTileX);
+    const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b * t.splits;
+    if (blocks == 0) return;
+    hipLaunchKernelGGL((linear_tile_kernel<E, PLANES, AA, BA, kTileX, kTileX, 2, 2, END>), dim3((unsigned)blocks), dim3(256), 0, st, t);
+}
+
+// Parts of a sum over k where `tiles` tiles alone would leave most of the card idle: as many as fill it twice, none shorter than 256 terms.
+static int splits_of(int64_t tiles, int64_t k)
+{
+    const int64_t want = tiles > 0 ? 512 / tiles : 1, most = k / 256;
+    const int64_t s = want < most ? want : most;
+    return (int)(s > 1 ? s : 1);
+}
+static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), kTileK) * kTileK; }
+
+// ---- a layer's plan --------------------------------------------------------------------------------
+struct Plan {
+    bool pack_x, pack_w;
+    size_t slope, x, w;  // bytes of each in a saved block, in this order
+    int64_t quads;
+    int sum_blocks;      // ranges of rows the bias's gradient is summed over
+    int64_t sum_rows;
+    int dw_splits;
+};
+
+static Plan plan_of(const kge_linear *l)
+{
+    Plan p;
+    p.quads = ceil_div(l->out, 4);
+    p.pack_x = !lies_ready(l->type, l->x, l->x_stride, l->in);
+    p.pack_w = !lies_ready(l->type, l->weight, l->weight_stride, l->in);
+    p.slope = l->act == KGE_ACT_NONE ? 0 : up256((size_t)l->rows * p.quads * 4 * type_bytes(l->type));
+    p.x = p.pack_x ? packed_bytes(l->type, l->rows, l->in) : 0;
+    p.w = p.pack_w ? packed_bytes(l->type, l->out, l->in) : 0;
+    // ranges of at least 16 rows, about 1024 workgroups in all
+    const int64_t across = ceil_div(up8(l->out), 256), want = across > 0 && across < 1024 ? 1024 / across : 1;
+    p.sum_rows = ceil_div(l->rows, want);
+    if (p.sum_rows < 16) p.sum_rows = 16;
+    p.sum_blocks = (int)ceil_div(l->rows, p.sum_rows);
+    p.dw_splits = splits_of(ceil_div(l->in, kTileX) * ceil_div(l->out, kTileX), l->rows);
+    return p;
+}
+
+static int check(const kge_linear *l)
+{
+    if (!l) return KGE_EINVAL;
+    if (!known_type(l->type) || (l->out_type != l->type && l->out_type != KGE_F32)) return KGE_EINVAL;
+    if (l->act < KGE_ACT_NONE || l->act > KGE_ACT_SILU || !drop_ok(l->p)) return KGE_EINVAL;
+    const int64_t most = (int64_t)1 << 31;
+    if (l->rows < 0 || l->in < 0 || l->out < 0 || l->rows >= most || l->in >= most || l->out >= most) return KGE_ESHAPE;
+    if (l->x_stride < l->in || l->weight_stride < l->in || (l->residual && l->residual_stride < l->out)) return KGE_ESHAPE;
+    // (every launch's workgroups are counted in 31 bits)
+    if (ceil_div(l->rows, 32) * ceil_div(l->out, 32) >= most || ceil_div(l->rows, 32) * ceil_div(l->in, 32) >= most ||
+        ceil_div(l->in, 32) * ceil_div(l->out, 32) >= most)
+        return KGE_ESHAPE;
+    if ((l->rows > 0 && l->in > 0 && !l->x) || (l->in > 0 && l->out > 0 && !l->weight)) return KGE_EINVAL;
+    return KGE_OK;
+}
+
+static int grid_for(int64_t items)
+{
+    const int64_t b = ceil_div(items, 256);
+    return (int)(b < 8192 ? b : 8192);
+}
+
+template <class T>
+static void launch_pack(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst, hipStream_t st)
+{
+    if (rows == 0 || width == 0) return;
+    hipLaunchKernelGGL(pack_kernel<T>, dim3(grid_for(rows * up8(width) / 4)), dim3(256), 0, st, static_cast<const T *>(src), stride, rows, width,
+                       up8(width), static_cast<StoredAs<T> *>(dst));
+}
+
+// an operand where it lies, or its packed copy
+static Side side_of(const void *p, int64_t stride, bool packed, const void *copy, int64_t rows, int64_t width, int64_t extent)
+{
+    if (packed) return Side{copy, up8(width), rows * up8(width), extent};
+    return Side{p, stride, 0, extent};
+}
+
+template <class T>
+static int forward(const kge_linear *l, const Plan &p, void *y, int64_t y_stride, char *slope, char *px, char *pw, hipStream_t st)
+{
+    using E = StoredAs<T>;
+    constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+    if (p.pack_x) launch_pack<T>(l->x, l->x_stride, l->rows, l->in, px, st);
+    if (p.pack_w) launch_pack<T>(l->weight, l->weight_stride, l->out, l->in, pw, st);
+    TileArgs t{};
+    t.a = side_of(l->weight, l->weight_stride, p.pack_w, pw, l->out, l->in, l->out);
+    t.b = side_of(l->x, l->x_stride, p.pack_x, px, l->rows, l->in, l->rows);
+    t.k = l->in, t.splits = 1, t.k_each = split_length(l->in, 1);
+    t.e = Ends{y, y_stride, l->bias, l->residual, l->residual_stride, slope, l->rows, l->out, p.quads,
+               make_drop(l->p, l->seed, l->step, l->step_dev, l->out), l->act, l->out_type == KGE_F32};
+    launch_tiles<E, kPlanes, false, false, kEndLayer>(t, st);
+    KGE_CHECK_LAUNCH();
+    return KGE_OK;
+}
+
+template <class T>
+static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t dy_stride, const char *saved, void *dx, void *dw, void *db,
+                    char *ws, hipStream_t st)
+{
+    using E = StoredAs<T>;
+    constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
+    const int64_t width8 = up8(l->out);
+    const bool ready = l->act == KGE_ACT_NONE && nearbyint(l->p * 65536.0) == 0.0 && l->out_type == l->type && lies_ready(l->type, dy, dy_stride, l->out);
+    char *dz = ws;
+    float *sums = reinterpret_cast<float *>(ws + packed_bytes(l->type, l->rows, l->out));
+    float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(sums) + up256((size_t)p.sum_blocks * p.quads * 16));
+    const bool want_dz = !ready && (dx || dw);
+    if ((want_dz || db) && l->rows > 0 && l->out > 0) {
+        GradArgs g{dy, dy_stride, p.slope ? saved : nullptr, l->rows, l->out, p.quads, p.sum_rows,
+                   make_drop(l->p, l->seed, l->step, l->step_dev, l->out), want_dz ? dz : nullptr, width8, db ? sums : nullptr};
+        const dim3 grid((unsigned)ceil_div(width8, 256), (unsigned)p.sum_blocks);
+        if (l->out_type == KGE_F32) hipLaunchKernelGGL((linear_dz_kernel<T, float>), grid, dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((linear_dz_kernel<T, T>), grid, dim3(256), 0, st, g);
+    }
+    const Side gz = side_of(dy, dy_stride, !ready, dz, l->rows, l->out, 0);
+    if (dx) {
+        TileArgs t{};
+        t.a = side_of(l->weight, l->weight_stride, p.pack_w, saved + p.slope + p.x, l->out, l->in, l->in);
+        t.b = gz, t.b.extent = l->rows;
+        t.k = l->out, t.splits = 1, t.k_each = split_length(l->out, 1);
+        t.e.y = dx, t.e.y_stride = l->in, t.e.rows = l->rows, t.e.cols = l->in, t.e.quads = ceil_div(l->in, 4);
+        launch_tiles<E, kPlanes, true, false, kEndStore>(t, st);
+    }
+    JoinArgs j{};
+    if (dw) {
+        TileArgs t{};
+        t.a = side_of(l->x, l->x_stride, p.pack_x, saved + p.slope, l->rows, l->in, l->in);
+        t.b = gz, t.b.extent = l->out;
+        t.k = l->rows, t.splits = p.dw_splits, t.k_each = split_length(l->rows, t.splits);
+        t.partial = part;
+        t.e.y = dw, t.e.y_stride = l->in, t.e.rows = l->out, t.e.cols = l->in, t.e.quads = ceil_div(l->in, 4);
+        if (t.splits == 1) {
+            launch_tiles<E, kPlanes, true, true, kEndStore>(t, st);
+        } else {
+            launch_tiles<E, kPlanes, true, true, kEndPartial>(t, st);
+            j.part[0] = part, j.rows[0] = l->out, j.cols[0] = l->in, j.quads[0] = t.e.quads, j.n[0] = t.splits, j.out[0] = dw;
+            j.blocks0 = ceil_div(j.rows[0] * j.quads[0], 256);
+        }
+    }
+    if (db) j.part[1] = sums, j.rows[1] = 1, j.cols[1] = l->out, j.quads[1] = p.quads, j.n[1] = p.sum_blocks, j.out[1] = db;
+    const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 256) : 0);
+    if (blocks) hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, j);
+    KGE_CHECK_LAUNCH();
+    return KGE_OK;
+}
+
+}  // namespace kge
+
+using namespace kge;
+
+extern "C" {
+
+size_t kge_linear_saved_bytes(const kge_linear *lin)
+{
+    if (check(lin)) return 0;
+    const Plan p = plan_of(lin);
+    return p.slope + p.x + p.w;
+}
+
+size_t kge_linear_fwd_workspace(const kge_linear *lin, int for_backward)
+{
+    if (check(lin)) return 0;
+    const Plan p = plan_of(lin);
+    return for_backward ? 0 : p.x + p.w;
+}
+
+int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_backward, void *saved, size_t saved_bytes, void *workspace,
+                   size_t workspace_bytes, void *stream)
+{
+    if (const int rc = check(lin)) return rc;
+    if (lin->rows == 0 || lin->out == 0) return KGE_OK;
+    if (!y) return KGE_EINVAL;
+    if (y_stride < lin->out) return KGE_ESHAPE;
+    const Plan p = plan_of(lin);
+    const size_t need_saved = for_backward ? p.slope + p.x + p.w : 0, need = for_backward ? 0 : p.x + p.w;
+    if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
+    char *slope = for_backward && p.slope ? static_cast<char *>(saved) : nullptr;
+    char *px = for_backward ? static_cast<char *>(saved) + p.slope : static_cast<char *>(workspace);
+    hipStream_t st = as_stream(stream);
+    KGE_CLEAR_LAUNCH_ERRORS();
+    if (lin->type == KGE_F32) return forward<float>(lin, p, y, y_stride, slope, px, px + p.x, st);
+    if (lin->type == KGE_BF16) return forward<bf16_t>(lin, p, y, y_stride, slope, px, px + p.x, st);
+    return forward<half_t>(lin, p, y, y_stride, slope, px, px + p.x, st);
+}
+
+size_t kge_linear_bwd_workspace(const kge_linear *lin)
+{
+    if (check(lin)) return 0;
+    const Plan p = plan_of(lin);
+    return packed_bytes(lin->type, lin->rows, lin->out) + up256((size_t)p.sum_blocks * p.quads * 16) +
+           (p.dw_splits > 1 ? (size_t)p.dw_splits * lin->out * ceil_div(lin->in, 4) * 16 : 0);
+}
+
+int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx, void *dweight,
+                   void *dbias, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (const int rc = check(lin)) return rc;
+    if (dy_stride < lin->out) return KGE_ESHAPE;
+    if (lin->rows > 0 && lin->out > 0 && !dy) return KGE_EINVAL;
+    const Plan p = plan_of(lin);
+    const size_t need_saved = p.slope + p.x + p.w, need = kge_linear_bwd_workspace(lin);
+    if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
+    hipStream_t st = as_stream(stream);
+    KGE_CLEAR_LAUNCH_ERRORS();
+    const char *s = static_cast<const char *>(saved);
+    char *ws = static_cast<char *>(workspace);
+    if (lin->type == KGE_F32) return backward<float>(lin, p, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+    if (lin->type == KGE_BF16) return backward<bf16_t>(lin, p, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+    return backward<half_t>(lin, p, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+}
+
+}  // extern "C"

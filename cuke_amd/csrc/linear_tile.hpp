@@ -1,0 +1,284 @@
+// Matrix products of the linear layers on the matrix cores: out[m][n] = sum over k of side a (n, k) and side b (m, k).
+//
+// Each side lies in memory in one of two ways: ALONG rows (row = its index, the sum runs inside the row) or ACROSS them (the sum runs
+// over rows, the index inside).  y = x W^T has both sides along, dx = dz W one across, dW = dz^T x both: no operand is ever transposed in
+// memory.  Tiles go to LDS 16 bytes a lane without passing through registers; a tile that lies across is turned by the transposing LDS
+// reads on its way to the matrix cores.  fp32 sides come as three bf16 planes (mfma_split.hpp), of whose nine products six are formed.
+#pragma once
+
+#include "features.hpp"
+#include "mfma_split.hpp"
+
+namespace kge {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+template <class E>
+struct Mfma;
+template <>
+struct Mfma<bf16_t> {
+    __device__ __forceinline__ static floatx16 go(s16x8 a, s16x8 b, floatx16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Mfma<half_t> {
+    __device__ __forceinline__ static floatx16 go(s16x8 a, s16x8 b, floatx16 c)
+    {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+
+// One side of a product.  Rows start 16-byte aligned and a multiple of 8 elements apart; elements between the last one and the next
+// multiple of 8 belong to the row and, where the sum runs inside it, are zero.
+struct Side {
+    const void *p;
+    int64_t stride;  // elements between rows
+    int64_t plane;   // elements between the planes of an fp32 side
+    int64_t extent;  // indices
+};
+
+// Where sums go: through the epilogue of the layer, rounded to the layer's type, or as fp32 partial sums of a split.
+enum EndKind { kEndLayer, kEndStore, kEndPartial };
+
+struct Ends {
+    void *y;
+    int64_t y_stride;
+    const void *bias;
+    const void *residual;
+    int64_t residual_stride;
+    void *slope;  // [rows][quads * 4], or NULL
+    int64_t rows, cols, quads;
+    Drop drop;
+    int act;
+    int out_f32;  // y and residual in fp32
+};
+
+struct TileArgs {
+    Side a, b;      // a: the columns of the output, b: its rows
+    int64_t k;      // terms of every sum
+    int64_t k_each; // per split, a multiple of kTileK
+    int tiles_a, tiles_b, splits;
+    float *partial; // [splits][rows][quads * 4]
+    Ends e;
+};
+
+constexpr int kTileK = 32;
+
+static __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};  // what chunks outside a side read
+
+__device__ __forceinline__ void chunk_to_lds(const void *src, void *lds)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+// A tile of X indices by 32 terms in LDS, as 16-byte chunks.  Along: four chunks a row, chunk j in slot j ^ (row / 2 % 4), so that the
+// 128-bit reads of eight consecutive rows fall on distinct banks.  Across: X / 8 chunks a row of terms, pairs of chunks permuted by the row so
+// that the transposing reads of four rows (and of both halves of a wave, where the row is long enough) do.
+template <int X, bool ACROSS, int THREADS>
+struct Tile {
+    static constexpr int kChunks = X * kTileK / 8;
+    static constexpr int kRounds = kChunks / THREADS;
+    static constexpr int kRow = ACROSS ? X / 8 : 4;  // chunks a row
+    static_assert(kChunks % THREADS == 0, "whole rounds");
+
+    __device__ __forceinline__ static int turn(int row)
+    {
+        if (!ACROSS) return (row >> 1) & 3;
+        return X >= 256 ? 2 * (2 * (row & 3) + 8 * ((row >> 3) & 1)) : (X >= 128 ? 4 * (row & 3) : 2 * (row & 3));
+    }
+
+    // the chunks of terms [k, k + 32) this thread brings in
+    template <class E>
+    __device__ __forceinline__ static void load(const Side &s, const E *p, int64_t first, int64_t k, int64_t k_end, char *lds)
+    {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+        for (int r = 0; r < kRounds; ++r) {
+            const int c = r * THREADS + (int)threadIdx.x;
+            const int row = c / kRow, j = (c % kRow) ^ turn(row);
+            const int64_t index = first + (ACROSS ? 8 * j : row), term = k + (ACROSS ? row : 8 * j);
+            const E *src = p + (ACROSS ? term * s.stride + index : index * s.stride + term);
+            const void *from = index < s.extent && term < k_end ? (const void *)src : (const void *)zero_chunk;
+            chunk_to_lds(from, lds + 16 * (r * THREADS + wave * 64));
+        }
+    }
+
+    // eight terms of an index for each lane: index at + lane % 32, terms 16 step + 8 (lane / 32) .. + 7
+    __device__ __forceinline__ static s16x8 read(const char *lds, int at, int step, int lane)
+    {
+        if (!ACROSS) {
+            const int row = at + (lane & 31), j = 2 * step + (lane >> 5);
+            return *reinterpret_cast<const s16x8 *>(lds + 16 * (row * 4 + (j ^ turn(row))));
+        }
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const int row = 16 * step + 8 * (lane >> 5) + ((lane & 15) >> 2), index = at + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const char *p = lds + 16 * (row * kRow + ((index >> 3) ^ turn(row))) + 2 * (index & 7);
+        const char *q = lds + 16 * ((row + 4) * kRow + ((index >> 3) ^ turn(row + 4))) + 2 * (index & 7);
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)q);
+        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// The sum of one output element by fp32 instructions, from the planes (which add up to the value, infinities and NaNs included).
+template <bool A_ACROSS, bool B_ACROSS>
+__device__ __noinline__ float plain_sum(const Side &a, const Side &b, int64_t n, int64_t m, int64_t k0, int64_t k1)
+{
+    const bf16_t *pa = static_cast<const bf16_t *>(a.p), *pb = static_cast<const bf16_t *>(b.p);
+    float s = 0.0f;
+    for (int64_t k = k0; k < k1; ++k) {
+        const bf16_t *x = pa + (A_ACROSS ? k * a.stride + n : n * a.stride + k), *y = pb + (B_ACROSS ? k * b.stride + m : m * b.stride + k);
+        s = fmaf((float)x[0] + (float)x[a.plane] + (float)x[2 * a.plane], (float)y[0] + (float)y[b.plane] + (float)y[2 * b.plane], s);
+    }
+    return s;
+}
+
+// Four consecutive columns of a row through the layer's epilogue.  T: the layer's type.
+template <class T>
+__device__ __forceinline__ void finish_quad(const Ends &e, uint64_t base, int64_t row, int64_t col, float4 z)
+{
+    const int valid = (int)(e.cols - col < 4 ? e.cols - col : 4);
+    if (e.bias) {
+        const float4 b = load4(static_cast<const T *>(e.bias) + col, valid);
+        z.x += b.x, z.y += b.y, z.z += b.z, z.w += b.w;
+    }
+    if (e.act != KGE_ACT_NONE) {
+        float4 s;
+        z.x = activate(z.x, e.act, &s.x), z.y = activate(z.y, e.act, &s.y), z.z = activate(z.z, e.act, &s.z), z.w = activate(z.w, e.act, &s.w);
+        if (e.slope) {  // (rows of whole quads)
+            const int64_t at = row * 4 * e.quads + col;
+            if (sizeof(T) == 4) {
+                *reinterpret_cast<float4 *>(static_cast<float *>(e.slope) + at) = s;
+            } else {
+                const ushort4 q = {slope_to_fixed(s.x), slope_to_fixed(s.y), slope_to_fixed(s.z), slope_to_fixed(s.w)};
+                *reinterpret_cast<ushort4 *>(static_cast<uint16_t *>(e.slope) + at) = q;
+            }
+        }
+    }
+    if (e.drop.cut) z = e.drop.apply(z, e.drop.word(base, row, col >> 2));
+    if (e.residual) {
+        const int64_t at = row * e.residual_stride + col;
+        const float4 r = sizeof(T) == 4 || e.out_f32 ? load4(static_cast<const float *>(e.residual) + at, valid)
+                                                     : load4(static_cast<const T *>(e.residual) + at, valid);
+        z.x += r.x, z.y += r.y, z.z += r.z, z.w += r.w;
+    }
+    const int64_t at = row * e.y_stride + col;
+    if (sizeof(T) == 4 || e.out_f32) store4(static_cast<float *>(e.y) + at, z, valid);
+    else store4(static_cast<T *>(e.y) + at, z, valid);
+}
+
+// Workgroups are dealt to the eight XCDs in turn; consecutive tiles go to one XCD, whose L2 then holds the rows and columns they share:
+// eight rows of tiles at a time, walked column by column.
+__device__ __forceinline__ void tile_of(int64_t block, int64_t blocks, const TileArgs &t, int *ta, int *tb, int *split)
+{
+    const int64_t xcd = block & 7, each = blocks >> 3, more = blocks & 7;
+    const int64_t id = xcd * each + (xcd < more ? xcd : more) + (block >> 3);
+    const int64_t tiles = (int64_t)t.tiles_a * t.tiles_b;
+    *split = (int)(id / tiles);
+    const int64_t q = id % tiles, band = (int64_t)8 * t.tiles_a;
+    const int64_t first = q / band * 8, wide = t.tiles_b - first < 8 ? t.tiles_b - first : 8;
+    *tb = (int)(first + q % band % wide), *ta = (int)(q % band / wide);
+}
+
+// E: what the matrix cores multiply, PLANES: 3 for fp32.  A workgroup of WA x WB waves computes XA columns by XB rows.
+template <class E, int PLANES, bool A_ACROSS, bool B_ACROSS, int XA, int XB, int WA, int WB, EndKind END>
+__global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
+{
+    using T = typename std::conditional<PLANES == 3, float, E>::type;
+    constexpr int kThreads = WA * WB * kWave;
+    using A = Tile<XA, A_ACROSS, kThreads>;
+    using B = Tile<XB, B_ACROSS, kThreads>;
+    constexpr int kBytesA = XA * kTileK * 2, kBytesB = XB * kTileK * 2, kStage = PLANES * (kBytesA + kBytesB);
+    constexpr int FA = XA / WA / 32, FB = XB / WB / 32;
+    __shared__ __align__(16) char stage0[kStage], stage1[kStage];
+
+    int ta, tb, split;
+    tile_of(blockIdx.x, gridDim.x, t, &ta, &tb, &split);
+    const int64_t n0 = (int64_t)ta * XA, m0 = (int64_t)tb * XB;
+    const int64_t k0 = split * t.k_each, k1 = k0 + t.k_each < t.k ? k0 + t.k_each : t.k;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wa = (wave % WA) * (XA / WA), wb = (wave / WA) * (XB / WB);
+
+    floatx16 acc[FA][FB] = {}, low[PLANES == 3 ? FA : 1][PLANES == 3 ? FB : 1] = {};
+
+    auto load = [&](int64_t k, char *lds) {
+#pragma unroll
+        for (int p = 0; p < PLANES; ++p) {
+            A::load(t.a, static_cast<const E *>(t.a.p) + p * t.a.plane, n0, k, k1, lds + p * kBytesA);
+            B::load(t.b, static_cast<const E *>(t.b.p) + p * t.b.plane, m0, k, k1, lds + PLANES * kBytesA + p * kBytesB);
+        }
+    };
+    auto multiply = [&](const char *lds) {
+#pragma unroll
+        for (int step = 0; step < kTileK / 16; ++step) {
+            s16x8 a[FA][PLANES], b[FB][PLANES];
+#pragma unroll
+            for (int p = 0; p < PLANES; ++p) {
+#pragma unroll
+                for (int i = 0; i < FA; ++i) a[i][p] = A::read(lds + p * kBytesA, wa + 32 * i, step, lane);
+#pragma unroll
+                for (int j = 0; j < FB; ++j) b[j][p] = B::read(lds + PLANES * kBytesA + p * kBytesB, wb + 32 * j, step, lane);
+            }
+#pragma unroll
+            for (int i = 0; i < FA; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j) {
+                    if constexpr (PLANES == 1) {
+                        acc[i][j] = Mfma<E>::go(a[i][0], b[j][0], acc[i][j]);
+                    } else {
+#pragma unroll
+                        for (int u = 0; u < kSplitTerms - 1; ++u) low[i][j] = Mfma<E>::go(a[i][kTermA[u]], b[j][kTermB[u]], low[i][j]);
+                        acc[i][j] = Mfma<E>::go(a[i][0], b[j][0], acc[i][j]);
+                    }
+                }
+        }
+    };
+
+    if (k0 < k1) load(k0, stage0);
+    for (int64_t k = k0; k < k1; k += 2 * kTileK) {
+        __syncthreads();  // (the stage has landed, and everyone is done with the other one)
+        if (k + kTileK < k1) load(k + kTileK, stage1);
+        multiply(stage0);
+        if (k + kTileK >= k1) break;
+        __syncthreads();
+        if (k + 2 * kTileK < k1) load(k + 2 * kTileK, stage0);
+        multiply(stage1);
+    }
+
+    // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
+    const uint64_t base = END == kEndLayer ? t.e.drop.base() : 0;
+#pragma unroll
+    for (int i = 0; i < FA; ++i)
+#pragma unroll
+        for (int j = 0; j < FB; ++j) {
+            const int64_t row = m0 + wb + 32 * j + (lane & 31);
+            if (row >= t.e.rows) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t col = n0 + wa + 32 * i + 8 * q + 4 * (lane >> 5);
+                if (col >= t.e.cols) continue;
+                float z[4];
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    z[v] = acc[i][j][4 * q + v];
+                    if constexpr (PLANES == 3) {
+                        z[v] += low[i][j][4 * q + v];
+                        // (an infinite operand's planes, or leading parts that were rounded up, may have made this of a finite sum)
+                        if (not_finite(z[v]) && col + v < t.e.cols) z[v] = plain_sum<A_ACROSS, B_ACROSS>(t.a, t.b, col + v, row, k0, k1);
+                    }
+                }
+                const float4 four = make_float4(z[0], z[1], z[2], z[3]);
+                if constexpr (END == kEndPartial)
+                    *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = four;
+                else if constexpr (END == kEndLayer)
+                    finish_quad<T>(t.e, base, row, col, four);
+                else
+                    store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, four, (int)(t.e.cols - col < 4 ? t.e.cols - col : 4));
+            }
+        }
+}
+
+}  // namespace kge

@@ -544,6 +544,106 @@ int kge_train_step_staged(const kge_tables *tab, kge_step_batch *cur, kge_step_b
 int kge_train_step(const kge_tables *tab, kge_step_batch *cur, const kge_step_buffers *buf, int fused, void *stream,
                    void *side_stream);
 
+/* ---- operators that make entity rows from features, and a loss against a frozen model --------------------------------------
+ *
+ * No counterpart in the reference, whose rows are always looked up.  Arrays are row-major with a stride in elements between
+ * rows (>= the row's length) and consecutive elements inside a row; they may start at any element.
+ */
+typedef enum kge_type_t { KGE_F32 = 0, KGE_BF16 = 1, KGE_F16 = 2 } kge_type_t;
+typedef enum kge_act_t {
+    KGE_ACT_NONE = 0,
+    KGE_ACT_RELU = 1, /* max(0, z) */
+    KGE_ACT_GELU = 2, /* z Phi(z), Phi the normal distribution */
+    KGE_ACT_SILU = 3  /* z / (1 + exp(-z)) */
+} kge_act_t;
+
+/*
+ * Dropout by a counter-based generator; no mask is stored.  With T = the whole number nearest to 65536 p, element (i, j) of [rows, cols] is
+ * dropped (zero, whatever x holds) iff
+ *   16 bits number j % 4 (the lowest first) of  splitmix64(base ^ ((i * ceil(cols / 4) + j / 4) * 0x9E3779B97F4A7C15))  are < T,
+ *   base = splitmix64(splitmix64(seed ^ 0xD1B54A32D192ED03) ^ (step + (step_dev ? *step_dev : 0))),
+ * and x * 65536 / (65536 - T) otherwise, rounded once.  step_dev is a word in device memory that the kernel reads, so that replays of a captured
+ * graph draw new masks.  The gradient of x is the same call on the gradient of y.  y == x is allowed; type: kge_type_t of x and y.
+ */
+int kge_dropout(int32_t type, const void *x, int64_t x_stride, void *y, int64_t y_stride, int64_t rows, int64_t cols, double p,
+                uint64_t seed, uint64_t step, const uint64_t *step_dev, void *stream);
+
+/*
+ * A linear layer with its epilogue:  y = drop(act(x weight^T + bias)) + residual, and its gradients.
+ *   x [rows, in], weight [out, in], bias [out] (NULL: none) have the type `type`; y and residual [rows, out] (NULL: none), and the
+ *   gradient of y, have the type `out_type`: `type` or KGE_F32.  The gradient of the residual is the gradient of y.  drop is kge_dropout of
+ *   the [rows, out] block with p, seed, step, step_dev (p = 0: none).  16-bit products are summed in fp32 on the matrix cores, fp32 ones
+ *   as three-part bf16 products (no larger an error against 64 bits than fp32 products); everything up to the last rounding is fp32.
+ *   rows, in, out: 0 .. 2^31 - 1 (in = 0: an empty sum).
+ */
+typedef struct kge_linear {
+    int32_t type, out_type; /* kge_type_t */
+    int32_t act;            /* kge_act_t */
+    int32_t reserved;
+    int64_t rows, in, out;
+    const void *x;
+    int64_t x_stride;
+    const void *weight;
+    int64_t weight_stride;
+    const void *bias;
+    const void *residual;
+    int64_t residual_stride;
+    double p;
+    uint64_t seed, step;
+    const uint64_t *step_dev;
+} kge_linear;
+
+/*
+ * saved: NULL for inference; else kge_linear_saved_bytes() bytes, 16-byte aligned, which kge_linear_fwd fills for kge_linear_bwd: act'(z)
+ * (16-bit layers: in 16 bits of fixed point, to 1.02e-5), and x and weight as the matrix cores take them where their own memory is not
+ * that (fp32, row widths that are no multiple of 8, odd addresses).  x and weight have to be unchanged when kge_linear_bwd runs, and *step_dev too.
+ * The byte counts depend on the types, sizes, strides, the low bits of addresses and whether there is an activation; a saved block of no bytes may be NULL.
+ */
+size_t kge_linear_saved_bytes(const kge_linear *lin);
+size_t kge_linear_fwd_workspace(const kge_linear *lin, int for_backward);
+int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_backward, void *saved, size_t saved_bytes, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/*
+ * dx [rows, in], dweight [out, in], dbias [out]: contiguous, of type `type`; each may be NULL and is then not computed.  The gradient at the
+ * products, dz = drop(dy) act'(z), enters them rounded to `type` (dbias sums it unrounded).  Sums over rows are split and joined in a fixed order:
+ * the same call gives the same bits.
+ */
+size_t kge_linear_bwd_workspace(const kge_linear *lin);
+int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx,
+                   void *dweight, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * A preference loss over the positive and negative scores of a batch, against those a frozen reference gives the same triples:
+ *   d[b][n] = sign * ((pos[b] - ref_pos[b]) - (neg[b][n] - ref_neg[b][n]))       (ref_* NULL: 0; both or neither)
+ *   f(d):  KGE_PREFER_SIGMOID  (1 - smoothing) log(1 + exp(-beta d)) + smoothing log(1 + exp(beta d))
+ *          KGE_PREFER_HINGE    max(0, 1 - beta d)
+ *          KGE_PREFER_SQUARE   (d - 1 / (2 beta))^2
+ *   a[b][.] = softmax over the row's valid n of temperature * sign * neg[b][n]  (0: uniform); a constant to the gradient
+ *   loss[0] = 1 / batch * sum_b sum_n a[b][n] f(d[b][n]),   dpos [batch], dneg [batch, n_neg]: its gradients, fp32, contiguous (NULL: not wanted)
+ * mask: one byte per pair, 0 = the pair does not exist (what the score arrays hold there is not looked at, its gradient is 0), NULL = all
+ * exist.  A row of no valid pair adds nothing, and its dpos is 0.  Scores and reference scores: kge_type_t `type`; sums and exponentials in fp32,
+ * the loss over rows in 64 bits, joined in a fixed order.  sign: +1 where higher scores are better, -1 for distances.
+ */
+typedef enum kge_prefer_t { KGE_PREFER_SIGMOID = 0, KGE_PREFER_HINGE = 1, KGE_PREFER_SQUARE = 2 } kge_prefer_t;
+typedef struct kge_preference {
+    int32_t type; /* kge_type_t */
+    int32_t kind; /* kge_prefer_t */
+    int64_t batch, n_neg;
+    const void *pos; /* [batch] */
+    const void *neg;
+    int64_t neg_stride;
+    const void *ref_pos; /* [batch] */
+    const void *ref_neg;
+    int64_t ref_neg_stride;
+    const uint8_t *mask;
+    int64_t mask_stride;
+    float beta, sign, smoothing, temperature;
+} kge_preference;
+size_t kge_preference_workspace(const kge_preference *pref);
+int kge_preference_loss(const kge_preference *pref, float *loss, float *dpos, float *dneg, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
 /* Sets flag[0] (int32, caller-zeroed) to 1 if any idx[i] is outside [0, n_rows). */
 int kge_check_indices(const int64_t *idx, int64_t n, int64_t n_rows, int32_t *flag, void *stream);
 

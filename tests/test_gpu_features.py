@@ -1,0 +1,547 @@
+"""Linear layers, dropout and the preference loss on the GPU against plain formulas in 64 bits.
+
+Tolerances, element by element, from the roundings a result goes through (u: half a unit in the last place of a type, eps = 2^-24):
+  a sum of K products in fp32, in any order     (K + 16) eps sum |a_k b_k|     (16: bias, activation, scale, residual, each a few eps)
+  the last rounding                             u |result|
+  a derivative kept in 16 bits of fixed point   1.02e-5, + 4 eps of its own evaluation and of z's error (|act''| <= 1.2)
+  dz in a 16-bit layer's type                   u |dz|, carried through the products by sum |w|
+Sums of relu layers are made of multiples of 1/8 that every type holds exactly, so that both sides agree on which of them are zero.
+"""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+U = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}   # (bf16, f16: to nearest, one bit to spare for bf16)
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}             # half the spacing of f16's subnormal numbers
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda:0"
+
+
+def kept(rows, cols, p, seed, step):
+    """[rows, cols] factors of the generator in the C header, on the host."""
+    cut = int(np.rint(p * 65536))
+    with np.errstate(over="ignore"):
+        def mix(z):
+            z = z + np.uint64(0x9E3779B97F4A7C15)
+            z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+            z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+            return z ^ (z >> np.uint64(31))
+        base = mix(mix(np.array([(seed % (1 << 64)) ^ 0xD1B54A32D192ED03], dtype=np.uint64)) ^ np.uint64(step % (1 << 64)))
+        i, j = np.meshgrid(np.arange(rows, dtype=np.uint64), np.arange(cols, dtype=np.uint64), indexing="ij")
+        word = mix(base ^ ((i * np.uint64((cols + 3) // 4) + j // np.uint64(4)) * np.uint64(0x9E3779B97F4A7C15)))
+        bits = (word >> (np.uint64(16) * (j % np.uint64(4)))) & np.uint64(0xFFFF)
+    scale = 65536.0 / (65536 - cut) if cut < 65536 else 0.0
+    return torch.from_numpy(np.where(bits >= np.uint64(cut), scale, 0.0)).to(DEV)
+
+
+def act64(z, act):
+    if act == "gelu":
+        c = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    if act == "relu":
+        return torch.clamp(z, min=0), (z > 0).double()
+    return z, torch.ones_like(z)
+
+
+def draw(gen, shape, dtype, scale=1.0, grid=False):
+    t = torch.randn(shape, generator=gen, dtype=torch.float64) * scale
+    if grid:
+        t = torch.clamp(torch.round(t * 8), -16, 16) / 8
+    return t.to(DEV).to(dtype)
+
+
+def within(got, want, tol, what):
+    got = got.double()
+    assert got.shape == want.shape, what
+    bad = ~((got - want).abs() <= tol)
+    if bad.any():
+        i = torch.nonzero(bad)[0].tolist()
+        raise AssertionError(f"{what}: {int(bad.sum())} of {bad.numel()} off, first at {i}: {got[tuple(i)].item()} for "
+                             f"{want[tuple(i)].item()} +- {tol.expand_as(want)[tuple(i)].item()}")
+
+
+class Layer:
+    """Inputs of a layer, its 64-bit results and their tolerances."""
+
+    def __init__(self, rows, fin, fout, dtype, act="none", drop=0.0, bias=True, residual=False, out=None, seed=0, layout="plain"):
+        g = torch.Generator().manual_seed(1000 * seed + rows + 7 * fin + 13 * fout)
+        grid = act == "relu"
+
+        def make(r, c, t, scale):
+            if layout == "plain":
+                return draw(g, (r, c), t, scale, grid)
+            if layout == "slice":                                  # an odd offset into wider rows
+                return draw(g, (r, c + 5), t, scale, grid)[:, 3:3 + c]
+            if layout == "wide":                                   # rows on 16 bytes, a stride that is not their length
+                return draw(g, (r, (c + 7) // 8 * 8 + 8), t, scale, grid)[:, :c]
+            return draw(g, (c, r), t, scale, grid).t()             # columns contiguous
+        self.out = out or dtype
+        self.x = make(rows, fin, dtype, 1.0)
+        self.w = make(fout, fin, dtype, 1.0 if grid else fin ** -0.5)
+        self.b = draw(g, (fout,), dtype, 0.3, grid) if bias else None
+        self.res = make(rows, fout, self.out, 0.5) if residual else None
+        self.dy = make(rows, fout, self.out, 0.5)
+        self.dtype, self.act, self.drop, self.seed, self.step = dtype, act, drop, 77 + seed, 5
+        x, w, dy = self.x.double(), self.w.double(), self.dy.double()
+        z = x @ w.T + (self.b.double() if bias else 0.0)
+        size = x.abs() @ w.abs().T + (self.b.double().abs() if bias else 0.0)
+        k = kept(rows, fout, drop, self.seed, self.step) if drop else torch.ones_like(z)
+        a, slope = act64(z, act)
+        self.y = a * k + (self.res.double() if residual else 0.0)
+        inner = (fin + 16) * EPS * (size + 1.0)
+        self.y_tol = U[self.out] * self.y.abs() + TINY[self.out] + 1.2 * k * inner + 16 * EPS * (self.y.abs() + (self.res.double().abs() if residual else 0.0))
+        dz = dy * k * slope
+        exact_dz = act == "none" and not drop and self.out == dtype
+        low = dtype != torch.float32
+        dz_tol = torch.zeros_like(dz)
+        if not exact_dz:
+            dz_tol = dy.abs() * k * (1.2 * inner * (act not in ("none", "relu")) + 16 * EPS + (1.1e-5 if low and act != "none" else 0.0))
+        db_tol = dz_tol
+        if low and not exact_dz:
+            dz_tol = dz_tol + U[dtype] * (dz.abs() + dz_tol) + TINY[dtype]
+        self.dx, self.dw, self.db = dz @ w, dz.T.contiguous() @ x, dz.sum(0)
+        self.dx_tol = dz_tol @ w.abs() + (fout + 16) * EPS * (dz.abs() @ w.abs()) + U[dtype] * self.dx.abs() + TINY[dtype]
+        self.dw_tol = dz_tol.T.contiguous() @ x.abs() + (rows + 16) * EPS * (dz.abs().T.contiguous() @ x.abs()) + U[dtype] * self.dw.abs() + TINY[dtype]
+        self.db_tol = db_tol.sum(0) + (rows + 16) * EPS * dz.abs().sum(0) + U[dtype] * self.db.abs() + TINY[dtype]
+
+    def kw(self):
+        return dict(act=self.act, drop=self.drop, seed=self.seed, step=self.step, residual=self.res, out_dtype=self.out)
+
+    def check(self):
+        from cuke_amd import features
+        within(features.linear(self.x, self.w, self.b, **self.kw()), self.y, self.y_tol, "y without a backward pass")
+        fw = features.linear_forward(self.x, self.w, self.b, **self.kw())
+        within(fw.y, self.y, self.y_tol, "y")
+        assert fw.y.dtype == self.out
+        g = features.linear_backward(fw, self.dy)
+        within(g.x, self.dx, self.dx_tol, "dx")
+        within(g.weight, self.dw, self.dw_tol, "dw")
+        if self.b is None:
+            assert g.bias is None
+        else:
+            within(g.bias, self.db, self.db_tol, "db")
+        again = features.linear_backward(fw, self.dy)
+        assert torch.equal(again.x, g.x) and torch.equal(again.weight, g.weight), "the same call gives the same bits"
+        return fw, g
+
+
+# one row to many, one term to many, whole tiles and none: on both sides of every tile and chunk width
+SHAPES = [(1, 1, 1), (1, 64, 64), (1, 1000, 33), (2, 7, 5), (3, 129, 257), (16, 8, 16), (17, 40, 24), (31, 96, 130), (33, 33, 31), (63, 300, 200),
+          (64, 32, 96), (65, 31, 129), (100, 50, 400), (127, 128, 128), (129, 256, 136), (200, 2048, 72), (257, 264, 520), (300, 17, 3),
+          (1000, 24, 8), (1025, 72, 264)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+def test_layer_shapes(shape, dtype):
+    print("layer", shape, dtype, flush=True)
+    Layer(*shape, dtype, act="gelu").check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu"])
+@pytest.mark.parametrize("drop,bias,residual", [(0.0, False, False), (0.0, True, True), (0.3, True, False), (0.1, False, True)])
+def test_layer_epilogues(dtype, act, drop, bias, residual):
+    print("epilogue", dtype, act, drop, bias, residual, flush=True)
+    Layer(70, 88, 150, dtype, act=act, drop=drop, bias=bias, residual=residual).check()
+    if dtype != torch.float32:
+        Layer(70, 88, 150, dtype, act=act, drop=drop, bias=bias, residual=residual, out=torch.float32).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["slice", "wide", "columns"])
+@pytest.mark.parametrize("shape", [(40, 64, 72), (150, 130, 66), (5, 33, 31)])
+def test_layer_layouts(shape, layout, dtype):
+    print("layout", shape, layout, dtype, flush=True)
+    Layer(*shape, dtype, act="silu", drop=0.2, residual=True, layout=layout).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(5000, 72, 40), (2500, 520, 264), (4096, 256, 512)])
+def test_layer_long_sums_over_rows(shape, dtype):
+    """Sums over rows that are split between workgroups."""
+    print("long", shape, dtype, flush=True)
+    Layer(*shape, dtype, act="gelu", drop=0.1, residual=True).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_large(dtype):
+    print("large", dtype, flush=True)
+    Layer(8200, 520, 776, dtype, act="gelu", drop=0.1).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_gradients_against_differences(dtype):
+    """The slope of sum(y dy) along random directions, by central differences of the 64-bit formula."""
+    from cuke_amd import features
+    L = Layer(37, 45, 52, dtype, act="gelu", drop=0.25, residual=True, seed=3)
+    fw = features.linear_forward(L.x, L.w, L.b, **L.kw())
+    g = features.linear_backward(fw, L.dy)
+    k = kept(37, 52, L.drop, L.seed, L.step)
+    gen = torch.Generator().manual_seed(9)
+
+    def total(x, w, b):
+        return ((act64(x @ w.T + b, "gelu")[0] * k + L.res.double()) * L.dy.double()).sum()
+
+    at = [L.x.double(), L.w.double(), L.b.double()]
+    for i, (grad, tol) in enumerate([(g.x, L.dx_tol), (g.weight, L.dw_tol), (g.bias, L.db_tol)]):
+        v = torch.randn(at[i].shape, generator=gen, dtype=torch.float64).to(DEV)
+        h = 1e-4
+        lo, hi = [list(at) for _ in range(2)]
+        lo[i], hi[i] = at[i] - h * v, at[i] + h * v
+        slope = (total(*hi) - total(*lo)) / (2 * h)
+        # the differences' own error: h^2 / 6 |third derivative| (below 2e3 for these sizes) + rounding
+        assert abs((grad.double() * v).sum() - slope) <= (tol * v.abs()).sum() + 2e3 * h * h
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_of_nothing(dtype):
+    from cuke_amd import features
+    for rows, fin, fout in [(0, 8, 8), (5, 0, 8), (5, 8, 0), (0, 0, 0), (0, 8, 0)]:
+        x, w = torch.randn(rows, fin, device=DEV).to(dtype), torch.randn(fout, fin, device=DEV).to(dtype)
+        b = torch.randn(fout, device=DEV).to(dtype)
+        fw = features.linear_forward(x, w, b, act="silu")
+        want = torch.nn.functional.silu(b.double()).expand(rows, fout)
+        assert torch.allclose(fw.y.double(), want, rtol=2 * U[dtype], atol=1e-6)
+        g = features.linear_backward(fw, torch.ones_like(fw.y))
+        assert g.x.shape == (rows, fin) and g.weight.shape == (fout, fin) and g.bias.shape == (fout,)
+        assert not g.x.any() and not g.weight.any()
+        if rows == 0:
+            assert not g.bias.any()
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_infinities_and_nans(dtype, rows):
+    """They reach the rows and columns whose sums hold them, as fp32 sums would have it, and no others."""
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(3)
+    x, w = draw(g, (rows, 80), dtype), draw(g, (90, 80), dtype, 0.1)
+    x[0, 5], x[1, 7], w[4, 9] = float("inf"), float("nan"), -float("inf")
+    w[6, 5] = 0.0                                    # infinity times zero
+    y = features.linear(x, w)
+    want = (x.float().cpu() @ w.float().cpu().T).to(DEV)
+    assert torch.equal(torch.isnan(y), torch.isnan(want))
+    assert torch.equal(torch.isinf(y), torch.isinf(want)) and torch.equal(torch.sign(y[torch.isinf(y)]).float(), torch.sign(want[torch.isinf(want)]))
+    fw = features.linear_forward(x, w)
+    dy = torch.ones_like(fw.y)
+    dy[2, 3] = float("inf")
+    got = features.linear_backward(fw, dy)
+    for have, want in [(got.x, dy.float().cpu() @ w.float().cpu()), (got.weight, dy.float().cpu().T @ x.float().cpu())]:
+        assert torch.equal(torch.isnan(have).cpu(), torch.isnan(want)) and torch.equal(torch.isinf(have).cpu(), torch.isinf(want))
+
+
+def test_layer_fp32_at_the_edge_of_its_range():
+    """fp32 values whose leading bf16 part would round to infinity, products near the largest number, and very small ones."""
+    from cuke_amd import features
+    x = torch.full((5, 24), 3.4e38, device=DEV)
+    w = torch.zeros((7, 24), device=DEV)
+    w[:, 3], w[1, 4], w[2, 3] = 1.0, -1.0, 2.0
+    y = features.linear(x, w)
+    want = (x.double() @ w.double().T).float()
+    assert torch.equal(y, want)
+    small = torch.full((200, 24), 1e-30, device=DEV)
+    y = features.linear(small, torch.full((7, 24), 1e-3, device=DEV))
+    assert torch.allclose(y.double(), torch.full_like(y, 24e-33).double(), rtol=1e-5)
+
+
+def test_layer_derivative_reaches_its_ends():
+    """Saturated and dead units, whose derivatives the fixed point holds exactly or to its spacing."""
+    from cuke_amd import features
+    for dtype in (torch.bfloat16, torch.float16):
+        z = torch.tensor([-60000.0, -40.0, -6.0, -1.0, 0.0, 1.0, 6.0, 40.0, 60000.0], device=DEV).to(dtype)
+        for act in ("relu", "gelu", "silu"):
+            fw = features.linear_forward(z[:, None], torch.ones(1, 1, device=DEV, dtype=dtype), act=act)
+            g = features.linear_backward(fw, torch.ones_like(fw.y))
+            a, s = act64(z.double(), act)
+            within(fw.y[:, 0], a, U[dtype] * a.abs() + 4e-7 * (1 + z.double().abs()) * (a != 0) + TINY[dtype], f"{act} {dtype}")
+            within(g.x[:, 0], s, 1.1e-5 + 2 * U[dtype] * s.abs() + 2 * TINY[dtype], f"{act}' {dtype}")
+
+
+def test_layer_on_another_stream_and_in_a_graph():
+    from cuke_amd import features
+    L = Layer(300, 264, 136, torch.bfloat16, act="gelu", drop=0.2, residual=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fw = features.linear_forward(L.x, L.w, L.b, **L.kw())
+        g = features.linear_backward(fw, L.dy)
+    torch.cuda.current_stream().wait_stream(side)
+    within(fw.y, L.y, L.y_tol, "y")
+    within(g.weight, L.dw, L.dw_tol, "dw")
+    # a graph whose mask goes by a word in device memory
+    step = torch.tensor([5], device=DEV)
+    kw = dict(L.kw(), step=step)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fw = features.linear_forward(L.x, L.w, L.b, **kw)
+        g = features.linear_backward(fw, L.dy)
+        d = features.dropout(L.x, 0.5, 3, step)
+        step += 1
+    for replay in range(4):
+        step.fill_(5 + replay % 2)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = features.linear_forward(L.x, L.w, L.b, **dict(L.kw(), step=5 + replay % 2))
+        want = features.linear_backward(eager, L.dy)
+        assert int(step.item()) == 6 + replay % 2
+        assert torch.equal(fw.y, eager.y) and torch.equal(g.x, want.x) and torch.equal(g.weight, want.weight) and torch.equal(g.bias, want.bias)
+        assert torch.equal(d, features.dropout(L.x, 0.5, 3, 5 + replay % 2))
+        if replay % 2 == 0:
+            within(fw.y, L.y, L.y_tol, "y of a replay")
+
+
+# ---- dropout ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (1, 7), (3, 4), (5, 50), (64, 8), (33, 130), (7, 1001), (2, 70001), (1500, 3)])
+@pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
+def test_dropout(shape, p, dtype):
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(shape[1])
+    x = draw(g, shape, dtype)
+    k = kept(*shape, p, 12345, 9)
+    want = x.double() * k
+    y = features.dropout(x, p, 12345, 9)
+    within(y, want, U[dtype] * want.abs() + EPS * want.abs() + TINY[dtype], "y")
+    assert torch.equal(y == 0, (k == 0) | (x == 0)) or dtype == torch.float16
+    dy = draw(g, shape, dtype)
+    within(features.dropout_backward(dy, p, 12345, 9), dy.double() * k, (U[dtype] + EPS) * (dy.double() * k).abs() + TINY[dtype], "dx")
+    if p == 0.0:
+        assert torch.equal(y, x)
+    wide = draw(g, (shape[0], shape[1] + 5), dtype)
+    part = wide[:, 3:3 + shape[1]]
+    was = wide.clone()
+    assert torch.equal(features.dropout(part, p, 12345, 9, out=part), features.dropout(was[:, 3:3 + shape[1]], p, 12345, 9))
+    assert torch.equal(wide[:, :3], was[:, :3]) and torch.equal(wide[:, 3 + shape[1]:], was[:, 3 + shape[1]:])
+    assert torch.equal(features.dropout(x.t().contiguous().t(), p, 12345, 9), y)
+
+
+def test_dropout_masks():
+    """Seeds, steps and rows have masks of their own, at the rate asked for; a row's does not depend on how many there are."""
+    from cuke_amd import features
+    x = torch.ones(4096, 257, device=DEV)
+    n = x.numel()
+    a = features.dropout(x, 0.1, 1, 0) == 0
+    for other in (features.dropout(x, 0.1, 2, 0), features.dropout(x, 0.1, 1, 1), features.dropout(x, 0.1, -1, 0)):
+        b = other == 0
+        assert abs(int(b.sum()) - 0.1 * n) < 6 * math.sqrt(n * 0.09)           # six standard deviations
+        assert abs(int((a & b).sum()) - 0.01 * n) < 6 * math.sqrt(n * 0.0099)   # independent masks
+    assert abs(int((a[1:] & a[:-1]).sum()) - 0.01 * n) < 6 * math.sqrt(n * 0.0099)
+    assert abs(int((a[:, 1:] & a[:, :-1]).sum()) - 0.01 * n) < 6 * math.sqrt(n * 0.0099)
+    assert torch.equal(features.dropout(x[:100], 0.1, 1, 0), features.dropout(x, 0.1, 1, 0)[:100])
+
+
+def test_dropout_drops_whatever_is_there():
+    from cuke_amd import features
+    x = torch.full((64, 64), float("nan"), device=DEV)
+    x[:, ::2] = float("inf")
+    y = features.dropout(x, 0.5, 4, 2)
+    gone = kept(64, 64, 0.5, 4, 2) == 0
+    assert bool((y[gone] == 0).all()) and not bool(torch.isfinite(y[~gone]).any())
+
+
+# ---- preference loss -------------------------------------------------------------------------------
+def prefer64(pos, neg, rpos, rneg, beta, kind, smoothing, temperature, mask, sign):
+    pos, neg = pos.double(), neg.double()
+    on = torch.ones_like(neg, dtype=torch.bool) if mask is None else mask.bool()
+    z0 = torch.zeros_like(neg)
+    n = torch.where(on, neg, z0)
+    gap = pos[:, None] - n
+    size = pos.abs()[:, None] + n.abs()
+    if rpos is not None:
+        r = torch.where(on, rneg.double(), z0)
+        gap = gap - (rpos.double()[:, None] - r)
+        size = size + rpos.double().abs()[:, None] + r.abs()
+    d = sign * gap
+    d_tol = 2 * EPS * size                                       # two roundings of differences
+    if kind == "sigmoid":
+        f = (1 - smoothing) * torch.nn.functional.softplus(-beta * d) + smoothing * torch.nn.functional.softplus(beta * d)
+        s = beta * (smoothing - torch.sigmoid(-beta * d))
+        f_tol, s_tol = beta * d_tol + 16 * EPS * (1 + beta * d.abs()), beta * (beta * d_tol / 4 + 16 * EPS * (1 + beta * d.abs()))
+    elif kind == "hinge":
+        f, s = torch.clamp(1 - beta * d, min=0), torch.where(beta * d < 1, -beta, 0.0).to(d)
+        f_tol = beta * d_tol + 8 * EPS * (1 + beta * d.abs())
+        s_tol = torch.where((1 - beta * d).abs() <= f_tol, beta, 2 * EPS * beta).to(d)     # the corner's side
+    else:
+        f, s = (d - 0.5 / beta) ** 2, 2 * (d - 0.5 / beta)
+        s_tol = 2 * d_tol + 8 * EPS * (d.abs() + 0.5 / beta)
+        f_tol = s_tol * s.abs() + s_tol ** 2
+    t = torch.where(on, temperature * sign * n, torch.full_like(n, -math.inf))
+    t_tol = 8 * EPS * (1 + temperature * n.abs().amax(1, keepdim=True)) if n.shape[1] else 0.0
+    a = torch.nan_to_num(torch.softmax(t, 1)) * on
+    B, N = n.shape
+    a_tol = a * (3 * t_tol + (N + 16) * EPS)
+    loss = (a * f).sum() / B
+    loss_tol = (a_tol * f.abs() + a * f_tol + (N + 16) * EPS * a * f.abs()).sum() / B + 2 * EPS * loss.abs()
+    g = sign * a * s / B
+    g_tol = (a_tol * s.abs() + a * s_tol) / B + 8 * EPS * g.abs()
+    return loss, g.sum(1), -g, loss_tol, g_tol.sum(1) + (N + 16) * EPS * g.abs().sum(1), g_tol
+
+
+def check_prefer(B, N, dtype, ref=True, mask=None, layout="plain", seed=0, **kw):
+    from cuke_amd import features
+    kw = dict(dict(beta=0.5, kind="sigmoid", smoothing=0.0, temperature=0.0, sign=1.0), **kw)
+    g = torch.Generator().manual_seed(seed + 31 * B + N)
+    wide = (lambda t: t) if layout == "plain" else (lambda t: torch.cat([t, t, t], 1)[:, 1:1 + N] if N else t)
+    pos, neg = draw(g, (B,), dtype, 2.0), wide(draw(g, (B, N), dtype, 2.0))
+    rpos, rneg = (draw(g, (B,), dtype, 2.0), wide(draw(g, (B, N), dtype, 2.0))) if ref else (None, None)
+    m = None
+    if mask is not None:
+        m = torch.rand(B, N, generator=g) >= mask
+        m[::5] = False
+        m = wide(m.to(DEV))
+        neg = neg.clone()
+        neg[~m] = float("nan")
+        if layout != "plain":
+            neg = torch.cat([neg, neg], 1)[:, :N]
+        if ref:
+            rneg = rneg.clone()
+            rneg[~m] = float("inf")
+    loss, dpos, dneg = features.preference_loss(pos, neg, rpos, rneg, mask=m, **kw)
+    want = prefer64(pos, neg, rpos, rneg, mask=m, **kw)
+    within(loss, want[0].view(1), want[3].view(1), "loss")
+    within(dpos, want[1], want[4], "dpos")
+    within(dneg, want[2], want[5], "dneg")
+    if m is not None:
+        assert not dneg[~m].any() and not dpos[::5].any()
+    again = features.preference_loss(pos, neg, rpos, rneg, mask=m, **kw)
+    assert torch.equal(loss, again[0]) and torch.equal(dpos, again[1]) and torch.equal(dneg, again[2])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (3, 1), (1000, 1), (5000, 2), (300, 3), (64, 4), (77, 7), (33, 16), (40, 25), (65, 63), (20, 64), (9, 65),
+                                   (30, 100), (17, 129), (12, 256), (500, 25), (8, 300), (6, 511), (6, 512), (5, 513), (4, 1000), (5, 1024), (5, 1025),
+                                   (3, 2047), (3, 2049), (2, 4096), (2, 4099), (7, 8191), (1, 8200), (3, 14951), (1, 70001)])
+def test_preference_shapes(shape, dtype):
+    print("preference", shape, dtype, flush=True)
+    check_prefer(*shape, dtype)
+    check_prefer(*shape, dtype, mask=0.3, temperature=1.0, smoothing=0.1, layout="wide")
+    check_prefer(*shape, dtype, ref=False, mask=0.9, kind="square", sign=-1.0)
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "square"])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("masked", [None, 0.2])
+@pytest.mark.parametrize("ref", [True, False])
+def test_preference_forms(kind, temperature, sign, masked, ref):
+    for B, N in ((50, 37), (6, 1500), (2, 9000)):
+        check_prefer(B, N, torch.float32, ref=ref, mask=masked, kind=kind, temperature=temperature, sign=sign, beta=0.3)
+
+
+def test_preference_extremes():
+    """Scores far apart neither overflow nor lose the small side; a temperature with scores of thousands stays a softmax."""
+    from cuke_amd import features
+    pos = torch.tensor([0.0, 0.0, 1e4, -1e4], device=DEV)
+    neg = torch.tensor([[1e4, -1e4], [60.0, -60.0], [0.0, 1.0], [0.0, 1.0]], device=DEV)
+    for temperature in (0.0, 1.0):
+        want = prefer64(pos, neg, None, None, 1.0, "sigmoid", 0.0, temperature, None, 1.0)
+        loss, dpos, dneg = features.preference_loss(pos, neg, temperature=temperature)
+        within(loss, want[0].view(1), want[3].view(1), "loss")
+        within(dneg, want[2], want[5], "dneg")
+        assert bool(torch.isfinite(dpos).all())
+    # the type's lowest value is a score like any other where it is not masked: it takes no share of the softmax
+    neg = torch.tensor([[1.0, torch.finfo(torch.float32).min]], device=DEV)
+    loss, _, dneg = features.preference_loss(pos[:1], neg, temperature=1.0)
+    assert abs(loss.item() - math.log1p(math.exp(1.0))) < 1e-6 and dneg[0, 1] == 0
+
+
+def test_preference_of_nothing():
+    from cuke_amd import features
+    for B, N in ((0, 5), (4, 0), (0, 0)):
+        loss, dpos, dneg = features.preference_loss(torch.zeros(B, device=DEV), torch.zeros(B, N, device=DEV))
+        assert loss.item() == 0 and dpos.shape == (B,) and dneg.shape == (B, N) and not dpos.any()
+
+
+def test_preference_gradient_against_differences():
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(1)
+    for kind in ("sigmoid", "square"):
+        pos, neg = draw(g, (6,), torch.float32), draw(g, (6, 9), torch.float32)
+        rp, rn = draw(g, (6,), torch.float32), draw(g, (6, 9), torch.float32)
+        _, dpos, dneg = features.preference_loss(pos, neg, rp, rn, beta=0.7, kind=kind)
+        vp, vn = draw(g, (6,), torch.float64), draw(g, (6, 9), torch.float64)
+        h = 1e-5
+        up, down = (prefer64(pos.double() + s * h * vp, neg.double() + s * h * vn, rp, rn, 0.7, kind, 0.0, 0.0, None, 1.0)[0] for s in (1, -1))
+        slope = (dpos.double() * vp).sum() + (dneg.double() * vn).sum()
+        size = (dpos.double() * vp).abs().sum() + (dneg.double() * vn).abs().sum()
+        assert abs((up - down) / (2 * h) - slope) <= 64 * EPS * (size + 1) + 1e-8
+
+
+# ---- together --------------------------------------------------------------------------------------
+def test_encoder_training_step():
+    """Features -> rows -> scores -> preference loss -> gradients, against the same chain in 64 bits with torch's own derivatives."""
+    from cuke_amd import features
+    from cuke_amd.kge import KGEModel
+    g = torch.Generator().manual_seed(5)
+    n, f, hid, dim, B, N = 96, 40, 56, 32, 64, 16
+    x, base = draw(g, (n, f), torch.float32), draw(g, (n, dim), torch.float32, 0.3)
+    w = [draw(g, (hid, f), torch.float32, f ** -0.5), draw(g, (hid,), torch.float32, 0.1), draw(g, (dim, hid), torch.float32, hid ** -0.5),
+         draw(g, (dim,), torch.float32, 0.1)]
+    R = draw(g, (5, dim), torch.float32, 0.5)
+    h, t = (torch.arange(B, device=DEV), torch.arange(B, device=DEV) + 32)
+    r, neg = torch.randint(0, 5, (B,), generator=g).to(DEV), torch.randint(0, n, (B // 16 * N,), generator=g).to(DEV)
+    rp, rn = draw(g, (B,), torch.float32), draw(g, (B, N), torch.float32)
+    enc = features.FeatureEncoder(*w, drop=0.2, row_drop=0.1, seed=11)
+    fw = enc.forward(x, base, step=3)
+    m = KGEModel("DistMult", fw.rows, R)
+    sc = m.score(h, r, t, neg, 16)
+    loss, dpos, dneg = features.preference_loss(sc.pos, sc.neg, rp, rn, beta=0.5, temperature=0.5)
+    sg = m.backward(sc, dpos, dneg)
+    drows = torch.zeros_like(fw.rows)
+    drows[sg.ent_ids] = sg.ent_rows
+    got = enc.backward(fw, drows, need_x=True)
+
+    leaf = [v.double().requires_grad_() for v in (x, base, *w)]
+    X, Bs, W1, B1, W2, B2 = leaf
+    z = X @ W1.T + B1
+    rows = (z * 0.5 * torch.erfc(-z / math.sqrt(2)) * kept(n, hid, 0.2, 11, 3)) @ W2.T + B2 + Bs
+    rows = rows * kept(n, dim, 0.1, 12, 3)
+    Rd = R.double()
+    ps = (rows[h] * Rd[r] * rows[t]).sum(1)
+    ns = ((rows[h] * Rd[r]).view(B // 16, 16, dim) @ rows[neg].view(B // 16, N, dim).transpose(1, 2).contiguous()).view(B, N)
+    a = torch.softmax(0.5 * ns, 1).detach()
+    total = (a * torch.nn.functional.softplus(-0.5 * ((ps - rp.double())[:, None] - (ns - rn.double())))).sum() / B
+    total.backward()
+    assert abs(loss.item() - total.item()) < 1e-5
+    for have, want in zip([got.hidden.x, got.base, got.hidden.weight, got.hidden.bias, got.last.weight, got.last.bias], [v.grad for v in leaf]):
+        # a chain of six fp32 stages, sums of at most 96 terms each: 6 * 112 eps of the largest values involved
+        assert (have.double() - want).abs().max() <= 6 * 112 * EPS * want.abs().max() + 1e-9
+    within(enc.encode(x, base), (act64(z, "gelu")[0] @ W2.T + B2 + Bs).detach(), torch.tensor(2e-5, device=DEV), "rows to answer with")
+
+
+def test_arguments_that_are_refused():
+    from cuke_amd import features
+    from cuke_amd.kge import KgeError
+    x, w, b = torch.zeros(4, 8, device=DEV), torch.zeros(6, 8, device=DEV), torch.zeros(6, device=DEV)
+    F = features
+    for bad, call in [
+            (KgeError, lambda: F.linear(x.cpu(), w)), (KgeError, lambda: F.linear(x, w.cpu())), (TypeError, lambda: F.linear(x.double(), w.double())),
+            (TypeError, lambda: F.linear(x, w.half())), (ValueError, lambda: F.linear(x, w[:, :7])), (ValueError, lambda: F.linear(x[0], w)),
+            (ValueError, lambda: F.linear(x, w, b[:5])), (TypeError, lambda: F.linear(x, w, b.half())), (ValueError, lambda: F.linear(x, w, act="tanh")),
+            (ValueError, lambda: F.linear(x, w, drop=1.5)), (ValueError, lambda: F.linear(x, w, drop=float("nan"))),
+            (ValueError, lambda: F.linear(x, w, residual=x)), (TypeError, lambda: F.linear(x, w, out_dtype=torch.float16)),
+            (TypeError, lambda: F.linear(x.half(), w.half(), residual=torch.zeros(4, 6, device=DEV, dtype=torch.bfloat16))),
+            (TypeError, lambda: F.linear([1.0], w)), (TypeError, lambda: F.linear_backward(x, x)),
+            (ValueError, lambda: F.linear_backward(F.linear_forward(x, w), x)), (TypeError, lambda: F.linear_backward(F.linear_forward(x, w), torch.zeros(4, 6, device=DEV).half())),
+            (TypeError, lambda: F.dropout(x.long(), 0.5, 1)), (ValueError, lambda: F.dropout(x, -0.1, 1)), (ValueError, lambda: F.dropout(b, 0.5, 1)),
+            (ValueError, lambda: F.dropout(x, 0.5, 1, out=w)), (TypeError, lambda: F.dropout(x, 0.5, 1, step=torch.zeros(1, device=DEV))),
+            (ValueError, lambda: F.dropout(x, 0.5, 1, out=torch.zeros(8, 4, device=DEV).t())),
+            (ValueError, lambda: F.preference_loss(b, x)), (TypeError, lambda: F.preference_loss(x[:, 0].half(), x)),
+            (ValueError, lambda: F.preference_loss(x[:, 0], x, ref_pos=x[:, 0])), (ValueError, lambda: F.preference_loss(x[:, 0], x, kind="none")),
+            (TypeError, lambda: F.preference_loss(x[:, 0], x, mask=x)), (ValueError, lambda: F.preference_loss(x[:, 0], x, mask=x[:, :3] > 0)),
+            (KgeError, lambda: F.preference_loss(x[:, 0], x, beta=0.0)), (KgeError, lambda: F.preference_loss(x[:, 0], x, sign=0.5)),
+            (KgeError, lambda: F.preference_loss(x[:, 0], x, temperature=-1.0)), (KgeError, lambda: F.preference_loss(x[:, 0], x, smoothing=2.0)),
+            (KgeError, lambda: F.preference_loss(x[:, 0], x, smoothing=0.1, kind="hinge")),
+            (KgeError, lambda: F.preference_loss(x[:, 0], x, temperature=float("inf"))), (KgeError, lambda: F.preference_loss(x[:, 0], x, beta=float("nan"))),
+            (ValueError, lambda: F.FeatureEncoder(w, b, w, b))]:
+        with pytest.raises(bad):
+            call()
