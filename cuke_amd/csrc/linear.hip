@@ -141,13 +141,24 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 // ---- products --------------------------------------------------------------------------------------
 constexpr int kTileX = 128;
 
+template <class E, int PLANES, bool AA, bool BA, int X, int WA, int WB, int STAGES, EndKind END>
+static void launch_sized(TileArgs &t, hipStream_t st)
+{
+    t.tiles_a = (int)ceil_div(t.a.extent, X), t.tiles_b = (int)ceil_div(t.b.extent, X);
+    const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b * t.splits;
+    if (blocks == 0) return;
+    hipLaunchKernelGGL((linear_tile_kernel<E, PLANES, AA, BA, X, X, WA, WB, STAGES, END>), dim3((unsigned)blocks), dim3(WA * WB * kWave), 0, st, t);
+}
+
 template <class E, int PLANES, bool AA, bool BA, EndKind END>
 static void launch_tiles(TileArgs &t, hipStream_t st)
 {
-    t.tiles_a = (int)ceil_div(t.a.extent, kTileX), t.tiles_b = (int)ceil_div(t.b.extent, kTileX);
-    const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b * t.splits;
-    if (blocks == 0) return;
-    hipLaunchKernelGGL((linear_tile_kernel<E, PLANES, AA, BA, kTileX, kTileX, 2, 2, END>), dim3((unsigned)blocks), dim3(256), 0, st, t);
+    if constexpr (PLANES == 3) {
+        launch_sized<E, PLANES, AA, BA, 128, 2, 4, 3, END>(t, st);
+    } else {
+        if (ceil_div(t.a.extent, 256) * ceil_div(t.b.extent, 256) * t.splits >= 200) launch_sized<E, PLANES, AA, BA, 256, 2, 4, 4, END>(t, st);
+        else launch_sized<E, PLANES, AA, BA, 128, 2, 2, 4, END>(t, st);
+    }
 }
 
 // Parts of a sum over k where `tiles` tiles alone would leave most of the card idle: as many as fill it twice, none shorter than 256 terms.

@@ -91,21 +91,38 @@ struct Tile {
         return X >= 256 ? 2 * (2 * (row & 3) + 8 * ((row >> 3) & 1)) : (X >= 128 ? 4 * (row & 3) : 2 * (row & 3));
     }
 
-    // the chunks of terms [k, k + 32) this thread brings in
+    // The chunks a thread brings in: where the next ones come from, and how far they are from the ones behind them.
     template <class E>
-    __device__ __forceinline__ static void load(const Side &s, const E *p, int64_t first, int64_t k, int64_t k_end, char *lds)
-    {
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    struct Feed {
+        const char *from[kRounds];
+        int64_t step[kRounds];
+        int term[kRounds];  // of the chunk, within the tile
+
+        __device__ __forceinline__ void start(const Side &s, int plane, int64_t first, int64_t k)
+        {
+            const E *p = static_cast<const E *>(s.p) + plane * s.plane;
 #pragma unroll
-        for (int r = 0; r < kRounds; ++r) {
-            const int c = r * THREADS + (int)threadIdx.x;
-            const int row = c / kRow, j = (c % kRow) ^ turn(row);
-            const int64_t index = first + (ACROSS ? 8 * j : row), term = k + (ACROSS ? row : 8 * j);
-            const E *src = p + (ACROSS ? term * s.stride + index : index * s.stride + term);
-            const void *from = index < s.extent && term < k_end ? (const void *)src : (const void *)zero_chunk;
-            chunk_to_lds(from, lds + 16 * (r * THREADS + wave * 64));
+            for (int r = 0; r < kRounds; ++r) {
+                const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
+                const int64_t index = first + (ACROSS ? 8 * j : row);
+                term[r] = ACROSS ? row : 8 * j;
+                const bool there = index < s.extent;
+                from[r] = there ? reinterpret_cast<const char *>(p + (ACROSS ? (k + row) * s.stride + index : index * s.stride + k + 8 * j))
+                                : reinterpret_cast<const char *>(zero_chunk);
+                step[r] = there ? (ACROSS ? kTileK * s.stride : kTileK) * (int64_t)sizeof(E) : 0;
+            }
         }
-    }
+        // the next tile, of which `left` terms exist (none, behind the end)
+        __device__ __forceinline__ void load(int64_t left, char *lds)
+        {
+            const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                chunk_to_lds(term[r] < left ? from[r] : reinterpret_cast<const char *>(zero_chunk), lds + 16 * (r * THREADS + wave * 64));
+                from[r] += step[r];
+            }
+        }
+    };
 
     // eight terms of an index for each lane: index at + lane % 32, terms 16 step + 8 (lane / 32) .. + 7
     __device__ __forceinline__ static s16x8 read(const char *lds, int at, int step, int lane)
@@ -123,28 +140,26 @@ struct Tile {
     }
 };
 
-// The sum of one output element by fp32 instructions, from the planes (which add up to the value, infinities and NaNs included).
+// The sums of four (`valid`) output elements of a row by fp32 instructions, from the planes (which add up to the value, infinities and NaNs
+// included).  Not for speed: it runs where a sum is not finite.
 template <bool A_ACROSS, bool B_ACROSS>
-__device__ __noinline__ float plain_sum(const Side &a, const Side &b, int64_t n, int64_t m, int64_t k0, int64_t k1)
+__device__ __noinline__ float4 plain_sums(Side a, Side b, int64_t n, int valid, int64_t m, int64_t k0, int64_t k1)
 {
     const bf16_t *pa = static_cast<const bf16_t *>(a.p), *pb = static_cast<const bf16_t *>(b.p);
-    float s = 0.0f;
-    for (int64_t k = k0; k < k1; ++k) {
-        const bf16_t *x = pa + (A_ACROSS ? k * a.stride + n : n * a.stride + k), *y = pb + (B_ACROSS ? k * b.stride + m : m * b.stride + k);
-        s = fmaf((float)x[0] + (float)x[a.plane] + (float)x[2 * a.plane], (float)y[0] + (float)y[b.plane] + (float)y[2 * b.plane], s);
-    }
-    return s;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int v = 0; v < valid; ++v)
+        for (int64_t k = k0; k < k1; ++k) {
+            const bf16_t *x = pa + (A_ACROSS ? k * a.stride + n + v : (n + v) * a.stride + k), *y = pb + (B_ACROSS ? k * b.stride + m : m * b.stride + k);
+            s[v] = fmaf((float)x[0] + (float)x[a.plane] + (float)x[2 * a.plane], (float)y[0] + (float)y[b.plane] + (float)y[2 * b.plane], s[v]);
+        }
+    return make_float4(s[0], s[1], s[2], s[3]);
 }
 
 // Four consecutive columns of a row through the layer's epilogue.  T: the layer's type.
 template <class T>
-__device__ __forceinline__ void finish_quad(const Ends &e, uint64_t base, int64_t row, int64_t col, float4 z)
+__device__ __forceinline__ void finish_quad(const Ends &e, uint64_t base, int64_t row, int64_t col, int valid, float4 z, float4 bias)
 {
-    const int valid = (int)(e.cols - col < 4 ? e.cols - col : 4);
-    if (e.bias) {
-        const float4 b = load4(static_cast<const T *>(e.bias) + col, valid);
-        z.x += b.x, z.y += b.y, z.z += b.z, z.w += b.w;
-    }
+    z.x += bias.x, z.y += bias.y, z.z += bias.z, z.w += bias.w;
     if (e.act != KGE_ACT_NONE) {
         float4 s;
         z.x = activate(z.x, e.act, &s.x), z.y = activate(z.y, e.act, &s.y), z.z = activate(z.z, e.act, &s.z), z.w = activate(z.w, e.act, &s.w);
@@ -183,8 +198,21 @@ __device__ __forceinline__ void tile_of(int64_t block, int64_t blocks, const Til
     *tb = (int)(first + q % band % wide), *ta = (int)(q % band / wide);
 }
 
-// E: what the matrix cores multiply, PLANES: 3 for fp32.  A workgroup of WA x WB waves computes XA columns by XB rows.
-template <class E, int PLANES, bool A_ACROSS, bool B_ACROSS, int XA, int XB, int WA, int WB, EndKind END>
+// A wave's own loads have landed but for the last `out` (LDS reads all have), and every wave's have: what the stage in turn holds may be
+// read, and the stage read last may be written.
+template <int OUT>
+__device__ __forceinline__ void stage_ready()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((OUT & 15) | (OUT >> 4) << 14 | 7 << 4);  // vmcnt(OUT) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// E: what the matrix cores multiply, PLANES: 3 for fp32.  A workgroup of WA x WB waves computes XA columns by XB rows.  STAGES tiles of 32 terms
+// are in LDS, in arrays of their own (so that the compiler sees that the one being read is none of those being written): STAGES - 1 are
+// requested ahead, and one barrier a tile both publishes the next and frees the last.
+template <class E, int PLANES, bool A_ACROSS, bool B_ACROSS, int XA, int XB, int WA, int WB, int STAGES, EndKind END>
 __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
 {
     using T = typename std::conditional<PLANES == 3, float, E>::type;
@@ -192,8 +220,10 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
     using A = Tile<XA, A_ACROSS, kThreads>;
     using B = Tile<XB, B_ACROSS, kThreads>;
     constexpr int kBytesA = XA * kTileK * 2, kBytesB = XB * kTileK * 2, kStage = PLANES * (kBytesA + kBytesB);
+    constexpr int kLoads = PLANES * (A::kRounds + B::kRounds);  // per thread and tile
     constexpr int FA = XA / WA / 32, FB = XB / WB / 32;
-    __shared__ __align__(16) char stage0[kStage], stage1[kStage];
+    static_assert(STAGES >= 2 && STAGES <= 4, "stages");
+    __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[STAGES > 2 ? kStage : 16], stage3[STAGES > 3 ? kStage : 16];
 
     int ta, tb, split;
     tile_of(blockIdx.x, gridDim.x, t, &ta, &tb, &split);
@@ -204,12 +234,18 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
 
     floatx16 acc[FA][FB] = {}, low[PLANES == 3 ? FA : 1][PLANES == 3 ? FB : 1] = {};
 
-    auto load = [&](int64_t k, char *lds) {
+    typename A::template Feed<E> feed_a[PLANES];
+    typename B::template Feed<E> feed_b[PLANES];
+#pragma unroll
+    for (int p = 0; p < PLANES; ++p) feed_a[p].start(t.a, p, n0, k0), feed_b[p].start(t.b, p, m0, k0);
+    int64_t left = k1 - k0;  // terms not requested yet
+    auto load = [&](char *lds) {
 #pragma unroll
         for (int p = 0; p < PLANES; ++p) {
-            A::load(t.a, static_cast<const E *>(t.a.p) + p * t.a.plane, n0, k, k1, lds + p * kBytesA);
-            B::load(t.b, static_cast<const E *>(t.b.p) + p * t.b.plane, m0, k, k1, lds + PLANES * kBytesA + p * kBytesB);
+            feed_a[p].load(left, lds + p * kBytesA);
+            feed_b[p].load(left, lds + PLANES * kBytesA + p * kBytesB);
         }
+        left -= kTileK;
     };
     auto multiply = [&](const char *lds) {
 #pragma unroll
@@ -218,9 +254,9 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
 #pragma unroll
             for (int p = 0; p < PLANES; ++p) {
 #pragma unroll
-                for (int i = 0; i < FA; ++i) a[i][p] = A::read(lds + p * kBytesA, wa + 32 * i, step, lane);
-#pragma unroll
                 for (int j = 0; j < FB; ++j) b[j][p] = B::read(lds + PLANES * kBytesA + p * kBytesB, wb + 32 * j, step, lane);
+#pragma unroll
+                for (int i = 0; i < FA; ++i) a[i][p] = A::read(lds + p * kBytesA, wa + 32 * i, step, lane);
             }
 #pragma unroll
             for (int i = 0; i < FA; ++i)
@@ -236,49 +272,76 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
                 }
         }
     };
+    auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
 
-    if (k0 < k1) load(k0, stage0);
-    for (int64_t k = k0; k < k1; k += 2 * kTileK) {
-        __syncthreads();  // (the stage has landed, and everyone is done with the other one)
-        if (k + kTileK < k1) load(k + kTileK, stage1);
-        multiply(stage0);
-        if (k + kTileK >= k1) break;
-        __syncthreads();
-        if (k + 2 * kTileK < k1) load(k + 2 * kTileK, stage0);
-        multiply(stage1);
+    // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
+    const int tiles = (int)((k1 - k0 + kTileK - 1) / kTileK);
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
+    int at = 0;
+    for (; at + STAGES <= tiles; at += STAGES)
+#pragma unroll
+        for (int u = 0; u < STAGES; ++u) {
+            stage_ready<kLoads * (STAGES - 2)>();
+            load(stage((u + STAGES - 1) % STAGES));
+            multiply(stage(u));
+        }
+#pragma unroll
+    for (int u = 0; u < STAGES - 1; ++u) {
+        if (at + u >= tiles) break;
+        stage_ready<kLoads * (STAGES - 2)>();
+        load(stage((u + STAGES - 1) % STAGES));
+        multiply(stage(u));
     }
 
-    // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
-    const uint64_t base = END == kEndLayer ? t.e.drop.base() : 0;
+    // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows of the wave's columns at a time, so that they come back
+    // row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.
+    stage_ready<0>();
+    constexpr int kQuads = 8 * FA, kStrip = 32 * kQuads * 16, kPerStage = kStage / kStrip;
+    static_assert(kPerStage >= 1 && (WA * WB + kPerStage - 1) / kPerStage <= STAGES, "a strip for every wave");
+    char *strip = stage(wave / kPerStage) + wave % kPerStage * kStrip;
+    const int quad = lane % kQuads;
+    const int64_t col = n0 + wa + 4 * quad;
+    const int valid = (int)(t.e.cols - col < 4 ? t.e.cols - col : 4);
+    uint64_t base = 0;
+    float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if constexpr (END == kEndLayer) {
+        base = t.e.drop.base();
+        if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + (valid > 0 ? col : 0), valid);
+    }
 #pragma unroll
-    for (int i = 0; i < FA; ++i)
+    for (int j = 0; j < FB; ++j) {
+        // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
 #pragma unroll
-        for (int j = 0; j < FB; ++j) {
-            const int64_t row = m0 + wb + 32 * j + (lane & 31);
-            if (row >= t.e.rows) continue;
+        for (int i = 0; i < FA; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const int64_t col = n0 + wa + 32 * i + 8 * q + 4 * (lane >> 5);
-                if (col >= t.e.cols) continue;
                 float z[4];
 #pragma unroll
                 for (int v = 0; v < 4; ++v) {
                     z[v] = acc[i][j][4 * q + v];
-                    if constexpr (PLANES == 3) {
-                        z[v] += low[i][j][4 * q + v];
-                        // (an infinite operand's planes, or leading parts that were rounded up, may have made this of a finite sum)
-                        if (not_finite(z[v]) && col + v < t.e.cols) z[v] = plain_sum<A_ACROSS, B_ACROSS>(t.a, t.b, col + v, row, k0, k1);
-                    }
+                    if constexpr (PLANES == 3) z[v] += low[i][j][4 * q + v];
                 }
-                const float4 four = make_float4(z[0], z[1], z[2], z[3]);
-                if constexpr (END == kEndPartial)
-                    *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = four;
-                else if constexpr (END == kEndLayer)
-                    finish_quad<T>(t.e, base, row, col, four);
-                else
-                    store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, four, (int)(t.e.cols - col < 4 ? t.e.cols - col : 4));
+                const int row = lane & 31, at = 8 * i + 2 * q + (lane >> 5);
+                *reinterpret_cast<float4 *>(strip + 16 * (row * kQuads + (at ^ (row & 7)))) = make_float4(z[0], z[1], z[2], z[3]);
             }
+#pragma unroll 2
+        for (int r = lane / kQuads; r < 32; r += 64 / kQuads) {
+            float4 z = *reinterpret_cast<const float4 *>(strip + 16 * (r * kQuads + (quad ^ (r & 7))));
+            const int64_t row = m0 + wb + 32 * j + r;
+            if (row >= t.e.rows || valid <= 0) continue;
+            if constexpr (PLANES == 3) {
+                // (an infinite operand's planes, or leading parts that were rounded up, may have made this of a finite sum)
+                if (not_finite(z.x) || not_finite(z.y) || not_finite(z.z) || not_finite(z.w)) z = plain_sums<A_ACROSS, B_ACROSS>(t.a, t.b, col, valid, row, k0, k1);
+            }
+            if constexpr (END == kEndPartial)
+                *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = z;
+            else if constexpr (END == kEndLayer)
+                finish_quad<T>(t.e, base, row, col, valid, z, bias);
+            else
+                store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, z, valid);
         }
+    }
 }
 
 }  // namespace kge
