@@ -11,9 +11,10 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T *x, int64_t x_stri
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i / drop.quads, quad = i % drop.quads, col = 4 * quad, left = cols - col;
         const int valid = (int)(left < 4 ? left : 4);
-        float4 v = load4(x + row * x_stride + col, valid);
-        if (drop.cut) v = drop.apply(v, drop.word(base, row, quad));
-        store4(y + row * y_stride + col, v, valid);
+        const float4 q = load4(x + row * x_stride + col, valid);
+        float v[4] = {q.x, q.y, q.z, q.w};
+        if (drop.cut) drop.apply(v, drop.word(base, drop.place(row, quad)));
+        store4(y + row * y_stride + col, make_float4(v[0], v[1], v[2], v[3]), valid);
     }
 }
 

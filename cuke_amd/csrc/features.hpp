@@ -24,6 +24,34 @@ struct Pack {
     __device__ __forceinline__ void store(E *p) const { *reinterpret_cast<type *>(p) = v; }
 };
 
+// eight elements of which `valid` exist (any number: none below 1, all above 7), as floats; the rest are zero
+template <class E>
+__device__ __forceinline__ void load8(const E *p, int valid, float (&v)[8])
+{
+    if (valid >= 8) {
+        const auto q = Pack<E, 8>::load(p).v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)q[e];
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < valid ? (float)p[e] : 0.0f;
+}
+template <class E>
+__device__ __forceinline__ void store8(E *p, const float (&v)[8], int valid)
+{
+    if (valid >= 8) {
+        Pack<E, 8> q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q.v[e] = (E)v[e];
+        q.store(p);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (e < valid) p[e] = (E)v[e];
+}
+
 // four elements of which `valid` (0 .. 4) exist, as floats; the rest are zero
 template <class E>
 __device__ __forceinline__ float4 load4(const E *p, int valid)
@@ -71,33 +99,39 @@ __device__ __forceinline__ void normal_cdf(float z, float *cdf, float *bell)
     *bell = e;
 }
 
-// act(z); *slope = act'(z)
-__device__ __forceinline__ float activate(float z, int act, float *slope)
+// act(z) in place, and act'(z), of V values (the branch is the launch's, not the value's)
+template <int V>
+__device__ __forceinline__ void activate(float (&z)[V], int act, float (&slope)[V])
 {
     if (act == KGE_ACT_GELU) {
-        float cdf, bell;
-        normal_cdf(z, &cdf, &bell);
-        *slope = fmaf(z * 0.39894228f, bell, cdf);
-        return z * cdf;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float cdf, bell;
+            normal_cdf(z[v], &cdf, &bell);
+            slope[v] = fmaf(z[v] * 0.39894228f, bell, cdf);
+            z[v] *= cdf;
+        }
+    } else if (act == KGE_ACT_SILU) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z[v]));
+            slope[v] = s * fmaf(z[v], 1.0f - s, 1.0f);
+            z[v] *= s;
+        }
+    } else if (act == KGE_ACT_RELU) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            slope[v] = z[v] > 0.0f ? 1.0f : (z[v] <= 0.0f ? 0.0f : z[v]);  // (a NaN stays one)
+            z[v] = z[v] < 0.0f ? 0.0f : z[v];
+        }
     }
-    if (act == KGE_ACT_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z));
-        *slope = s * fmaf(z, 1.0f - s, 1.0f);
-        return z * s;
-    }
-    if (act == KGE_ACT_RELU) {
-        *slope = z > 0.0f ? 1.0f : (z <= 0.0f ? 0.0f : z);  // (a NaN stays one)
-        return z < 0.0f ? 0.0f : z;
-    }
-    *slope = 1.0f;
-    return z;
 }
 
 // The derivative as it is kept for the backward pass of 16-bit layers: every one of them lies in [-0.13, 1.13], so 16 bits of fixed
-// point hold it to 1.02e-5 (0 and 1 exactly), where bf16 would add an error as large as that of the gradient's own rounding; 65535 is NaN.
-// Layers in fp32 keep it in fp32.
-__device__ __forceinline__ uint16_t slope_to_fixed(float s) { return s == s ? (uint16_t)(int)(fmaf(s, 49152.0f, 8192.5f)) : (uint16_t)65535; }
-__device__ __forceinline__ float slope_from_fixed(uint32_t q) { return q == 65535u ? __builtin_nanf("") : ((float)(int)(q - 8192u)) * (1.0f / 49152.0f); }
+// point hold it to 1.02e-5 (0 and 1 exactly), where bf16 would add an error as large as that of the gradient's own rounding; 0, which no derivative
+// comes near, is NaN.  Layers in fp32 keep it in fp32.
+__device__ __forceinline__ uint16_t slope_to_fixed(float s) { return (uint16_t)(uint32_t)fmaxf(fmaf(s, 49152.0f, 8192.5f), 0.0f); }
+__device__ __forceinline__ float slope_from_fixed(float q) { return q == 0.0f ? __builtin_nanf("") : (q - 8192.0f) * (1.0f / 49152.0f); }
 
 // ---- random bits -----------------------------------------------------------------------------------
 __host__ __device__ __forceinline__ uint64_t mix64(uint64_t z)  // splitmix64
@@ -118,17 +152,15 @@ struct Drop {
     float scale;
     int64_t quads;             // words per row
     __device__ __forceinline__ uint64_t base() const { return cut ? mix64(mixed_seed ^ (step + (step_dev ? *step_dev : 0))) : 0; }
-    __device__ __forceinline__ uint64_t word(uint64_t base, int64_t row, int64_t quad) const
+    // a quad's place in the sequence: places of rows a fixed distance apart differ by a constant (no product per quad)
+    __device__ __forceinline__ uint64_t place(int64_t row, int64_t quad) const { return (uint64_t)(row * quads + quad) * 0x9E3779B97F4A7C15ull; }
+    __device__ __forceinline__ static uint64_t word(uint64_t base, uint64_t place) { return mix64(base ^ place); }
+    __device__ __forceinline__ void apply(float *v, uint64_t w) const
     {
-        return mix64(base ^ ((uint64_t)(row * quads + quad) * 0x9E3779B97F4A7C15ull));
-    }
-    __device__ __forceinline__ float4 apply(float4 v, uint64_t w) const
-    {
-        // (a dropped element is zero whatever it was)
+        // (four elements; a dropped one is zero whatever it was)
         const uint32_t lo = (uint32_t)w, hi = (uint32_t)(w >> 32);
-        v.x = (lo & 0xFFFFu) >= cut ? v.x * scale : 0.0f, v.y = (lo >> 16) >= cut ? v.y * scale : 0.0f;
-        v.z = (hi & 0xFFFFu) >= cut ? v.z * scale : 0.0f, v.w = (hi >> 16) >= cut ? v.w * scale : 0.0f;
-        return v;
+        v[0] = (lo & 0xFFFFu) >= cut ? v[0] * scale : 0.0f, v[1] = (lo >> 16) >= cut ? v[1] * scale : 0.0f;
+        v[2] = (hi & 0xFFFFu) >= cut ? v[2] * scale : 0.0f, v[3] = (hi >> 16) >= cut ? v[3] * scale : 0.0f;
     }
 };
 

@@ -56,8 +56,9 @@ __global__ __launch_bounds__(256) void pack_kernel(const T *src, int64_t stride,
 }
 
 // ---- gradient at the products ----------------------------------------------------------------------
-// dz = drop(dy) act'(z) in the layer's type, and its column sums over a range of rows.  Bound by memory (dy and act' read, dz written); a wave
-// takes 256 columns of a row, four elements a lane, so that the sums stay in registers from row to row.
+// dz = drop(dy) act'(z) in the layer's type, and its column sums over a range of rows.  Bound by memory (dy and act' read, dz written).  Eight
+// elements a lane, kGradRows rows at a time per group of lanes, so that enough loads are in flight; `lanes` of a wave (a power of two) take a
+// row, or 512 columns of it, and the sums stay in registers from row to row.
 struct GradArgs {
     const void *dy;
     int64_t dy_stride;
@@ -67,108 +68,164 @@ struct GradArgs {
     void *dz;  // [rows][width8], planes rows * width8 apart; or NULL
     int64_t width8;
     float *sums;  // [gridDim.y][4 quads] or NULL
+    int lanes;
 };
+constexpr int kGradRows = 2;
 
 template <class T, class O>
 __global__ __launch_bounds__(256) void linear_dz_kernel(GradArgs g)
 {
-    __shared__ float4 s_sum[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t quad = (int64_t)blockIdx.x * 64 + lane, col = 4 * quad;
+    __shared__ float s_sum[256][8];
+    const int lane = threadIdx.x % g.lanes, group = threadIdx.x / g.lanes, groups = 256 / g.lanes;
+    const int64_t col = ((int64_t)blockIdx.x * g.lanes + lane) * 8;
     const int64_t first = (int64_t)blockIdx.y * g.rows_each, last = first + g.rows_each < g.rows ? first + g.rows_each : g.rows;
     const int64_t left = g.cols - col;
-    const int valid = (int)(left < 4 ? left : 4);
-    const uint64_t base = g.drop.base();
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int valid = (int)(left < 8 ? left : 8);
+    const uint64_t base = g.drop.base(), step = g.drop.place(groups, 0);
+    float sum[8] = {};
     if (col < g.width8) {
-        for (int64_t row = first + wave; row < last; row += 4) {
-            float4 v = load4(static_cast<const O *>(g.dy) + row * g.dy_stride + col, valid);
-            if (g.slope && valid > 0) {
-                const int64_t at = row * 4 * g.quads + col;
-                float4 s;
-                if (sizeof(T) == 4) {
-                    s = *reinterpret_cast<const float4 *>(static_cast<const float *>(g.slope) + at);
-                } else {
-                    const ushort4 q = *reinterpret_cast<const ushort4 *>(static_cast<const uint16_t *>(g.slope) + at);
-                    s = make_float4(slope_from_fixed(q.x), slope_from_fixed(q.y), slope_from_fixed(q.z), slope_from_fixed(q.w));
+        uint64_t place = g.drop.place(first + group, col >> 2);
+        for (int64_t row0 = first + group; row0 < last; row0 += kGradRows * groups) {
+            float v[kGradRows][8], s[kGradRows][8];
+#pragma unroll
+            for (int r = 0; r < kGradRows; ++r) {
+                const int64_t row = row0 + r * groups < last ? row0 + r * groups : row0;
+                load8(static_cast<const O *>(g.dy) + row * g.dy_stride + col, valid, v[r]);
+                if (g.slope) {
+                    const int64_t at = row * 4 * g.quads + col;
+                    const int kept = (int)(4 * g.quads - col < 8 ? 4 * g.quads - col : 8);
+                    if (sizeof(T) == 4) load8(static_cast<const float *>(g.slope) + at, kept, s[r]);
+                    else load8(static_cast<const uint16_t *>(g.slope) + at, kept, s[r]);
                 }
-                v.x *= s.x, v.y *= s.y, v.z *= s.z, v.w *= s.w;
             }
-            if (g.drop.cut && valid > 0) v = g.drop.apply(v, g.drop.word(base, row, quad));  // (last: a dropped element's gradient is zero)
-            if (g.dz) store_packed<T>(static_cast<StoredAs<T> *>(g.dz) + row * g.width8 + col, g.rows * g.width8, v);
-            sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+#pragma unroll
+            for (int r = 0; r < kGradRows; ++r, place += step) {
+                const int64_t row = row0 + r * groups;
+                if (row >= last) break;
+                if (g.slope) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < valid) v[r][e] *= sizeof(T) == 4 ? s[r][e] : slope_from_fixed(s[r][e]);
+                }
+                if (g.drop.cut) {  // (last: a dropped element's gradient is zero)
+                    g.drop.apply(v[r], Drop::word(base, place));
+                    g.drop.apply(v[r] + 4, Drop::word(base, place + 0x9E3779B97F4A7C15ull));
+                }
+                if (g.dz) {
+                    StoredAs<T> *to = static_cast<StoredAs<T> *>(g.dz) + row * g.width8 + col;
+                    if constexpr (sizeof(T) == 4) {
+                        store_packed<T>(to, g.rows * g.width8, make_float4(v[r][0], v[r][1], v[r][2], v[r][3]));
+                        store_packed<T>(to + 4, g.rows * g.width8, make_float4(v[r][4], v[r][5], v[r][6], v[r][7]));
+                    } else {
+                        store8(to, v[r], 8);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e] += v[r][e];
+            }
         }
     }
     if (!g.sums) return;
-    s_sum[wave][lane] = sum;
-    __syncthreads();
-    if (wave || quad >= g.quads) return;
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        const float4 o = s_sum[w][lane];
-        sum.x += o.x, sum.y += o.y, sum.z += o.z, sum.w += o.w;
-    }
-    *reinterpret_cast<float4 *>(g.sums + ((int64_t)blockIdx.y * g.quads + quad) * 4) = sum;
+    for (int e = 0; e < 8; ++e) s_sum[threadIdx.x][e] = sum[e];
+    __syncthreads();
+    if (group || valid <= 0) return;
+    for (int k = 1; k < groups; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] += s_sum[k * g.lanes + lane][e];
+    float *to = g.sums + (int64_t)blockIdx.y * g.quads * 4 + col;
+    *reinterpret_cast<float4 *>(to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    if (valid > 4) *reinterpret_cast<float4 *>(to + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
 }
 
 // ---- partial sums joined ---------------------------------------------------------------------------
-// out[row][col] = sum over n parts of part[.][row][col], for up to two blocks of partial sums in one launch (a weight's and a bias's gradient).
+// out[row][col] = sum over n parts of part[.][row][col].  The weight's gradient has few parts of many quads: a thread takes a quad.  The bias's
+// has many parts of few quads: sixteen threads share one, or a call waited for its last 512 loads one after another (64 us).
 struct JoinArgs {
     const float *part[2];
-    int64_t rows[2], cols[2], quads[2];
+    int64_t rows, cols[2], quads[2];
     int n[2];
     void *out[2];
-    int64_t blocks0;  // workgroups of the first block
+    int64_t blocks0;  // workgroups of the weight's gradient
 };
 
 template <class T>
 __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 {
-    const int which = (int64_t)blockIdx.x < j.blocks0 ? 0 : 1;
-    const int64_t i = ((int64_t)blockIdx.x - (which ? j.blocks0 : 0)) * 256 + threadIdx.x;
-    const int64_t quads = j.quads[which], each = j.rows[which] * quads;
-    if (i >= each) return;
+    __shared__ float4 s_sum[256];
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float4 *p = reinterpret_cast<const float4 *>(j.part[which]) + i;
-    for (int k = 0; k < j.n[which]; ++k, p += each) {
-        const float4 v = *p;
+    if ((int64_t)blockIdx.x < j.blocks0) {
+        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, quads = j.quads[0], each = j.rows * quads;
+        if (i >= each) return;
+        const float4 *p = reinterpret_cast<const float4 *>(j.part[0]) + i;
+#pragma unroll 4
+        for (int k = 0; k < j.n[0]; ++k) {
+            const float4 v = p[k * each];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        const int64_t row = i / quads, col = 4 * (i % quads), left = j.cols[0] - col;
+        store4(static_cast<T *>(j.out[0]) + row * j.cols[0] + col, s, (int)(left < 4 ? left : 4));
+        return;
+    }
+    const int64_t quad = ((int64_t)blockIdx.x - j.blocks0) * 16 + threadIdx.x % 16;
+    if (quad < j.quads[1]) {
+        const float4 *p = reinterpret_cast<const float4 *>(j.part[1]) + quad;
+#pragma unroll 4
+        for (int k = threadIdx.x / 16; k < j.n[1]; k += 16) {
+            const float4 v = p[k * j.quads[1]];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+    }
+    s_sum[threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.x >= 16 || quad >= j.quads[1]) return;
+    for (int k = 1; k < 16; ++k) {
+        const float4 v = s_sum[16 * k + threadIdx.x];
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const int64_t row = i / quads, col = 4 * (i % quads), left = j.cols[which] - col;
-    store4(static_cast<T *>(j.out[which]) + row * j.cols[which] + col, s, (int)(left < 4 ? left : 4));
+    const int64_t left = j.cols[1] - 4 * quad;
+    store4(static_cast<T *>(j.out[1]) + 4 * quad, s, (int)(left < 4 ? left : 4));
 }
 
 // ---- products --------------------------------------------------------------------------------------
-constexpr int kTileX = 128;
-
-template <class E, int PLANES, bool AA, bool BA, int X, int WA, int WB, int STAGES, EndKind END>
+template <class E, int PLANES, bool AA, bool BA, int XA, int XB, int K, int WA, int WB, int STAGES, EndKind END>
 static void launch_sized(TileArgs &t, hipStream_t st)
 {
-    t.tiles_a = (int)ceil_div(t.a.extent, X), t.tiles_b = (int)ceil_div(t.b.extent, X);
+    t.tiles_a = (int)ceil_div(t.a.extent, XA), t.tiles_b = (int)ceil_div(t.b.extent, XB);
     const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b * t.splits;
     if (blocks == 0) return;
-    hipLaunchKernelGGL((linear_tile_kernel<E, PLANES, AA, BA, X, X, WA, WB, STAGES, END>), dim3((unsigned)blocks), dim3(WA * WB * kWave), 0, st, t);
+    hipLaunchKernelGGL((linear_tile_kernel<E, PLANES, AA, BA, XA, XB, K, WA, WB, STAGES, END>), dim3((unsigned)blocks), dim3(WA * WB * kWave), 0, st, t);
 }
 
+// Larger tiles read less and multiply faster (dx of 32768 x 2048 x 2048 bf16: 256 x 256 237 us, 128 x 128 297, 64 x 64 425), smaller ones
+// fill the card where there are few (forward of 4096 x 1024 x 512: 43.6, 18.9 and 11.8 us): the largest of which there are 256.
 template <class E, int PLANES, bool AA, bool BA, EndKind END>
 static void launch_tiles(TileArgs &t, hipStream_t st)
 {
+    auto tiles = [&](int x) { return ceil_div(t.a.extent, x) * ceil_div(t.b.extent, x) * t.splits; };
     if constexpr (PLANES == 3) {
-        launch_sized<E, PLANES, AA, BA, 128, 2, 4, 3, END>(t, st);
+        if (tiles(128) >= 200) launch_sized<E, PLANES, AA, BA, 128, 128, 32, 2, 4, 3, END>(t, st);
+        else launch_sized<E, PLANES, AA, BA, 64, 64, 32, 2, 2, 3, END>(t, st);
     } else {
-        if (ceil_div(t.a.extent, 256) * ceil_div(t.b.extent, 256) * t.splits >= 200) launch_sized<E, PLANES, AA, BA, 256, 2, 4, 4, END>(t, st);
-        else launch_sized<E, PLANES, AA, BA, 128, 2, 2, 4, END>(t, st);
+        if (tiles(256) >= 256) launch_sized<E, PLANES, AA, BA, 256, 256, 32, 2, 4, 4, END>(t, st);
+        else if (tiles(128) >= 256) launch_sized<E, PLANES, AA, BA, 128, 128, 32, 2, 2, 4, END>(t, st);
+        else launch_sized<E, PLANES, AA, BA, 64, 64, 64, 2, 2, 2, END>(t, st);
     }
 }
 
-// Parts of a sum over k where `tiles` tiles alone would leave most of the card idle: as many as fill it twice, none shorter than 256 terms.
-static int splits_of(int64_t tiles, int64_t k)
+// Parts of a sum over k where the tiles of an a x b output alone would leave most of the card idle: as many as make 256 large tiles, or 512 of the
+// middle ones, none shorter than 256 terms (their join costs 4 bytes written and read an element and part).
+static int splits_of(int64_t a, int64_t b, int64_t k)
 {
-    const int64_t want = tiles > 0 ? 512 / tiles : 1, most = k / 256;
-    const int64_t s = want < most ? want : most;
+    const int64_t large = ceil_div(a, 256) * ceil_div(b, 256), middle = ceil_div(a, 128) * ceil_div(b, 128);
+    if (large == 0) return 1;
+    int64_t s = ceil_div(256, large);
+    if (s * 512 > k) s = 512 / middle;  // (parts for large tiles would be short)
+    const int64_t most = k / 256;
+    s = s < most ? s : most;
     return (int)(s > 1 ? s : 1);
 }
-static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), kTileK) * kTileK; }
+static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), 64) * 64; }
 
 // ---- a layer's plan --------------------------------------------------------------------------------
 struct Plan {
@@ -190,11 +247,11 @@ static Plan plan_of(const kge_linear *l)
     p.x = p.pack_x ? packed_bytes(l->type, l->rows, l->in) : 0;
     p.w = p.pack_w ? packed_bytes(l->type, l->out, l->in) : 0;
     // ranges of at least 16 rows, about 1024 workgroups in all
-    const int64_t across = ceil_div(up8(l->out), 256), want = across > 0 && across < 1024 ? 1024 / across : 1;
+    const int64_t across = ceil_div(up8(l->out), 512), want = across > 0 && across < 1024 ? 1024 / across : 1;
     p.sum_rows = ceil_div(l->rows, want);
     if (p.sum_rows < 16) p.sum_rows = 16;
     p.sum_blocks = (int)ceil_div(l->rows, p.sum_rows);
-    p.dw_splits = splits_of(ceil_div(l->in, kTileX) * ceil_div(l->out, kTileX), l->rows);
+    p.dw_splits = splits_of(l->in, l->out, l->rows);
     return p;
 }
 
@@ -267,8 +324,9 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
     const bool want_dz = !ready && (dx || dw);
     if ((want_dz || db) && l->rows > 0 && l->out > 0) {
         GradArgs g{dy, dy_stride, p.slope ? saved : nullptr, l->rows, l->out, p.quads, p.sum_rows,
-                   make_drop(l->p, l->seed, l->step, l->step_dev, l->out), want_dz ? dz : nullptr, width8, db ? sums : nullptr};
-        const dim3 grid((unsigned)ceil_div(width8, 256), (unsigned)p.sum_blocks);
+                   make_drop(l->p, l->seed, l->step, l->step_dev, l->out), want_dz ? dz : nullptr, width8, db ? sums : nullptr, 4};
+        while (g.lanes < 64 && 8 * g.lanes < width8) g.lanes *= 2;
+        const dim3 grid((unsigned)ceil_div(width8, 8 * g.lanes), (unsigned)p.sum_blocks);
         if (l->out_type == KGE_F32) hipLaunchKernelGGL((linear_dz_kernel<T, float>), grid, dim3(256), 0, st, g);
         else hipLaunchKernelGGL((linear_dz_kernel<T, T>), grid, dim3(256), 0, st, g);
     }
@@ -293,12 +351,12 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
             launch_tiles<E, kPlanes, true, true, kEndStore>(t, st);
         } else {
             launch_tiles<E, kPlanes, true, true, kEndPartial>(t, st);
-            j.part[0] = part, j.rows[0] = l->out, j.cols[0] = l->in, j.quads[0] = t.e.quads, j.n[0] = t.splits, j.out[0] = dw;
-            j.blocks0 = ceil_div(j.rows[0] * j.quads[0], 256);
+            j.part[0] = part, j.rows = l->out, j.cols[0] = l->in, j.quads[0] = t.e.quads, j.n[0] = t.splits, j.out[0] = dw;
+            j.blocks0 = ceil_div(j.rows * j.quads[0], 256);
         }
     }
-    if (db) j.part[1] = sums, j.rows[1] = 1, j.cols[1] = l->out, j.quads[1] = p.quads, j.n[1] = p.sum_blocks, j.out[1] = db;
-    const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 256) : 0);
+    if (db) j.part[1] = sums, j.cols[1] = l->out, j.quads[1] = p.quads, j.n[1] = p.sum_blocks, j.out[1] = db;
+    const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 16) : 0);
     if (blocks) hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, j);
     KGE_CHECK_LAUNCH();
     return KGE_OK;

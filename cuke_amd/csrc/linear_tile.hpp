@@ -60,13 +60,11 @@ struct Ends {
 struct TileArgs {
     Side a, b;      // a: the columns of the output, b: its rows
     int64_t k;      // terms of every sum
-    int64_t k_each; // per split, a multiple of kTileK
+    int64_t k_each; // per split, a multiple of 64
     int tiles_a, tiles_b, splits;
     float *partial; // [splits][rows][quads * 4]
     Ends e;
 };
-
-constexpr int kTileK = 32;
 
 static __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};  // what chunks outside a side read
 
@@ -75,19 +73,19 @@ __device__ __forceinline__ void chunk_to_lds(const void *src, void *lds)
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
 }
 
-// A tile of X indices by 32 terms in LDS, as 16-byte chunks.  Along: four chunks a row, chunk j in slot j ^ (row / 2 % 4), so that the
-// 128-bit reads of eight consecutive rows fall on distinct banks.  Across: X / 8 chunks a row of terms, pairs of chunks permuted by the row so
+// A tile of X indices by K (32 or 64) terms in LDS, as 16-byte chunks.  Along: K / 8 chunks a row, chunk j in slot j ^ (row / 2 % 8) (K = 32: j ^
+// (row / 4 % 4)), so that the 128-bit reads of sixteen consecutive rows fall on distinct banks of the 64.  Across: X / 8 chunks a row of terms, pairs of chunks permuted by the row so
 // that the transposing reads of four rows (and of both halves of a wave, where the row is long enough) do.
-template <int X, bool ACROSS, int THREADS>
+template <int X, int K, bool ACROSS, int THREADS>
 struct Tile {
-    static constexpr int kChunks = X * kTileK / 8;
+    static constexpr int kChunks = X * K / 8;
     static constexpr int kRounds = kChunks / THREADS;
-    static constexpr int kRow = ACROSS ? X / 8 : 4;  // chunks a row
+    static constexpr int kRow = ACROSS ? X / 8 : K / 8;  // chunks a row
     static_assert(kChunks % THREADS == 0, "whole rounds");
 
     __device__ __forceinline__ static int turn(int row)
     {
-        if (!ACROSS) return (row >> 1) & 3;
+        if (!ACROSS) return K == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
         return X >= 256 ? 2 * (2 * (row & 3) + 8 * ((row >> 3) & 1)) : (X >= 128 ? 4 * (row & 3) : 2 * (row & 3));
     }
 
@@ -109,7 +107,7 @@ struct Tile {
                 const bool there = index < s.extent;
                 from[r] = there ? reinterpret_cast<const char *>(p + (ACROSS ? (k + row) * s.stride + index : index * s.stride + k + 8 * j))
                                 : reinterpret_cast<const char *>(zero_chunk);
-                step[r] = there ? (ACROSS ? kTileK * s.stride : kTileK) * (int64_t)sizeof(E) : 0;
+                step[r] = there ? (ACROSS ? K * s.stride : K) * (int64_t)sizeof(E) : 0;
             }
         }
         // the next tile, of which `left` terms exist (none, behind the end)
@@ -129,7 +127,7 @@ struct Tile {
     {
         if (!ACROSS) {
             const int row = at + (lane & 31), j = 2 * step + (lane >> 5);
-            return *reinterpret_cast<const s16x8 *>(lds + 16 * (row * 4 + (j ^ turn(row))));
+            return *reinterpret_cast<const s16x8 *>(lds + 16 * (row * kRow + (j ^ turn(row))));
         }
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         const int row = 16 * step + 8 * (lane >> 5) + ((lane & 15) >> 2), index = at + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -155,34 +153,63 @@ __device__ __noinline__ float4 plain_sums(Side a, Side b, int64_t n, int valid, 
     return make_float4(s[0], s[1], s[2], s[3]);
 }
 
-// Four consecutive columns of a row through the layer's epilogue.  T: the layer's type.
-template <class T>
-__device__ __forceinline__ void finish_quad(const Ends &e, uint64_t base, int64_t row, int64_t col, int valid, float4 z, float4 bias)
+// Four consecutive columns (`valid` of them exist) of R rows, `apart` rows from one to the next, through the layer's epilogue.  T: the layer's
+// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.
+template <class T, int R>
+__device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64_t first, int apart, int64_t col, int valid, float (&z)[R][4], float4 bias)
 {
-    z.x += bias.x, z.y += bias.y, z.z += bias.z, z.w += bias.w;
+    float res[R][4];
+    if (e.residual) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int64_t row = first + r * apart, at = (row < e.rows ? row : e.rows - 1) * e.residual_stride + col;
+            const float4 v = sizeof(T) == 4 || e.out_f32 ? load4(static_cast<const float *>(e.residual) + at, valid)
+                                                         : load4(static_cast<const T *>(e.residual) + at, valid);
+            res[r][0] = v.x, res[r][1] = v.y, res[r][2] = v.z, res[r][3] = v.w;
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) z[r][0] += bias.x, z[r][1] += bias.y, z[r][2] += bias.z, z[r][3] += bias.w;
     if (e.act != KGE_ACT_NONE) {
-        float4 s;
-        z.x = activate(z.x, e.act, &s.x), z.y = activate(z.y, e.act, &s.y), z.z = activate(z.z, e.act, &s.z), z.w = activate(z.w, e.act, &s.w);
+        float flat[4 * R], slope[4 * R];
+#pragma unroll
+        for (int i = 0; i < 4 * R; ++i) flat[i] = z[i / 4][i % 4];
+        activate(flat, e.act, slope);
+#pragma unroll
+        for (int i = 0; i < 4 * R; ++i) z[i / 4][i % 4] = flat[i];
         if (e.slope) {  // (rows of whole quads)
-            const int64_t at = row * 4 * e.quads + col;
-            if (sizeof(T) == 4) {
-                *reinterpret_cast<float4 *>(static_cast<float *>(e.slope) + at) = s;
-            } else {
-                const ushort4 q = {slope_to_fixed(s.x), slope_to_fixed(s.y), slope_to_fixed(s.z), slope_to_fixed(s.w)};
-                *reinterpret_cast<ushort4 *>(static_cast<uint16_t *>(e.slope) + at) = q;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int64_t row = first + r * apart, at = row * 4 * e.quads + col;
+                if (row >= e.rows) continue;
+                if (sizeof(T) == 4) {
+                    *reinterpret_cast<float4 *>(static_cast<float *>(e.slope) + at) = make_float4(slope[4 * r], slope[4 * r + 1], slope[4 * r + 2], slope[4 * r + 3]);
+                } else {
+                    const ushort4 q = {slope_to_fixed(slope[4 * r]), slope_to_fixed(slope[4 * r + 1]), slope_to_fixed(slope[4 * r + 2]), slope_to_fixed(slope[4 * r + 3])};
+                    *reinterpret_cast<ushort4 *>(static_cast<uint16_t *>(e.slope) + at) = q;
+                }
             }
         }
     }
-    if (e.drop.cut) z = e.drop.apply(z, e.drop.word(base, row, col >> 2));
-    if (e.residual) {
-        const int64_t at = row * e.residual_stride + col;
-        const float4 r = sizeof(T) == 4 || e.out_f32 ? load4(static_cast<const float *>(e.residual) + at, valid)
-                                                     : load4(static_cast<const T *>(e.residual) + at, valid);
-        z.x += r.x, z.y += r.y, z.z += r.z, z.w += r.w;
+    if (e.drop.cut) {
+        const uint64_t place = e.drop.place(first, col >> 2), step = e.drop.place(apart, 0);
+#pragma unroll
+        for (int r = 0; r < R; ++r) e.drop.apply(z[r], Drop::word(base, place + r * step));
     }
-    const int64_t at = row * e.y_stride + col;
-    if (sizeof(T) == 4 || e.out_f32) store4(static_cast<float *>(e.y) + at, z, valid);
-    else store4(static_cast<T *>(e.y) + at, z, valid);
+    if (e.residual) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) z[r][v] += res[r][v];
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int64_t row = first + r * apart, at = row * e.y_stride + col;
+        if (row >= e.rows) continue;
+        const float4 v = make_float4(z[r][0], z[r][1], z[r][2], z[r][3]);
+        if (sizeof(T) == 4 || e.out_f32) store4(static_cast<float *>(e.y) + at, v, valid);
+        else store4(static_cast<T *>(e.y) + at, v, valid);
+    }
 }
 
 // Workgroups are dealt to the eight XCDs in turn; consecutive tiles go to one XCD, whose L2 then holds the rows and columns they share:
@@ -209,17 +236,17 @@ __device__ __forceinline__ void stage_ready()
     asm volatile("" ::: "memory");
 }
 
-// E: what the matrix cores multiply, PLANES: 3 for fp32.  A workgroup of WA x WB waves computes XA columns by XB rows.  STAGES tiles of 32 terms
+// E: what the matrix cores multiply, PLANES: 3 for fp32.  A workgroup of WA x WB waves computes XA columns by XB rows.  STAGES tiles of K terms
 // are in LDS, in arrays of their own (so that the compiler sees that the one being read is none of those being written): STAGES - 1 are
 // requested ahead, and one barrier a tile both publishes the next and frees the last.
-template <class E, int PLANES, bool A_ACROSS, bool B_ACROSS, int XA, int XB, int WA, int WB, int STAGES, EndKind END>
+template <class E, int PLANES, bool A_ACROSS, bool B_ACROSS, int XA, int XB, int K, int WA, int WB, int STAGES, EndKind END>
 __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
 {
     using T = typename std::conditional<PLANES == 3, float, E>::type;
     constexpr int kThreads = WA * WB * kWave;
-    using A = Tile<XA, A_ACROSS, kThreads>;
-    using B = Tile<XB, B_ACROSS, kThreads>;
-    constexpr int kBytesA = XA * kTileK * 2, kBytesB = XB * kTileK * 2, kStage = PLANES * (kBytesA + kBytesB);
+    using A = Tile<XA, K, A_ACROSS, kThreads>;
+    using B = Tile<XB, K, B_ACROSS, kThreads>;
+    constexpr int kBytesA = XA * K * 2, kBytesB = XB * K * 2, kStage = PLANES * (kBytesA + kBytesB);
     constexpr int kLoads = PLANES * (A::kRounds + B::kRounds);  // per thread and tile
     constexpr int FA = XA / WA / 32, FB = XB / WB / 32;
     static_assert(STAGES >= 2 && STAGES <= 4, "stages");
@@ -245,11 +272,11 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
             feed_a[p].load(left, lds + p * kBytesA);
             feed_b[p].load(left, lds + PLANES * kBytesA + p * kBytesB);
         }
-        left -= kTileK;
+        left -= K;
     };
     auto multiply = [&](const char *lds) {
 #pragma unroll
-        for (int step = 0; step < kTileK / 16; ++step) {
+        for (int step = 0; step < K / 16; ++step) {
             s16x8 a[FA][PLANES], b[FB][PLANES];
 #pragma unroll
             for (int p = 0; p < PLANES; ++p) {
@@ -275,7 +302,7 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
 
     // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
-    const int tiles = (int)((k1 - k0 + kTileK - 1) / kTileK);
+    const int tiles = (int)((k1 - k0 + K - 1) / K);
 #pragma unroll
     for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
     int at = 0;
@@ -294,52 +321,69 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
         multiply(stage(u));
     }
 
-    // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows of the wave's columns at a time, so that they come back
-    // row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.
+    // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows by 64 (or 32) of the wave's columns at a time, so that they
+    // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.
     stage_ready<0>();
-    constexpr int kQuads = 8 * FA, kStrip = 32 * kQuads * 16, kPerStage = kStage / kStrip;
-    static_assert(kPerStage >= 1 && (WA * WB + kPerStage - 1) / kPerStage <= STAGES, "a strip for every wave");
+    constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16, kPerStage = kStage / kStrip;
+    static_assert(FA % kGroup == 0 && kPerStage >= 1 && (WA * WB + kPerStage - 1) / kPerStage <= STAGES, "a strip for every wave");
+    auto skew = [](int row) { return kQuads == 16 ? row & 15 : (row >> 1) & 7; };
     char *strip = stage(wave / kPerStage) + wave % kPerStage * kStrip;
     const int quad = lane % kQuads;
-    const int64_t col = n0 + wa + 4 * quad;
-    const int valid = (int)(t.e.cols - col < 4 ? t.e.cols - col : 4);
     uint64_t base = 0;
-    float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if constexpr (END == kEndLayer) {
-        base = t.e.drop.base();
-        if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + (valid > 0 ? col : 0), valid);
-    }
+    if constexpr (END == kEndLayer) base = t.e.drop.base();
 #pragma unroll
-    for (int j = 0; j < FB; ++j) {
-        // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
+    for (int g = 0; g < FA; g += kGroup) {
+        const int64_t col = n0 + wa + 32 * g + 4 * quad;
+        const int valid = (int)(t.e.cols - col < 4 ? t.e.cols - col : 4);
+        float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if constexpr (END == kEndLayer)
+            if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + (valid > 0 ? col : 0), valid);
 #pragma unroll
-        for (int i = 0; i < FA; ++i)
+        for (int j = 0; j < FB; ++j) {
+            // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float z[4];
+            for (int i = 0; i < kGroup; ++i)
 #pragma unroll
-                for (int v = 0; v < 4; ++v) {
-                    z[v] = acc[i][j][4 * q + v];
-                    if constexpr (PLANES == 3) z[v] += low[i][j][4 * q + v];
+                for (int q = 0; q < 4; ++q) {
+                    float z[4];
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        z[v] = acc[g + i][j][4 * q + v];
+                        if constexpr (PLANES == 3) z[v] += low[g + i][j][4 * q + v];
+                    }
+                    const int row = lane & 31, at = 8 * i + 2 * q + (lane >> 5);
+                    *reinterpret_cast<float4 *>(strip + 16 * (row * kQuads + (at ^ skew(row)))) = make_float4(z[0], z[1], z[2], z[3]);
                 }
-                const int row = lane & 31, at = 8 * i + 2 * q + (lane >> 5);
-                *reinterpret_cast<float4 *>(strip + 16 * (row * kQuads + (at ^ (row & 7)))) = make_float4(z[0], z[1], z[2], z[3]);
+            if (valid <= 0) continue;
+            constexpr int kApart = 64 / kQuads, kRows = 4;  // rows a read covers, reads a turn
+            for (int r0 = lane / kQuads; r0 < 32; r0 += kApart * kRows) {
+                const int64_t first = m0 + wb + 32 * j + r0;
+                float z[kRows][4];
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    const int r = r0 + k * kApart;
+                    const int64_t row = first + k * kApart;
+                    float4 v = *reinterpret_cast<const float4 *>(strip + 16 * (r * kQuads + (quad ^ skew(r))));
+                    if constexpr (PLANES == 3) {
+                        // (an infinite operand's planes, or leading parts that were rounded up, may have made this of a finite sum)
+                        if ((not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) && row < t.e.rows)
+                            v = plain_sums<A_ACROSS, B_ACROSS>(t.a, t.b, col, valid, row, k0, k1);
+                    }
+                    z[k][0] = v.x, z[k][1] = v.y, z[k][2] = v.z, z[k][3] = v.w;
+                }
+                if constexpr (END == kEndLayer) {
+                    finish_quads<T, kRows>(t.e, base, first, kApart, col, valid, z, bias);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kRows; ++k) {
+                        const int64_t row = first + k * kApart;
+                        const float4 v = make_float4(z[k][0], z[k][1], z[k][2], z[k][3]);
+                        if (row >= t.e.rows) continue;
+                        if constexpr (END == kEndPartial) *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = v;
+                        else store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, v, valid);
+                    }
+                }
             }
-#pragma unroll 2
-        for (int r = lane / kQuads; r < 32; r += 64 / kQuads) {
-            float4 z = *reinterpret_cast<const float4 *>(strip + 16 * (r * kQuads + (quad ^ (r & 7))));
-            const int64_t row = m0 + wb + 32 * j + r;
-            if (row >= t.e.rows || valid <= 0) continue;
-            if constexpr (PLANES == 3) {
-                // (an infinite operand's planes, or leading parts that were rounded up, may have made this of a finite sum)
-                if (not_finite(z.x) || not_finite(z.y) || not_finite(z.z) || not_finite(z.w)) z = plain_sums<A_ACROSS, B_ACROSS>(t.a, t.b, col, valid, row, k0, k1);
-            }
-            if constexpr (END == kEndPartial)
-                *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = z;
-            else if constexpr (END == kEndLayer)
-                finish_quad<T>(t.e, base, row, col, valid, z, bias);
-            else
-                store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, z, valid);
         }
     }
 }
