@@ -1,5 +1,5 @@
 // The eager surface's host path: what KGEModel.score / backward, margin_loss, the sparse optimizer steps, the
-// positional score functions and the sampler do between Python and the library's entry points, in native code.
+// positional score functions, the sampler and the feature operators do between Python and the library's entry points, in native code.
 //
 // A batch of a few hundred triples is 50 to 100 us of small kernels; the same calls issued through Python's
 // ctypes -- argument checks, structure building, a dozen torch.empty calls, one synchronisation per distinct-row
@@ -16,6 +16,7 @@
 #include <c10/hip/HIPCachingAllocator.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -664,6 +665,180 @@ PyObject *py_sample_batch(PyObject *, PyObject *const *args, Py_ssize_t)
     END_HANDLE_TH_ERRORS
 }
 
+// ---- feature operators (features.py) ----------------------------------------------------------------
+// kge_type_t of a tensor this module can hand on, or -1
+int type_of(const at::Tensor *t, int dev)
+{
+    if (!t || !t->is_cuda() || t->device().index() != dev) return -1;
+    switch (t->scalar_type()) {
+        case at::kFloat: return KGE_F32;
+        case at::kBFloat16: return KGE_BF16;
+        case at::kHalf: return KGE_F16;
+        default: return -1;
+    }
+}
+
+// [rows, cols] of a type with contiguous rows, whatever the stride between them
+bool rows_of(const at::Tensor *t, int type, int64_t rows, int64_t cols, int dev, int64_t *stride)
+{
+    if (type_of(t, dev) != type || t->dim() != 2 || t->size(0) != rows || t->size(1) != cols) return false;
+    if (cols > 1 && t->stride(1) != 1) return false;
+    if (rows > 1 && t->stride(0) < cols) return false;
+    *stride = rows > 1 ? t->stride(0) : std::max(t->stride(0), cols);
+    return true;
+}
+
+bool vector_of(const at::Tensor *t, int type, int64_t n, int dev)
+{
+    return type_of(t, dev) == type && t->dim() == 1 && t->size(0) == n && t->is_contiguous();
+}
+
+bool word(PyObject *o, uint64_t *out)
+{
+    if (!PyLong_Check(o)) return false;
+    *out = PyLong_AsUnsignedLongLongMask(o);
+    return true;
+}
+
+// linear(x, weight, bias, act, residual, out_dtype or None, drop, seed, step, for_backward) -> y, or (y, saved, kge_linear as bytes), or None
+PyObject *py_linear(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = tensor(args[0]), *w = tensor(args[1]), *b = tensor(args[2]), *res = tensor(args[4]);
+    if (!x || !x->is_cuda()) NOT_HERE;  // (first: without a GPU there is no current device)
+    const int dev = c10::hip::current_device();
+    kge_linear l{};
+    l.type = type_of(x, dev);
+    if (l.type < 0 || x->dim() != 2 || !w || w->dim() != 2) NOT_HERE;
+    l.rows = x->size(0), l.in = x->size(1), l.out = w->size(0);
+    if (!rows_of(x, l.type, l.rows, l.in, dev, &l.x_stride) || !rows_of(w, l.type, l.out, l.in, dev, &l.weight_stride)) NOT_HERE;
+    if (args[2] != Py_None && !vector_of(b, l.type, l.out, dev)) NOT_HERE;
+    if (!PyLong_Check(args[3])) NOT_HERE;
+    l.act = (int32_t)PyLong_AsLong(args[3]);
+    l.out_type = l.type;
+    if (args[5] != Py_None) {
+        if (!THPDtype_Check(args[5])) NOT_HERE;
+        const at::ScalarType want = reinterpret_cast<THPDtype *>(args[5])->scalar_type;
+        if (want == at::kFloat) l.out_type = KGE_F32;
+        else if (want != x->scalar_type()) NOT_HERE;
+    } else if (args[4] != Py_None && type_of(res, dev) == KGE_F32) {
+        l.out_type = KGE_F32;
+    }
+    if (args[4] != Py_None && !rows_of(res, l.out_type, l.rows, l.out, dev, &l.residual_stride)) NOT_HERE;
+    if (!number(args[6], &l.p) || !word(args[7], &l.seed) || !word(args[8], &l.step)) NOT_HERE;
+    if (!(l.p >= 0.0 && l.p <= 1.0)) NOT_HERE;
+    const bool keep = PyObject_IsTrue(args[9]);
+    l.x = x->data_ptr(), l.weight = w->data_ptr();
+    l.bias = args[2] != Py_None ? b->data_ptr() : nullptr, l.residual = args[4] != Py_None ? res->data_ptr() : nullptr;
+    const auto opt = x->options().requires_grad(false);
+    at::Tensor y = at::empty({l.rows, l.out}, l.out_type == KGE_F32 ? opt.dtype(at::kFloat) : opt), saved;
+    const size_t saved_bytes = keep ? kge_linear_saved_bytes(&l) : 0, ws_bytes = kge_linear_fwd_workspace(&l, keep);
+    if (saved_bytes) saved = at::empty({(int64_t)saved_bytes}, opt.dtype(at::kByte));
+    c10::DataPtr ws;
+    if (ws_bytes) ws = scratch(ws_bytes);
+    void *st = stream(), *to = y.data_ptr(), *kept = saved_bytes ? saved.data_ptr() : nullptr;
+    const int rc = nogil([&] { return kge_linear_fwd(&l, to, std::max<int64_t>(l.out, 1), keep, kept, saved_bytes, ws.get(), ws_bytes, st); });
+    if (rc) return fail(rc, "kge_linear_fwd"), nullptr;
+    if (!keep) return wrap(y);
+    return Py_BuildValue("(NNy#)", wrap(y), wrap(saved), reinterpret_cast<const char *>(&l), (Py_ssize_t)sizeof(l));
+    END_HANDLE_TH_ERRORS
+}
+
+// linear_backward(kge_linear as bytes, x, saved, dy, need x, need weight, need bias) -> (dx, dweight, dbias), or None.  The bytes, x and saved are
+// those of the forward call, which linear_backward() of features.py has checked.
+PyObject *py_linear_backward(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    kge_linear l;
+    if (!PyBytes_Check(args[0]) || PyBytes_GET_SIZE(args[0]) != (Py_ssize_t)sizeof(l)) NOT_HERE;
+    std::memcpy(&l, PyBytes_AS_STRING(args[0]), sizeof(l));
+    const at::Tensor *x = tensor(args[1]), *saved = tensor(args[2]), *dy = tensor(args[3]);
+    if (!x || !x->is_cuda()) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    int64_t dy_stride;
+    if (type_of(x, dev) != l.type || !rows_of(dy, l.out_type, l.rows, l.out, dev, &dy_stride)) NOT_HERE;
+    const auto opt = x->options().requires_grad(false);
+    at::Tensor dx, dw, db;
+    if (PyObject_IsTrue(args[4])) dx = at::empty({l.rows, l.in}, opt);
+    if (PyObject_IsTrue(args[5])) dw = at::empty({l.out, l.in}, opt);
+    if (PyObject_IsTrue(args[6])) db = at::empty({l.out}, opt);
+    const size_t ws_bytes = kge_linear_bwd_workspace(&l);
+    const c10::DataPtr ws = scratch(ws_bytes);
+    auto at = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    void *st = stream(), *px = at(dx), *pw = at(dw), *pb = at(db);
+    const void *kept = saved ? saved->data_ptr() : nullptr, *from = dy->data_ptr();
+    const size_t kept_bytes = saved ? saved->numel() : 0;
+    const int rc = nogil([&] { return kge_linear_bwd(&l, from, dy_stride, kept, kept_bytes, px, pw, pb, ws.get(), ws_bytes, st); });
+    if (rc) return fail(rc, "kge_linear_bwd"), nullptr;
+    return Py_BuildValue("(NNN)", wrap(dx), wrap(dw), wrap(db));
+    END_HANDLE_TH_ERRORS
+}
+
+// dropout(x, p, seed, step) -> y, or None
+PyObject *py_dropout(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = tensor(args[0]);
+    if (!x || !x->is_cuda()) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    const int type = type_of(x, dev);
+    int64_t stride;
+    double p;
+    uint64_t seed, step;
+    if (type < 0 || x->dim() != 2 || !rows_of(x, type, x->size(0), x->size(1), dev, &stride)) NOT_HERE;
+    if (!number(args[1], &p) || !(p >= 0.0 && p <= 1.0) || !word(args[2], &seed) || !word(args[3], &step)) NOT_HERE;
+    const int64_t rows = x->size(0), cols = x->size(1);
+    at::Tensor y = at::empty({rows, cols}, x->options().requires_grad(false));
+    void *st = stream(), *to = y.data_ptr();
+    const void *from = x->data_ptr();
+    const int rc = nogil([&] { return kge_dropout(type, from, stride, to, cols, rows, cols, p, seed, step, nullptr, st); });
+    if (rc) return fail(rc, "kge_dropout"), nullptr;
+    return wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// preference_loss(pos, neg, ref_pos, ref_neg, mask, kind, beta, sign, smoothing, temperature) -> (loss, dpos, dneg), or None
+PyObject *py_preference_loss(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *pos = tensor(args[0]), *neg = tensor(args[1]), *rp = tensor(args[2]), *rn = tensor(args[3]), *mask = tensor(args[4]);
+    if (!neg || !neg->is_cuda()) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    kge_preference q{};
+    q.type = type_of(neg, dev);
+    if (q.type < 0 || neg->dim() != 2) NOT_HERE;
+    q.batch = neg->size(0), q.n_neg = neg->size(1);
+    if (!rows_of(neg, q.type, q.batch, q.n_neg, dev, &q.neg_stride) || !vector_of(pos, q.type, q.batch, dev)) NOT_HERE;
+    if ((args[2] == Py_None) != (args[3] == Py_None)) NOT_HERE;
+    if (args[2] != Py_None) {
+        if (!vector_of(rp, q.type, q.batch, dev) || !rows_of(rn, q.type, q.batch, q.n_neg, dev, &q.ref_neg_stride)) NOT_HERE;
+        q.ref_pos = rp->data_ptr(), q.ref_neg = rn->data_ptr();
+    }
+    if (args[4] != Py_None) {
+        if (!mask || !mask->is_cuda() || mask->device().index() != dev || mask->dim() != 2) NOT_HERE;
+        if (mask->scalar_type() != at::kBool && mask->scalar_type() != at::kByte) NOT_HERE;
+        if (mask->size(0) != q.batch || mask->size(1) != q.n_neg || (q.n_neg > 1 && mask->stride(1) != 1)) NOT_HERE;
+        if (q.batch > 1 && mask->stride(0) < q.n_neg) NOT_HERE;
+        q.mask_stride = q.batch > 1 ? mask->stride(0) : std::max(mask->stride(0), q.n_neg);
+        q.mask = static_cast<const uint8_t *>(mask->data_ptr());
+    }
+    double beta, sign, smoothing, temperature;
+    if (!PyLong_Check(args[5]) || !number(args[6], &beta) || !number(args[7], &sign) || !number(args[8], &smoothing) || !number(args[9], &temperature)) NOT_HERE;
+    q.kind = (int32_t)PyLong_AsLong(args[5]);
+    q.beta = (float)beta, q.sign = (float)sign, q.smoothing = (float)smoothing, q.temperature = (float)temperature;
+    q.pos = pos->data_ptr(), q.neg = neg->data_ptr();
+    const auto f32 = neg->options().dtype(at::kFloat).requires_grad(false);
+    at::Tensor loss = at::empty({1}, f32), dpos = at::empty({q.batch}, f32), dneg = at::empty({q.batch, q.n_neg}, f32);
+    const size_t ws_bytes = kge_preference_workspace(&q);
+    const c10::DataPtr ws = scratch(ws_bytes);
+    void *st = stream();
+    float *pl = loss.data_ptr<float>(), *pp = dpos.data_ptr<float>(), *pn = dneg.data_ptr<float>();
+    const int rc = nogil([&] { return kge_preference_loss(&q, pl, pp, pn, ws.get(), ws_bytes, st); });
+    if (rc) return fail(rc, "kge_preference_loss"), nullptr;
+    return Py_BuildValue("(NNN)", wrap(loss), wrap(dpos), wrap(dneg));
+    END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"set_error", py_set_error, METH_O, nullptr},
                          FAST(inspect),
@@ -674,6 +849,10 @@ PyMethodDef methods[] = {{"set_error", py_set_error, METH_O, nullptr},
                          FAST(sparse_step),
                          {"sampler_stage", py_sampler_stage, METH_O, nullptr},
                          FAST(sample_batch),
+                         FAST(linear),
+                         FAST(linear_backward),
+                         FAST(dropout),
+                         FAST(preference_loss),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -8,7 +8,8 @@ The score functions of :mod:`cuke_amd.kge` look rows up.  The operators here sta
   FeatureEncoder                              two linear layers that turn feature rows into entity rows
 
 Like the rest of the package they work on the current stream, allocate their outputs, give every gradient by an explicit call,
-and raise where an argument is not what the kernels take: there is no fallback.  16-bit and fp32 tensors are taken as they are; one whose rows
+and raise where an argument is not what the kernels take: there is no fallback.  The ordinary call goes through csrc/host.cpp, what that does
+not take through the code here, which converts or raises.  16-bit and fp32 tensors are taken as they are; one whose rows
 are not contiguous is copied.  No counterpart in the reference.
 """
 from __future__ import annotations
@@ -93,9 +94,9 @@ def _bytes(n: int, device):
 class LinearForward:
     """A layer's output, and what its backward pass needs (x and weight have to stay as they are until then)."""
     y: torch.Tensor
-    desc: _lib.Linear
+    desc: bytes     # a kge_linear
     saved: torch.Tensor | None
-    tensors: tuple  # what desc points to
+    tensors: tuple  # what desc points to: x, weight, bias, residual, step
 
 
 @dataclass
@@ -120,10 +121,8 @@ def _describe(x, weight, bias, act, drop, seed, step, residual, out_dtype):
         raise TypeError(f"out_dtype must be {x.dtype} or float32 (got {out_dtype})")
     if residual is not None:
         residual = _rows(residual, "residual", out_dtype, shape=(rows, out))
-    if (act or "none") not in _lib.ACTS:
-        raise ValueError(f"act must be one of {sorted(_lib.ACTS)} (got {act!r})")
     seed, step, word = _random(seed, step)
-    desc = _lib.Linear(_TYPES[x.dtype], _TYPES[out_dtype], _lib.ACTS[act or "none"], 0, rows, x.shape[1], out, _p(x), _row_stride(x),
+    desc = _lib.Linear(_TYPES[x.dtype], _TYPES[out_dtype], _act(act), 0, rows, x.shape[1], out, _p(x), _row_stride(x),
                        _p(weight), _row_stride(weight), _p(bias), _p(residual), _row_stride(residual) if residual is not None else 0,
                        _probability(drop), seed, step, _p(word))
     return desc, (x, weight, bias, residual, word), out_dtype
@@ -140,26 +139,44 @@ def _linear_call(desc, tensors, out_dtype, for_backward):
     return y, saved
 
 
+def _act(act) -> int:
+    code = _lib.ACTS.get(act or "none")
+    if code is None:
+        raise ValueError(f"act must be one of {sorted(_lib.ACTS)} (got {act!r})")
+    return code
+
+
 def linear(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, drop=0.0, seed=0, step=0) -> torch.Tensor:
     """``drop(act(x weight^T + bias)) + residual``: x [rows, in], weight [out, in], bias [out], residual [rows, out].
 
     act: "none", "relu", "gelu" or "silu"; drop, seed, step as in :func:`dropout`.  The output has x's type, or float32 by out_dtype (or
     because the residual is); 16-bit products are summed in fp32 and nothing is rounded before the end."""
+    y = _lib.host().linear(x, weight, bias, _act(act), residual, out_dtype, drop, seed, step, False)
+    if y is not None:
+        return y
     return _linear_call(*_describe(x, weight, bias, act, drop, seed, step, residual, out_dtype), False)[0]
 
 
 def linear_forward(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, drop=0.0, seed=0, step=0) -> LinearForward:
     """:func:`linear`, with what :func:`linear_backward` needs."""
+    got = _lib.host().linear(x, weight, bias, _act(act), residual, out_dtype, drop, seed, step, True)
+    if got is not None:
+        y, saved, desc = got
+        return LinearForward(y, desc, saved, (x, weight, bias, residual, None))
     desc, tensors, out_dtype = _describe(x, weight, bias, act, drop, seed, step, residual, out_dtype)
     y, saved = _linear_call(desc, tensors, out_dtype, True)
-    return LinearForward(y, desc, saved, tensors)
+    return LinearForward(y, bytes(desc), saved, tensors)
 
 
 def linear_backward(fw: LinearForward, dy, need_x: bool = True, need_weight: bool = True, need_bias: bool = True) -> LinearGrads:
     """Gradients of x, weight and bias from the gradient of y (of y's type)."""
     if not isinstance(fw, LinearForward):
         raise TypeError("fw must come from linear_forward()")
-    d, (x, weight, bias, _, _) = fw.desc, fw.tensors
+    x, _, bias = fw.tensors[:3]
+    got = _lib.host().linear_backward(fw.desc, x, fw.saved, dy, need_x, need_weight, need_bias and bias is not None)
+    if got is not None:
+        return LinearGrads(*got)
+    d = _lib.Linear.from_buffer_copy(fw.desc)
     dy = _rows(dy, "dy", fw.y.dtype, shape=fw.y.shape)
     dx = torch.empty((d.rows, d.in_), dtype=x.dtype, device=x.device) if need_x else None
     dw = torch.empty((d.out, d.in_), dtype=x.dtype, device=x.device) if need_weight else None
@@ -179,6 +196,10 @@ def dropout(x, p, seed, step=0, out=None) -> torch.Tensor:
     Which elements go is a function of (seed, step, row, column) alone, defined at kge_dropout in the C header; nothing is stored.  step: an
     integer, or one int64 on the GPU that the kernel reads (a captured graph then draws a new mask at every replay).  out: where to, x
     itself included."""
+    if out is None:
+        y = _lib.host().dropout(x, p, seed, step)
+        if y is not None:
+            return y
     x = _rows(x, "x")
     p = _probability(p)
     seed, step, word = _random(seed, step)
@@ -205,6 +226,12 @@ def preference_loss(pos, neg, ref_pos=None, ref_neg=None, *, beta=1.0, kind="sig
     ("sigmoid"), max(0, 1 - beta d) ("hinge") or (d - 1 / (2 beta))^2 ("square").  A row's pairs are averaged, evenly or by
     softmax(temperature sign neg) (a constant to the gradient), rows evenly.  mask [B, N] (bool or uint8): False where there is no pair; what the
     scores hold there is not looked at, and a row without a pair costs nothing.  Gradients and loss are float32."""
+    code = _lib.PREFERENCES.get(kind)
+    if code is None:
+        raise ValueError(f"kind must be one of {sorted(_lib.PREFERENCES)} (got {kind!r})")
+    got = _lib.host().preference_loss(pos, neg, ref_pos, ref_neg, mask, code, beta, sign, smoothing, temperature)
+    if got is not None:
+        return got
     neg = _rows(neg, "neg")
     B, N = neg.shape
     pos = _rows(pos, "pos", neg.dtype, ndim=1, shape=(B,))
@@ -216,9 +243,7 @@ def preference_loss(pos, neg, ref_pos=None, ref_neg=None, *, beta=1.0, kind="sig
         if isinstance(mask, torch.Tensor) and mask.dtype == torch.bool:
             mask = mask.view(torch.uint8)
         mask = _rows(mask, "mask", torch.uint8, shape=(B, N))
-    if kind not in _lib.PREFERENCES:
-        raise ValueError(f"kind must be one of {sorted(_lib.PREFERENCES)} (got {kind!r})")
-    desc = _lib.Preference(_TYPES[neg.dtype], _lib.PREFERENCES[kind], B, N, _p(pos), _p(neg), _row_stride(neg), _p(ref_pos), _p(ref_neg),
+    desc = _lib.Preference(_TYPES[neg.dtype], code, B, N, _p(pos), _p(neg), _row_stride(neg), _p(ref_pos), _p(ref_neg),
                            _row_stride(ref_neg) if ref_neg is not None else 0, _p(mask), _row_stride(mask) if mask is not None else 0,
                            float(beta), float(sign), float(smoothing), float(temperature))
     L = _lib.lib()
