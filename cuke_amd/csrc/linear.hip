@@ -8,50 +8,26 @@ namespace kge {
 // ---- operands as the matrix cores take them --------------------------------------------------------
 static int64_t up8(int64_t n) { return (n + 7) & ~int64_t(7); }
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+static size_t packed_bytes(int type, int64_t rows, int64_t width) { return up256((size_t)rows * up8(width) * type_bytes(type)); }
 
-static int planes_of(int type) { return type == KGE_F32 ? 3 : 1; }
-static size_t packed_bytes(int type, int64_t rows, int64_t width) { return up256((size_t)planes_of(type) * rows * up8(width) * 2); }
+// Whether an array can be read as it lies: fp32 always, 16 bits where rows start on 16 bytes and are whole chunks of 8 elements.
+static bool lies_ready(int type, const void *p, int64_t stride, int64_t width) { return type == KGE_F32 || (aligned16(p) && stride % 8 == 0 && width % 8 == 0); }
 
-// Whether an array can be read as it lies: 16 bits, rows that start on 16 bytes and are whole chunks of 8 elements.
-static bool lies_ready(int type, const void *p, int64_t stride, int64_t width) { return type != KGE_F32 && aligned16(p) && stride % 8 == 0 && width % 8 == 0; }
-
-// v = parts[0] + parts[1] + parts[2] exactly (down to 2^-108), also where v is infinite, is NaN or would round to infinity.
-__device__ __forceinline__ void split_value(float v, bf16_t (&part)[3])
+// Rows of 16-bit elements copied to whole chunks, zeros behind their end.  One pass at memory speed.
+__global__ __launch_bounds__(256) void pack_kernel(const uint16_t *src, int64_t stride, int64_t rows, int64_t width, int64_t width8, uint16_t *dst)
 {
-    bf16_t a = (bf16_t)v;
-    if (__builtin_isinf((float)a)) a = __builtin_bit_cast(bf16_t, (uint16_t)(__builtin_bit_cast(uint32_t, v) >> 16));
-    const float r = (float)a == v ? 0.0f : v - (float)a;
-    const bf16_t b = (bf16_t)r;
-    part[0] = a, part[1] = b, part[2] = (bf16_t)(r - (float)b);
-}
-
-template <class T>
-using StoredAs = typename std::conditional<sizeof(T) == 4, bf16_t, T>::type;
-
-// four elements of a packed row (8-byte aligned), in one plane or in three
-template <class T>
-__device__ __forceinline__ void store_packed(StoredAs<T> *p, int64_t plane, float4 v)
-{
-    typedef StoredAs<T> quad __attribute__((ext_vector_type(4)));
-    if constexpr (sizeof(T) == 4) {
-        bf16_t x[3], y[3], z[3], w[3];
-        split_value(v.x, x), split_value(v.y, y), split_value(v.z, z), split_value(v.w, w);
-#pragma unroll
-        for (int k = 0; k < 3; ++k) *reinterpret_cast<quad *>(p + k * plane) = quad{x[k], y[k], z[k], w[k]};
-    } else {
-        *reinterpret_cast<quad *>(p) = quad{(T)v.x, (T)v.y, (T)v.z, (T)v.w};
-    }
-}
-
-// Rows copied to whole chunks, zeros behind their end; fp32 as three planes.  One pass at memory speed (fp32: 4 bytes in, 6 out an element).
-template <class T>
-__global__ __launch_bounds__(256) void pack_kernel(const T *src, int64_t stride, int64_t rows, int64_t width, int64_t width8, StoredAs<T> *dst)
-{
-    const int64_t quads = width8 / 4, total = rows * quads;
+    typedef uint16_t chunk __attribute__((ext_vector_type(8)));
+    const int64_t chunks = width8 / 8, total = rows * chunks;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / quads, col = 4 * (i % quads);
-        const int64_t left = width - col;
-        store_packed<T>(dst + row * width8 + col, rows * width8, load4(src + row * stride + col, (int)(left < 4 ? left : 4)));
+        const int64_t row = i / chunks, col = 8 * (i % chunks), left = width - col;
+        chunk v;
+        if (left >= 8) {
+            v = Pack<uint16_t, 8>::load(src + row * stride + col).v;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = e < left ? src[row * stride + col + e] : (uint16_t)0;
+        }
+        *reinterpret_cast<chunk *>(dst + row * width8 + col) = v;
     }
 }
 
@@ -65,7 +41,7 @@ struct GradArgs {
     const void *slope;  // [rows][4 quads] or NULL
     int64_t rows, cols, quads, rows_each;
     Drop drop;
-    void *dz;  // [rows][width8], planes rows * width8 apart; or NULL
+    void *dz;  // [rows][width8] or NULL
     int64_t width8;
     float *sums;  // [gridDim.y][4 quads] or NULL
     int lanes;
@@ -111,15 +87,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(GradArgs g)
                     g.drop.apply(v[r], Drop::word(base, place));
                     g.drop.apply(v[r] + 4, Drop::word(base, place + 0x9E3779B97F4A7C15ull));
                 }
-                if (g.dz) {
-                    StoredAs<T> *to = static_cast<StoredAs<T> *>(g.dz) + row * g.width8 + col;
-                    if constexpr (sizeof(T) == 4) {
-                        store_packed<T>(to, g.rows * g.width8, make_float4(v[r][0], v[r][1], v[r][2], v[r][3]));
-                        store_packed<T>(to + 4, g.rows * g.width8, make_float4(v[r][4], v[r][5], v[r][6], v[r][7]));
-                    } else {
-                        store8(to, v[r], 8);
-                    }
-                }
+                if (g.dz) store8(static_cast<T *>(g.dz) + row * g.width8 + col, v[r], 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) sum[e] += v[r][e];
             }
@@ -188,43 +156,84 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 }
 
 // ---- products --------------------------------------------------------------------------------------
-template <class E, int PLANES, bool AA, bool BA, int XA, int XB, int K, int WA, int WB, int STAGES, EndKind END>
-static void launch_sized(TileArgs &t, hipStream_t st)
+// 16 bits: larger tiles read less and multiply faster, smaller ones fill the card where there are few, and several to a CU hide each other's
+// epilogues.  Forward of 32768 x 2048 x 2048 bf16 with gelu and drop: 256 x 256 322 us, 128 x 128 368, 64 x 64 468; of 4096 x 1024 x 512: 43.6, 18.9
+// and 11.8.  Columns by rows 64 x 128 take 65536 x 512 -> 400 with an fp32 residual in 76 us (256 x 256: 97), 32768 x 1024 -> 1024 plainly in 101
+// (77).  fp32: 128 x 128, or 64 x 64.
+using Large = Shape<256, 256, 32, 2, 4, 4>;
+using Middle = Shape<128, 128, 64, 2, 2, 2>;
+using Tall = Shape<64, 128, 64, 2, 2, 2>;
+using Small = Shape<64, 64, 64, 2, 2, 2>;
+using MiddleF = Shape<128, 128, 32, 2, 4, 2>;
+using SmallF = Shape<64, 64, 32, 2, 2, 2>;
+
+static int64_t tiles_of(int64_t a, int64_t b, int x) { return ceil_div(a, x) * ceil_div(b, x); }
+
+template <class T, class S>
+static void launch_forward(TileArgs &t, hipStream_t st)
 {
-    t.tiles_a = (int)ceil_div(t.a.extent, XA), t.tiles_b = (int)ceil_div(t.b.extent, XB);
-    const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b * t.splits;
-    if (blocks == 0) return;
-    hipLaunchKernelGGL((linear_tile_kernel<E, PLANES, AA, BA, XA, XB, K, WA, WB, STAGES, END>), dim3((unsigned)blocks), dim3(WA * WB * kWave), 0, st, t);
+    t.tiles_a = (int)ceil_div(t.a.extent, S::XA), t.tiles_b = (int)ceil_div(t.b.extent, S::XB);
+    const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b;
+    if (blocks) hipLaunchKernelGGL((linear_forward_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
-// Larger tiles read less and multiply faster (dx of 32768 x 2048 x 2048 bf16: 256 x 256 237 us, 128 x 128 297, 64 x 64 425), smaller ones
-// fill the card where there are few (forward of 4096 x 1024 x 512: 43.6, 18.9 and 11.8 us): the largest of which there are 256.
-template <class E, int PLANES, bool AA, bool BA, EndKind END>
-static void launch_tiles(TileArgs &t, hipStream_t st)
+template <class T>
+static void launch_forward(TileArgs &t, hipStream_t st)
 {
-    auto tiles = [&](int x) { return ceil_div(t.a.extent, x) * ceil_div(t.b.extent, x) * t.splits; };
-    if constexpr (PLANES == 3) {
-        if (tiles(128) >= 200) launch_sized<E, PLANES, AA, BA, 128, 128, 32, 2, 4, 3, END>(t, st);
-        else launch_sized<E, PLANES, AA, BA, 64, 64, 32, 2, 2, 3, END>(t, st);
+    const int64_t a = t.a.extent, b = t.b.extent;
+    if constexpr (sizeof(T) == 4) {
+        if (tiles_of(a, b, 128) >= 200) launch_forward<T, MiddleF>(t, st);
+        else launch_forward<T, SmallF>(t, st);
     } else {
-        if (tiles(256) >= 256) launch_sized<E, PLANES, AA, BA, 256, 256, 32, 2, 4, 4, END>(t, st);
-        else if (tiles(128) >= 256) launch_sized<E, PLANES, AA, BA, 128, 128, 32, 2, 2, 4, END>(t, st);
-        else launch_sized<E, PLANES, AA, BA, 64, 64, 64, 2, 2, 2, END>(t, st);
+        // bytes that the epilogue moves an element, beside the sum's length
+        const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 2 : 0);
+        if (tiles_of(a, b, 128) >= 256 && 128 * moved >= t.k) launch_forward<T, Tall>(t, st);
+        else if (tiles_of(a, b, 256) >= 256) launch_forward<T, Large>(t, st);
+        else if (tiles_of(a, b, 128) >= 256) launch_forward<T, Middle>(t, st);
+        else launch_forward<T, Small>(t, st);
     }
 }
 
-// Parts of a sum over k where the tiles of an a x b output alone would leave most of the card idle: as many as make 256 large tiles, or 512 of the
-// middle ones, none shorter than 256 terms (their join costs 4 bytes written and read an element and part).
-static int splits_of(int64_t a, int64_t b, int64_t k)
+// The tiles of a backward pass and the parts that dW's sums over rows are split into.  Both products share a launch and `slots` workgroups run at
+// once: dW is split until its sums are no longer than a slot's share of the work (none shorter than 256 terms; a part costs 4 bytes written and
+// read an element).
+struct GradPlan {
+    int tile, dw_splits;  // tile: 256, 128 or 64
+};
+static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
 {
-    const int64_t large = ceil_div(a, 256) * ceil_div(b, 256), middle = ceil_div(a, 128) * ceil_div(b, 128);
-    if (large == 0) return 1;
-    int64_t s = ceil_div(256, large);
-    if (s * 512 > k) s = 512 / middle;  // (parts for large tiles would be short)
-    const int64_t most = k / 256;
-    s = s < most ? s : most;
-    return (int)(s > 1 ? s : 1);
+    auto at_most = [&](int x) { return tiles_of(rows, in, x) + tiles_of(out, in, x) * (rows >= 512 ? rows / 512 : 1); };
+    GradPlan p;
+    if (type == KGE_F32) p.tile = at_most(128) >= 320 ? 128 : 64;
+    else p.tile = at_most(256) >= 384 ? 256 : (at_most(128) >= 320 ? 128 : 64);
+    const int64_t slots = p.tile == 256 ? 256 : (p.tile == 128 ? (type == KGE_F32 ? 256 : 512) : 1024);
+    const int64_t share = (tiles_of(rows, in, p.tile) * out + tiles_of(out, in, p.tile) * rows) / slots;
+    p.dw_splits = (int)ceil_div(rows, share > 256 ? share : 256);
+    if (p.dw_splits < 1) p.dw_splits = 1;
+    return p;
 }
+
+template <class T, class S>
+static void launch_grads(TileArgs &dw, TileArgs &dx, bool want_dw, bool want_dx, hipStream_t st)
+{
+    for (TileArgs *t : {&dw, &dx}) t->tiles_a = (int)ceil_div(t->a.extent, S::XA), t->tiles_b = (int)ceil_div(t->b.extent, S::XB);
+    const int64_t nw = want_dw ? (int64_t)dw.tiles_a * dw.tiles_b * dw.splits : 0, nx = want_dx ? (int64_t)dx.tiles_a * dx.tiles_b : 0;
+    if (nw + nx) hipLaunchKernelGGL((linear_grads_kernel<T, S>), dim3((unsigned)(nw + nx)), dim3(S::kThreads), 0, st, dw, dx, nw);
+}
+
+template <class T>
+static void launch_grads(int tile, TileArgs &dw, TileArgs &dx, bool want_dw, bool want_dx, hipStream_t st)
+{
+    if constexpr (sizeof(T) == 4) {
+        if (tile == 128) launch_grads<T, MiddleF>(dw, dx, want_dw, want_dx, st);
+        else launch_grads<T, SmallF>(dw, dx, want_dw, want_dx, st);
+    } else {
+        if (tile == 256) launch_grads<T, Large>(dw, dx, want_dw, want_dx, st);
+        else if (tile == 128) launch_grads<T, Middle>(dw, dx, want_dw, want_dx, st);
+        else launch_grads<T, Small>(dw, dx, want_dw, want_dx, st);
+    }
+}
+
 static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), 64) * 64; }
 
 // ---- a layer's plan --------------------------------------------------------------------------------
@@ -234,7 +243,7 @@ struct Plan {
     int64_t quads;
     int sum_blocks;      // ranges of rows the bias's gradient is summed over
     int64_t sum_rows;
-    int dw_splits;
+    GradPlan grads;
 };
 
 static Plan plan_of(const kge_linear *l)
@@ -246,12 +255,12 @@ static Plan plan_of(const kge_linear *l)
     p.slope = l->act == KGE_ACT_NONE ? 0 : up256((size_t)l->rows * p.quads * 4 * type_bytes(l->type));
     p.x = p.pack_x ? packed_bytes(l->type, l->rows, l->in) : 0;
     p.w = p.pack_w ? packed_bytes(l->type, l->out, l->in) : 0;
-    // ranges of at least 16 rows, about 1024 workgroups in all
+    // ranges of at least 8 rows, about 1024 workgroups in all
     const int64_t across = ceil_div(up8(l->out), 512), want = across > 0 && across < 1024 ? 1024 / across : 1;
     p.sum_rows = ceil_div(l->rows, want);
-    if (p.sum_rows < 16) p.sum_rows = 16;
+    if (p.sum_rows < 8) p.sum_rows = 8;
     p.sum_blocks = (int)ceil_div(l->rows, p.sum_rows);
-    p.dw_splits = splits_of(l->in, l->out, l->rows);
+    p.grads = grad_plan(l->type, l->rows, l->in, l->out);
     return p;
 }
 
@@ -277,35 +286,32 @@ static int grid_for(int64_t items)
     return (int)(b < 8192 ? b : 8192);
 }
 
-template <class T>
 static void launch_pack(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst, hipStream_t st)
 {
     if (rows == 0 || width == 0) return;
-    hipLaunchKernelGGL(pack_kernel<T>, dim3(grid_for(rows * up8(width) / 4)), dim3(256), 0, st, static_cast<const T *>(src), stride, rows, width,
-                       up8(width), static_cast<StoredAs<T> *>(dst));
+    hipLaunchKernelGGL(pack_kernel, dim3(grid_for(rows * up8(width) / 8)), dim3(256), 0, st, static_cast<const uint16_t *>(src), stride, rows, width,
+                       up8(width), static_cast<uint16_t *>(dst));
 }
 
 // an operand where it lies, or its packed copy
-static Side side_of(const void *p, int64_t stride, bool packed, const void *copy, int64_t rows, int64_t width, int64_t extent)
+static Side side_of(const void *p, int64_t stride, bool packed, const void *copy, int64_t width, int64_t extent)
 {
-    if (packed) return Side{copy, up8(width), rows * up8(width), extent};
-    return Side{p, stride, 0, extent};
+    if (packed) return Side{copy, up8(width), extent};
+    return Side{p, stride, extent};
 }
 
 template <class T>
 static int forward(const kge_linear *l, const Plan &p, void *y, int64_t y_stride, char *slope, char *px, char *pw, hipStream_t st)
 {
-    using E = StoredAs<T>;
-    constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
-    if (p.pack_x) launch_pack<T>(l->x, l->x_stride, l->rows, l->in, px, st);
-    if (p.pack_w) launch_pack<T>(l->weight, l->weight_stride, l->out, l->in, pw, st);
+    if (p.pack_x) launch_pack(l->x, l->x_stride, l->rows, l->in, px, st);
+    if (p.pack_w) launch_pack(l->weight, l->weight_stride, l->out, l->in, pw, st);
     TileArgs t{};
-    t.a = side_of(l->weight, l->weight_stride, p.pack_w, pw, l->out, l->in, l->out);
-    t.b = side_of(l->x, l->x_stride, p.pack_x, px, l->rows, l->in, l->rows);
+    t.a = side_of(l->weight, l->weight_stride, p.pack_w, pw, l->in, l->out);
+    t.b = side_of(l->x, l->x_stride, p.pack_x, px, l->in, l->rows);
     t.k = l->in, t.splits = 1, t.k_each = split_length(l->in, 1);
     t.e = Ends{y, y_stride, l->bias, l->residual, l->residual_stride, slope, l->rows, l->out, p.quads,
                make_drop(l->p, l->seed, l->step, l->step_dev, l->out), l->act, l->out_type == KGE_F32};
-    launch_tiles<E, kPlanes, false, false, kEndLayer>(t, st);
+    launch_forward<T>(t, st);
     KGE_CHECK_LAUNCH();
     return KGE_OK;
 }
@@ -314,8 +320,6 @@ template <class T>
 static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t dy_stride, const char *saved, void *dx, void *dw, void *db,
                     char *ws, hipStream_t st)
 {
-    using E = StoredAs<T>;
-    constexpr int kPlanes = sizeof(T) == 4 ? 3 : 1;
     const int64_t width8 = up8(l->out);
     const bool ready = l->act == KGE_ACT_NONE && nearbyint(l->p * 65536.0) == 0.0 && l->out_type == l->type && lies_ready(l->type, dy, dy_stride, l->out);
     char *dz = ws;
@@ -330,30 +334,22 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
         if (l->out_type == KGE_F32) hipLaunchKernelGGL((linear_dz_kernel<T, float>), grid, dim3(256), 0, st, g);
         else hipLaunchKernelGGL((linear_dz_kernel<T, T>), grid, dim3(256), 0, st, g);
     }
-    const Side gz = side_of(dy, dy_stride, !ready, dz, l->rows, l->out, 0);
-    if (dx) {
-        TileArgs t{};
-        t.a = side_of(l->weight, l->weight_stride, p.pack_w, saved + p.slope + p.x, l->out, l->in, l->in);
-        t.b = gz, t.b.extent = l->rows;
-        t.k = l->out, t.splits = 1, t.k_each = split_length(l->out, 1);
-        t.e.y = dx, t.e.y_stride = l->in, t.e.rows = l->rows, t.e.cols = l->in, t.e.quads = ceil_div(l->in, 4);
-        launch_tiles<E, kPlanes, true, false, kEndStore>(t, st);
-    }
+    const int64_t in_quads = ceil_div(l->in, 4);
+    TileArgs tx{}, tw{};
+    tx.a = side_of(l->weight, l->weight_stride, p.pack_w, saved + p.slope + p.x, l->in, l->in);
+    tx.b = side_of(dy, dy_stride, !ready, dz, l->out, l->rows);
+    tx.k = l->out, tx.splits = 1, tx.k_each = split_length(l->out, 1);
+    tx.e.y = dx, tx.e.y_stride = l->in, tx.e.rows = l->rows, tx.e.cols = l->in, tx.e.quads = in_quads;
+    tw.a = side_of(l->x, l->x_stride, p.pack_x, saved + p.slope, l->in, l->in);
+    tw.b = tx.b, tw.b.extent = l->out;
+    tw.k = l->rows, tw.splits = p.grads.dw_splits, tw.k_each = split_length(l->rows, tw.splits);
+    tw.partial = tw.splits > 1 ? part : nullptr;
+    tw.e.y = dw, tw.e.y_stride = l->in, tw.e.rows = l->out, tw.e.cols = l->in, tw.e.quads = in_quads;
+    launch_grads<T>(p.grads.tile, tw, tx, dw != nullptr, dx != nullptr, st);
     JoinArgs j{};
-    if (dw) {
-        TileArgs t{};
-        t.a = side_of(l->x, l->x_stride, p.pack_x, saved + p.slope, l->rows, l->in, l->in);
-        t.b = gz, t.b.extent = l->out;
-        t.k = l->rows, t.splits = p.dw_splits, t.k_each = split_length(l->rows, t.splits);
-        t.partial = part;
-        t.e.y = dw, t.e.y_stride = l->in, t.e.rows = l->out, t.e.cols = l->in, t.e.quads = ceil_div(l->in, 4);
-        if (t.splits == 1) {
-            launch_tiles<E, kPlanes, true, true, kEndStore>(t, st);
-        } else {
-            launch_tiles<E, kPlanes, true, true, kEndPartial>(t, st);
-            j.part[0] = part, j.rows = l->out, j.cols[0] = l->in, j.quads[0] = t.e.quads, j.n[0] = t.splits, j.out[0] = dw;
-            j.blocks0 = ceil_div(j.rows * j.quads[0], 256);
-        }
+    if (dw && tw.partial) {
+        j.part[0] = part, j.rows = l->out, j.cols[0] = l->in, j.quads[0] = in_quads, j.n[0] = tw.splits, j.out[0] = dw;
+        j.blocks0 = ceil_div(j.rows * j.quads[0], 256);
     }
     if (db) j.part[1] = sums, j.cols[1] = l->out, j.quads[1] = p.quads, j.n[1] = p.sum_blocks, j.out[1] = db;
     const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 16) : 0);
@@ -407,7 +403,7 @@ size_t kge_linear_bwd_workspace(const kge_linear *lin)
     if (check(lin)) return 0;
     const Plan p = plan_of(lin);
     return packed_bytes(lin->type, lin->rows, lin->out) + up256((size_t)p.sum_blocks * p.quads * 16) +
-           (p.dw_splits > 1 ? (size_t)p.dw_splits * lin->out * ceil_div(lin->in, 4) * 16 : 0);
+           (p.grads.dw_splits > 1 ? (size_t)p.grads.dw_splits * lin->out * ceil_div(lin->in, 4) * 16 : 0);
 }
 
 int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx, void *dweight,

@@ -2,8 +2,9 @@
 //
 // Each side lies in memory in one of two ways: ALONG rows (row = its index, the sum runs inside the row) or ACROSS them (the sum runs
 // over rows, the index inside).  y = x W^T has both sides along, dx = dz W one across, dW = dz^T x both: no operand is ever transposed in
-// memory.  Tiles go to LDS 16 bytes a lane without passing through registers; a tile that lies across is turned by the transposing LDS
-// reads on its way to the matrix cores.  fp32 sides come as three bf16 planes (mfma_split.hpp), of whose nine products six are formed.
+// memory.  A tile that lies across is turned by the transposing LDS reads on its way to the matrix cores.  16-bit tiles go to LDS 16 bytes a lane
+// without passing through registers; fp32 ones are taken through registers, where every value becomes three bf16 parts (mfma_split.hpp), of
+// whose nine products six are formed.
 #pragma once
 
 #include "features.hpp"
@@ -32,17 +33,13 @@ struct Mfma<half_t> {
     }
 };
 
-// One side of a product.  Rows start 16-byte aligned and a multiple of 8 elements apart; elements between the last one and the next
-// multiple of 8 belong to the row and, where the sum runs inside it, are zero.
+// One side of a product.  16 bits: rows start 16-byte aligned and a multiple of 8 elements apart; elements between the last one and the next
+// multiple of 8 belong to the row and, where the sum runs inside it, are zero.  fp32: rows as they lie.
 struct Side {
     const void *p;
     int64_t stride;  // elements between rows
-    int64_t plane;   // elements between the planes of an fp32 side
     int64_t extent;  // indices
 };
-
-// Where sums go: through the epilogue of the layer, rounded to the layer's type, or as fp32 partial sums of a split.
-enum EndKind { kEndLayer, kEndStore, kEndPartial };
 
 struct Ends {
     void *y;
@@ -62,7 +59,7 @@ struct TileArgs {
     int64_t k;      // terms of every sum
     int64_t k_each; // per split, a multiple of 64
     int tiles_a, tiles_b, splits;
-    float *partial; // [splits][rows][quads * 4]
+    float *partial; // where a sum is split: [splits][rows][quads * 4] in fp32, to be joined; else NULL
     Ends e;
 };
 
@@ -96,9 +93,9 @@ struct Tile {
         int64_t step[kRounds];
         int term[kRounds];  // of the chunk, within the tile
 
-        __device__ __forceinline__ void start(const Side &s, int plane, int64_t first, int64_t k)
+        __device__ __forceinline__ void start(const Side &s, int64_t first, int64_t k)
         {
-            const E *p = static_cast<const E *>(s.p) + plane * s.plane;
+            const E *p = static_cast<const E *>(s.p);
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
                 const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
@@ -122,6 +119,58 @@ struct Tile {
         }
     };
 
+    // The same of an fp32 side: a chunk's eight values wait in registers while the tile before is multiplied, then go to LDS as parts.
+    struct FloatFeed {
+        const float *from[kRounds];
+        int64_t step;
+        int term[kRounds], there[kRounds];  // there: of a chunk's indices (across; along: whether its row exists)
+        float held[kRounds][8];
+
+        __device__ __forceinline__ void start(const Side &s, int64_t first, int64_t k)
+        {
+            const float *p = static_cast<const float *>(s.p);
+            step = ACROSS ? K * s.stride : K;
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
+                const int64_t index = first + (ACROSS ? 8 * j : row), rest = s.extent - index;
+                term[r] = ACROSS ? row : 8 * j;
+                there[r] = (int)(rest < 8 ? rest : 8);
+                from[r] = p + (ACROSS ? (k + row) * s.stride + index : index * s.stride + k + 8 * j);
+            }
+        }
+        __device__ __forceinline__ void fetch(int64_t left)
+        {
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int64_t rest = left - term[r];
+                const int valid = ACROSS ? (rest > 0 ? there[r] : 0) : (there[r] > 0 ? (int)(rest < 8 ? rest : 8) : 0);
+                load8(from[r], valid, held[r]);
+                from[r] += step;
+            }
+        }
+        __device__ __forceinline__ void put(char *lds, int plane_bytes)
+        {
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                // (an infinite value, or one that rounds to infinity, and NaN make NaN of the second part and so of every sum they enter, which is
+                // then formed again)
+                bf16x4 lo[kSplitParts], hi[kSplitParts];
+                bf16x8 part[kSplitParts];
+                // (The compiler has been seen to let the parts overwrite the values they are still to be taken from, where both are tuples of
+                // registers: each value passes through a register of its own.)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) asm("" : "+v"(held[r][e]));
+                split_quad(make_float4(held[r][0], held[r][1], held[r][2], held[r][3]), lo);
+                split_quad(make_float4(held[r][4], held[r][5], held[r][6], held[r][7]), hi);
+#pragma unroll
+                for (int k = 0; k < kSplitParts; ++k) part[k] = __builtin_shufflevector(lo[k], hi[k], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                for (int k = 0; k < kSplitParts; ++k) *reinterpret_cast<bf16x8 *>(lds + k * plane_bytes + 16 * (r * THREADS + (int)threadIdx.x)) = part[k];
+            }
+        }
+    };
+
     // eight terms of an index for each lane: index at + lane % 32, terms 16 step + 8 (lane / 32) .. + 7
     __device__ __forceinline__ static s16x8 read(const char *lds, int at, int step, int lane)
     {
@@ -138,18 +187,15 @@ struct Tile {
     }
 };
 
-// The sums of four (`valid`) output elements of a row by fp32 instructions, from the planes (which add up to the value, infinities and NaNs
-// included).  Not for speed: it runs where a sum is not finite.
+// The sums of four (`valid`) output elements of a row by fp32 instructions, for fp32 sides.  Not for speed: it runs where a sum is not finite.
 template <bool A_ACROSS, bool B_ACROSS>
 __device__ __noinline__ float4 plain_sums(Side a, Side b, int64_t n, int valid, int64_t m, int64_t k0, int64_t k1)
 {
-    const bf16_t *pa = static_cast<const bf16_t *>(a.p), *pb = static_cast<const bf16_t *>(b.p);
+    const float *pa = static_cast<const float *>(a.p), *pb = static_cast<const float *>(b.p);
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int v = 0; v < valid; ++v)
-        for (int64_t k = k0; k < k1; ++k) {
-            const bf16_t *x = pa + (A_ACROSS ? k * a.stride + n + v : (n + v) * a.stride + k), *y = pb + (B_ACROSS ? k * b.stride + m : m * b.stride + k);
-            s[v] = fmaf((float)x[0] + (float)x[a.plane] + (float)x[2 * a.plane], (float)y[0] + (float)y[b.plane] + (float)y[2 * b.plane], s[v]);
-        }
+        for (int64_t k = k0; k < k1; ++k)
+            s[v] = fmaf(pa[A_ACROSS ? k * a.stride + n + v : (n + v) * a.stride + k], pb[B_ACROSS ? k * b.stride + m : m * b.stride + k], s[v]);
     return make_float4(s[0], s[1], s[2], s[3]);
 }
 
@@ -212,7 +258,7 @@ __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64
     }
 }
 
-// Workgroups are dealt to the eight XCDs in turn; consecutive tiles go to one XCD, whose L2 then holds the rows and columns they share:
+// Workgroups are dealt to the eight XCDs in turn (wherever the count starts); consecutive tiles go to one XCD, whose L2 then holds the rows and columns they share:
 // eight rows of tiles at a time, walked column by column.
 __device__ __forceinline__ void tile_of(int64_t block, int64_t blocks, const TileArgs &t, int *ta, int *tb, int *split)
 {
@@ -225,8 +271,8 @@ __device__ __forceinline__ void tile_of(int64_t block, int64_t blocks, const Til
     *tb = (int)(first + q % band % wide), *ta = (int)(q % band / wide);
 }
 
-// A wave's own loads have landed but for the last `out` (LDS reads all have), and every wave's have: what the stage in turn holds may be
-// read, and the stage read last may be written.
+// A wave's own loads have landed but for the last `out` (LDS reads and writes all have), and every wave's have: what the stage in turn holds
+// may be read, and the stage read last may be written.
 template <int OUT>
 __device__ __forceinline__ void stage_ready()
 {
@@ -235,45 +281,48 @@ __device__ __forceinline__ void stage_ready()
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
-
-// E: what the matrix cores multiply, PLANES: 3 for fp32.  A workgroup of WA x WB waves computes XA columns by XB rows.  STAGES tiles of K terms
-// are in LDS, in arrays of their own (so that the compiler sees that the one being read is none of those being written): STAGES - 1 are
-// requested ahead, and one barrier a tile both publishes the next and frees the last.
-template <class E, int PLANES, bool A_ACROSS, bool B_ACROSS, int XA, int XB, int K, int WA, int WB, int STAGES, EndKind END>
-__global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
+__device__ __forceinline__ void lds_ready()
 {
-    using T = typename std::conditional<PLANES == 3, float, E>::type;
-    constexpr int kThreads = WA * WB * kWave;
-    using A = Tile<XA, K, A_ACROSS, kThreads>;
-    using B = Tile<XB, K, B_ACROSS, kThreads>;
-    constexpr int kBytesA = XA * K * 2, kBytesB = XB * K * 2, kStage = PLANES * (kBytesA + kBytesB);
-    constexpr int kLoads = PLANES * (A::kRounds + B::kRounds);  // per thread and tile
-    constexpr int FA = XA / WA / 32, FB = XB / WB / 32;
-    static_assert(STAGES >= 2 && STAGES <= 4, "stages");
-    __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[STAGES > 2 ? kStage : 16], stage3[STAGES > 3 ? kStage : 16];
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 7 << 4);  // lgkmcnt(0): loads to registers stay in flight
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A workgroup of WA x WB waves computes XA columns by XB rows, K terms at a time.  16 bits: STAGES tiles are in LDS, in arrays of their own (so
+// that the compiler sees that the one being read is none of those being written); STAGES - 1 are requested ahead, and one barrier a tile both
+// publishes the next and frees the last.  fp32: two stages, a third tile in registers.
+template <int XA_, int XB_, int K_, int WA_, int WB_, int STAGES_>
+struct Shape {
+    static constexpr int XA = XA_, XB = XB_, K = K_, WA = WA_, WB = WB_, STAGES = STAGES_, kThreads = WA * WB * kWave;
+};
+template <class T, class S>
+constexpr int stage_bytes() { return (S::XA + S::XB) * S::K * 2 * (sizeof(T) == 4 ? kSplitParts : 1); }
+
+// T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.
+template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER>
+__device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, int64_t blocks, char *stage0, char *stage1, char *stage2, char *stage3)
+{
+    constexpr bool kFloat = sizeof(T) == 4;
+    using E = typename std::conditional<kFloat, bf16_t, T>::type;
+    constexpr int PLANES = kFloat ? kSplitParts : 1, K = S::K, STAGES = S::STAGES, WA = S::WA, WB = S::WB;
+    using A = Tile<S::XA, K, A_ACROSS, S::kThreads>;
+    using B = Tile<S::XB, K, B_ACROSS, S::kThreads>;
+    constexpr int kBytesA = S::XA * K * 2, kBytesB = S::XB * K * 2, kStage = stage_bytes<T, S>();
+    constexpr int FA = S::XA / WA / 32, FB = S::XB / WB / 32;
+    static_assert(STAGES >= 2 && STAGES <= 4 && (!kFloat || STAGES == 2), "stages");
 
     int ta, tb, split;
-    tile_of(blockIdx.x, gridDim.x, t, &ta, &tb, &split);
-    const int64_t n0 = (int64_t)ta * XA, m0 = (int64_t)tb * XB;
+    tile_of(block, blocks, t, &ta, &tb, &split);
+    const int64_t n0 = (int64_t)ta * S::XA, m0 = (int64_t)tb * S::XB;
     const int64_t k0 = split * t.k_each, k1 = k0 + t.k_each < t.k ? k0 + t.k_each : t.k;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wa = (wave % WA) * (XA / WA), wb = (wave / WA) * (XB / WB);
+    const int wa = (wave % WA) * (S::XA / WA), wb = (wave / WA) * (S::XB / WB);
 
-    floatx16 acc[FA][FB] = {}, low[PLANES == 3 ? FA : 1][PLANES == 3 ? FB : 1] = {};
-
-    typename A::template Feed<E> feed_a[PLANES];
-    typename B::template Feed<E> feed_b[PLANES];
-#pragma unroll
-    for (int p = 0; p < PLANES; ++p) feed_a[p].start(t.a, p, n0, k0), feed_b[p].start(t.b, p, m0, k0);
+    floatx16 acc[FA][FB] = {}, low[kFloat ? FA : 1][kFloat ? FB : 1] = {};
     int64_t left = k1 - k0;  // terms not requested yet
-    auto load = [&](char *lds) {
-#pragma unroll
-        for (int p = 0; p < PLANES; ++p) {
-            feed_a[p].load(left, lds + p * kBytesA);
-            feed_b[p].load(left, lds + PLANES * kBytesA + p * kBytesB);
-        }
-        left -= K;
-    };
+    const int tiles = left > 0 ? (int)((left + K - 1) / K) : 0;
+    auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
     auto multiply = [&](const char *lds) {
 #pragma unroll
         for (int step = 0; step < K / 16; ++step) {
@@ -289,7 +338,7 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
             for (int i = 0; i < FA; ++i)
 #pragma unroll
                 for (int j = 0; j < FB; ++j) {
-                    if constexpr (PLANES == 1) {
+                    if constexpr (!kFloat) {
                         acc[i][j] = Mfma<E>::go(a[i][0], b[j][0], acc[i][j]);
                     } else {
 #pragma unroll
@@ -299,26 +348,48 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
                 }
         }
     };
-    auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
-
-    // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
-    const int tiles = (int)((k1 - k0 + K - 1) / K);
+    if constexpr (kFloat) {
+        typename A::FloatFeed feed_a;
+        typename B::FloatFeed feed_b;
+        feed_a.start(t.a, n0, k0), feed_b.start(t.b, m0, k0);
+        auto fetch = [&] { feed_a.fetch(left), feed_b.fetch(left), left -= K; };
+        auto put = [&](char *lds) { feed_a.put(lds, kBytesA), feed_b.put(lds + PLANES * kBytesA, kBytesB); };
+        fetch();
+        put(stage0);
+        fetch();
+        for (int at = 0; at < tiles; at += 2)
 #pragma unroll
-    for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
-    int at = 0;
-    for (; at + STAGES <= tiles; at += STAGES)
+            for (int u = 0; u < 2; ++u) {
+                if (at + u >= tiles) break;
+                lds_ready();
+                put(stage(1 - u));
+                fetch();
+                multiply(stage(u));
+            }
+    } else {
+        typename A::template Feed<E> feed_a;
+        typename B::template Feed<E> feed_b;
+        constexpr int kLoads = A::kRounds + B::kRounds;  // per thread and tile
+        feed_a.start(t.a, n0, k0), feed_b.start(t.b, m0, k0);
+        auto load = [&](char *lds) { feed_a.load(left, lds), feed_b.load(left, lds + kBytesA), left -= K; };
+        // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
 #pragma unroll
-        for (int u = 0; u < STAGES; ++u) {
+        for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
+        int at = 0;
+        for (; at + STAGES <= tiles; at += STAGES)
+#pragma unroll
+            for (int u = 0; u < STAGES; ++u) {
+                stage_ready<kLoads * (STAGES - 2)>();
+                load(stage((u + STAGES - 1) % STAGES));
+                multiply(stage(u));
+            }
+#pragma unroll
+        for (int u = 0; u < STAGES - 1; ++u) {
+            if (at + u >= tiles) break;
             stage_ready<kLoads * (STAGES - 2)>();
             load(stage((u + STAGES - 1) % STAGES));
             multiply(stage(u));
         }
-#pragma unroll
-    for (int u = 0; u < STAGES - 1; ++u) {
-        if (at + u >= tiles) break;
-        stage_ready<kLoads * (STAGES - 2)>();
-        load(stage((u + STAGES - 1) % STAGES));
-        multiply(stage(u));
     }
 
     // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows by 64 (or 32) of the wave's columns at a time, so that they
@@ -330,13 +401,13 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
     char *strip = stage(wave / kPerStage) + wave % kPerStage * kStrip;
     const int quad = lane % kQuads;
     uint64_t base = 0;
-    if constexpr (END == kEndLayer) base = t.e.drop.base();
+    if constexpr (LAYER) base = t.e.drop.base();
 #pragma unroll
     for (int g = 0; g < FA; g += kGroup) {
         const int64_t col = n0 + wa + 32 * g + 4 * quad;
         const int valid = (int)(t.e.cols - col < 4 ? t.e.cols - col : 4);
         float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if constexpr (END == kEndLayer)
+        if constexpr (LAYER)
             if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + (valid > 0 ? col : 0), valid);
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
@@ -349,7 +420,7 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         z[v] = acc[g + i][j][4 * q + v];
-                        if constexpr (PLANES == 3) z[v] += low[g + i][j][4 * q + v];
+                        if constexpr (kFloat) z[v] += low[g + i][j][4 * q + v];
                     }
                     const int row = lane & 31, at = 8 * i + 2 * q + (lane >> 5);
                     *reinterpret_cast<float4 *>(strip + 16 * (row * kQuads + (at ^ skew(row)))) = make_float4(z[0], z[1], z[2], z[3]);
@@ -364,14 +435,14 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
                     const int r = r0 + k * kApart;
                     const int64_t row = first + k * kApart;
                     float4 v = *reinterpret_cast<const float4 *>(strip + 16 * (r * kQuads + (quad ^ skew(r))));
-                    if constexpr (PLANES == 3) {
-                        // (an infinite operand's planes, or leading parts that were rounded up, may have made this of a finite sum)
+                    if constexpr (kFloat) {
+                        // (an infinite operand's parts, or leading parts that were rounded up, may have made this of a finite sum)
                         if ((not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) && row < t.e.rows)
                             v = plain_sums<A_ACROSS, B_ACROSS>(t.a, t.b, col, valid, row, k0, k1);
                     }
                     z[k][0] = v.x, z[k][1] = v.y, z[k][2] = v.z, z[k][3] = v.w;
                 }
-                if constexpr (END == kEndLayer) {
+                if constexpr (LAYER) {
                     finish_quads<T, kRows>(t.e, base, first, kApart, col, valid, z, bias);
                 } else {
 #pragma unroll
@@ -379,13 +450,32 @@ __global__ __launch_bounds__(WA *WB *kWave) void linear_tile_kernel(TileArgs t)
                         const int64_t row = first + k * kApart;
                         const float4 v = make_float4(z[k][0], z[k][1], z[k][2], z[k][3]);
                         if (row >= t.e.rows) continue;
-                        if constexpr (END == kEndPartial) *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = v;
+                        if (t.partial) *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = v;
                         else store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, v, valid);
                     }
                 }
             }
         }
     }
+}
+
+// y = drop(act(x W^T + b)) + residual
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads) void linear_forward_kernel(TileArgs t)
+{
+    constexpr int kStage = stage_bytes<T, S>();
+    __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
+    compute_tile<T, false, false, S, true>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
+}
+
+// dW = dz^T x and dx = dz W in one launch: the first `dw_blocks` workgroups, which have the longer sums, take dW.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, TileArgs dx, int64_t dw_blocks)
+{
+    constexpr int kStage = stage_bytes<T, S>();
+    __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
+    if ((int64_t)blockIdx.x < dw_blocks) compute_tile<T, true, true, S, false>(dw, blockIdx.x, dw_blocks, stage0, stage1, stage2, stage3);
+    else compute_tile<T, true, false, S, false>(dx, blockIdx.x - dw_blocks, gridDim.x - dw_blocks, stage0, stage1, stage2, stage3);
 }
 
 }  // namespace kge

@@ -595,8 +595,8 @@ typedef struct kge_linear {
 
 /*
  * saved: NULL for inference; else kge_linear_saved_bytes() bytes, 16-byte aligned, which kge_linear_fwd fills for kge_linear_bwd: act'(z)
- * (16-bit layers: in 16 bits of fixed point, to 1.02e-5), and x and weight as the matrix cores take them where their own memory is not
- * that (fp32, row widths that are no multiple of 8, odd addresses).  x and weight have to be unchanged when kge_linear_bwd runs, and *step_dev too.
+ * (16-bit layers: in 16 bits of fixed point, to 1.02e-5), and copies of x and weight where the matrix cores cannot take them as they lie
+ * (16 bits, with rows that do not start on 16 bytes or whose width is no multiple of 8).  x and weight have to be unchanged when kge_linear_bwd runs, and *step_dev too.
  * The byte counts depend on the types, sizes, strides, the low bits of addresses and whether there is an activation; a saved block of no bytes may be NULL.
  */
 size_t kge_linear_saved_bytes(const kge_linear *lin);

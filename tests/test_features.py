@@ -91,15 +91,15 @@ def test_linear_outputs_and_workspaces_are_checked():
 
 
 def test_linear_saves_no_more_than_it_needs():
-    """Rows of whole 16-byte chunks are read where they lie; fp32, odd widths, strides and addresses take a packed copy."""
+    """Rows of whole 16-byte chunks are read where they lie, and so is fp32; odd 16-bit widths, strides and addresses take a packed copy."""
     _, L = lib()
     size = lambda **kw: L.kge_linear_saved_bytes(C.byref(linear(rows=64, fin=64, fout=32, **kw)))
     assert size() == 0
     assert size(act=1) == 64 * 32 * 2
     assert size(xs=68) == 64 * 64 * 2 and size(x=FAKE + 2) == 64 * 64 * 2 and size(xs=72) == 0
     assert size(w=FAKE + 8) == 32 * 64 * 2
-    assert size(type=0, out_type=0) == 3 * 2 * (64 * 64 + 32 * 64)
-    assert size(type=0, out_type=0, act=3) == 4 * 64 * 32 + 3 * 2 * (64 * 64 + 32 * 64)
+    assert size(type=0, out_type=0) == 0 and size(type=0, out_type=0, x=FAKE + 4, xs=65) == 0
+    assert size(type=0, out_type=0, act=3) == 4 * 64 * 32
 
 
 @pytest.mark.parametrize("bad,rc", [
