@@ -169,12 +169,12 @@ using SmallF = Shape<64, 64, 32, 2, 2, 2>;
 
 static int64_t tiles_of(int64_t a, int64_t b, int x) { return ceil_div(a, x) * ceil_div(b, x); }
 
-template <class T, class S>
+template <class T, class S, bool WHOLE = true>
 static void launch_forward(TileArgs &t, hipStream_t st)
 {
     t.tiles_a = (int)ceil_div(t.a.extent, S::XA), t.tiles_b = (int)ceil_div(t.b.extent, S::XB);
     const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b;
-    if (blocks) hipLaunchKernelGGL((linear_forward_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
+    if (blocks) hipLaunchKernelGGL((linear_forward_kernel<T, S, WHOLE>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
 template <class T>
@@ -182,8 +182,9 @@ static void launch_forward(TileArgs &t, hipStream_t st)
 {
     const int64_t a = t.a.extent, b = t.b.extent;
     if constexpr (sizeof(T) == 4) {
-        if (tiles_of(a, b, 128) >= 200) launch_forward<T, MiddleF>(t, st);
-        else launch_forward<T, SmallF>(t, st);
+        const bool whole = t.k % 4 == 0;
+        if (tiles_of(a, b, 128) >= 200) whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
+        else whole ? launch_forward<T, SmallF, true>(t, st) : launch_forward<T, SmallF, false>(t, st);
     } else {
         // bytes that the epilogue moves an element, beside the sum's length
         const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 2 : 0);
@@ -213,20 +214,21 @@ static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
     return p;
 }
 
-template <class T, class S>
+template <class T, class S, bool WHOLE = true>
 static void launch_grads(TileArgs &dw, TileArgs &dx, bool want_dw, bool want_dx, hipStream_t st)
 {
     for (TileArgs *t : {&dw, &dx}) t->tiles_a = (int)ceil_div(t->a.extent, S::XA), t->tiles_b = (int)ceil_div(t->b.extent, S::XB);
     const int64_t nw = want_dw ? (int64_t)dw.tiles_a * dw.tiles_b * dw.splits : 0, nx = want_dx ? (int64_t)dx.tiles_a * dx.tiles_b : 0;
-    if (nw + nx) hipLaunchKernelGGL((linear_grads_kernel<T, S>), dim3((unsigned)(nw + nx)), dim3(S::kThreads), 0, st, dw, dx, nw);
+    if (nw + nx) hipLaunchKernelGGL((linear_grads_kernel<T, S, WHOLE>), dim3((unsigned)(nw + nx)), dim3(S::kThreads), 0, st, dw, dx, nw);
 }
 
 template <class T>
 static void launch_grads(int tile, TileArgs &dw, TileArgs &dx, bool want_dw, bool want_dx, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
-        if (tile == 128) launch_grads<T, MiddleF>(dw, dx, want_dw, want_dx, st);
-        else launch_grads<T, SmallF>(dw, dx, want_dw, want_dx, st);
+        const bool whole = dw.a.extent % 4 == 0 && dw.b.extent % 4 == 0;  // in and out
+        if (tile == 128) whole ? launch_grads<T, MiddleF, true>(dw, dx, want_dw, want_dx, st) : launch_grads<T, MiddleF, false>(dw, dx, want_dw, want_dx, st);
+        else whole ? launch_grads<T, SmallF, true>(dw, dx, want_dw, want_dx, st) : launch_grads<T, SmallF, false>(dw, dx, want_dw, want_dx, st);
     } else {
         if (tile == 256) launch_grads<T, Large>(dw, dx, want_dw, want_dx, st);
         else if (tile == 128) launch_grads<T, Middle>(dw, dx, want_dw, want_dx, st);

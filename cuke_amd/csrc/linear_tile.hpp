@@ -119,12 +119,14 @@ struct Tile {
         }
     };
 
-    // The same of an fp32 side: a chunk's eight values wait in registers while the tile before is multiplied, then go to LDS as parts.
+    // The same of an fp32 side: a chunk's eight values wait in registers (two tiles' at a time) until they go to LDS as parts.  WHOLE: rows are
+    // whole quads, of which each exists or not, and loads need no branch (behind which they would be waited for); other rows end inside one.
+    template <bool WHOLE>
     struct FloatFeed {
         const float *from[kRounds];
         int64_t step;
-        int term[kRounds], there[kRounds];  // there: of a chunk's indices (across; along: whether its row exists)
-        float held[kRounds][8];
+        int term[kRounds], there[kRounds];  // there: how many of a chunk's indices exist (across; along: of its row, all or none)
+        float held[2][kRounds][8];
 
         __device__ __forceinline__ void start(const Side &s, int64_t first, int64_t k)
         {
@@ -135,21 +137,30 @@ struct Tile {
                 const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
                 const int64_t index = first + (ACROSS ? 8 * j : row), rest = s.extent - index;
                 term[r] = ACROSS ? row : 8 * j;
-                there[r] = (int)(rest < 8 ? rest : 8);
+                there[r] = rest <= 0 ? 0 : (ACROSS && rest < 8 ? (int)rest : 8);
                 from[r] = p + (ACROSS ? (k + row) * s.stride + index : index * s.stride + k + 8 * j);
             }
         }
-        __device__ __forceinline__ void fetch(int64_t left)
+        __device__ __forceinline__ void fetch(int set, int64_t left)
         {
+            const int most = (int)(left < K ? left : K);
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
-                const int64_t rest = left - term[r];
-                const int valid = ACROSS ? (rest > 0 ? there[r] : 0) : (there[r] > 0 ? (int)(rest < 8 ? rest : 8) : 0);
-                load8(from[r], valid, held[r]);
+                const int rest = most - term[r], valid = ACROSS ? (rest > 0 ? there[r] : 0) : (rest < there[r] ? rest : there[r]);
+                if constexpr (WHOLE) {
+                    const float *zero = reinterpret_cast<const float *>(zero_chunk);
+                    // (said to be global memory: the choice between two objects would make flat loads of these, which count with the LDS's)
+                    typedef const __attribute__((address_space(1))) f4u *quad;
+                    const f4u a = *(quad)(valid > 0 ? from[r] : zero), b = *(quad)(valid > 4 ? from[r] + 4 : zero);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) held[set][r][e] = a[e], held[set][r][4 + e] = b[e];
+                } else {
+                    load8(from[r], valid, held[set][r]);
+                }
                 from[r] += step;
             }
         }
-        __device__ __forceinline__ void put(char *lds, int plane_bytes)
+        __device__ __forceinline__ void put(int set, char *lds, int plane_bytes)
         {
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
@@ -159,10 +170,14 @@ struct Tile {
                 bf16x8 part[kSplitParts];
                 // (The compiler has been seen to let the parts overwrite the values they are still to be taken from, where both are tuples of
                 // registers: each value passes through a register of its own.)
+                float v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) asm("" : "+v"(held[r][e]));
-                split_quad(make_float4(held[r][0], held[r][1], held[r][2], held[r][3]), lo);
-                split_quad(make_float4(held[r][4], held[r][5], held[r][6], held[r][7]), hi);
+                for (int e = 0; e < 8; ++e) {
+                    v[e] = held[set][r][e];
+                    asm("" : "+v"(v[e]));
+                }
+                split_quad(make_float4(v[0], v[1], v[2], v[3]), lo);
+                split_quad(make_float4(v[4], v[5], v[6], v[7]), hi);
 #pragma unroll
                 for (int k = 0; k < kSplitParts; ++k) part[k] = __builtin_shufflevector(lo[k], hi[k], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
@@ -291,7 +306,8 @@ __device__ __forceinline__ void lds_ready()
 
 // A workgroup of WA x WB waves computes XA columns by XB rows, K terms at a time.  16 bits: STAGES tiles are in LDS, in arrays of their own (so
 // that the compiler sees that the one being read is none of those being written); STAGES - 1 are requested ahead, and one barrier a tile both
-// publishes the next and frees the last.  fp32: two stages, a third tile in registers.
+// publishes the next and frees the last.  fp32: two stages, two more tiles in
+// registers.
 template <int XA_, int XB_, int K_, int WA_, int WB_, int STAGES_>
 struct Shape {
     static constexpr int XA = XA_, XB = XB_, K = K_, WA = WA_, WB = WB_, STAGES = STAGES_, kThreads = WA * WB * kWave;
@@ -299,8 +315,9 @@ struct Shape {
 template <class T, class S>
 constexpr int stage_bytes() { return (S::XA + S::XB) * S::K * 2 * (sizeof(T) == 4 ? kSplitParts : 1); }
 
-// T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.
-template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER>
+// T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.  WHOLE: an fp32
+// side's rows are whole quads.
+template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER, bool WHOLE>
 __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, int64_t blocks, char *stage0, char *stage1, char *stage2, char *stage3)
 {
     constexpr bool kFloat = sizeof(T) == 4;
@@ -349,23 +366,29 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
         }
     };
     if constexpr (kFloat) {
-        typename A::FloatFeed feed_a;
-        typename B::FloatFeed feed_b;
+        typename A::template FloatFeed<WHOLE> feed_a;
+        typename B::template FloatFeed<WHOLE> feed_b;
         feed_a.start(t.a, n0, k0), feed_b.start(t.b, m0, k0);
-        auto fetch = [&] { feed_a.fetch(left), feed_b.fetch(left), left -= K; };
-        auto put = [&](char *lds) { feed_a.put(lds, kBytesA), feed_b.put(lds + PLANES * kBytesA, kBytesB); };
-        fetch();
-        put(stage0);
-        fetch();
-        for (int at = 0; at < tiles; at += 2)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (at + u >= tiles) break;
-                lds_ready();
-                put(stage(1 - u));
-                fetch();
-                multiply(stage(u));
-            }
+        auto fetch = [&](int set) { feed_a.fetch(set, left), feed_b.fetch(set, left), left -= K; };
+        auto put = [&](int set, char *lds) { feed_a.put(set, lds, kBytesA), feed_b.put(set, lds + PLANES * kBytesA, kBytesB); };
+        // (in this order: the loop waits for the older of two tiles' loads only where the entry leaves them in the loop's own order)
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(1);
+        __builtin_amdgcn_sched_barrier(0);
+        put(0, stage0);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+        auto turn = [&](int u) {
+            lds_ready();
+            put(1 - u, stage(1 - u));
+            fetch(1 - u);
+            multiply(stage(u));
+        };
+        int at = 0;
+        for (; at + 2 <= tiles; at += 2) turn(0), turn(1);
+        if (at < tiles) turn(0);
     } else {
         typename A::template Feed<E> feed_a;
         typename B::template Feed<E> feed_b;
@@ -460,22 +483,22 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
 }
 
 // y = drop(act(x W^T + b)) + residual
-template <class T, class S>
+template <class T, class S, bool WHOLE>
 __global__ __launch_bounds__(S::kThreads) void linear_forward_kernel(TileArgs t)
 {
     constexpr int kStage = stage_bytes<T, S>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
-    compute_tile<T, false, false, S, true>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
+    compute_tile<T, false, false, S, true, WHOLE>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
 }
 
 // dW = dz^T x and dx = dz W in one launch: the first `dw_blocks` workgroups, which have the longer sums, take dW.
-template <class T, class S>
+template <class T, class S, bool WHOLE>
 __global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, TileArgs dx, int64_t dw_blocks)
 {
     constexpr int kStage = stage_bytes<T, S>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
-    if ((int64_t)blockIdx.x < dw_blocks) compute_tile<T, true, true, S, false>(dw, blockIdx.x, dw_blocks, stage0, stage1, stage2, stage3);
-    else compute_tile<T, true, false, S, false>(dx, blockIdx.x - dw_blocks, gridDim.x - dw_blocks, stage0, stage1, stage2, stage3);
+    if ((int64_t)blockIdx.x < dw_blocks) compute_tile<T, true, true, S, false, WHOLE>(dw, blockIdx.x, dw_blocks, stage0, stage1, stage2, stage3);
+    else compute_tile<T, true, false, S, false, WHOLE>(dx, blockIdx.x - dw_blocks, gridDim.x - dw_blocks, stage0, stage1, stage2, stage3);
 }
 
 }  // namespace kge
