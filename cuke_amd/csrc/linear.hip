@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(GradArgs g)
 
 // ---- partial sums joined ---------------------------------------------------------------------------
 // out[row][col] = sum over n parts of part[.][row][col].  The weight's gradient has few parts of many quads: a thread takes a quad.  The bias's
-// has many parts of few quads: sixteen threads share one, or a call waited for its last 512 loads one after another (64 us).
+// has many parts of few quads: 64 threads share one, or a call waited for its last 512 loads one after another (64 us).
 struct JoinArgs {
     const float *part[2];
     int64_t rows, cols[2], quads[2];
@@ -135,22 +135,26 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
         store4(static_cast<T *>(j.out[0]) + row * j.cols[0] + col, s, (int)(left < 4 ? left : 4));
         return;
     }
-    const int64_t quad = ((int64_t)blockIdx.x - j.blocks0) * 16 + threadIdx.x % 16;
+    const int64_t quad = ((int64_t)blockIdx.x - j.blocks0) * 4 + threadIdx.x % 4;
     if (quad < j.quads[1]) {
         const float4 *p = reinterpret_cast<const float4 *>(j.part[1]) + quad;
 #pragma unroll 4
-        for (int k = threadIdx.x / 16; k < j.n[1]; k += 16) {
+        for (int k = threadIdx.x / 4; k < j.n[1]; k += 64) {
             const float4 v = p[k * j.quads[1]];
             s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
         }
     }
-    s_sum[threadIdx.x] = s;
-    __syncthreads();
-    if (threadIdx.x >= 16 || quad >= j.quads[1]) return;
-    for (int k = 1; k < 16; ++k) {
-        const float4 v = s_sum[16 * k + threadIdx.x];
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    // (a tree: the order of the sums is the same in every call)
+    for (int o = 128; o >= 4; o >>= 1) {
+        s_sum[threadIdx.x] = s;
+        __syncthreads();
+        if ((int)threadIdx.x < o) {
+            const float4 v = s_sum[threadIdx.x + o];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        __syncthreads();
     }
+    if (threadIdx.x >= 4 || quad >= j.quads[1]) return;
     const int64_t left = j.cols[1] - 4 * quad;
     store4(static_cast<T *>(j.out[1]) + 4 * quad, s, (int)(left < 4 ? left : 4));
 }
@@ -193,6 +197,24 @@ static void launch_forward(TileArgs &t, hipStream_t st)
         else if (tiles_of(a, b, 128) >= 256) launch_forward<T, Middle>(t, st);
         else launch_forward<T, Small>(t, st);
     }
+}
+
+// Few output elements: how many times 16 rows a workgroup of linear_few_kernel takes, or 0 where tiles are faster.  Measured with gelu and drop
+// (us; tiles, 16 rows, 32 rows): 1 x 768 -> 512 bf16 7.2, 3.4, 3.6; 512 x 768 -> 400 7.8, 7.0, 6.4; 512 x 2048 -> 512 13.0, 17.0, 13.4; fp32, whose
+// tiles wait for one another longer: 37 x 300 -> 200 12.1, 3.3, 4.0; 256 x 768 -> 2048 21.9, 24.4, 19.4; 512 x 2048 -> 2048 49.7, 113, 87.
+static int few_rows(int type, int64_t rows, int64_t out)
+{
+    const int64_t blocks = tiles_of(rows, out, 16);
+    if (blocks <= 512) return 1;
+    return blocks <= (type == KGE_F32 ? 2048 : 1024) ? 2 : 0;
+}
+
+template <class T>
+static void launch_few(int few, const TileArgs &t, hipStream_t st)
+{
+    const dim3 grid((unsigned)ceil_div(t.a.extent, 16), (unsigned)ceil_div(t.b.extent, 16 * few)), block(kFewWaves * kWave);
+    if (few == 1) hipLaunchKernelGGL((linear_few_kernel<T, 1>), grid, block, 0, st, t);
+    else hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, st, t);
 }
 
 // The tiles of a backward pass and the parts that dW's sums over rows are split into.  Both products share a launch and `slots` workgroups run at
@@ -241,6 +263,7 @@ static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k,
 // ---- a layer's plan --------------------------------------------------------------------------------
 struct Plan {
     bool pack_x, pack_w;
+    int few;             // few_rows() of the forward pass
     size_t slope, x, w;  // bytes of each in a saved block, in this order
     int64_t quads;
     int sum_blocks;      // ranges of rows the bias's gradient is summed over
@@ -252,13 +275,14 @@ static Plan plan_of(const kge_linear *l)
 {
     Plan p;
     p.quads = ceil_div(l->out, 4);
+    p.few = few_rows(l->type, l->rows, l->out);
     p.pack_x = !lies_ready(l->type, l->x, l->x_stride, l->in);
     p.pack_w = !lies_ready(l->type, l->weight, l->weight_stride, l->in);
     p.slope = l->act == KGE_ACT_NONE ? 0 : up256((size_t)l->rows * p.quads * 4 * type_bytes(l->type));
     p.x = p.pack_x ? packed_bytes(l->type, l->rows, l->in) : 0;
     p.w = p.pack_w ? packed_bytes(l->type, l->out, l->in) : 0;
-    // ranges of at least 8 rows, about 1024 workgroups in all
-    const int64_t across = ceil_div(up8(l->out), 512), want = across > 0 && across < 1024 ? 1024 / across : 1;
+    // ranges of at least 8 rows, at most 512 of them, about 1024 workgroups in all
+    const int64_t across = ceil_div(up8(l->out), 512), want = across > 0 && across < 1024 ? (across < 2 ? 512 : 1024 / across) : 1;
     p.sum_rows = ceil_div(l->rows, want);
     if (p.sum_rows < 8) p.sum_rows = 8;
     p.sum_blocks = (int)ceil_div(l->rows, p.sum_rows);
@@ -303,17 +327,18 @@ static Side side_of(const void *p, int64_t stride, bool packed, const void *copy
 }
 
 template <class T>
-static int forward(const kge_linear *l, const Plan &p, void *y, int64_t y_stride, char *slope, char *px, char *pw, hipStream_t st)
+static int forward(const kge_linear *l, const Plan &p, bool pack, void *y, int64_t y_stride, char *slope, char *px, char *pw, hipStream_t st)
 {
-    if (p.pack_x) launch_pack(l->x, l->x_stride, l->rows, l->in, px, st);
-    if (p.pack_w) launch_pack(l->weight, l->weight_stride, l->out, l->in, pw, st);
+    if (pack && p.pack_x) launch_pack(l->x, l->x_stride, l->rows, l->in, px, st);
+    if (pack && p.pack_w) launch_pack(l->weight, l->weight_stride, l->out, l->in, pw, st);
     TileArgs t{};
-    t.a = side_of(l->weight, l->weight_stride, p.pack_w, pw, l->in, l->out);
-    t.b = side_of(l->x, l->x_stride, p.pack_x, px, l->in, l->rows);
+    t.a = side_of(l->weight, l->weight_stride, p.pack_w && !p.few, pw, l->in, l->out);
+    t.b = side_of(l->x, l->x_stride, p.pack_x && !p.few, px, l->in, l->rows);
     t.k = l->in, t.splits = 1, t.k_each = split_length(l->in, 1);
     t.e = Ends{y, y_stride, l->bias, l->residual, l->residual_stride, slope, l->rows, l->out, p.quads,
                make_drop(l->p, l->seed, l->step, l->step_dev, l->out), l->act, l->out_type == KGE_F32};
-    launch_forward<T>(t, st);
+    if (p.few) launch_few<T>(p.few, t, st);
+    else launch_forward<T>(t, st);
     KGE_CHECK_LAUNCH();
     return KGE_OK;
 }
@@ -354,7 +379,7 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
         j.blocks0 = ceil_div(j.rows * j.quads[0], 256);
     }
     if (db) j.part[1] = sums, j.cols[1] = l->out, j.quads[1] = p.quads, j.n[1] = p.sum_blocks, j.out[1] = db;
-    const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 16) : 0);
+    const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 4) : 0);
     if (blocks) hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, j);
     KGE_CHECK_LAUNCH();
     return KGE_OK;
@@ -377,7 +402,7 @@ size_t kge_linear_fwd_workspace(const kge_linear *lin, int for_backward)
 {
     if (check(lin)) return 0;
     const Plan p = plan_of(lin);
-    return for_backward ? 0 : p.x + p.w;
+    return for_backward || p.few ? 0 : p.x + p.w;
 }
 
 int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_backward, void *saved, size_t saved_bytes, void *workspace,
@@ -388,16 +413,17 @@ int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_bac
     if (!y) return KGE_EINVAL;
     if (y_stride < lin->out) return KGE_ESHAPE;
     const Plan p = plan_of(lin);
-    const size_t need_saved = for_backward ? p.slope + p.x + p.w : 0, need = for_backward ? 0 : p.x + p.w;
+    const size_t need_saved = for_backward ? p.slope + p.x + p.w : 0, need = for_backward || p.few ? 0 : p.x + p.w;
+    const bool pack = for_backward || !p.few;  // (few rows are read where they lie; the backward pass wants the copies)
     if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
     char *slope = for_backward && p.slope ? static_cast<char *>(saved) : nullptr;
     char *px = for_backward ? static_cast<char *>(saved) + p.slope : static_cast<char *>(workspace);
     hipStream_t st = as_stream(stream);
     KGE_CLEAR_LAUNCH_ERRORS();
-    if (lin->type == KGE_F32) return forward<float>(lin, p, y, y_stride, slope, px, px + p.x, st);
-    if (lin->type == KGE_BF16) return forward<bf16_t>(lin, p, y, y_stride, slope, px, px + p.x, st);
-    return forward<half_t>(lin, p, y, y_stride, slope, px, px + p.x, st);
+    if (lin->type == KGE_F32) return forward<float>(lin, p, pack, y, y_stride, slope, px, px + p.x, st);
+    if (lin->type == KGE_BF16) return forward<bf16_t>(lin, p, pack, y, y_stride, slope, px, px + p.x, st);
+    return forward<half_t>(lin, p, pack, y, y_stride, slope, px, px + p.x, st);
 }
 
 size_t kge_linear_bwd_workspace(const kge_linear *lin)

@@ -15,6 +15,7 @@ namespace kge {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 
 template <class E>
 struct Mfma;
@@ -499,6 +500,121 @@ __global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, 
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
     if ((int64_t)blockIdx.x < dw_blocks) compute_tile<T, true, true, S, false, WHOLE>(dw, blockIdx.x, dw_blocks, stage0, stage1, stage2, stage3);
     else compute_tile<T, true, false, S, false, WHOLE>(dx, blockIdx.x - dw_blocks, gridDim.x - dw_blocks, stage0, stage1, stage2, stage3);
+}
+
+// ---- few rows --------------------------------------------------------------------------------------
+// The forward pass of a few rows reads the weight once and does next to nothing with it, so what counts is how soon all of it is on its way: a
+// workgroup takes 16 columns and up to 64 rows, its eight waves take every eighth stretch of the sum, straight from memory into the matrix
+// cores' registers (fp32: by fp32 instructions), and join their sums in LDS.  Rows may lie anywhere.
+constexpr int kFewWaves = 8;
+
+template <class T>
+struct Few;  // what a lane holds of a row for one step of kTerms terms: those from 8 (or 4) * (lane / 16) on
+template <class T>
+struct FewHalf {
+    static constexpr int kTerms = 32, kEach = 8;
+    typedef short piece __attribute__((ext_vector_type(8)));
+    __device__ __forceinline__ static piece load(const T *p) { return Pack<short, 8>::load(reinterpret_cast<const short *>(p)).v; }
+    __device__ __forceinline__ static piece load(const T *p, int valid)
+    {
+        piece v;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < valid ? reinterpret_cast<const short *>(p)[e] : (short)0;
+        return v;
+    }
+};
+template <>
+struct Few<bf16_t> : FewHalf<bf16_t> {
+    __device__ __forceinline__ static f4 multiply(piece a, piece b, f4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Few<half_t> : FewHalf<half_t> {
+    __device__ __forceinline__ static f4 multiply(piece a, piece b, f4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+};
+template <>
+struct Few<float> {
+    static constexpr int kTerms = 16, kEach = 4;
+    typedef f4 piece;
+    __device__ __forceinline__ static piece load(const float *p) { return Pack<float, 4>::load(p).v; }
+    __device__ __forceinline__ static piece load(const float *p, int valid)
+    {
+        const float4 v = load4(p, valid);
+        return f4{v.x, v.y, v.z, v.w};
+    }
+    __device__ __forceinline__ static f4 multiply(piece a, piece b, f4 c)
+    {
+        // (an instruction takes one term of each lane; which four terms meet in it does not matter)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <class T, int MF>
+__global__ __launch_bounds__(kFewWaves *kWave) void linear_few_kernel(TileArgs t)
+{
+    using F = Few<T>;
+    constexpr int kAhead = 4;  // steps whose loads are in flight together
+    __shared__ f4 sums[kFewWaves][MF][kWave];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, k0 = F::kEach * (lane >> 4);
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MF;
+    const int64_t n = n0 + r < t.a.extent ? n0 + r : t.a.extent - 1;  // (rows that do not exist: others, whose sums nobody asks for)
+    const T *a = static_cast<const T *>(t.a.p) + n * t.a.stride + k0, *b[MF];
+#pragma unroll
+    for (int j = 0; j < MF; ++j) {
+        const int64_t m = m0 + 16 * j + r;
+        b[j] = static_cast<const T *>(t.b.p) + (m < t.b.extent ? m : t.b.extent - 1) * t.b.stride + k0;
+    }
+    f4 acc[MF] = {};
+    const int64_t full = t.k / F::kTerms;
+    int64_t s = wave;
+    for (; s + (kAhead - 1) * kFewWaves < full; s += kAhead * kFewWaves) {
+        typename F::piece x[kAhead], y[kAhead][MF];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t at = (s + u * kFewWaves) * F::kTerms;
+            x[u] = F::load(a + at);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) y[u][j] = F::load(b[j] + at);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (int j = 0; j < MF; ++j) acc[j] = F::multiply(x[u], y[u][j], acc[j]);
+    }
+    for (; s < full; s += kFewWaves) {
+        const typename F::piece x = F::load(a + s * F::kTerms);
+#pragma unroll
+        for (int j = 0; j < MF; ++j) acc[j] = F::multiply(x, F::load(b[j] + s * F::kTerms), acc[j]);
+    }
+    if (s == full && full * F::kTerms < t.k) {  // the wave whose turn it is takes what is left
+        const int64_t at = full * F::kTerms, left = t.k - at - k0;
+        const int valid = left < 0 ? 0 : (int)(left < F::kEach ? left : F::kEach);
+        const typename F::piece x = F::load(a + at, valid);
+#pragma unroll
+        for (int j = 0; j < MF; ++j) acc[j] = F::multiply(x, F::load(b[j] + at, valid), acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < MF; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= MF) return;
+    // wave j finishes rows 16 j ..: lane l holds columns 4 (l / 16) .. + 3 of row l % 16
+    f4 z = sums[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) z += sums[w][wave][lane];
+    const int64_t row = m0 + 16 * wave + r, col = n0 + 4 * (lane >> 4), left = t.e.cols - col;
+    if (row >= t.e.rows || left <= 0) return;
+    const int valid = (int)(left < 4 ? left : 4);
+    float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + col, valid);
+    float out[1][4] = {{z[0], z[1], z[2], z[3]}};
+    finish_quads<T, 1>(t.e, t.e.drop.base(), row, 1, col, valid, out, bias);
 }
 
 }  // namespace kge

@@ -178,6 +178,53 @@ def test_layer_large(dtype):
     Layer(8200, 520, 776, dtype, act="gelu", drop=0.1).check()
 
 
+# (rows, in, out, options): outputs too large for the kernel of few rows, on both sides of every rule that picks tiles
+TILED = [(1100, 72, 264, {}), (2100, 130, 264, {}), (2100, 132, 265, dict(act="silu", drop=0.2)), (1537, 64, 400, dict(act="relu", residual=True)),
+         (4000, 33, 150, dict(act="gelu")), (8200, 520, 776, {}), (8200, 520, 776, dict(act="gelu", drop=0.1, residual=True)),
+         (8200, 521, 777, dict(act="silu", residual=True)), (16640, 264, 1030, {}), (16640, 264, 1030, dict(act="gelu", drop=0.1)),
+         (33000, 64, 130, dict(act="gelu", residual=True))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", TILED, ids=lambda c: "%dx%dx%d%s" % (c[0], c[1], c[2], "".join("-" + str(v) for v in c[3].values())))
+def test_layer_tiles(case, dtype):
+    print("tiles", case, dtype, flush=True)
+    Layer(*case[:3], dtype, **case[3]).check()
+    if dtype != torch.float32 and case[3].get("residual"):
+        Layer(*case[:3], dtype, out=torch.float32, **case[3]).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("layout", ["slice", "wide", "columns"])
+@pytest.mark.parametrize("shape", [(2100, 136, 264), (2100, 130, 270)])
+def test_layer_tiles_of_other_layouts(shape, layout, dtype):
+    print("layout of tiles", shape, layout, dtype, flush=True)
+    Layer(*shape, dtype, act="gelu", drop=0.2, residual=True, layout=layout).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_layer_tiles_with_infinities_and_nans(dtype):
+    """As of few rows, where the sums are made in tiles (and fp32 ones from bf16 parts)."""
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(4)
+    x, w = draw(g, (2100, 136), dtype), draw(g, (264, 136), dtype, 0.1)
+    x[0, 5], x[100, 7], w[4, 9] = float("inf"), float("nan"), -float("inf")
+    w[6, 5] = 0.0
+    if dtype == torch.float32:
+        x[7, 3], w[9, 3] = 3.4e38, 0.5      # rounds to infinity as bf16
+    want = (x.float().cpu() @ w.float().cpu().T).to(DEV)
+    y = features.linear(x, w)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    assert torch.equal(torch.sign(y[torch.isinf(y)]).float(), torch.sign(want[torch.isinf(want)]))
+    if dtype == torch.float32:
+        assert abs(y[7, 9].item() / 1.7e38 - 1) < 1e-6
+    dy = torch.ones_like(y)
+    dy[2, 3] = float("inf")
+    got = features.linear_backward(features.linear_forward(x, w), dy)
+    for have, want in [(got.x, dy.float().cpu() @ w.float().cpu()), (got.weight, dy.float().cpu().T @ x.float().cpu())]:
+        assert torch.equal(torch.isnan(have).cpu(), torch.isnan(want)) and torch.equal(torch.isinf(have).cpu(), torch.isinf(want))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_layer_gradients_against_differences(dtype):
     """The slope of sum(y dy) along random directions, by central differences of the 64-bit formula."""
