@@ -107,56 +107,28 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(GradArgs g)
 }
 
 // ---- partial sums joined ---------------------------------------------------------------------------
-// out[row][col] = sum over n parts of part[.][row][col].  The weight's gradient has few parts of many quads: a thread takes a quad.  The bias's
-// has many parts of few quads: 64 threads share one, or a call waited for its last 512 loads one after another (64 us).
+// A weight's gradient: out[row][col] = sum over n parts of part[.][row][col], a quad a thread.
 struct JoinArgs {
-    const float *part[2];
-    int64_t rows, cols[2], quads[2];
-    int n[2];
-    void *out[2];
-    int64_t blocks0;  // workgroups of the weight's gradient
+    const float *part;
+    int64_t rows, cols, quads;
+    int n;
+    void *out;
 };
 
 template <class T>
 __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 {
-    __shared__ float4 s_sum[256];
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, each = j.rows * j.quads;
+    if (i >= each) return;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if ((int64_t)blockIdx.x < j.blocks0) {
-        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, quads = j.quads[0], each = j.rows * quads;
-        if (i >= each) return;
-        const float4 *p = reinterpret_cast<const float4 *>(j.part[0]) + i;
+    const float4 *p = reinterpret_cast<const float4 *>(j.part) + i;
 #pragma unroll 4
-        for (int k = 0; k < j.n[0]; ++k) {
-            const float4 v = p[k * each];
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-        const int64_t row = i / quads, col = 4 * (i % quads), left = j.cols[0] - col;
-        store4(static_cast<T *>(j.out[0]) + row * j.cols[0] + col, s, (int)(left < 4 ? left : 4));
-        return;
+    for (int k = 0; k < j.n; ++k) {
+        const float4 v = p[k * each];
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const int64_t quad = ((int64_t)blockIdx.x - j.blocks0) * 4 + threadIdx.x % 4;
-    if (quad < j.quads[1]) {
-        const float4 *p = reinterpret_cast<const float4 *>(j.part[1]) + quad;
-#pragma unroll 4
-        for (int k = threadIdx.x / 4; k < j.n[1]; k += 64) {
-            const float4 v = p[k * j.quads[1]];
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-    }
-    // (a tree: the order of the sums is the same in every call)
-    for (int o = 128; o >= 4; o >>= 1) {
-        s_sum[threadIdx.x] = s;
-        __syncthreads();
-        if ((int)threadIdx.x < o) {
-            const float4 v = s_sum[threadIdx.x + o];
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-        __syncthreads();
-    }
-    if (threadIdx.x >= 4 || quad >= j.quads[1]) return;
-    const int64_t left = j.cols[1] - 4 * quad;
-    store4(static_cast<T *>(j.out[1]) + 4 * quad, s, (int)(left < 4 ? left : 4));
+    const int64_t row = i / j.quads, col = 4 * (i % j.quads), left = j.cols - col;
+    store4(static_cast<T *>(j.out) + row * j.cols + col, s, (int)(left < 4 ? left : 4));
 }
 
 // ---- products --------------------------------------------------------------------------------------
@@ -219,7 +191,7 @@ static void launch_few(int few, const TileArgs &t, hipStream_t st)
 
 // The tiles of a backward pass and the parts that dW's sums over rows are split into.  Both products share a launch and `slots` workgroups run at
 // once: dW is split until its sums are no longer than a slot's share of the work (none shorter than 256 terms; a part costs 4 bytes written and
-// read an element).
+// read an element).  Where rows are few, one part alone saves the launch that joins them: 512 x 768 -> 400.
 struct GradPlan {
     int tile, dw_splits;  // tile: 256, 128 or 64
 };
@@ -231,30 +203,31 @@ static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
     else p.tile = at_most(256) >= 384 ? 256 : (at_most(128) >= 320 ? 128 : 64);
     const int64_t slots = p.tile == 256 ? 256 : (p.tile == 128 ? (type == KGE_F32 ? 256 : 512) : 1024);
     const int64_t share = (tiles_of(rows, in, p.tile) * out + tiles_of(out, in, p.tile) * rows) / slots;
-    p.dw_splits = (int)ceil_div(rows, share > 256 ? share : 256);
+    p.dw_splits = rows <= 1024 ? 1 : (int)ceil_div(rows, share > 256 ? share : 256);
     if (p.dw_splits < 1) p.dw_splits = 1;
     return p;
 }
 
 template <class T, class S, bool WHOLE = true>
-static void launch_grads(TileArgs &dw, TileArgs &dx, bool want_dw, bool want_dx, hipStream_t st)
+static void launch_grads(TileArgs &dw, TileArgs &dx, const SumArgs &db, bool want_dw, bool want_dx, hipStream_t st)
 {
     for (TileArgs *t : {&dw, &dx}) t->tiles_a = (int)ceil_div(t->a.extent, S::XA), t->tiles_b = (int)ceil_div(t->b.extent, S::XB);
     const int64_t nw = want_dw ? (int64_t)dw.tiles_a * dw.tiles_b * dw.splits : 0, nx = want_dx ? (int64_t)dx.tiles_a * dx.tiles_b : 0;
-    if (nw + nx) hipLaunchKernelGGL((linear_grads_kernel<T, S, WHOLE>), dim3((unsigned)(nw + nx)), dim3(S::kThreads), 0, st, dw, dx, nw);
+    const int64_t nb = db.out ? ceil_div(db.quads, 4) : 0;
+    if (nw + nx + nb) hipLaunchKernelGGL((linear_grads_kernel<T, S, WHOLE>), dim3((unsigned)(nw + nx + nb)), dim3(S::kThreads), 0, st, dw, dx, db, nw, nx);
 }
 
 template <class T>
-static void launch_grads(int tile, TileArgs &dw, TileArgs &dx, bool want_dw, bool want_dx, hipStream_t st)
+static void launch_grads(int tile, TileArgs &dw, TileArgs &dx, const SumArgs &db, bool want_dw, bool want_dx, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
         const bool whole = dw.a.extent % 4 == 0 && dw.b.extent % 4 == 0;  // in and out
-        if (tile == 128) whole ? launch_grads<T, MiddleF, true>(dw, dx, want_dw, want_dx, st) : launch_grads<T, MiddleF, false>(dw, dx, want_dw, want_dx, st);
-        else whole ? launch_grads<T, SmallF, true>(dw, dx, want_dw, want_dx, st) : launch_grads<T, SmallF, false>(dw, dx, want_dw, want_dx, st);
+        if (tile == 128) whole ? launch_grads<T, MiddleF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, MiddleF, false>(dw, dx, db, want_dw, want_dx, st);
+        else whole ? launch_grads<T, SmallF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, SmallF, false>(dw, dx, db, want_dw, want_dx, st);
     } else {
-        if (tile == 256) launch_grads<T, Large>(dw, dx, want_dw, want_dx, st);
-        else if (tile == 128) launch_grads<T, Middle>(dw, dx, want_dw, want_dx, st);
-        else launch_grads<T, Small>(dw, dx, want_dw, want_dx, st);
+        if (tile == 256) launch_grads<T, Large>(dw, dx, db, want_dw, want_dx, st);
+        else if (tile == 128) launch_grads<T, Middle>(dw, dx, db, want_dw, want_dx, st);
+        else launch_grads<T, Small>(dw, dx, db, want_dw, want_dx, st);
     }
 }
 
@@ -372,15 +345,12 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
     tw.k = l->rows, tw.splits = p.grads.dw_splits, tw.k_each = split_length(l->rows, tw.splits);
     tw.partial = tw.splits > 1 ? part : nullptr;
     tw.e.y = dw, tw.e.y_stride = l->in, tw.e.rows = l->out, tw.e.cols = l->in, tw.e.quads = in_quads;
-    launch_grads<T>(p.grads.tile, tw, tx, dw != nullptr, dx != nullptr, st);
-    JoinArgs j{};
+    launch_grads<T>(p.grads.tile, tw, tx, SumArgs{sums, p.sum_blocks, l->out, p.quads, db}, dw != nullptr, dx != nullptr, st);
     if (dw && tw.partial) {
-        j.part[0] = part, j.rows = l->out, j.cols[0] = l->in, j.quads[0] = in_quads, j.n[0] = tw.splits, j.out[0] = dw;
-        j.blocks0 = ceil_div(j.rows * j.quads[0], 256);
+        const JoinArgs j{part, l->out, l->in, in_quads, tw.splits, dw};
+        const int64_t blocks = ceil_div(j.rows * j.quads, 256);
+        if (blocks) hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, j);
     }
-    if (db) j.part[1] = sums, j.cols[1] = l->out, j.quads[1] = p.quads, j.n[1] = p.sum_blocks, j.out[1] = db;
-    const int64_t blocks = j.blocks0 + (db ? ceil_div(p.quads, 4) : 0);
-    if (blocks) hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, j);
     KGE_CHECK_LAUNCH();
     return KGE_OK;
 }

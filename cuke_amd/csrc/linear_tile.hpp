@@ -492,14 +492,52 @@ __global__ __launch_bounds__(S::kThreads) void linear_forward_kernel(TileArgs t)
     compute_tile<T, false, false, S, true, WHOLE>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
 }
 
-// dW = dz^T x and dx = dz W in one launch: the first `dw_blocks` workgroups, which have the longer sums, take dW.
+// out[col] = sum over n parts of part[.][col]: few columns, many parts, so a quad is shared by a quarter of the workgroup.
+struct SumArgs {
+    const float *part;  // [n][4 quads]
+    int n;
+    int64_t cols, quads;
+    void *out;
+};
+template <class T, int THREADS>
+__device__ __forceinline__ void join_sums(const SumArgs &j, int64_t block, float4 *lds)
+{
+    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const int64_t quad = block * 4 + threadIdx.x % 4;
+    if (quad < j.quads) {
+        const float4 *p = reinterpret_cast<const float4 *>(j.part) + quad;
+#pragma unroll 4
+        for (int k = threadIdx.x / 4; k < j.n; k += THREADS / 4) {
+            const float4 v = p[k * j.quads];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+    }
+    // (a tree: the order of the sums is the same in every call)
+    for (int o = THREADS / 2; o >= 4; o >>= 1) {
+        lds[threadIdx.x] = s;
+        __syncthreads();
+        if ((int)threadIdx.x < o) {
+            const float4 v = lds[threadIdx.x + o];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x >= 4 || quad >= j.quads) return;
+    const int64_t left = j.cols - 4 * quad;
+    store4(static_cast<T *>(j.out) + 4 * quad, s, (int)(left < 4 ? left : 4));
+}
+
+// dW = dz^T x, dx = dz W and the bias's gradient in one launch: the first `dw_blocks` workgroups, which have the longer sums, take dW, the next
+// `dx_blocks` dx, the rest join the column sums that the kernel before this one has left.
 template <class T, class S, bool WHOLE>
-__global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, TileArgs dx, int64_t dw_blocks)
+__global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, TileArgs dx, SumArgs db, int64_t dw_blocks, int64_t dx_blocks)
 {
     constexpr int kStage = stage_bytes<T, S>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
-    if ((int64_t)blockIdx.x < dw_blocks) compute_tile<T, true, true, S, false, WHOLE>(dw, blockIdx.x, dw_blocks, stage0, stage1, stage2, stage3);
-    else compute_tile<T, true, false, S, false, WHOLE>(dx, blockIdx.x - dw_blocks, gridDim.x - dw_blocks, stage0, stage1, stage2, stage3);
+    const int64_t block = blockIdx.x;
+    if (block < dw_blocks) compute_tile<T, true, true, S, false, WHOLE>(dw, block, dw_blocks, stage0, stage1, stage2, stage3);
+    else if (block < dw_blocks + dx_blocks) compute_tile<T, true, false, S, false, WHOLE>(dx, block - dw_blocks, dx_blocks, stage0, stage1, stage2, stage3);
+    else join_sums<T, S::kThreads>(db, block - dw_blocks - dx_blocks, reinterpret_cast<float4 *>(stage0));
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
