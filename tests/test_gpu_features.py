@@ -592,3 +592,21 @@ def test_arguments_that_are_refused():
             (ValueError, lambda: F.FeatureEncoder(w, b, w, b))]:
         with pytest.raises(bad):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_example_learns(dtype):
+    """The example's loss starts at that of a model against itself and falls well below it."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "feature_preference.py")
+    spec = importlib.util.spec_from_file_location("feature_preference", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    # Without drops the frozen model is the model itself: d = 0 but for rows that another kernel encoded.  Of those a hidden value may be rounded
+    # the other way, 2^-8 of it in bf16: rows, and scores of about 2, are then off by as much, and a loss by beta / 2 of four times that
+    first = mod.train(steps=1, n_ent=500, batch=256, dtype=dtype, drop=0.0)[0]
+    assert abs(first - math.log(2)) < 0.25 * 4 * 2.0 ** -8 * 2
+    losses = mod.train(steps=40, n_ent=500, batch=256, dtype=dtype)
+    assert all(math.isfinite(v) for v in losses)
+    assert sum(losses[-5:]) / 5 < 0.8 * losses[0]
