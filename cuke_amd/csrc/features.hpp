@@ -130,7 +130,12 @@ __device__ __forceinline__ void activate(float (&z)[V], int act, float (&slope)[
 // The derivative as it is kept for the backward pass of 16-bit layers: every one of them lies in [-0.13, 1.13], so 16 bits of fixed
 // point hold it to 1.02e-5 (0 and 1 exactly), where bf16 would add an error as large as that of the gradient's own rounding; 0, which no derivative
 // comes near, is NaN.  Layers in fp32 keep it in fp32.
-__device__ __forceinline__ uint16_t slope_to_fixed(float s) { return (uint16_t)(uint32_t)fmaxf(fmaf(s, 49152.0f, 8192.5f), 0.0f); }
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ us2 slopes_to_fixed(float a, float b)  // (one conversion to two unsigned normalised numbers; it makes 0 of NaN)
+{
+    constexpr float k1 = 49152.0f / 65535.0f, k0 = 8192.0f / 65535.0f;
+    return __builtin_bit_cast(us2, __builtin_amdgcn_cvt_pknorm_u16(fmaf(a, k1, k0), fmaf(b, k1, k0)));
+}
 __device__ __forceinline__ float slope_from_fixed(float q) { return q == 0.0f ? __builtin_nanf("") : (q - 8192.0f) * (1.0f / 49152.0f); }
 
 // ---- random bits -----------------------------------------------------------------------------------

@@ -139,10 +139,12 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 }
 
 // ---- products --------------------------------------------------------------------------------------
-// 16 bits: larger tiles read less and multiply faster, smaller ones fill the card where there are few, and several to a CU hide each other's
-// epilogues.  Forward of 32768 x 2048 x 2048 bf16 with gelu and drop: 256 x 256 322 us, 128 x 128 368, 64 x 64 468; of 4096 x 1024 x 512: 43.6, 18.9
-// and 11.8.  Columns by rows 64 x 128 take 65536 x 512 -> 400 with an fp32 residual in 76 us (256 x 256: 97), 32768 x 1024 -> 1024 plainly in 101
-// (77).  fp32: 128 x 128, or 64 x 64.
+// Larger tiles read less and multiply faster, smaller ones waste less at the edges and in the last round over the card, and where several share a
+// CU each hides the other's epilogue.  Forward passes by tile (us; 256 x 256, 128 x 128, 64 columns x 128 rows, 64 x 64):
+//   32768 x 2048 -> 2048 bf16, gelu and drop   322  368        468        65536 x 512 -> 400, plain           50  58  57  70
+//   20000 x 304 -> 800, plain                   35   32   28    30        16384 x 768 -> 512, plain           29  21  25  25
+//   65536 x 256 -> 128, plain                   20   14   15    15        32768 x 1024 -> 1024, fp32 residual 112 133 134 166
+// fp32 (128 x 128, 64 x 64): 8192 x 1024 -> 1024 110 136; 4096 x 512 -> 256 26 18.
 using Large = Shape<256, 256, 32, 2, 4, 4>;
 using Middle = Shape<128, 128, 64, 2, 2, 2>;
 using Tall = Shape<64, 128, 64, 2, 2, 2>;
@@ -160,20 +162,33 @@ static void launch_forward(TileArgs &t, hipStream_t st)
     if (blocks) hipLaunchKernelGGL((linear_forward_kernel<T, S, WHOLE>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
+// What a forward pass costs in tiles of a shape, in terms of one sum at the largest tiles' pace: rounds over the card, times what a round holds on a
+// CU (`share` tiles at most), each tile's area times its terms and as many again as its epilogue is worth (64 for a byte moved an element).
+// The paces are those of the sizes above; a CU that holds fewer tiles than it could waits more (4096 x 1024 -> 512: one 64 x 128 tile a CU 18.7 us,
+// two 64 x 64 ones 15.3).
+template <class S>
+static double forward_cost(const TileArgs &t, int share, double pace, int64_t moved)
+{
+    const int64_t tiles = ceil_div(t.a.extent, S::XA) * ceil_div(t.b.extent, S::XB), a_cu = ceil_div(tiles, 256);
+    const int64_t at_once = a_cu < share ? a_cu : share, rounds = ceil_div(tiles, 256 * (at_once > 0 ? at_once : 1));
+    return (double)rounds * at_once * S::XA * S::XB * (double)(t.k + 64 * moved) / (pace * (0.4 + 0.6 * at_once / share));
+}
+
 template <class T>
 static void launch_forward(TileArgs &t, hipStream_t st)
 {
-    const int64_t a = t.a.extent, b = t.b.extent;
+    const int64_t out = sizeof(T) == 4 || t.e.out_f32 ? 4 : 2, moved = out * (t.e.residual ? 2 : 1) + (t.e.slope ? (int64_t)sizeof(T) : 0);
     if constexpr (sizeof(T) == 4) {
         const bool whole = t.k % 4 == 0;
-        if (tiles_of(a, b, 128) >= 200) whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
+        if (forward_cost<MiddleF>(t, 1, 1.0, moved) <= forward_cost<SmallF>(t, 3, 0.8, moved))
+            whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
         else whole ? launch_forward<T, SmallF, true>(t, st) : launch_forward<T, SmallF, false>(t, st);
     } else {
-        // bytes that the epilogue moves an element, beside the sum's length
-        const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 2 : 0);
-        if (tiles_of(a, b, 128) >= 256 && 128 * moved >= t.k) launch_forward<T, Tall>(t, st);
-        else if (tiles_of(a, b, 256) >= 256) launch_forward<T, Large>(t, st);
-        else if (tiles_of(a, b, 128) >= 256) launch_forward<T, Middle>(t, st);
+        const double large = forward_cost<Large>(t, 1, 1.0, moved), middle = forward_cost<Middle>(t, 2, 0.83, moved);
+        const double tall = forward_cost<Tall>(t, 3, 0.75, moved), small = forward_cost<Small>(t, 4, 0.65, moved);
+        if (large <= middle && large <= tall && large <= small) launch_forward<T, Large>(t, st);
+        else if (middle <= tall && middle <= small) launch_forward<T, Middle>(t, st);
+        else if (tall <= small) launch_forward<T, Tall>(t, st);
         else launch_forward<T, Small>(t, st);
     }
 }

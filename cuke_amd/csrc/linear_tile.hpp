@@ -215,13 +215,48 @@ __device__ __noinline__ float4 plain_sums(Side a, Side b, int64_t n, int valid, 
     return make_float4(s[0], s[1], s[2], s[3]);
 }
 
+// Four elements of a residual's row as they lie in memory, requested ahead of their use (a 16-bit row's fill half of it).
+struct Raw4 {
+    f4 v;
+    template <class T>
+    __device__ __forceinline__ void fetch(const Ends &e, int64_t row, int64_t col)
+    {
+        const int64_t at = (row < e.rows ? row : e.rows - 1) * e.residual_stride + (col < e.cols ? col : e.cols - 4);
+        typedef float pair __attribute__((ext_vector_type(2), aligned(2)));
+        if (sizeof(T) == 4 || e.out_f32) {
+            v = Pack<float, 4>::load(static_cast<const float *>(e.residual) + at).v;
+        } else {
+            const pair q = *reinterpret_cast<const pair *>(static_cast<const T *>(e.residual) + at);
+            v[0] = q[0], v[1] = q[1];
+        }
+    }
+    template <class T>
+    __device__ __forceinline__ f4 value(const Ends &e) const
+    {
+        if constexpr (sizeof(T) == 2) {
+            typedef T quad __attribute__((ext_vector_type(4)));
+            typedef float pair __attribute__((ext_vector_type(2)));
+            const quad q = __builtin_bit_cast(quad, pair{v[0], v[1]});
+            if (!e.out_f32) return f4{(float)q[0], (float)q[1], (float)q[2], (float)q[3]};
+        }
+        return v;
+    }
+};
+
 // Four consecutive columns (`valid` of them exist) of R rows, `apart` rows from one to the next, through the layer's epilogue.  T: the layer's
-// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.
+// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.  ahead: the rows' residuals, or NULL.
 template <class T, int R>
-__device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64_t first, int apart, int64_t col, int valid, float (&z)[R][4], float4 bias)
+__device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64_t first, int apart, int64_t col, int valid, float (&z)[R][4], float4 bias,
+                                             const Raw4 *ahead)
 {
     float res[R][4];
-    if (e.residual) {
+    if (ahead) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const f4 v = ahead[r].value<T>(e);
+            res[r][0] = v[0], res[r][1] = v[1], res[r][2] = v[2], res[r][3] = v[3];
+        }
+    } else if (e.residual) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = first + r * apart, at = (row < e.rows ? row : e.rows - 1) * e.residual_stride + col;
@@ -247,7 +282,8 @@ __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64
                 if (sizeof(T) == 4) {
                     *reinterpret_cast<float4 *>(static_cast<float *>(e.slope) + at) = make_float4(slope[4 * r], slope[4 * r + 1], slope[4 * r + 2], slope[4 * r + 3]);
                 } else {
-                    const ushort4 q = {slope_to_fixed(slope[4 * r]), slope_to_fixed(slope[4 * r + 1]), slope_to_fixed(slope[4 * r + 2]), slope_to_fixed(slope[4 * r + 3])};
+                    const us2 lo = slopes_to_fixed(slope[4 * r], slope[4 * r + 1]), hi = slopes_to_fixed(slope[4 * r + 2], slope[4 * r + 3]);
+                    const ushort4 q = {lo[0], lo[1], hi[0], hi[1]};
                     *reinterpret_cast<ushort4 *>(static_cast<uint16_t *>(e.slope) + at) = q;
                 }
             }
@@ -417,25 +453,44 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     }
 
     // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows by 64 (or 32) of the wave's columns at a time, so that they
-    // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.
-    stage_ready<0>();
+    // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.  A
+    // strip's residuals are requested all at once and ahead of everything else that is done with it.
     constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16, kPerStage = kStage / kStrip;
+    constexpr int kApart = 64 / kQuads, kRows = 4, kTurns = 32 / (kApart * kRows);  // rows a read covers, reads a turn, turns a strip
+    constexpr int kStrips = FA / kGroup * FB;
     static_assert(FA % kGroup == 0 && kPerStage >= 1 && (WA * WB + kPerStage - 1) / kPerStage <= STAGES, "a strip for every wave");
+    const int quad = lane % kQuads, row0 = lane / kQuads;
+    const bool ahead = LAYER && t.e.residual && t.e.cols % 4 == 0;
+    Raw4 held[kTurns][kRows];
+    auto column = [&](int strip) { return n0 + wa + strip / FB * 32 * kGroup + 4 * quad; };
+    auto line = [&](int strip, int turn) { return m0 + wb + strip % FB * 32 + row0 + turn * kApart * kRows; };
+    auto fetch_strip = [&](int strip) {
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u)
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) held[u][k].template fetch<T>(t.e, line(strip, u) + k * kApart, column(strip));
+    };
+    if constexpr (LAYER)
+        if (ahead) fetch_strip(0);
+    stage_ready<0>();
     auto skew = [](int row) { return kQuads == 16 ? row & 15 : (row >> 1) & 7; };
-    char *strip = stage(wave / kPerStage) + wave % kPerStage * kStrip;
-    const int quad = lane % kQuads;
+    char *lds = stage(wave / kPerStage) + wave % kPerStage * kStrip;
     uint64_t base = 0;
     if constexpr (LAYER) base = t.e.drop.base();
-#pragma unroll
-    for (int g = 0; g < FA; g += kGroup) {
-        const int64_t col = n0 + wa + 32 * g + 4 * quad;
+    // (one copy of what is done with a strip: unrolled, the epilogue alone would fill the instruction cache)
+#pragma unroll 1
+    for (int strip = 0; strip < kStrips; ++strip) {
+        const int64_t col = column(strip);
         const int valid = (int)(t.e.cols - col < 4 ? t.e.cols - col : 4);
         float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if constexpr (LAYER)
+        if constexpr (LAYER) {
             if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + (valid > 0 ? col : 0), valid);
+            if (ahead && strip > 0) fetch_strip(strip);
+        }
+        // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
 #pragma unroll
-        for (int j = 0; j < FB; ++j) {
-            // lane l holds columns 8 (v / 4) + 4 (l / 32) + v % 4 of row l % 32
+        for (int f = 0; f < kStrips; ++f) {
+            if (f != strip) continue;
 #pragma unroll
             for (int i = 0; i < kGroup; ++i)
 #pragma unroll
@@ -443,40 +498,40 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                     float z[4];
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
-                        z[v] = acc[g + i][j][4 * q + v];
-                        if constexpr (kFloat) z[v] += low[g + i][j][4 * q + v];
+                        z[v] = acc[f / FB * kGroup + i][f % FB][4 * q + v];
+                        if constexpr (kFloat) z[v] += low[f / FB * kGroup + i][f % FB][4 * q + v];
                     }
                     const int row = lane & 31, at = 8 * i + 2 * q + (lane >> 5);
-                    *reinterpret_cast<float4 *>(strip + 16 * (row * kQuads + (at ^ skew(row)))) = make_float4(z[0], z[1], z[2], z[3]);
+                    *reinterpret_cast<float4 *>(lds + 16 * (row * kQuads + (at ^ skew(row)))) = make_float4(z[0], z[1], z[2], z[3]);
                 }
-            if (valid <= 0) continue;
-            constexpr int kApart = 64 / kQuads, kRows = 4;  // rows a read covers, reads a turn
-            for (int r0 = lane / kQuads; r0 < 32; r0 += kApart * kRows) {
-                const int64_t first = m0 + wb + 32 * j + r0;
-                float z[kRows][4];
+        }
+        if (valid <= 0) continue;
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+            const int64_t first = line(strip, u);
+            float z[kRows][4];
+#pragma unroll
+            for (int k = 0; k < kRows; ++k) {
+                const int r = row0 + (u * kRows + k) * kApart;
+                float4 v = *reinterpret_cast<const float4 *>(lds + 16 * (r * kQuads + (quad ^ skew(r))));
+                if constexpr (kFloat) {
+                    // (an infinite operand's parts, or leading parts that were rounded up, may have made this of a finite sum)
+                    const int64_t row = first + k * kApart;
+                    if ((not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) && row < t.e.rows)
+                        v = plain_sums<A_ACROSS, B_ACROSS>(t.a, t.b, col, valid, row, k0, k1);
+                }
+                z[k][0] = v.x, z[k][1] = v.y, z[k][2] = v.z, z[k][3] = v.w;
+            }
+            if constexpr (LAYER) {
+                finish_quads<T, kRows>(t.e, base, first, kApart, col, valid, z, bias, ahead ? held[u] : nullptr);
+            } else {
 #pragma unroll
                 for (int k = 0; k < kRows; ++k) {
-                    const int r = r0 + k * kApart;
                     const int64_t row = first + k * kApart;
-                    float4 v = *reinterpret_cast<const float4 *>(strip + 16 * (r * kQuads + (quad ^ skew(r))));
-                    if constexpr (kFloat) {
-                        // (an infinite operand's parts, or leading parts that were rounded up, may have made this of a finite sum)
-                        if ((not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) && row < t.e.rows)
-                            v = plain_sums<A_ACROSS, B_ACROSS>(t.a, t.b, col, valid, row, k0, k1);
-                    }
-                    z[k][0] = v.x, z[k][1] = v.y, z[k][2] = v.z, z[k][3] = v.w;
-                }
-                if constexpr (LAYER) {
-                    finish_quads<T, kRows>(t.e, base, first, kApart, col, valid, z, bias);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < kRows; ++k) {
-                        const int64_t row = first + k * kApart;
-                        const float4 v = make_float4(z[k][0], z[k][1], z[k][2], z[k][3]);
-                        if (row >= t.e.rows) continue;
-                        if (t.partial) *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = v;
-                        else store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, v, valid);
-                    }
+                    const float4 v = make_float4(z[k][0], z[k][1], z[k][2], z[k][3]);
+                    if (row >= t.e.rows) continue;
+                    if (t.partial) *reinterpret_cast<float4 *>(t.partial + ((int64_t)split * t.e.rows + row) * 4 * t.e.quads + col) = v;
+                    else store4(static_cast<T *>(t.e.y) + row * t.e.y_stride + col, v, valid);
                 }
             }
         }
@@ -652,7 +707,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear_few_kernel(TileArgs t
     float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + col, valid);
     float out[1][4] = {{z[0], z[1], z[2], z[3]}};
-    finish_quads<T, 1>(t.e, t.e.drop.base(), row, 1, col, valid, out, bias);
+    finish_quads<T, 1>(t.e, t.e.drop.base(), row, 1, col, valid, out, bias, nullptr);
 }
 
 }  // namespace kge

@@ -313,6 +313,22 @@ def test_layer_derivative_reaches_its_ends():
             within(g.x[:, 0], s, 1.1e-5 + 2 * U[dtype] * s.abs() + 2 * TINY[dtype], f"{act}' {dtype}")
 
 
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [4, 3000])
+def test_layer_derivative_of_nan(rows, dtype, act):
+    """A NaN among the features reaches the gradients of its row, also through the derivative that is kept, and no other row's."""
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(2)
+    x, w = draw(g, (rows, 24), dtype), draw(g, (40, 24), dtype, 0.2)
+    x[1, 3] = float("nan")
+    fw = features.linear_forward(x, w, act=act)
+    assert bool(torch.isnan(fw.y[1]).all()) and int(torch.isnan(fw.y).sum()) == 40
+    got = features.linear_backward(fw, torch.ones_like(fw.y))
+    assert bool(torch.isnan(got.x[1]).all()) and int(torch.isnan(got.x).sum()) == 24
+    assert bool(torch.isnan(got.weight).all())
+
+
 def test_layer_on_another_stream_and_in_a_graph():
     from cuke_amd import features
     L = Layer(300, 264, 136, torch.bfloat16, act="gelu", drop=0.2, residual=True)
