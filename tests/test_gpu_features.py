@@ -182,7 +182,7 @@ def test_layer_large(dtype):
 TILED = [(1100, 72, 264, {}), (2100, 130, 264, {}), (2100, 132, 265, dict(act="silu", drop=0.2)), (1537, 64, 400, dict(act="relu", residual=True)),
          (4000, 33, 150, dict(act="gelu")), (8200, 520, 776, {}), (8200, 520, 776, dict(act="gelu", drop=0.1, residual=True)),
          (8200, 521, 777, dict(act="silu", residual=True)), (16640, 264, 1030, {}), (16640, 264, 1030, dict(act="gelu", drop=0.1)),
-         (33000, 64, 130, dict(act="gelu", residual=True))]
+         (33000, 64, 130, dict(act="gelu", residual=True)), (16300, 520, 1000, {}), (16300, 520, 1000, dict(act="silu", drop=0.1, residual=True))]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -537,6 +537,65 @@ def test_preference_gradient_against_differences():
         slope = (dpos.double() * vp).sum() + (dneg.double() * vn).sum()
         size = (dpos.double() * vp).abs().sum() + (dneg.double() * vn).abs().sum()
         assert abs((up - down) / (2 * h) - slope) <= 64 * EPS * (size + 1) + 1e-8
+
+
+# ---- past 32 bits ----------------------------------------------------------------------------------
+def test_arrays_of_more_elements_than_32_bits_count():
+    """The last rows of arrays whose offsets pass 2^31 and 2^32 elements are those of a call of their own."""
+    from cuke_amd import features
+    free = torch.cuda.mem_get_info()[0]
+    if free < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    bf = torch.bfloat16
+    x = torch.zeros(70_000, 65_536, device=DEV, dtype=bf)                 # 4.6e9 elements
+    x[-3:] = torch.randn(3, 65_536, device=DEV).to(bf)
+    y = features.dropout(x, 0.5, 7)
+    k = torch.from_numpy(np.ascontiguousarray(last_kept(70_000, 65_536, 3, 0.5, 7))).to(DEV)
+    assert torch.equal(y[-3:].double(), x[-3:].double() * k)
+    del y
+    # a sum over 65536 terms of the last rows, and the gradient that comes back to them
+    w = torch.randn(16, 65_536, device=DEV).to(bf) * 0.01
+    fw = features.linear_forward(x, w)
+    want = x[-3:].double() @ w.double().T
+    tol = (65_536 + 16) * EPS * (x[-3:].double().abs() @ w.double().abs().T) + U[bf] * want.abs()
+    within(fw.y[-3:], want, tol, "y")
+    assert not fw.y[:-3].any()
+    dy = torch.zeros_like(fw.y)
+    dy[-3:] = torch.randn(3, 16, device=DEV).to(bf)
+    g = features.linear_backward(fw, dy)
+    want = dy[-3:].double() @ w.double()
+    within(g.x[-3:], want, 32 * EPS * (dy[-3:].double().abs() @ w.double().abs()) + U[bf] * want.abs(), "dx")
+    want = dy[-3:].double().T @ x[-3:].double()
+    within(g.weight, want, (70_000 + 16) * EPS * (dy[-3:].double().abs().T @ x[-3:].double().abs()) + U[bf] * want.abs(), "dw")
+    del x, fw, g, dy
+    torch.cuda.empty_cache()
+    for B, N in ((40_000, 60_000), (2_400_000, 1000)):                     # rows in segments, and rows in registers: 2.4e9 pairs
+        neg = torch.zeros(B, N, device=DEV, dtype=bf)
+        neg[-2:] = torch.randn(2, N, device=DEV).to(bf)
+        pos = torch.zeros(B, device=DEV, dtype=bf)
+        loss, dpos, dneg = features.preference_loss(pos, neg, temperature=0.5)
+        want = prefer64(pos[-2:], neg[-2:], None, None, 1.0, "sigmoid", 0.0, 0.5, None, 1.0)
+        within(dneg[-2:], want[2] * 2 / B, want[5] * 2 / B + 8 * EPS * (want[2] * 2 / B).abs(), "dneg")
+        within(dpos[-2:], want[1] * 2 / B, want[4] * 2 / B + 8 * EPS * (want[1] * 2 / B).abs(), "dpos")
+        assert abs(loss.item() - math.log(2)) < 1e-4
+        del neg, pos, dneg, dpos
+        torch.cuda.empty_cache()
+
+
+def last_kept(rows, cols, last, p, seed, step=0):
+    """kept() of the last rows of a large block."""
+    with np.errstate(over="ignore"):
+        def mix(z):
+            z = z + np.uint64(0x9E3779B97F4A7C15)
+            z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)
+            z = (z ^ (z >> np.uint64(27))) * np.uint64(0x94D049BB133111EB)
+            return z ^ (z >> np.uint64(31))
+        base = mix(mix(np.array([seed ^ 0xD1B54A32D192ED03], dtype=np.uint64)) ^ np.uint64(step))
+        i, j = np.meshgrid(np.arange(rows - last, rows, dtype=np.uint64), np.arange(cols, dtype=np.uint64), indexing="ij")
+        word = mix(base ^ ((i * np.uint64((cols + 3) // 4) + j // np.uint64(4)) * np.uint64(0x9E3779B97F4A7C15)))
+        bits = (word >> (np.uint64(16) * (j % np.uint64(4)))) & np.uint64(0xFFFF)
+    cut = int(round(p * 65536))
+    return np.where(bits >= np.uint64(cut), 65536.0 / (65536 - cut), 0.0)
 
 
 # ---- together --------------------------------------------------------------------------------------
