@@ -162,16 +162,16 @@ static void launch_forward(TileArgs &t, hipStream_t st)
     if (blocks) hipLaunchKernelGGL((linear_forward_kernel<T, S, WHOLE>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
-// What a forward pass costs in tiles of a shape, in terms of one sum at the largest tiles' pace: rounds over the card, times what a round holds on a
-// CU (`share` tiles at most), each tile's area times its terms and as many again as its epilogue is worth (64 for a byte moved an element).
-// The paces are those of the sizes above; a CU that holds fewer tiles than it could waits more (4096 x 1024 -> 512: one 64 x 128 tile a CU 18.7 us,
-// two 64 x 64 ones 15.3).
+// What a forward pass costs in tiles of a shape: rounds over the card, times the tiles a round holds on a CU (`share` at most), times a tile's area,
+// times its terms and its epilogue's worth of terms (64 for a byte moved an element), each at the shape's pace beside the largest tiles'.  The paces
+// are those of the sizes above; a CU that holds fewer tiles than it could waits more (4096 x 1024 -> 512: one 64 x 128 tile a CU 18.7 us, two 64 x 64
+// ones 15.3).
 template <class S>
-static double forward_cost(const TileArgs &t, int share, double pace, int64_t moved)
+static double forward_cost(const TileArgs &t, int64_t moved, int share, double pace, double epilogue_pace)
 {
     const int64_t tiles = ceil_div(t.a.extent, S::XA) * ceil_div(t.b.extent, S::XB), a_cu = ceil_div(tiles, 256);
     const int64_t at_once = a_cu < share ? a_cu : share, rounds = ceil_div(tiles, 256 * (at_once > 0 ? at_once : 1));
-    return (double)rounds * at_once * S::XA * S::XB * (double)(t.k + 64 * moved) / (pace * (0.4 + 0.6 * at_once / share));
+    return (double)rounds * at_once * S::XA * S::XB * ((double)t.k / pace + 64.0 * moved / epilogue_pace) / (0.4 + 0.6 * at_once / share);
 }
 
 template <class T>
@@ -180,12 +180,12 @@ static void launch_forward(TileArgs &t, hipStream_t st)
     const int64_t out = sizeof(T) == 4 || t.e.out_f32 ? 4 : 2, moved = out * (t.e.residual ? 2 : 1) + (t.e.slope ? (int64_t)sizeof(T) : 0);
     if constexpr (sizeof(T) == 4) {
         const bool whole = t.k % 4 == 0;
-        if (forward_cost<MiddleF>(t, 1, 1.0, moved) <= forward_cost<SmallF>(t, 3, 0.8, moved))
+        if (forward_cost<MiddleF>(t, moved, 1, 1.0, 1.0) <= forward_cost<SmallF>(t, moved, 3, 0.8, 1.6))
             whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
         else whole ? launch_forward<T, SmallF, true>(t, st) : launch_forward<T, SmallF, false>(t, st);
     } else {
-        const double large = forward_cost<Large>(t, 1, 1.0, moved), middle = forward_cost<Middle>(t, 2, 0.83, moved);
-        const double tall = forward_cost<Tall>(t, 3, 0.75, moved), small = forward_cost<Small>(t, 4, 0.65, moved);
+        const double large = forward_cost<Large>(t, moved, 1, 1.0, 1.0), middle = forward_cost<Middle>(t, moved, 2, 0.83, 1.2);
+        const double tall = forward_cost<Tall>(t, moved, 3, 0.75, 1.5), small = forward_cost<Small>(t, moved, 4, 0.55, 2.0);
         if (large <= middle && large <= tall && large <= small) launch_forward<T, Large>(t, st);
         else if (middle <= tall && middle <= small) launch_forward<T, Middle>(t, st);
         else if (tall <= small) launch_forward<T, Tall>(t, st);
@@ -220,10 +220,15 @@ struct GradPlan {
 static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
 {
     auto at_most = [&](int x) { return tiles_of(rows, in, x) + tiles_of(out, in, x) * (rows >= 512 ? rows / 512 : 1); };
+    // (padded work at the shape's pace)
+    auto work = [&](int x, double pace) { return (double)(tiles_of(rows, in, x) * out + tiles_of(out, in, x) * rows) * x * x / pace; };
+    const bool f32 = type == KGE_F32;
+    const double small = work(64, f32 ? 0.8 : 0.6), middle = work(128, f32 ? 1.0 : 0.83), large = work(256, 1.0);
     GradPlan p;
-    if (type == KGE_F32) p.tile = at_most(128) >= 320 ? 128 : 64;
-    else p.tile = at_most(256) >= 384 ? 256 : (at_most(128) >= 320 ? 128 : 64);
-    const int64_t slots = p.tile == 256 ? 256 : (p.tile == 128 ? (type == KGE_F32 ? 256 : 512) : 1024);
+    p.tile = 64;
+    if (at_most(128) >= 320 && middle <= small) p.tile = 128;
+    if (!f32 && at_most(256) >= 384 && large <= middle && large <= small) p.tile = 256;
+    const int64_t slots = p.tile == 256 ? 256 : (p.tile == 128 ? (f32 ? 256 : 512) : 1024);
     const int64_t share = (tiles_of(rows, in, p.tile) * out + tiles_of(out, in, p.tile) * rows) / slots;
     p.dw_splits = rows <= 1024 ? 1 : (int)ceil_div(rows, share > 256 ? share : 256);
     if (p.dw_splits < 1) p.dw_splits = 1;
@@ -259,6 +264,7 @@ static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k,
 struct Plan {
     bool pack_x, pack_w;
     int few;             // few_rows() of the forward pass
+    bool pack_few;       // whether its operands are copied for it where they have to be for tiles
     size_t slope, x, w;  // bytes of each in a saved block, in this order
     int64_t quads;
     int sum_blocks;      // ranges of rows the bias's gradient is summed over
@@ -275,11 +281,14 @@ static Plan plan_of(const kge_linear *l)
     p.pack_w = !lies_ready(l->type, l->weight, l->weight_stride, l->in);
     // (a weight whose rows share a channel is worth copying where many rows are multiplied by it)
     if (l->type != KGE_F32 && l->weight_stride % 2048 == 0 && l->in >= 1024 && l->out >= 1024 && l->rows >= 8192) p.pack_w = true;
+    // (rows that start anywhere are read as they lie, at a third of the pace: 2110 x 1283 -> 56 21 us; that is less than the copies' launches up to
+    // some 8 MB)
+    p.pack_few = p.few && (ceil_div(l->rows, 16 * p.few) * ceil_div(l->out, 16) * (16 + 16 * p.few)) * l->in * 2 > 8 << 20;
     p.slope = l->act == KGE_ACT_NONE ? 0 : up256((size_t)l->rows * p.quads * 4 * type_bytes(l->type));
     p.x = p.pack_x ? packed_bytes(l->type, l->rows, l->in) : 0;
     p.w = p.pack_w ? packed_bytes(l->type, l->out, l->in) : 0;
-    // ranges of at least 8 rows, at most 512 of them, about 1024 workgroups in all
-    const int64_t across = ceil_div(up8(l->out), 512), want = across > 0 && across < 1024 ? (across < 2 ? 512 : 1024 / across) : 1;
+    // ranges of at least 8 rows, about 2048 workgroups in all: few turns each, so that a range is not one wait after another
+    const int64_t across = ceil_div(up8(l->out), 512), want = across > 0 && across < 2048 ? 2048 / across : 1;
     p.sum_rows = ceil_div(l->rows, want);
     if (p.sum_rows < 8) p.sum_rows = 8;
     p.sum_blocks = (int)ceil_div(l->rows, p.sum_rows);
@@ -329,8 +338,8 @@ static int forward(const kge_linear *l, const Plan &p, bool pack, void *y, int64
     if (pack && p.pack_x) launch_pack(l->x, l->x_stride, l->rows, l->in, px, st);
     if (pack && p.pack_w) launch_pack(l->weight, l->weight_stride, l->out, l->in, pw, st);
     TileArgs t{};
-    t.a = side_of(l->weight, l->weight_stride, p.pack_w && !p.few, pw, l->type, l->in, l->out);
-    t.b = side_of(l->x, l->x_stride, p.pack_x && !p.few, px, l->type, l->in, l->rows);
+    t.a = side_of(l->weight, l->weight_stride, p.pack_w && pack, pw, l->type, l->in, l->out);
+    t.b = side_of(l->x, l->x_stride, p.pack_x && pack, px, l->type, l->in, l->rows);
     t.k = l->in, t.splits = 1, t.k_each = split_length(l->in, 1);
     t.e = Ends{y, y_stride, l->bias, l->residual, l->residual_stride, slope, l->rows, l->out, p.quads,
                make_drop(l->p, l->seed, l->step, l->step_dev, l->out), l->act, l->out_type == KGE_F32};
@@ -396,7 +405,7 @@ size_t kge_linear_fwd_workspace(const kge_linear *lin, int for_backward)
 {
     if (check(lin)) return 0;
     const Plan p = plan_of(lin);
-    return for_backward || p.few ? 0 : p.x + p.w;
+    return for_backward || (p.few && !p.pack_few) ? 0 : p.x + p.w;
 }
 
 int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_backward, void *saved, size_t saved_bytes, void *workspace,
@@ -407,8 +416,8 @@ int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_bac
     if (!y) return KGE_EINVAL;
     if (y_stride < lin->out) return KGE_ESHAPE;
     const Plan p = plan_of(lin);
-    const size_t need_saved = for_backward ? p.slope + p.x + p.w : 0, need = for_backward || p.few ? 0 : p.x + p.w;
-    const bool pack = for_backward || !p.few;  // (few rows are read where they lie; the backward pass wants the copies)
+    const size_t need_saved = for_backward ? p.slope + p.x + p.w : 0, need = for_backward || (p.few && !p.pack_few) ? 0 : p.x + p.w;
+    const bool pack = for_backward || !p.few || p.pack_few;
     if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
     char *slope = for_backward && p.slope ? static_cast<char *>(saved) : nullptr;

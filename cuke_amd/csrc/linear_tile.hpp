@@ -120,19 +120,22 @@ struct Tile {
         }
     };
 
-    // The same of an fp32 side: a chunk's eight values wait in registers (two tiles' at a time) until they go to LDS as parts.  WHOLE: rows are
-    // whole quads, of which each exists or not, and loads need no branch (behind which they would be waited for); other rows end inside one.
+    // The same of an fp32 side: a chunk's eight values wait in registers (two tiles' at a time) until they go to LDS as parts.  A quad that
+    // exists as a whole or not at all needs no branch, behind which its load would be waited for; only where rows are no whole quads (not WHOLE) and
+    // a tile holds their end are values taken one at a time.
     template <bool WHOLE>
     struct FloatFeed {
         const float *from[kRounds];
         int64_t step;
         int term[kRounds], there[kRounds];  // there: how many of a chunk's indices exist (across; along: of its row, all or none)
+        bool ends;                          // across: the tile holds the end of its rows, inside a quad
         float held[2][kRounds][8];
 
         __device__ __forceinline__ void start(const Side &s, int64_t first, int64_t k)
         {
             const float *p = static_cast<const float *>(s.p);
             step = ACROSS ? K * s.stride : K;
+            ends = ACROSS && first + X > s.extent && s.extent % 4 != 0;
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
                 const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
@@ -145,18 +148,19 @@ struct Tile {
         __device__ __forceinline__ void fetch(int set, int64_t left)
         {
             const int most = (int)(left < K ? left : K);
+            const bool single = !WHOLE && (ACROSS ? ends : most > 0 && most % 4 != 0);
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
                 const int rest = most - term[r], valid = ACROSS ? (rest > 0 ? there[r] : 0) : (rest < there[r] ? rest : there[r]);
-                if constexpr (WHOLE) {
+                if (single) {
+                    load8(from[r], valid, held[set][r]);
+                } else {
                     const float *zero = reinterpret_cast<const float *>(zero_chunk);
                     // (said to be global memory: the choice between two objects would make flat loads of these, which count with the LDS's)
                     typedef const __attribute__((address_space(1))) f4u *quad;
                     const f4u a = *(quad)(valid > 0 ? from[r] : zero), b = *(quad)(valid > 4 ? from[r] + 4 : zero);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) held[set][r][e] = a[e], held[set][r][4 + e] = b[e];
-                } else {
-                    load8(from[r], valid, held[set][r]);
                 }
                 from[r] += step;
             }
