@@ -1,4 +1,6 @@
 // Linear layers with a fused epilogue, y = drop(act(x W^T + b)) + residual, and their gradients (kge_linear_fwd, kge_linear_bwd).
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "linear_tile.hpp"
@@ -140,15 +142,20 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 
 // ---- products --------------------------------------------------------------------------------------
 // Larger tiles read less and multiply faster, smaller ones waste less at the edges and in the last round over the card, and where several share a
-// CU each hides the other's epilogue.  Forward passes by tile (us; 256 x 256, 128 x 128, 64 columns x 128 rows, 64 x 64):
-//   32768 x 2048 -> 2048 bf16, gelu and drop   322  368        468        65536 x 512 -> 400, plain           50  58  57  70
-//   20000 x 304 -> 800, plain                   35   32   28    30        16384 x 768 -> 512, plain           29  21  25  25
-//   65536 x 256 -> 128, plain                   20   14   15    15        32768 x 1024 -> 1024, fp32 residual 112 133 134 166
-// fp32 (128 x 128, 64 x 64): 8192 x 1024 -> 1024 110 136; 4096 x 512 -> 256 26 18.
+// CU each hides the other's epilogue.  Forward passes by tile (us; Large, Middle, Tall, Lone, Small; what is chosen in brackets):
+//   32768 x 2048 -> 2048 bf16, gelu and drop   [349] 382  424  521  485       65536 x 512 -> 400, plain         [50] 50  56  75  62
+//   65536 x 512 -> 400, fp32 residual            88 [75]  80  102   84        20000 x 304 -> 800, plain          36 [26] 29  37  30
+//   16384 x 768 -> 512, plain                    29 [20]  27   27   25         8192 x 768 -> 512, fp32 residual  37  19 [17] 20  20
+//    4096 x 1024 -> 512, gelu and drop           45  18   15  [12]  13         2500 x 520 -> 264, gelu and drop  36  19  12   9  [8]
+// Lone's four stages keep a CU busy that has one tile.  Middle has eight waves (four: 27.6 us where it takes 25.6, 16384 x 768 -> 512) and shorter
+// stages in the gradients, whose epilogue is short (8192 x 768 -> 512 38.7 and 36.1 us); Tall is slower with eight (20000 x 304 -> 800 40 and 44).
+// fp32 (MiddleF, SmallF): 4033 x 1200 -> 1352 [117] 131; 8192 x 1024 -> 1024 [110] 140; 4096 x 512 -> 256 26 [18]; 2048 x 1024 -> 1024 47 [40].
 using Large = Shape<256, 256, 32, 2, 4, 4>;
-using Middle = Shape<128, 128, 64, 2, 2, 2>;
+using Middle = Shape<128, 128, 64, 2, 4, 2>;
+using MiddleG = Shape<128, 128, 32, 2, 4, 4>;
 using Tall = Shape<64, 128, 64, 2, 2, 2>;
-using Small = Shape<64, 64, 64, 2, 2, 2>;
+using Lone = Shape<64, 128, 64, 2, 4, 4>;
+using Small = Shape<64, 64, 64, 2, 2, 3>;
 using MiddleF = Shape<128, 128, 32, 2, 4, 2>;
 using SmallF = Shape<64, 64, 32, 2, 2, 2>;
 
@@ -163,30 +170,33 @@ static void launch_forward(TileArgs &t, hipStream_t st)
 }
 
 // What a forward pass costs in tiles of a shape: rounds over the card, times the tiles a round holds on a CU (`share` at most), times a tile's area,
-// times its terms and its epilogue's worth of terms (64 for a byte moved an element), each at the shape's pace beside the largest tiles'.  The paces
-// are those of the sizes above; a CU that holds fewer tiles than it could waits more (4096 x 1024 -> 512: one 64 x 128 tile a CU 18.7 us, two 64 x 64
-// ones 15.3).
+// times its terms and its epilogue's worth of terms (64 for a byte moved an element, 192 for gelu or silu and 192 for dropping), each at the shape's
+// pace beside the largest tiles'; a CU that holds fewer tiles than it could waits more.  Over 15 sizes, each with three epilogues, the shape chosen
+// takes 0.4 % longer than the best one on average, and 13 % at most.
 template <class S>
-static double forward_cost(const TileArgs &t, int64_t moved, int share, double pace, double epilogue_pace)
+static double forward_cost(const TileArgs &t, int64_t epilogue, int share, double pace, double epilogue_pace)
 {
     const int64_t tiles = ceil_div(t.a.extent, S::XA) * ceil_div(t.b.extent, S::XB), a_cu = ceil_div(tiles, 256);
     const int64_t at_once = a_cu < share ? a_cu : share, rounds = ceil_div(tiles, 256 * (at_once > 0 ? at_once : 1));
-    return (double)rounds * at_once * S::XA * S::XB * ((double)t.k / pace + 64.0 * moved / epilogue_pace) / (0.4 + 0.6 * at_once / share);
+    return (double)rounds * at_once * S::XA * S::XB * ((double)t.k / pace + epilogue / epilogue_pace) / (0.4 + 0.6 * at_once / share);
 }
 
 template <class T>
 static void launch_forward(TileArgs &t, hipStream_t st)
 {
     const int64_t out = sizeof(T) == 4 || t.e.out_f32 ? 4 : 2, moved = out * (t.e.residual ? 2 : 1) + (t.e.slope ? (int64_t)sizeof(T) : 0);
+    const int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
     if constexpr (sizeof(T) == 4) {
         const bool whole = t.k % 4 == 0;
-        if (forward_cost<MiddleF>(t, moved, 1, 1.0, 1.0) <= forward_cost<SmallF>(t, moved, 3, 0.8, 1.6))
+        if (forward_cost<MiddleF>(t, epilogue, 1, 1.0, 1.0) <= forward_cost<SmallF>(t, epilogue, 3, 0.7, 0.7))
             whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
         else whole ? launch_forward<T, SmallF, true>(t, st) : launch_forward<T, SmallF, false>(t, st);
     } else {
-        const double large = forward_cost<Large>(t, moved, 1, 1.0, 1.0), middle = forward_cost<Middle>(t, moved, 2, 0.83, 1.2);
-        const double tall = forward_cost<Tall>(t, moved, 3, 0.75, 1.5), small = forward_cost<Small>(t, moved, 4, 0.55, 2.0);
-        if (large <= middle && large <= tall && large <= small) launch_forward<T, Large>(t, st);
+        const double large = forward_cost<Large>(t, epilogue, 1, 1.0, 1.0), middle = forward_cost<Middle>(t, epilogue, 2, 0.73, 2.5);
+        const double tall = forward_cost<Tall>(t, epilogue, 3, 0.53, 2.3), small = forward_cost<Small>(t, epilogue, 3, 0.47, 0.9);
+        const double lone = forward_cost<Lone>(t, epilogue, 1, 0.41, 0.9);
+        if (lone < large && lone < middle && lone < tall && lone < small) launch_forward<T, Lone>(t, st);
+        else if (large <= middle && large <= tall && large <= small) launch_forward<T, Large>(t, st);
         else if (middle <= tall && middle <= small) launch_forward<T, Middle>(t, st);
         else if (tall <= small) launch_forward<T, Tall>(t, st);
         else launch_forward<T, Small>(t, st);
@@ -211,28 +221,55 @@ static void launch_few(int few, const TileArgs &t, hipStream_t st)
     else hipLaunchKernelGGL((linear_few_kernel<T, 2>), grid, block, 0, st, t);
 }
 
-// The tiles of a backward pass and the parts that dW's sums over rows are split into.  Both products share a launch and `slots` workgroups run at
-// once: dW is split until its sums are no longer than a slot's share of the work (none shorter than 256 terms; a part costs 4 bytes written and
-// read an element).  Where rows are few, one part alone saves the launch that joins them: 512 x 768 -> 400.
+static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), 64) * 64; }
+
+// The tiles of a backward pass and the parts that dW's sums over rows are split into: what is expected to end first.  dW's workgroups start first,
+// `slots` at a time, dx's fill what they leave; a tile takes so many ns a term and some us besides, and parts cost a launch, and bytes written and
+// read.  The paces are those that fit some six plans of each of 17 sizes, within 8 % on average.  Some of what they decide (us): 65536 x 256 -> 128
+// bf16 in 33 parts 41, in 128 49; 16384 x 768 -> 512 in tiles of 128 54, of 256 64; 32768 x 2048 -> 2048 745 and 632; 1500 x 4000 -> 120 in one part
+// of tiles of 64 17, in 6 of 128 22; 3000 x 700 -> 1000 fp32 in 2 parts 80, in 3 100.
 struct GradPlan {
     int tile, dw_splits;  // tile: 256, 128 or 64
 };
+// When n jobs of length a each, then m of length b, are done by `slots` workers.
+static double jobs_end(int64_t n, double a, int64_t m, double b, int64_t slots)
+{
+    const int64_t late = n % slots;
+    const double first = (double)(n / slots) * a, second = late ? first + a : first;  // when the workers without and with a last job of the first kind are free
+    if (m == 0) return second;
+    auto whole = [&](double from, double t) { return from + std::ceil((t - from) / b - 1e-6) * b; };
+    double t = first + (double)m * b / (double)(slots - late);
+    if (t <= second || !late) return std::max(second, whole(first, t));
+    t = ((double)m * b + (double)(slots - late) * first + (double)late * second) / (double)slots;
+    return std::max(second, std::min(whole(first, t), whole(second, t)));
+}
 static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
 {
-    auto at_most = [&](int x) { return tiles_of(rows, in, x) + tiles_of(out, in, x) * (rows >= 512 ? rows / 512 : 1); };
-    // (padded work at the shape's pace)
-    auto work = [&](int x, double pace) { return (double)(tiles_of(rows, in, x) * out + tiles_of(out, in, x) * rows) * x * x / pace; };
+    struct Pace {
+        int tile, slots;
+        double a_term, besides;  // us
+        double alone;            // how much longer a long sum takes where nothing else hides its waits
+    };
+    static const Pace kHalf[] = {{64, 256, 0.0026, 1.0, 2.3}, {128, 256, 0.0066, 3.0, 1.4}, {256, 256, 0.0260, 8.1, 1.0}};
+    static const Pace kFloat[] = {{64, 512, 0.0268, 3.5, 1.0}, {128, 256, 0.0393, 6.7, 1.0}};
     const bool f32 = type == KGE_F32;
-    const double small = work(64, f32 ? 0.8 : 0.6), middle = work(128, f32 ? 1.0 : 0.83), large = work(256, 1.0);
-    GradPlan p;
-    p.tile = 64;
-    if (at_most(128) >= 320 && middle <= small) p.tile = 128;
-    if (!f32 && at_most(256) >= 384 && large <= middle && large <= small) p.tile = 256;
-    const int64_t slots = p.tile == 256 ? 256 : (p.tile == 128 ? (f32 ? 256 : 512) : 1024);
-    const int64_t share = (tiles_of(rows, in, p.tile) * out + tiles_of(out, in, p.tile) * rows) / slots;
-    p.dw_splits = rows <= 1024 ? 1 : (int)ceil_div(rows, share > 256 ? share : 256);
-    if (p.dw_splits < 1) p.dw_splits = 1;
-    return p;
+    const Pace *paces = f32 ? kFloat : kHalf;
+    const double parts_launch = f32 ? 7.0 : 5.0, part = (double)out * (double)in * 8.0 / (f32 ? 16e6 : 40e6);  // us
+    GradPlan best{64, 1};
+    double best_end = INFINITY;
+    for (int i = 0; i < (f32 ? 2 : 3); ++i) {
+        const Pace &p = paces[i];
+        const int64_t dw = tiles_of(out, in, p.tile), dx = tiles_of(rows, in, p.tile);
+        for (int parts = 1; parts <= 64; parts += parts < 8 ? 1 : parts / 4) {
+            const int64_t each = split_length(rows, parts);
+            if (parts > 1 && each < 128) break;
+            double end = jobs_end(dw * ceil_div(rows, each > 0 ? each : 1), (double)each * p.a_term + p.besides, dx, (double)out * p.a_term + p.besides, p.slots);
+            end = std::max(end, p.alone * (double)each * p.a_term);
+            if (parts > 1) end += parts_launch + parts * part;
+            if (end < best_end) best_end = end, best = GradPlan{p.tile, parts};
+        }
+    }
+    return best;
 }
 
 template <class T, class S, bool WHOLE = true>
@@ -253,12 +290,10 @@ static void launch_grads(int tile, TileArgs &dw, TileArgs &dx, const SumArgs &db
         else whole ? launch_grads<T, SmallF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, SmallF, false>(dw, dx, db, want_dw, want_dx, st);
     } else {
         if (tile == 256) launch_grads<T, Large>(dw, dx, db, want_dw, want_dx, st);
-        else if (tile == 128) launch_grads<T, Middle>(dw, dx, db, want_dw, want_dx, st);
+        else if (tile == 128) launch_grads<T, MiddleG>(dw, dx, db, want_dw, want_dx, st);
         else launch_grads<T, Small>(dw, dx, db, want_dw, want_dx, st);
     }
 }
-
-static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), 64) * 64; }
 
 // ---- a layer's plan --------------------------------------------------------------------------------
 struct Plan {
@@ -269,7 +304,6 @@ struct Plan {
     int64_t quads;
     int sum_blocks;      // ranges of rows the bias's gradient is summed over
     int64_t sum_rows;
-    GradPlan grads;
 };
 
 static Plan plan_of(const kge_linear *l)
@@ -292,7 +326,6 @@ static Plan plan_of(const kge_linear *l)
     p.sum_rows = ceil_div(l->rows, want);
     if (p.sum_rows < 8) p.sum_rows = 8;
     p.sum_blocks = (int)ceil_div(l->rows, p.sum_rows);
-    p.grads = grad_plan(l->type, l->rows, l->in, l->out);
     return p;
 }
 
@@ -350,7 +383,7 @@ static int forward(const kge_linear *l, const Plan &p, bool pack, void *y, int64
 }
 
 template <class T>
-static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t dy_stride, const char *saved, void *dx, void *dw, void *db,
+static int backward(const kge_linear *l, const Plan &p, const GradPlan &g, const void *dy, int64_t dy_stride, const char *saved, void *dx, void *dw, void *db,
                     char *ws, hipStream_t st)
 {
     const int64_t width8 = up8(l->out);
@@ -360,12 +393,12 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
     float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(sums) + up256((size_t)p.sum_blocks * p.quads * 16));
     const bool want_dz = !ready && (dx || dw);
     if ((want_dz || db) && l->rows > 0 && l->out > 0) {
-        GradArgs g{dy, dy_stride, p.slope ? saved : nullptr, l->rows, l->out, p.quads, p.sum_rows,
+        GradArgs a{dy, dy_stride, p.slope ? saved : nullptr, l->rows, l->out, p.quads, p.sum_rows,
                    make_drop(l->p, l->seed, l->step, l->step_dev, l->out), want_dz ? dz : nullptr, width8, pitch_of(l->type, l->out), db ? sums : nullptr, 4};
-        while (g.lanes < 64 && 8 * g.lanes < width8) g.lanes *= 2;
-        const dim3 grid((unsigned)ceil_div(width8, 8 * g.lanes), (unsigned)p.sum_blocks);
-        if (l->out_type == KGE_F32) hipLaunchKernelGGL((linear_dz_kernel<T, float>), grid, dim3(256), 0, st, g);
-        else hipLaunchKernelGGL((linear_dz_kernel<T, T>), grid, dim3(256), 0, st, g);
+        while (a.lanes < 64 && 8 * a.lanes < width8) a.lanes *= 2;
+        const dim3 grid((unsigned)ceil_div(width8, 8 * a.lanes), (unsigned)p.sum_blocks);
+        if (l->out_type == KGE_F32) hipLaunchKernelGGL((linear_dz_kernel<T, float>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((linear_dz_kernel<T, T>), grid, dim3(256), 0, st, a);
     }
     const int64_t in_quads = ceil_div(l->in, 4);
     TileArgs tx{}, tw{};
@@ -375,10 +408,10 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
     tx.e.y = dx, tx.e.y_stride = l->in, tx.e.rows = l->rows, tx.e.cols = l->in, tx.e.quads = in_quads;
     tw.a = side_of(l->x, l->x_stride, p.pack_x, saved + p.slope, l->type, l->in, l->in);
     tw.b = tx.b, tw.b.extent = l->out;
-    tw.k = l->rows, tw.splits = p.grads.dw_splits, tw.k_each = split_length(l->rows, tw.splits);
+    tw.k = l->rows, tw.splits = g.dw_splits, tw.k_each = split_length(l->rows, tw.splits);
     tw.partial = tw.splits > 1 ? part : nullptr;
     tw.e.y = dw, tw.e.y_stride = l->in, tw.e.rows = l->out, tw.e.cols = l->in, tw.e.quads = in_quads;
-    launch_grads<T>(p.grads.tile, tw, tx, SumArgs{sums, p.sum_blocks, l->out, p.quads, db}, dw != nullptr, dx != nullptr, st);
+    launch_grads<T>(g.tile, tw, tx, SumArgs{sums, p.sum_blocks, l->out, p.quads, db}, dw != nullptr, dx != nullptr, st);
     if (dw && tw.partial) {
         const JoinArgs j{part, l->out, l->in, in_quads, tw.splits, dw};
         const int64_t blocks = ceil_div(j.rows * j.quads, 256);
@@ -391,6 +424,12 @@ static int backward(const kge_linear *l, const Plan &p, const void *dy, int64_t 
 }  // namespace kge
 
 using namespace kge;
+
+static size_t backward_bytes(const kge_linear *l, const Plan &p, const GradPlan &g)
+{
+    return packed_bytes(l->type, l->rows, l->out) + up256((size_t)p.sum_blocks * p.quads * 16) +
+           (g.dw_splits > 1 ? (size_t)g.dw_splits * l->out * ceil_div(l->in, 4) * 16 : 0);
+}
 
 extern "C" {
 
@@ -432,9 +471,7 @@ int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_bac
 size_t kge_linear_bwd_workspace(const kge_linear *lin)
 {
     if (check(lin)) return 0;
-    const Plan p = plan_of(lin);
-    return packed_bytes(lin->type, lin->rows, lin->out) + up256((size_t)p.sum_blocks * p.quads * 16) +
-           (p.grads.dw_splits > 1 ? (size_t)p.grads.dw_splits * lin->out * ceil_div(lin->in, 4) * 16 : 0);
+    return backward_bytes(lin, plan_of(lin), grad_plan(lin->type, lin->rows, lin->in, lin->out));
 }
 
 int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx, void *dweight,
@@ -444,16 +481,17 @@ int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, con
     if (dy_stride < lin->out) return KGE_ESHAPE;
     if (lin->rows > 0 && lin->out > 0 && !dy) return KGE_EINVAL;
     const Plan p = plan_of(lin);
-    const size_t need_saved = p.slope + p.x + p.w, need = kge_linear_bwd_workspace(lin);
+    const GradPlan g = grad_plan(lin->type, lin->rows, lin->in, lin->out);
+    const size_t need_saved = p.slope + p.x + p.w, need = backward_bytes(lin, p, g);
     if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
     hipStream_t st = as_stream(stream);
     KGE_CLEAR_LAUNCH_ERRORS();
     const char *s = static_cast<const char *>(saved);
     char *ws = static_cast<char *>(workspace);
-    if (lin->type == KGE_F32) return backward<float>(lin, p, dy, dy_stride, s, dx, dweight, dbias, ws, st);
-    if (lin->type == KGE_BF16) return backward<bf16_t>(lin, p, dy, dy_stride, s, dx, dweight, dbias, ws, st);
-    return backward<half_t>(lin, p, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+    if (lin->type == KGE_F32) return backward<float>(lin, p, g, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+    if (lin->type == KGE_BF16) return backward<bf16_t>(lin, p, g, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+    return backward<half_t>(lin, p, g, dy, dy_stride, s, dx, dweight, dbias, ws, st);
 }
 
 }  // extern "C"
