@@ -22,21 +22,32 @@ static size_t packed_bytes(int type, int64_t rows, int64_t width) { return up256
 // Whether an array can be read as it lies: fp32 always, 16 bits where rows start on 16 bytes and are whole chunks of 8 elements.
 static bool lies_ready(int type, const void *p, int64_t stride, int64_t width) { return type == KGE_F32 || (aligned16(p) && stride % 8 == 0 && width % 8 == 0); }
 
-// Rows of 16-bit elements copied to whole chunks, zeros behind their end.  One pass at memory speed.
-__global__ __launch_bounds__(256) void pack_kernel(const uint16_t *src, int64_t stride, int64_t rows, int64_t width, int64_t pitch, uint16_t *dst)
+// Rows of 16-bit elements of up to two arrays of one width (a layer's x and weight) copied to whole chunks, zeros behind their end, in one launch:
+// two cost 2 us more.  Bound by memory.
+struct PackArgs {
+    const uint16_t *src[2];
+    int64_t stride[2], rows[2];
+    uint16_t *dst[2];
+    int64_t width, pitch;
+};
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a)
 {
     typedef uint16_t chunk __attribute__((ext_vector_type(8)));
-    const int64_t chunks = (width + 7) / 8, total = rows * chunks;
+    const int64_t chunks = (a.width + 7) / 8, total = (a.rows[0] + a.rows[1]) * chunks;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / chunks, col = 8 * (i % chunks), left = width - col;
+        int64_t row = i / chunks;
+        const int64_t col = 8 * (i - row * chunks), left = a.width - col;
+        const bool second = row >= a.rows[0];
+        if (second) row -= a.rows[0];
+        const uint16_t *src = (second ? a.src[1] : a.src[0]) + row * (second ? a.stride[1] : a.stride[0]) + col;
         chunk v;
         if (left >= 8) {
-            v = Pack<uint16_t, 8>::load(src + row * stride + col).v;
+            v = Pack<uint16_t, 8>::load(src).v;
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = e < left ? src[row * stride + col + e] : (uint16_t)0;
+            for (int e = 0; e < 8; ++e) v[e] = e < left ? src[e] : (uint16_t)0;
         }
-        *reinterpret_cast<chunk *>(dst + row * pitch + col) = v;
+        *reinterpret_cast<chunk *>((second ? a.dst[1] : a.dst[0]) + row * a.pitch + col) = v;
     }
 }
 
@@ -203,14 +214,16 @@ static void launch_forward(TileArgs &t, hipStream_t st)
     }
 }
 
-// Few output elements: how many times 16 rows a workgroup of linear_few_kernel takes, or 0 where tiles are faster.  Measured with gelu and drop
-// (us; tiles, 16 rows, 32 rows): 1 x 768 -> 512 bf16 7.2, 3.4, 3.6; 512 x 768 -> 400 7.8, 7.0, 6.4; 512 x 2048 -> 512 13.0, 17.0, 13.4; fp32, whose
-// tiles wait for one another longer: 37 x 300 -> 200 12.1, 3.3, 4.0; 256 x 768 -> 2048 21.9, 24.4, 19.4; 512 x 2048 -> 2048 49.7, 113, 87.
-static int few_rows(int type, int64_t rows, int64_t out)
+// Few output elements: how many times 16 rows a workgroup of linear_few_kernel takes, or 0 where tiles are faster.  copies: whether tiles would need
+// an operand copied first.  Measured with gelu and drop (us; tiles, 16 rows, 32 rows): 1 x 768 -> 512 bf16 6.4, 3.5, 3.7; 256 x 4096 -> 512 17.1,
+// 16.8, 13.3; 512 x 768 -> 400 6.9, 8.0, 6.9; 512 x 2048 -> 512 11.0, 16.9, 13.5; 2000 x 200 -> 100 5.4, 4.0, 4.1; 1000 x 300 -> 200, with copies, 11.8, 9.5, 9.4; fp32, whose tiles
+// wait for one another longer: 37 x 300 -> 200 12.3, 3.4, 3.9; 256 x 768 -> 2048 22.2, 24.1, 19.3; 512 x 2048 -> 1024 48.8, 58.4, 44.9, and
+// 512 x 2048 -> 2048 49.7, 113, 87.
+static int few_rows(int type, int64_t rows, int64_t in, int64_t out, bool copies)
 {
     const int64_t blocks = tiles_of(rows, out, 16);
-    if (blocks <= 512) return 1;
-    return blocks <= (type == KGE_F32 ? 2048 : 1024) ? 2 : 0;
+    if (blocks <= 400) return 1;
+    return blocks <= (type == KGE_F32 ? 2048 : (copies || in <= 512 ? 1024 : 768)) ? 2 : 0;
 }
 
 template <class T>
@@ -310,9 +323,9 @@ static Plan plan_of(const kge_linear *l)
 {
     Plan p;
     p.quads = ceil_div(l->out, 4);
-    p.few = few_rows(l->type, l->rows, l->out);
     p.pack_x = !lies_ready(l->type, l->x, l->x_stride, l->in);
     p.pack_w = !lies_ready(l->type, l->weight, l->weight_stride, l->in);
+    p.few = few_rows(l->type, l->rows, l->in, l->out, p.pack_x || p.pack_w);
     // (a weight whose rows share a channel is worth copying where many rows are multiplied by it)
     if (l->type != KGE_F32 && l->weight_stride % 2048 == 0 && l->in >= 1024 && l->out >= 1024 && l->rows >= 8192) p.pack_w = true;
     // (rows that start anywhere are read as they lie, at a third of the pace: 2110 x 1283 -> 56 21 us; that is less than the copies' launches up to
@@ -351,11 +364,12 @@ static int grid_for(int64_t items)
     return (int)(b < 8192 ? b : 8192);
 }
 
-static void launch_pack(const void *src, int64_t stride, int64_t rows, int64_t width, void *dst, hipStream_t st)
+static void launch_pack(const kge_linear *l, bool x, bool weight, void *px, void *pw, hipStream_t st)
 {
-    if (rows == 0 || width == 0) return;
-    hipLaunchKernelGGL(pack_kernel, dim3(grid_for(rows * up8(width) / 8)), dim3(256), 0, st, static_cast<const uint16_t *>(src), stride, rows, width,
-                       pitch_of(KGE_BF16, width), static_cast<uint16_t *>(dst));
+    const PackArgs a{{static_cast<const uint16_t *>(l->x), static_cast<const uint16_t *>(l->weight)}, {l->x_stride, l->weight_stride},
+                     {x ? l->rows : 0, weight ? l->out : 0}, {static_cast<uint16_t *>(px), static_cast<uint16_t *>(pw)}, l->in, pitch_of(KGE_BF16, l->in)};
+    const int64_t total = (a.rows[0] + a.rows[1]) * (up8(l->in) / 8);
+    if (total) hipLaunchKernelGGL(pack_kernel, dim3(grid_for(total)), dim3(256), 0, st, a);
 }
 
 // an operand where it lies, or its packed copy
@@ -368,8 +382,7 @@ static Side side_of(const void *p, int64_t stride, bool packed, const void *copy
 template <class T>
 static int forward(const kge_linear *l, const Plan &p, bool pack, void *y, int64_t y_stride, char *slope, char *px, char *pw, hipStream_t st)
 {
-    if (pack && p.pack_x) launch_pack(l->x, l->x_stride, l->rows, l->in, px, st);
-    if (pack && p.pack_w) launch_pack(l->weight, l->weight_stride, l->out, l->in, pw, st);
+    if (pack && (p.pack_x || p.pack_w)) launch_pack(l, p.pack_x, p.pack_w, px, pw, st);
     TileArgs t{};
     t.a = side_of(l->weight, l->weight_stride, p.pack_w && pack, pw, l->type, l->in, l->out);
     t.b = side_of(l->x, l->x_stride, p.pack_x && pack, px, l->type, l->in, l->rows);
