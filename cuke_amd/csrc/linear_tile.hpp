@@ -347,8 +347,10 @@ __device__ __forceinline__ void lds_ready()
 
 // A workgroup of WA x WB waves computes XA columns by XB rows, K terms at a time.  16 bits: STAGES tiles are in LDS, in arrays of their own (so
 // that the compiler sees that the one being read is none of those being written); STAGES - 1 are requested ahead, and one barrier a tile both
-// publishes the next and frees the last.  fp32: two stages, two more tiles in
-// registers.
+// publishes the next and frees the last.  fp32: two stages, two more tiles in registers.
+// Bound by the matrix cores where sums are long: 32768 x 2048 -> 2048 bf16 plain 280 us (982 TFLOP/s; a large library product of this card 1383, both
+// held by its power), its gradients 470 (1170); fp32 8192 x 1024 -> 1024 103 us (1.0 PFLOP/s of bf16 products).  Where they are short, by waits: a
+// CU's first tiles and its epilogues, which more workgroups a CU hide.
 template <int XA_, int XB_, int K_, int WA_, int WB_, int STAGES_>
 struct Shape {
     static constexpr int XA = XA_, XB = XB_, K = K_, WA = WA_, WB = WB_, STAGES = STAGES_, kThreads = WA * WB * kWave;
@@ -542,7 +544,8 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     }
 }
 
-// y = drop(act(x W^T + b)) + residual
+// y = drop(act(x W^T + b)) + residual.  The epilogue is fused: with gelu, drop and act' kept 32768 x 2048 -> 2048 bf16 takes 333 us, 53 more than the
+// plain product, where a pass over memory of its own would take 100 or more.
 template <class T, class S, bool WHOLE>
 __global__ __launch_bounds__(S::kThreads) void linear_forward_kernel(TileArgs t)
 {
@@ -601,8 +604,9 @@ __global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, 
 
 // ---- few rows --------------------------------------------------------------------------------------
 // The forward pass of a few rows reads the weight once and does next to nothing with it, so what counts is how soon all of it is on its way: a
-// workgroup takes 16 columns and up to 64 rows, its eight waves take every eighth stretch of the sum, straight from memory into the matrix
-// cores' registers (fp32: by fp32 instructions), and join their sums in LDS.  Rows may lie anywhere.
+// workgroup takes 16 columns and 16 or 32 rows, its eight waves take every eighth stretch of the sum, straight from memory into the matrix
+// cores' registers (fp32: by fp32 instructions), and join their sums in LDS.  Rows may lie anywhere.  Bound by the latency of a launch and of two
+// loads: 1 x 1024 -> 512 bf16 3.5 us, 37 x 300 -> 200 fp32 3.4 (an empty launch takes 2).
 constexpr int kFewWaves = 8;
 
 template <class T>

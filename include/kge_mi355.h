@@ -573,7 +573,8 @@ int kge_dropout(int32_t type, const void *x, int64_t x_stride, void *y, int64_t 
  *   x [rows, in], weight [out, in], bias [out] (NULL: none) have the type `type`; y and residual [rows, out] (NULL: none), and the
  *   gradient of y, have the type `out_type`: `type` or KGE_F32.  The gradient of the residual is the gradient of y.  drop is kge_dropout of
  *   the [rows, out] block with p, seed, step, step_dev (p = 0: none).  16-bit products are summed in fp32 on the matrix cores, fp32 ones
- *   as three-part bf16 products (no larger an error against 64 bits than fp32 products); everything up to the last rounding is fp32.
+ *   as three-part bf16 products or by fp32 instructions (few rows), with no larger an error against 64 bits than fp32 products;
+ *   everything up to the last rounding is fp32.
  *   rows, in, out: 0 .. 2^31 - 1 (in = 0: an empty sum).
  */
 typedef struct kge_linear {
@@ -596,7 +597,7 @@ typedef struct kge_linear {
 /*
  * saved: NULL for inference; else kge_linear_saved_bytes() bytes, 16-byte aligned, which kge_linear_fwd fills for kge_linear_bwd: act'(z)
  * (16-bit layers: in 16 bits of fixed point, to 1.02e-5), and copies of x and weight where the matrix cores cannot take them as they lie
- * (16 bits, with rows that do not start on 16 bytes or whose width is no multiple of 8).  x and weight have to be unchanged when kge_linear_bwd runs, and *step_dev too.
+ * (16 bits, with rows that do not start on 16 bytes or whose width is no multiple of 8, or a large weight whose rows lie 4096 bytes apart).  x and weight have to be unchanged when kge_linear_bwd runs, and *step_dev too.
  * The byte counts depend on the types, sizes, strides, the low bits of addresses and whether there is an activation; a saved block of no bytes may be NULL.
  */
 size_t kge_linear_saved_bytes(const kge_linear *lin);
