@@ -60,6 +60,14 @@ def _rows(x, name: str, dtype=None, ndim: int = 2, shape=None) -> torch.Tensor:
     return x if (inner == 1 or x.shape[1] <= 1) and (outer >= x.shape[1] or x.shape[0] <= 1) else x.contiguous()
 
 
+def _apart(x, out) -> bool:
+    """Whether two blocks of equal rows are the very same one or do not overlap (as ranges of memory)."""
+    if x.data_ptr() == out.data_ptr() and (x.stride() == out.stride() or x.shape[0] <= 1):
+        return True
+    ends = [(t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _row_stride(t) + t.shape[1]) * t.element_size()) for t in (x, out)]
+    return x.numel() == 0 or ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]
+
+
 def _row_stride(x: torch.Tensor) -> int:
     """Elements between rows (of a single row: its length, whatever torch says)."""
     return x.stride(0) if x.shape[0] > 1 else max(x.stride(0), x.shape[1])
@@ -177,6 +185,7 @@ def linear_backward(fw: LinearForward, dy, need_x: bool = True, need_weight: boo
     if got is not None:
         return LinearGrads(*got)
     d = _lib.Linear.from_buffer_copy(fw.desc)
+    _tensor(x, "x of the forward call", 2)
     dy = _rows(dy, "dy", fw.y.dtype, shape=fw.y.shape)
     dx = torch.empty((d.rows, d.in_), dtype=x.dtype, device=x.device) if need_x else None
     dw = torch.empty((d.out, d.in_), dtype=x.dtype, device=x.device) if need_weight else None
@@ -207,6 +216,8 @@ def dropout(x, p, seed, step=0, out=None) -> torch.Tensor:
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     elif _rows(out, "out", x.dtype, shape=x.shape) is not out:
         raise ValueError("out must have contiguous rows: it is written in place")
+    elif not _apart(x, out):
+        raise ValueError("out must be x itself or share no memory with it")
     _lib.check(_lib.lib().kge_dropout(_TYPES[x.dtype], _p(x), _row_stride(x), _p(out), _row_stride(out), x.shape[0], x.shape[1], p, seed,
                                       step, _p(word), _stream()), "kge_dropout")
     return out

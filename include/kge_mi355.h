@@ -547,7 +547,8 @@ int kge_train_step(const kge_tables *tab, kge_step_batch *cur, const kge_step_bu
 /* ---- operators that make entity rows from features, and a loss against a frozen model --------------------------------------
  *
  * No counterpart in the reference, whose rows are always looked up.  Arrays are row-major with a stride in elements between
- * rows (>= the row's length) and consecutive elements inside a row; they may start at any element.
+ * rows (>= the row's length) and consecutive elements inside a row; they may start at any element.  Outputs share no memory with inputs or with
+ * one another, but for what a call says.
  */
 typedef enum kge_type_t { KGE_F32 = 0, KGE_BF16 = 1, KGE_F16 = 2 } kge_type_t;
 typedef enum kge_act_t {

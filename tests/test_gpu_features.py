@@ -685,3 +685,34 @@ def test_example_learns(dtype):
     losses = mod.train(steps=40, n_ent=500, batch=256, dtype=dtype)
     assert all(math.isfinite(v) for v in losses)
     assert sum(losses[-5:]) / 5 < 0.8 * losses[0]
+
+
+# (rows, in, out, options): sizes at which single tiles fill a CU, the largest tiles are used, and the gradients' sums are split into many parts
+WIDER = [(5520, 72, 130, {}), (5764, 179, 132, dict(act="gelu")), (4090, 1020, 510, dict(act="silu", drop=0.1, residual=True)),
+         (4090, 1021, 509, dict(act="gelu", drop=0.1, residual=True)), (1053, 982, 969, dict(act="gelu")), (35010, 272, 151, {}),
+         (34394, 698, 132, dict(act="gelu")), (35011, 1072, 130, dict(act="relu", residual=True)), (21508, 688, 136, dict(drop=0.1)),
+         (21508, 1333, 136, dict(act="relu", residual=True)), (16300, 1604, 1010, dict(act="gelu", drop=0.1, residual=True)),
+         (16300, 1601, 1011, dict(act="silu", drop=0.1, residual=True))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", WIDER, ids=lambda c: "%dx%dx%d%s" % (c[0], c[1], c[2], "".join("-" + str(v) for v in c[3].values())))
+def test_layer_wider_tiles(case, dtype):
+    print("wider", case, dtype, flush=True)
+    Layer(*case[:3], dtype, **case[3]).check()
+    if dtype != torch.float32 and case[3].get("residual"):
+        Layer(*case[:3], dtype, out=torch.float32, **case[3]).check()
+
+
+def test_dropout_into_what_overlaps_is_refused():
+    from cuke_amd import features
+    rows = torch.zeros(9, 16, device=DEV)
+    for x, out in [(rows[:8], rows[1:]), (rows[:, :8], rows[:, 4:12]), (rows[:4], rows.view(-1)[:128].view(4, 32)[:, :16])]:
+        with pytest.raises(ValueError):
+            features.dropout(x, 0.5, 1, out=out)
+    x = torch.randn(6, 16, device=DEV)
+    want = features.dropout(x, 0.5, 1)
+    both = torch.empty(12, 16, device=DEV)
+    both[:6] = x
+    assert torch.equal(features.dropout(both[:6], 0.5, 1, out=both[6:]), want)
+    assert features.dropout(x, 0.5, 1, out=x) is x and torch.equal(x, want)
