@@ -127,8 +127,9 @@ __global__ __launch_bounds__(256) void linear_dz_kernel(GradArgs g)
 }
 
 // ---- partial sums joined ---------------------------------------------------------------------------
-// A weight's gradient: out[row][col] = sum over n parts of part[.][row][col], a quad a thread.  Bound by memory: 4 parts of 2048 x 2048 (75 MB)
-// 18 us; below some 10 MB by its launch (3 us).
+// A weight's gradient: out[row][col] = sum over n parts of part[.][row][col].  SHARE threads take a quad, each every SHARE-th part: many parts of a
+// small gradient are many loads one after another otherwise (63 parts of 34 x 102: 7.2 us with one, 4.0 with eight).  Bound by memory where the
+// gradient is large: 4 parts of 2048 x 2048 (75 MB) 18 us.
 struct JoinArgs {
     const float *part;
     int64_t rows, cols, quads;
@@ -136,18 +137,32 @@ struct JoinArgs {
     void *out;
 };
 
-template <class T>
+template <class T, int SHARE>
 __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, each = j.rows * j.quads;
-    if (i >= each) return;
+    __shared__ float4 sums[SHARE > 1 ? 256 : 1];
+    constexpr int kQuads = 256 / SHARE;
+    const int64_t i = (int64_t)blockIdx.x * kQuads + threadIdx.x % kQuads, each = j.rows * j.quads;
     float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    const float4 *p = reinterpret_cast<const float4 *>(j.part) + i;
+    if (i < each) {
+        const float4 *p = reinterpret_cast<const float4 *>(j.part) + i;
 #pragma unroll 4
-    for (int k = 0; k < j.n; ++k) {
-        const float4 v = p[k * each];
-        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        for (int k = threadIdx.x / kQuads; k < j.n; k += SHARE) {
+            const float4 v = p[k * each];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
     }
+    if constexpr (SHARE > 1) {
+        sums[threadIdx.x] = s;
+        __syncthreads();
+        if (threadIdx.x >= kQuads) return;
+#pragma unroll
+        for (int k = 1; k < SHARE; ++k) {
+            const float4 v = sums[threadIdx.x + k * kQuads];
+            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+    }
+    if (i >= each) return;
     const int64_t row = i / j.quads, col = 4 * (i % j.quads), left = j.cols - col;
     store4(static_cast<T *>(j.out) + row * j.cols + col, s, (int)(left < 4 ? left : 4));
 }
@@ -161,7 +176,9 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 //    4096 x 1024 -> 512, gelu and drop           45  18   15  [12]  13         2500 x 520 -> 264, gelu and drop  36  19  12   9  [8]
 // Lone's four stages keep a CU busy that has one tile.  Middle has eight waves (four: 27.6 us where it takes 25.6, 16384 x 768 -> 512) and shorter
 // stages in the gradients, whose epilogue is short (8192 x 768 -> 512 38.7 and 36.1 us); Tall is slower with eight (20000 x 304 -> 800 40 and 44).
-// fp32 (MiddleF, SmallF): 4033 x 1200 -> 1352 [117] 131; 8192 x 1024 -> 1024 [110] 140; 4096 x 512 -> 256 26 [18]; 2048 x 1024 -> 1024 47 [40].
+// fp32 (MiddleF, SmallF, DeepF): 4033 x 1200 -> 1352 [117] 131; 8192 x 1024 -> 1024 [110] 140; 8192 x 768 -> 512 [45] 45 62; 2048 x 1024 -> 1024 47
+// [40]; 851 x 1968 -> 1016 48 [34]; 2500 x 520 -> 264 17 [13]; 27717 x 102 -> 34 [12] 15.  DeepF's eight waves share a tile's terms in halves, so
+// that a CU with one tile has two waves a SIMD to hide splitting and waits; the same in 16 bits loses to Small (2500 x 520 -> 264 7.0 and 7.3).
 using Large = Shape<256, 256, 32, 2, 4, 4>;
 using Middle = Shape<128, 128, 64, 2, 4, 2>;
 using MiddleG = Shape<128, 128, 32, 2, 4, 4>;
@@ -170,6 +187,7 @@ using Lone = Shape<64, 128, 64, 2, 4, 4>;
 using Small = Shape<64, 64, 64, 2, 2, 3>;
 using MiddleF = Shape<128, 128, 32, 2, 4, 2>;
 using SmallF = Shape<64, 64, 32, 2, 2, 2>;
+using DeepF = Shape<64, 64, 64, 2, 2, 2, 2>;
 
 static int64_t tiles_of(int64_t a, int64_t b, int x) { return ceil_div(a, x) * ceil_div(b, x); }
 
@@ -200,8 +218,10 @@ static void launch_forward(TileArgs &t, hipStream_t st)
     const int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
     if constexpr (sizeof(T) == 4) {
         const bool whole = t.k % 4 == 0;
-        if (forward_cost<MiddleF>(t, epilogue, 1, 1.0, 1.0) <= forward_cost<SmallF>(t, epilogue, 3, 0.7, 0.7))
-            whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
+        const double middle = forward_cost<MiddleF>(t, epilogue, 1, 1.0, 1.0), small = forward_cost<SmallF>(t, epilogue, 3, 0.7, 0.7);
+        const double deep = forward_cost<DeepF>(t, epilogue, 1, 0.55, 0.55);
+        if (deep < middle && deep < small) whole ? launch_forward<T, DeepF, true>(t, st) : launch_forward<T, DeepF, false>(t, st);
+        else if (middle <= small) whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
         else whole ? launch_forward<T, SmallF, true>(t, st) : launch_forward<T, SmallF, false>(t, st);
     } else {
         const double large = forward_cost<Large>(t, epilogue, 1, 1.0, 1.0), middle = forward_cost<Middle>(t, epilogue, 2, 0.73, 2.5);
@@ -244,6 +264,7 @@ static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k,
 // of tiles of 64 17, in 6 of 128 22; 3000 x 700 -> 1000 fp32 in 2 parts 80, in 3 100.
 struct GradPlan {
     int tile, dw_splits;  // tile: 256, 128 or 64
+    bool deep;            // DeepF
 };
 // When n jobs of length a each, then m of length b, are done by `slots` workers.
 static double jobs_end(int64_t n, double a, int64_t m, double b, int64_t slots)
@@ -263,15 +284,16 @@ static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
         int tile, slots;
         double a_term, besides;  // us
         double alone;            // how much longer a long sum takes where nothing else hides its waits
+        bool deep;
     };
-    static const Pace kHalf[] = {{64, 256, 0.0026, 1.0, 2.3}, {128, 256, 0.0066, 3.0, 1.4}, {256, 256, 0.0260, 8.1, 1.0}};
-    static const Pace kFloat[] = {{64, 512, 0.0268, 3.5, 1.0}, {128, 256, 0.0393, 6.7, 1.0}};
+    static const Pace kHalf[] = {{64, 256, 0.0026, 1.0, 2.3, false}, {128, 256, 0.0066, 3.0, 1.4, false}, {256, 256, 0.0260, 8.1, 1.0, false}};
+    static const Pace kFloat[] = {{64, 512, 0.0268, 3.5, 1.0, false}, {128, 256, 0.0393, 6.7, 1.0, false}, {64, 256, 0.0165, 5.0, 1.0, true}};
     const bool f32 = type == KGE_F32;
     const Pace *paces = f32 ? kFloat : kHalf;
     const double parts_launch = f32 ? 7.0 : 5.0, part = (double)out * (double)in * 8.0 / (f32 ? 16e6 : 40e6);  // us
-    GradPlan best{64, 1};
+    GradPlan best{64, 1, false};
     double best_end = INFINITY;
-    for (int i = 0; i < (f32 ? 2 : 3); ++i) {
+    for (int i = 0; i < 3; ++i) {
         const Pace &p = paces[i];
         const int64_t dw = tiles_of(out, in, p.tile), dx = tiles_of(rows, in, p.tile);
         for (int parts = 1; parts <= 64; parts += parts < 8 ? 1 : parts / 4) {
@@ -280,7 +302,7 @@ static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
             double end = jobs_end(dw * ceil_div(rows, each > 0 ? each : 1), (double)each * p.a_term + p.besides, dx, (double)out * p.a_term + p.besides, p.slots);
             end = std::max(end, p.alone * (double)each * p.a_term);
             if (parts > 1) end += parts_launch + parts * part;
-            if (end < best_end) best_end = end, best = GradPlan{p.tile, parts};
+            if (end < best_end) best_end = end, best = GradPlan{p.tile, parts, p.deep};
         }
     }
     return best;
@@ -296,15 +318,16 @@ static void launch_grads(TileArgs &dw, TileArgs &dx, const SumArgs &db, bool wan
 }
 
 template <class T>
-static void launch_grads(int tile, TileArgs &dw, TileArgs &dx, const SumArgs &db, bool want_dw, bool want_dx, hipStream_t st)
+static void launch_grads(const GradPlan &g, TileArgs &dw, TileArgs &dx, const SumArgs &db, bool want_dw, bool want_dx, hipStream_t st)
 {
     if constexpr (sizeof(T) == 4) {
         const bool whole = dw.a.extent % 4 == 0 && dw.b.extent % 4 == 0;  // in and out
-        if (tile == 128) whole ? launch_grads<T, MiddleF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, MiddleF, false>(dw, dx, db, want_dw, want_dx, st);
+        if (g.deep) whole ? launch_grads<T, DeepF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, DeepF, false>(dw, dx, db, want_dw, want_dx, st);
+        else if (g.tile == 128) whole ? launch_grads<T, MiddleF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, MiddleF, false>(dw, dx, db, want_dw, want_dx, st);
         else whole ? launch_grads<T, SmallF, true>(dw, dx, db, want_dw, want_dx, st) : launch_grads<T, SmallF, false>(dw, dx, db, want_dw, want_dx, st);
     } else {
-        if (tile == 256) launch_grads<T, Large>(dw, dx, db, want_dw, want_dx, st);
-        else if (tile == 128) launch_grads<T, MiddleG>(dw, dx, db, want_dw, want_dx, st);
+        if (g.tile == 256) launch_grads<T, Large>(dw, dx, db, want_dw, want_dx, st);
+        else if (g.tile == 128) launch_grads<T, MiddleG>(dw, dx, db, want_dw, want_dx, st);
         else launch_grads<T, Small>(dw, dx, db, want_dw, want_dx, st);
     }
 }
@@ -425,11 +448,12 @@ static int backward(const kge_linear *l, const Plan &p, const GradPlan &g, const
     tw.k = l->rows, tw.splits = g.dw_splits, tw.k_each = split_length(l->rows, tw.splits);
     tw.partial = tw.splits > 1 ? part : nullptr;
     tw.e.y = dw, tw.e.y_stride = l->in, tw.e.rows = l->out, tw.e.cols = l->in, tw.e.quads = in_quads;
-    launch_grads<T>(g.tile, tw, tx, SumArgs{sums, p.sum_blocks, l->out, p.quads, db}, dw != nullptr, dx != nullptr, st);
+    launch_grads<T>(g, tw, tx, SumArgs{sums, p.sum_blocks, l->out, p.quads, db}, dw != nullptr, dx != nullptr, st);
     if (dw && tw.partial) {
         const JoinArgs j{part, l->out, l->in, in_quads, tw.splits, dw};
-        const int64_t blocks = ceil_div(j.rows * j.quads, 256);
-        if (blocks) hipLaunchKernelGGL(linear_join_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, st, j);
+        const int64_t quads = j.rows * j.quads;
+        if (quads && quads <= 65536 && j.n >= 8) hipLaunchKernelGGL((linear_join_kernel<T, 8>), dim3((unsigned)ceil_div(quads, 32)), dim3(256), 0, st, j);
+        else if (quads) hipLaunchKernelGGL((linear_join_kernel<T, 1>), dim3((unsigned)ceil_div(quads, 256)), dim3(256), 0, st, j);
     }
     KGE_CHECK_LAUNCH();
     return KGE_OK;

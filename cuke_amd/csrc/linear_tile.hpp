@@ -83,7 +83,7 @@ struct Tile {
 
     __device__ __forceinline__ static int turn(int row)
     {
-        if (!ACROSS) return K == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
+        if (!ACROSS) return K == 128 ? row & 15 : (K == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
         return X >= 256 ? 2 * (2 * (row & 3) + 8 * ((row >> 3) & 1)) : (X >= 128 ? 4 * (row & 3) : 2 * (row & 3));
     }
 
@@ -347,13 +347,14 @@ __device__ __forceinline__ void lds_ready()
 
 // A workgroup of WA x WB waves computes XA columns by XB rows, K terms at a time.  16 bits: STAGES tiles are in LDS, in arrays of their own (so
 // that the compiler sees that the one being read is none of those being written); STAGES - 1 are requested ahead, and one barrier a tile both
-// publishes the next and frees the last.  fp32: two stages, two more tiles in registers.
+// publishes the next and frees the last.  fp32: two stages, two more tiles in registers.  SHARE > 1: as many groups of WA x WB waves each multiply
+// their share of every tile's terms, and join their sums in LDS before the epilogue.
 // Bound by the matrix cores where sums are long: 32768 x 2048 -> 2048 bf16 plain 280 us (982 TFLOP/s; a large library product of this card 1383, both
 // held by its power), its gradients 470 (1170); fp32 8192 x 1024 -> 1024 103 us (1.0 PFLOP/s of bf16 products).  Where they are short, by waits: a
 // CU's first tiles and its epilogues, which more workgroups a CU hide.
-template <int XA_, int XB_, int K_, int WA_, int WB_, int STAGES_>
+template <int XA_, int XB_, int K_, int WA_, int WB_, int STAGES_, int SHARE_ = 1>
 struct Shape {
-    static constexpr int XA = XA_, XB = XB_, K = K_, WA = WA_, WB = WB_, STAGES = STAGES_, kThreads = WA * WB * kWave;
+    static constexpr int XA = XA_, XB = XB_, K = K_, WA = WA_, WB = WB_, STAGES = STAGES_, SHARE = SHARE_, kThreads = WA * WB * SHARE * kWave;
 };
 template <class T, class S>
 constexpr int stage_bytes() { return (S::XA + S::XB) * S::K * 2 * (sizeof(T) == 4 ? kSplitParts : 1); }
@@ -365,7 +366,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
 {
     constexpr bool kFloat = sizeof(T) == 4;
     using E = typename std::conditional<kFloat, bf16_t, T>::type;
-    constexpr int PLANES = kFloat ? kSplitParts : 1, K = S::K, STAGES = S::STAGES, WA = S::WA, WB = S::WB;
+    constexpr int PLANES = kFloat ? kSplitParts : 1, K = S::K, STAGES = S::STAGES, WA = S::WA, WB = S::WB, SHARE = S::SHARE;
     using A = Tile<S::XA, K, A_ACROSS, S::kThreads>;
     using B = Tile<S::XB, K, B_ACROSS, S::kThreads>;
     constexpr int kBytesA = S::XA * K * 2, kBytesB = S::XB * K * 2, kStage = stage_bytes<T, S>();
@@ -377,7 +378,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     const int64_t n0 = (int64_t)ta * S::XA, m0 = (int64_t)tb * S::XB;
     const int64_t k0 = split * t.k_each, k1 = k0 + t.k_each < t.k ? k0 + t.k_each : t.k;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wa = (wave % WA) * (S::XA / WA), wb = (wave / WA) * (S::XB / WB);
+    const int wa = (wave % WA) * (S::XA / WA), wb = (wave / WA % WB) * (S::XB / WB), part = SHARE > 1 ? wave / (WA * WB) : 0;  // of every tile's terms
 
     floatx16 acc[FA][FB] = {}, low[kFloat ? FA : 1][kFloat ? FB : 1] = {};
     int64_t left = k1 - k0;  // terms not requested yet
@@ -385,7 +386,8 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
     auto multiply = [&](const char *lds) {
 #pragma unroll
-        for (int step = 0; step < K / 16; ++step) {
+        for (int u = 0; u < K / 16 / SHARE; ++u) {
+            const int step = part * (K / 16 / SHARE) + u;
             s16x8 a[FA][PLANES], b[FB][PLANES];
 #pragma unroll
             for (int p = 0; p < PLANES; ++p) {
@@ -462,10 +464,11 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.  A
     // strip's residuals are requested all at once and ahead of everything else that is done with it.
     constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16, kPerStage = kStage / kStrip;
-    constexpr int kApart = 64 / kQuads, kRows = 4, kTurns = 32 / (kApart * kRows);  // rows a read covers, reads a turn, turns a strip
+    constexpr int kApart = 64 / kQuads, kRows = 4 / SHARE, kTurns = 32 / (kApart * kRows * SHARE);  // rows a read covers, reads a turn, turns of a wave in a strip
     constexpr int kStrips = FA / kGroup * FB;
     static_assert(FA % kGroup == 0 && kPerStage >= 1 && (WA * WB + kPerStage - 1) / kPerStage <= STAGES, "a strip for every wave");
-    const int quad = lane % kQuads, row0 = lane / kQuads;
+    static_assert(SHARE == 1 || (kStrips == 1 && kPerStage >= SHARE * WA * WB), "waves that share a strip");
+    const int quad = lane % kQuads, row0 = lane / kQuads + part * kTurns * kApart * kRows;
     const bool ahead = LAYER && t.e.residual && t.e.cols % 4 == 0;
     Raw4 held[kTurns][kRows];
     auto column = [&](int strip) { return n0 + wa + strip / FB * 32 * kGroup + 4 * quad; };
@@ -511,6 +514,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                     *reinterpret_cast<float4 *>(lds + 16 * (row * kQuads + (at ^ skew(row)))) = make_float4(z[0], z[1], z[2], z[3]);
                 }
         }
+        if constexpr (SHARE > 1) lds_ready();  // (one strip: nothing is written to again)
         if (valid <= 0) continue;
 #pragma unroll
         for (int u = 0; u < kTurns; ++u) {
@@ -519,7 +523,13 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
 #pragma unroll
             for (int k = 0; k < kRows; ++k) {
                 const int r = row0 + (u * kRows + k) * kApart;
-                float4 v = *reinterpret_cast<const float4 *>(lds + 16 * (r * kQuads + (quad ^ skew(r))));
+                const char *from = (SHARE > 1 ? stage0 + wave % (WA * WB) * kStrip : lds) + 16 * (r * kQuads + (quad ^ skew(r)));
+                float4 v = *reinterpret_cast<const float4 *>(from);
+#pragma unroll
+                for (int p = 1; p < SHARE; ++p) {
+                    const float4 more = *reinterpret_cast<const float4 *>(from + p * WA * WB * kStrip);
+                    v.x += more.x, v.y += more.y, v.z += more.z, v.w += more.w;
+                }
                 if constexpr (kFloat) {
                     // (an infinite operand's parts, or leading parts that were rounded up, may have made this of a finite sum)
                     const int64_t row = first + k * kApart;

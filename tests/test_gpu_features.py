@@ -716,3 +716,33 @@ def test_dropout_into_what_overlaps_is_refused():
     both[:6] = x
     assert torch.equal(features.dropout(both[:6], 0.5, 1, out=both[6:]), want)
     assert features.dropout(x, 0.5, 1, out=x) is x and torch.equal(x, want)
+
+
+# (rows, in, out, options): a CU's only tile, whose terms the waves share (fp32), and many parts of a small weight's gradient
+SHARED = [(851, 1968, 1016, {}), (2500, 520, 264, dict(act="gelu", drop=0.1)), (2500, 523, 261, dict(act="silu", residual=True)),
+          (513, 768, 400, dict(act="gelu")), (701, 509, 699, dict(act="relu", drop=0.1, residual=True)), (27717, 102, 34, dict(act="silu", residual=True)),
+          (30000, 64, 64, {}), (30001, 65, 63, dict(act="gelu"))]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", SHARED, ids=lambda c: "%dx%dx%d%s" % (c[0], c[1], c[2], "".join("-" + str(v) for v in c[3].values())))
+def test_layer_shared_tiles_and_many_parts(case, dtype):
+    print("shared", case, dtype, flush=True)
+    Layer(*case[:3], dtype, **case[3]).check()
+
+
+def test_layer_shared_tiles_with_infinities():
+    """fp32 sums that are formed again where the parts of an infinite operand cancel, in tiles whose terms two groups of waves share."""
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(5)
+    x, w = torch.randn(2500, 520, generator=g).to(DEV), torch.randn(264, 520, generator=g).to(DEV)
+    x[17, 3], x[600, 519], x[2499, 260], x[40, 0] = float("inf"), float("-inf"), float("nan"), 3e38
+    w[:, 0] = 0.0
+    w[5, 3] = 0.0
+    y = features.linear(x, w)
+    want = x.double() @ w.double().T
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(y[inf].double(), want[inf])
+    fine = torch.isfinite(want)
+    tol = (520 + 16) * EPS * (torch.nan_to_num(x, 0.0, 0.0, 0.0).double().abs() @ w.double().abs().T + 1.0) + EPS * want.abs()
+    assert bool(((y.double() - want).abs() <= tol)[fine].all())
