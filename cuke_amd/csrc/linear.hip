@@ -257,11 +257,12 @@ static void launch_few(int few, const TileArgs &t, hipStream_t st)
 
 static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k, splits), 64) * 64; }
 
-// The tiles of a backward pass and the parts that dW's sums over rows are split into: what is expected to end first.  dW's workgroups start first,
-// `slots` at a time, dx's fill what they leave; a tile takes so many ns a term and some us besides, and parts cost a launch, and bytes written and
-// read.  The paces are those that fit some six plans of each of 17 sizes, within 8 % on average.  Some of what they decide (us): 65536 x 256 -> 128
-// bf16 in 33 parts 41, in 128 49; 16384 x 768 -> 512 in tiles of 128 54, of 256 64; 32768 x 2048 -> 2048 745 and 632; 1500 x 4000 -> 120 in one part
-// of tiles of 64 17, in 6 of 128 22; 3000 x 700 -> 1000 fp32 in 2 parts 80, in 3 100.
+// The tiles of a backward pass and the parts that dW's sums over rows are split into: what is expected to end first.  Workgroups for the longer
+// sums start first, `slots` at a time, the others fill what they leave; a tile takes so many us a term and some besides, and parts cost a launch, and
+// bytes written and read.  The paces are those that fit some six plans of each of 17 sizes, within 8 % on average.  Some of what they decide (us):
+// 65536 x 256 -> 128 bf16 in 33 parts 41, in 128 49; 16384 x 768 -> 512 in tiles of 128 54, of 256 64; 32768 x 2048 -> 2048 745 and 632; 1500 x 4000
+// -> 120 in one part of tiles of 64 17, in 6 of 128 22; fp32 9000 x 100 -> 1500 with dx's longer sums first 95, with dW's 105; 512 x 768 -> 400 in DeepF's
+// tiles 16, in SmallF's 20.
 struct GradPlan {
     int tile, dw_splits;  // tile: 256, 128 or 64
     bool deep;            // DeepF
@@ -296,11 +297,13 @@ static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
     for (int i = 0; i < 3; ++i) {
         const Pace &p = paces[i];
         const int64_t dw = tiles_of(out, in, p.tile), dx = tiles_of(rows, in, p.tile);
+        const double b = (double)out * p.a_term + p.besides;
         for (int parts = 1; parts <= 64; parts += parts < 8 ? 1 : parts / 4) {
-            const int64_t each = split_length(rows, parts);
+            const int64_t each = split_length(rows, parts), n = dw * ceil_div(rows, each > 0 ? each : 1);
             if (parts > 1 && each < 128) break;
-            double end = jobs_end(dw * ceil_div(rows, each > 0 ? each : 1), (double)each * p.a_term + p.besides, dx, (double)out * p.a_term + p.besides, p.slots);
-            end = std::max(end, p.alone * (double)each * p.a_term);
+            const double a = (double)each * p.a_term + p.besides;
+            double end = out > each ? jobs_end(dx, b, n, a, p.slots) : jobs_end(n, a, dx, b, p.slots);
+            end = std::max(end, p.alone * (double)std::max(each, out) * p.a_term);
             if (parts > 1) end += parts_launch + parts * part;
             if (end < best_end) best_end = end, best = GradPlan{p.tile, parts, p.deep};
         }

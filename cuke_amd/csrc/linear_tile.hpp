@@ -599,17 +599,17 @@ __device__ __forceinline__ void join_sums(const SumArgs &j, int64_t block, float
     store4(static_cast<T *>(j.out) + 4 * quad, s, (int)(left < 4 ? left : 4));
 }
 
-// dW = dz^T x, dx = dz W and the bias's gradient in one launch: the first `dw_blocks` workgroups, which have the longer sums, take dW, the next
-// `dx_blocks` dx, the rest join the column sums that the kernel before this one has left.
+// dW = dz^T x, dx = dz W and the bias's gradient in one launch: workgroups for the longer sums start first, the last ones join the column sums that
+// the kernel before this one has left.
 template <class T, class S, bool WHOLE>
 __global__ __launch_bounds__(S::kThreads) void linear_grads_kernel(TileArgs dw, TileArgs dx, SumArgs db, int64_t dw_blocks, int64_t dx_blocks)
 {
     constexpr int kStage = stage_bytes<T, S>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
-    const int64_t block = blockIdx.x;
-    if (block < dw_blocks) compute_tile<T, true, true, S, false, WHOLE>(dw, block, dw_blocks, stage0, stage1, stage2, stage3);
-    else if (block < dw_blocks + dx_blocks) compute_tile<T, true, false, S, false, WHOLE>(dx, block - dw_blocks, dx_blocks, stage0, stage1, stage2, stage3);
-    else join_sums<T, S::kThreads>(db, block - dw_blocks - dx_blocks, reinterpret_cast<float4 *>(stage0));
+    const int64_t block = blockIdx.x, products = dw_blocks + dx_blocks, before = dx.k > dw.k_each ? dx_blocks : 0;  // dx's in front of dW's
+    if (block >= products) join_sums<T, S::kThreads>(db, block - products, reinterpret_cast<float4 *>(stage0));
+    else if (block >= before && block < before + dw_blocks) compute_tile<T, true, true, S, false, WHOLE>(dw, block - before, dw_blocks, stage0, stage1, stage2, stage3);
+    else compute_tile<T, true, false, S, false, WHOLE>(dx, before ? block : block - dw_blocks, dx_blocks, stage0, stage1, stage2, stage3);
 }
 
 // ---- few rows --------------------------------------------------------------------------------------
