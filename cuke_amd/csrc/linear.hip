@@ -201,8 +201,8 @@ static void launch_forward(TileArgs &t, hipStream_t st)
 
 // What a forward pass costs in tiles of a shape: rounds over the card, times the tiles a round holds on a CU (`share` at most), times a tile's area,
 // times its terms and its epilogue's worth of terms (64 for a byte moved an element, 192 for gelu or silu and 192 for dropping), each at the shape's
-// pace beside the largest tiles'; a CU that holds fewer tiles than it could waits more.  Over 15 sizes, each with three epilogues, the shape chosen
-// takes 0.4 % longer than the best one on average, and 13 % at most.
+// pace beside the largest tiles'; a CU that holds fewer tiles than it could waits more.  Over 24 sizes, each with six epilogues, the shape chosen
+// takes 1 % longer than the best one on average, and 28 % at most.
 template <class S>
 static double forward_cost(const TileArgs &t, int64_t epilogue, int share, double pace, double epilogue_pace)
 {
@@ -224,7 +224,8 @@ static void launch_forward(TileArgs &t, hipStream_t st)
         else if (middle <= small) whole ? launch_forward<T, MiddleF, true>(t, st) : launch_forward<T, MiddleF, false>(t, st);
         else whole ? launch_forward<T, SmallF, true>(t, st) : launch_forward<T, SmallF, false>(t, st);
     } else {
-        const double large = forward_cost<Large>(t, epilogue, 1, 1.0, 1.0), middle = forward_cost<Middle>(t, epilogue, 2, 0.73, 2.5);
+        // (a residual hides behind nothing in the largest tiles: 30198 x 488 -> 1392, plain and with one, 90 and 124 us; Middle 91 and 95)
+        const double large = forward_cost<Large>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0), middle = forward_cost<Middle>(t, epilogue, 2, 0.73, 2.5);
         const double tall = forward_cost<Tall>(t, epilogue, 3, 0.53, 2.3), small = forward_cost<Small>(t, epilogue, 3, 0.47, 0.9);
         const double lone = forward_cost<Lone>(t, epilogue, 1, 0.41, 0.9);
         if (lone < large && lone < middle && lone < tall && lone < small) launch_forward<T, Lone>(t, st);

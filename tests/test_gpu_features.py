@@ -746,3 +746,12 @@ def test_layer_shared_tiles_with_infinities():
     fine = torch.isfinite(want)
     tol = (520 + 16) * EPS * (torch.nan_to_num(x, 0.0, 0.0, 0.0).double().abs() @ w.double().abs().T + 1.0) + EPS * want.abs()
     assert bool(((y.double() - want).abs() <= tol)[fine].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", [(16380, 2052, 1020, dict(act="silu", drop=0.1, residual=True)), (16380, 2049, 1019, dict(act="silu", drop=0.1, residual=True)),
+                                  (16380, 1604, 1020, dict(residual=True))], ids=lambda c: "%dx%dx%d" % c[:3])
+def test_layer_largest_tiles_with_residuals(case, dtype):
+    print("largest", case, dtype, flush=True)
+    for out in (dtype, torch.float32):
+        Layer(*case[:3], dtype, out=out, **case[3]).check()
