@@ -53,6 +53,7 @@ struct Ends {
     Drop drop;
     int act;
     int out_f32;  // y and residual in fp32
+    int passing;  // y, in fp32 and its quads on 16 bytes, is written past the caches
 };
 
 struct TileArgs {
@@ -309,6 +310,10 @@ __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64
         const int64_t row = first + r * apart, at = row * e.y_stride + col;
         if (row >= e.rows) continue;
         const float4 v = make_float4(z[r][0], z[r][1], z[r][2], z[r][3]);
+        if (e.passing && valid >= 4) {
+            __builtin_nontemporal_store(f4{v.x, v.y, v.z, v.w}, reinterpret_cast<f4 *>(static_cast<float *>(e.y) + at));
+            continue;
+        }
         if (sizeof(T) == 4 || e.out_f32) store4(static_cast<float *>(e.y) + at, v, valid);
         else store4(static_cast<T *>(e.y) + at, v, valid);
     }

@@ -755,3 +755,10 @@ def test_layer_largest_tiles_with_residuals(case, dtype):
     print("largest", case, dtype, flush=True)
     for out in (dtype, torch.float32):
         Layer(*case[:3], dtype, out=out, **case[3]).check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", [(33001, 72, 512, dict(act="gelu", drop=0.1, residual=True)), (33001, 70, 528, {})], ids=lambda c: "%dx%dx%d" % c[:3])
+def test_layer_large_fp32_outputs(case, dtype):
+    print("large output", case, dtype, flush=True)
+    Layer(*case[:3], dtype, out=torch.float32, **case[3]).check()
