@@ -35,11 +35,13 @@ __device__ __forceinline__ float prefer(const PreferArgs &a, float d, float *slo
         return z < 1.0f ? 1.0f - z : 0.0f;
     }
     // log(1 + exp(-z)) = max(-z, 0) + log(1 + e), e = exp(-|z|); what 1 + e rounds away is put back to first order, so that pairs far apart keep
-    // their small loss; sigma(-z) without cancellation
+    // their small loss; sigma(-z) without cancellation.  Of the two terms in |z| one is zero; a term whose factor is zero is not there, however
+    // large z is
     const float e = __builtin_amdgcn_exp2f(-1.44269504f * fabsf(z)), u = 1.0f + e, inv = __builtin_amdgcn_rcpf(u);
     const float soft = fmaf(e - (u - 1.0f), inv, 0.69314718f * __builtin_amdgcn_logf(u));
     *slope = a.beta * (a.smoothing - (z > 0.0f ? e : 1.0f) * inv);
-    return soft + (1.0f - a.smoothing) * fmaxf(-z, 0.0f) + a.smoothing * fmaxf(z, 0.0f);
+    const float share = z > 0.0f ? a.smoothing : 1.0f - a.smoothing;
+    return share != 0.0f ? fmaf(share, fabsf(z), soft) : soft;
 }
 
 // Sums and maxima over the lanes that share a row: `lanes` of a wave, or a whole workgroup of four waves.

@@ -1,0 +1,117 @@
+"""Linear layers, dropout and the preference loss where values, sizes or memory are at the edge of what they take.
+
+Tolerances as in test_gpu_features.py, element by element (EPS = 2^-24), from the roundings a result goes through; infinities and NaN have to stand
+where the formulas in 64 bits have them.  There a pair without a share adds nothing, also where its own loss is infinite.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS, LEAST = 2.0 ** -24, 2.0 ** -126         # (LEAST: what is smaller may become zero)
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = "cuda:0"
+
+
+def draw(gen, shape, dtype, scale=1.0):
+    return (torch.randn(shape, generator=gen, dtype=torch.float64) * scale).to(DEV).to(dtype)
+
+
+def like(got, want, tol, what):
+    """The same infinities and NaN, and finite values within tol."""
+    got = got.double()
+    assert got.shape == want.shape, what
+    assert torch.equal(torch.isnan(got), torch.isnan(want)), what
+    assert torch.equal(got[torch.isinf(got)], want[torch.isinf(want)]) and torch.equal(torch.isinf(got), torch.isinf(want)), what
+    off = torch.isfinite(want) & ~((got - want).abs() <= tol.expand_as(want))
+    if off.any():
+        i = tuple(torch.nonzero(off)[0].tolist())
+        raise AssertionError(f"{what}: {int(off.sum())} of {off.numel()} off, first at {i}: {got[i].item()} for {want[i].item()} +- {tol.expand_as(want)[i].item()}")
+
+
+# ---- preference loss -------------------------------------------------------------------------------
+def prefer64(pos, neg, rpos=None, rneg=None, *, beta=1.0, kind="sigmoid", smoothing=0.0, temperature=0.0, sign=1.0, mask=None):
+    """(loss, dpos, dneg) and their tolerances."""
+    pos, neg = pos.double(), neg.double()
+    on = torch.ones_like(neg, dtype=torch.bool) if mask is None else mask.bool()
+    zero = torch.zeros_like(neg)
+    n = torch.where(on, neg, zero)
+    rp = torch.zeros_like(pos) if rpos is None else rpos.double()
+    rn = zero if rneg is None else torch.where(on, rneg.double(), zero)
+    d = sign * ((pos - rp)[:, None] - (n - rn))
+    z = beta * d
+    # sizes of what is rounded; scores at the end of the range saturate, and what they come to is exact
+    small = lambda v: torch.where(v.abs() < 1e4, v.abs(), torch.zeros_like(v))
+    d_tol = 2 * EPS * (small(pos)[:, None] + small(n) + small(rp)[:, None] + small(rn))
+    z_tol = beta * d_tol
+    if kind == "sigmoid":
+        part = lambda c, v: c * torch.where(v > 0, v + torch.log1p(torch.exp(-v)), torch.log1p(torch.exp(v))) if c else zero
+        f = part(1 - smoothing, -z) + part(smoothing, z) + 0.0 * torch.where(torch.isnan(z), z, zero)
+        s = beta * (smoothing - torch.sigmoid(-z))
+        f_tol, s_tol = z_tol + 16 * EPS * (1 + small(z)), beta * (z_tol / 4 + 16 * EPS * (1 + small(z)))
+    elif kind == "hinge":
+        f, s = torch.clamp(1 - z, min=0), torch.where(z >= 1, zero, torch.where(z < 1, zero - beta, z))
+        f_tol = z_tol + 8 * EPS * (1 + small(z))
+        s_tol = torch.where((1 - z).abs() <= f_tol, beta, 2 * EPS * beta).to(z)
+    else:
+        f, s = (d - 0.5 / beta) ** 2, 2 * (d - 0.5 / beta)
+        s_tol = 2 * d_tol + 8 * EPS * (small(d) + 0.5 / beta)
+        f_tol = s_tol * small(s) + s_tol ** 2
+    B, N = n.shape
+    if temperature:
+        u = torch.where(on, sign * n, zero - math.inf)
+        top = u.amax(1, keepdim=True)
+        t = temperature * (u - torch.where(top == -math.inf, torch.zeros_like(top), top))
+        e = torch.where(on, torch.exp(t), zero)
+    else:
+        t, e = zero, on.double()
+    total = e.sum(1, keepdim=True)
+    a = torch.where(total == 0, zero, e / total)
+    # a weight: the difference, its product and the exponential; the sum of N of them
+    a_tol = a * (8 * EPS * (1 + torch.where(torch.isfinite(t), t.abs(), zero)) + (N + 16) * EPS) + LEAST * (a > 0)
+
+    def times(w, v):
+        return torch.where((w == 0) & torch.isinf(v) | ~on, zero, w * v)
+    loss = times(a, f).sum() / B
+    loss_tol = (times(a_tol, f.abs()) + a * f_tol + (N + 16) * EPS * times(a, f.abs())).nan_to_num(0, 0, 0).sum() / B + 2 * EPS * loss.abs()
+    g = sign * times(a, s) / B
+    g_tol = (times(a_tol, s.abs()) + a * s_tol) / B + 8 * EPS * g.abs() + LEAST * (a > 0)
+    return loss.view(1), g.sum(1), -g, loss_tol.view(1), g_tol.sum(1) + (N + 16) * EPS * g.abs().sum(1), g_tol
+
+
+def check_prefer(pos, neg, rpos=None, rneg=None, **kw):
+    from cuke_amd import features
+    loss, dpos, dneg = features.preference_loss(pos, neg, rpos, rneg, **kw)
+    want = prefer64(pos, neg, rpos, rneg, **kw)
+    like(loss, want[0], want[3], "loss")
+    like(dpos, want[1], want[4], "dpos")
+    like(dneg, want[2], want[5], "dneg")
+    return loss, dpos, dneg
+
+
+# one lane to a row and more, all quads a lane holds, and segments with and without a pass for the weights' sums
+WIDTHS = [1, 7, 300, 700, 2051]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_sigmoid_of_infinite_scores(n, sign, dtype):
+    """-log sigma(infinity) is 0, whatever the factor of a term that is not there: filters leave infinite scores where there is no mask."""
+    g = torch.Generator().manual_seed(n)
+    pos, neg = draw(g, (6,), dtype, 2.0), draw(g, (6, n), dtype, 2.0)
+    neg[1, n // 2] = neg[2, 0] = -sign * math.inf       # the better the lower they are: no loss, no gradient
+    pos[4] = sign * math.inf
+    for kw in (dict(sign=sign), dict(sign=sign, mask=torch.ones(6, n, device=DEV, dtype=torch.bool))):
+        loss, dpos, dneg = check_prefer(pos, neg, beta=0.5, **kw)
+        assert bool(torch.isfinite(loss)) and dneg[1, n // 2] == 0 and not dneg[4].any() and dpos[4] == 0
+        # the other side: all weight on the flipped labels
+        check_prefer(-pos, -neg, beta=0.5, smoothing=1.0, **kw)
+        # labels that are not certain make the loss infinite, the gradient stays what sigma's limit makes it
+        loss, _, dneg = check_prefer(pos, neg, beta=0.5, smoothing=0.25, **kw)
+        assert loss.item() == math.inf and bool(torch.isfinite(dneg).all())
+        # and a score on the wrong side
+        loss, _, dneg = check_prefer(-pos, -neg, beta=0.5, **kw)
+        assert loss.item() == math.inf and bool(torch.isfinite(dneg).all())
