@@ -31,8 +31,8 @@ __device__ __forceinline__ float prefer(const PreferArgs &a, float d, float *slo
     }
     const float z = __fmul_rn(a.beta, d);
     if (a.kind == KGE_PREFER_HINGE) {
-        *slope = z < 1.0f ? -a.beta : 0.0f;
-        return z < 1.0f ? 1.0f - z : 0.0f;
+        *slope = z < 1.0f ? -a.beta : (z >= 1.0f ? 0.0f : z);  // (a NaN stays one)
+        return z >= 1.0f ? 0.0f : 1.0f - z;
     }
     // log(1 + exp(-z)) = max(-z, 0) + log(1 + e), e = exp(-|z|); what 1 + e rounds away is put back to first order, so that pairs far apart keep
     // their small loss; sigma(-z) without cancellation.  Of the two terms in |z| one is zero; a term whose factor is zero is not there, however

@@ -115,3 +115,22 @@ def test_sigmoid_of_infinite_scores(n, sign, dtype):
         # and a score on the wrong side
         loss, _, dneg = check_prefer(-pos, -neg, beta=0.5, **kw)
         assert loss.item() == math.inf and bool(torch.isfinite(dneg).all())
+
+
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge", "square"])
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("where", ["pos", "neg", "ref_pos", "ref_neg"])
+def test_preference_of_nan(n, where, kind):
+    """A NaN that no mask excludes makes NaN of the loss, of its pair's (or row's) gradients and of no other's."""
+    g = torch.Generator().manual_seed(n + 1)
+    pos, neg, rpos, rneg = draw(g, (5,), torch.float32), draw(g, (5, n), torch.float32), draw(g, (5,), torch.float32), draw(g, (5, n), torch.float32)
+    bad = {"pos": pos, "neg": neg, "ref_pos": rpos, "ref_neg": rneg}[where]
+    row = where.endswith("pos")
+    bad[3 if row else (3, n // 2)] = math.nan
+    mask = torch.ones(5, n, device=DEV, dtype=torch.bool)
+    mask[1, 0] = False
+    for kw in (dict(), dict(mask=mask), dict(mask=mask, temperature=0.5)):
+        loss, dpos, dneg = check_prefer(pos, neg, rpos, rneg, beta=0.7, kind=kind, **kw)
+        assert bool(torch.isnan(loss)) and torch.isnan(dpos).nonzero().flatten().tolist() == [3]
+        whole = row or (where == "neg" and "temperature" in kw)          # (its weight is part of every other's)
+        assert int(torch.isnan(dneg).sum()) == (n if whole else 1) and bool(torch.isnan(dneg[3, n // 2]))
