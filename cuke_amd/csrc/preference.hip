@@ -9,11 +9,11 @@ struct PreferArgs {
     const void *pos, *neg, *ref_pos, *ref_neg;
     const uint8_t *mask;
     int64_t B, N, neg_stride, ref_stride, mask_stride;
-    float beta, sign, smoothing, heat, target, inv_batch;  // heat: temperature * sign * log2(e); target: 1 / (2 beta)
+    float beta, sign, smoothing, heat, target, inv_batch;  // heat: temperature * log2(e); target: 1 / (2 beta)
     int kind;
     float *dpos, *dneg, *loss;
     double *part_loss;  // one per workgroup of rows, or per segment
-    float2 *stats;      // [B][segments]: largest exponent, sum of weights relative to it
+    float2 *stats;      // [B][segments]: largest score, sum of weights relative to it
     float *part_back;   // [B][segments]
     int64_t segments;
     double scale;
@@ -78,6 +78,11 @@ struct Workgroup {
     }
 };
 
+// The weight of a score so far above (below) the one that has weight 1.
+__device__ __forceinline__ float weight_of(const PreferArgs &a, float above) { return __builtin_amdgcn_exp2f(a.heat * above); }
+// What scores are measured against where the largest is `top`.  Where there is none, or all are infinitely low, none of them has a weight.
+__device__ __forceinline__ float base_of(float top) { return top == -INFINITY ? 0.0f : top; }
+
 // The part of a row a lane holds in registers: C quads, `apart` elements from one to the next.
 template <class T, int C>
 struct Held {
@@ -112,13 +117,14 @@ struct Held {
             on |= bits << (4 * c);
         }
     }
-    // the largest exponent, then the weights relative to `top` and their sum
+    // The largest score (of distances: the smallest, negated), then the weights relative to `top` and their sum.  The maximum is a score, not an
+    // exponent: exponents of scores near the end of the range would be infinite, and those of scores far from zero lose their differences' bits.
     __device__ __forceinline__ float top(const PreferArgs &a) const
     {
         float t = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 4 * C; ++i)
-            if (on >> i & 1u) t = fmaxf(t, a.heat * v[i / 4][i % 4]);
+            if (on >> i & 1u) t = fmaxf(t, a.sign * v[i / 4][i % 4]);
         return t;
     }
     __device__ __forceinline__ float weigh(const PreferArgs &a, float top)
@@ -127,7 +133,7 @@ struct Held {
 #pragma unroll
         for (int i = 0; i < 4 * C; ++i) {
             float &x = w[i / 4][i % 4];
-            x = on >> i & 1u ? (a.heat != 0.0f ? __builtin_amdgcn_exp2f(a.heat * v[i / 4][i % 4] - top) : 1.0f) : 0.0f;
+            x = on >> i & 1u ? (a.heat != 0.0f ? weight_of(a, fmaf(a.sign, v[i / 4][i % 4], -top)) : 1.0f) : 0.0f;
             sum += x;
         }
         return sum;
@@ -190,7 +196,7 @@ __global__ __launch_bounds__(1024) void preference_rows_kernel(PreferArgs a)
         float p = 0.0f, loss = 0.0f, back = 0.0f;
         h.load(a, row ? b : 0, n0, apart, row ? a.N : 0, true);
         if (row) p = positive<T>(a, b);
-        const float top = a.heat != 0.0f ? g.max(h.top(a)) : 0.0f;
+        const float top = a.heat != 0.0f ? base_of(g.max(h.top(a))) : 0.0f;
         const float sum = g.sum(h.weigh(a, top));
         h.finish(a, row ? b : 0, n0, apart, row ? a.N : 0, p, sum != 0.0f ? 1.0f / sum : 0.0f, &loss, &back);
         loss = g.sum(loss), back = g.sum(back);
@@ -220,7 +226,7 @@ __global__ __launch_bounds__(256) void preference_stats_kernel(PreferArgs a)
     const int64_t b = blockIdx.x / a.segments, seg = blockIdx.x % a.segments, n0 = seg * kSegment + 4 * threadIdx.x;
     Held<T, kSegmentQuads> h;
     h.load(a, b, n0, 1024, a.N, false);
-    const float top = a.heat != 0.0f ? g.max(h.top(a)) : 0.0f;
+    const float top = a.heat != 0.0f ? base_of(g.max(h.top(a))) : 0.0f;
     const float sum = g.sum(h.weigh(a, top));
     if (threadIdx.x == 0) a.stats[b * a.segments + seg] = make_float2(top, sum);
 }
@@ -236,13 +242,14 @@ __global__ __launch_bounds__(256) void preference_segment_kernel(PreferArgs a)
     float top = 0.0f, sum = (float)a.N;
     if (a.stats) {
         const float2 *st = a.stats + b * a.segments;
+        // (a segment none of whose pairs has a weight is left out)
         float t = -INFINITY, u = 0.0f;
         for (int64_t i = threadIdx.x; i < a.segments; i += 256)
             if (st[i].y != 0.0f) t = fmaxf(t, st[i].x);
-        top = g.max(t);
+        top = base_of(g.max(t));
         for (int64_t i = threadIdx.x; i < a.segments; i += 256) {
             const float2 v = st[i];
-            if (v.y != 0.0f) u += v.y * (v.x == top ? 1.0f : __builtin_amdgcn_exp2f(v.x - top));
+            if (v.y != 0.0f) u += v.y * weight_of(a, v.x - top);
         }
         sum = g.sum(u);
     }
@@ -350,7 +357,7 @@ int kge_preference_loss(const kge_preference *pref, float *loss, float *dpos, fl
     PreferArgs a{};
     a.pos = pref->pos, a.neg = pref->neg, a.ref_pos = pref->ref_pos, a.ref_neg = pref->ref_neg, a.mask = pref->mask;
     a.B = pref->batch, a.N = pref->n_neg, a.neg_stride = pref->neg_stride, a.ref_stride = pref->ref_neg_stride, a.mask_stride = pref->mask_stride;
-    a.beta = pref->beta, a.sign = pref->sign, a.smoothing = pref->smoothing, a.heat = pref->temperature * pref->sign * 1.44269504f;
+    a.beta = pref->beta, a.sign = pref->sign, a.smoothing = pref->smoothing, a.heat = fminf(pref->temperature * 1.44269504f, FLT_MAX);
     a.target = 0.5f / pref->beta, a.inv_batch = a.B > 0 ? 1.0f / (float)a.B : 0.0f, a.scale = a.B > 0 ? 1.0 / (double)a.B : 0.0;
     a.kind = pref->kind, a.dpos = dpos, a.dneg = dneg, a.loss = loss, a.part_loss = static_cast<double *>(workspace);
     KGE_CLEAR_LAUNCH_ERRORS();

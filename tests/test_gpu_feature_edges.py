@@ -134,3 +134,58 @@ def test_preference_of_nan(n, where, kind):
         assert bool(torch.isnan(loss)) and torch.isnan(dpos).nonzero().flatten().tolist() == [3]
         whole = row or (where == "neg" and "temperature" in kw)          # (its weight is part of every other's)
         assert int(torch.isnan(dneg).sum()) == (n if whole else 1) and bool(torch.isnan(dneg[3, n // 2]))
+
+
+def lowest(dtype, infinite):
+    return -math.inf if infinite else torch.finfo(dtype).min
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("infinite", [False, True])
+@pytest.mark.parametrize("n,first,end", [(2, 1, 2), (7, 4, 7), (700, 256, 512), (2049, 2048, 2049), (4099, 2048, 4096), (4099, 4096, 4099), (6200, 0, 2048)])
+@pytest.mark.parametrize("kind", ["sigmoid", "hinge"])
+def test_scores_that_take_no_share(n, first, end, infinite, dtype, kind):
+    """A stretch of scores of the type's lowest value, or infinitely low, beside others: it takes no share of the softmax."""
+    g = torch.Generator().manual_seed(n + first)
+    for sign in (1.0, -1.0):
+        pos, neg = draw(g, (4,), dtype, 2.0), draw(g, (4, n), dtype, 2.0)
+        neg[:3, first:end] = sign * lowest(dtype, infinite)
+        mask = torch.rand(4, n, generator=g).to(DEV) >= 0.2
+        mask[:, 0 if first else end] = True                    # (something is left)
+        mask[1, first:end - 1] = False                         # in a row of its own, the last of them alone
+        for temperature in (0.5, 1.0, 30.0):
+            for m in (None, mask):
+                loss, dpos, dneg = check_prefer(pos, neg, beta=0.3, kind=kind, temperature=temperature, sign=sign, mask=m)
+                assert bool(torch.isfinite(loss)) and bool(torch.isfinite(dpos).all()) and not dneg[:3, first:end].any()
+                assert bool(dpos.any())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 6, 700, 4099])
+def test_rows_of_nothing_but_lowest_scores(n, dtype):
+    """Infinitely low: the row adds nothing, as one without a pair.  Of the lowest value: equal scores, that share evenly."""
+    g = torch.Generator().manual_seed(n)
+    pos, neg = draw(g, (4,), dtype, 2.0), draw(g, (4, n), dtype, 2.0)
+    neg[1], neg[2] = -math.inf, torch.finfo(dtype).min
+    for kind in ("sigmoid", "hinge"):
+        loss, dpos, dneg = check_prefer(pos, neg, beta=0.3, kind=kind, temperature=1.0)
+        assert bool(torch.isfinite(loss)) and not dneg[1:3].any() and not dpos[1:3].any()
+
+
+@pytest.mark.parametrize("n", [16, 300, 2048 + 16])
+def test_softmax_of_scores_far_from_zero(n):
+    """The weights are those of the scores' differences, which fp32 holds exactly beside a common offset of a thousand."""
+    g = torch.Generator().manual_seed(n)
+    neg = (1000.0 + draw(g, (64, n), torch.float64, 2.0)).float()
+    mask = torch.zeros(64, n, device=DEV, dtype=torch.bool)
+    mask[:, -16:] = True                                        # few enough that sums of them add little
+    pos = (1000.0 + draw(g, (64,), torch.float64, 2.0)).float()
+    from cuke_amd import features
+    _, _, dneg = features.preference_loss(pos, neg, temperature=1.0, mask=mask)
+    p, v = pos.double(), neg[:, -16:].double()
+    a = torch.softmax(v, 1)
+    want = a * torch.sigmoid(v - p[:, None]) / 64
+    top = v.amax(1, keepdim=True)
+    # 16 + 16 roundings of the sum and around it; the exponents' own, and the sigmoid's: both differences are exact
+    tol = want * (8 * EPS * (1 + (top - v)) + 32 * EPS + 16 * EPS * (1 + (v - p[:, None]).abs()))
+    like(dneg[:, -16:], want, tol, "dneg")
