@@ -150,7 +150,9 @@ struct Held {
             for (int e = 0; e < 4; ++e) {
                 float slope;
                 const float f = prefer(a, a.sign * (p - (v[c][e] - ref[c][e])), &slope), x = w[c][e] * inv;
-                const bool there = on >> (4 * c + e) & 1u;
+                // (A pair without a weight adds nothing, also where its loss, and then perhaps its slope, is infinite; a NaN stays one.  16384 x 1024
+                // takes 1.3 us for asking; a second pass over lanes that hold such a pair spills registers, and takes more.)
+                const bool there = (on >> (4 * c + e) & 1u) && !(x == 0.0f && f == INFINITY);
                 l += there ? x * f : 0.0f;
                 g[e] = there ? x * slope * up : 0.0f;
                 k += g[e];

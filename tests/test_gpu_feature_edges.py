@@ -189,3 +189,20 @@ def test_softmax_of_scores_far_from_zero(n):
     # 16 + 16 roundings of the sum and around it; the exponents' own, and the sigmoid's: both differences are exact
     tol = want * (8 * EPS * (1 + (top - v)) + 32 * EPS + 16 * EPS * (1 + (v - p[:, None]).abs()))
     like(dneg[:, -16:], want, tol, "dneg")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 7, 700, 2051])
+def test_pairs_without_a_share_add_nothing(n, dtype):
+    """A pair whose weight is zero adds neither loss nor gradient, also where its own loss is infinite or passes fp32's range."""
+    g = torch.Generator().manual_seed(n)
+    pos, neg = draw(g, (4,), dtype, 2.0), draw(g, (4, n), dtype, 2.0)
+    neg[1, n - 1], neg[2, n - 1] = torch.finfo(dtype).min, -math.inf
+    for kw in (dict(kind="square", beta=0.5), dict(smoothing=0.1, beta=4.0), dict(smoothing=0.1, beta=0.5)):
+        loss, dpos, dneg = check_prefer(pos, neg, temperature=1.0, **kw)
+        assert bool(torch.isfinite(loss)) and bool(torch.isfinite(dpos).all()) and not dneg[1:3, n - 1].any()
+    if n > 2:                                               # a NaN there is none the less one
+        rneg = torch.zeros_like(neg)
+        rneg[1, n - 1] = math.nan
+        loss, dpos, _ = check_prefer(pos, neg, torch.zeros_like(pos), rneg, temperature=1.0)
+        assert bool(torch.isnan(loss)) and bool(torch.isnan(dpos[1]))
