@@ -197,7 +197,7 @@ __global__ __launch_bounds__(1024) void preference_rows_kernel(PreferArgs a)
         Held<T, C> h;
         float p = 0.0f, loss = 0.0f, back = 0.0f;
         h.load(a, row ? b : 0, n0, apart, row ? a.N : 0, true);
-        if (row) p = positive<T>(a, b);
+        if (row && a.N > 0) p = positive<T>(a, b);  // (rows of no pairs: the arrays may be NULL)
         const float top = a.heat != 0.0f ? base_of(g.max(h.top(a))) : 0.0f;
         const float sum = g.sum(h.weigh(a, top));
         h.finish(a, row ? b : 0, n0, apart, row ? a.N : 0, p, sum != 0.0f ? 1.0f / sum : 0.0f, &loss, &back);

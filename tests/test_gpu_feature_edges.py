@@ -206,3 +206,18 @@ def test_pairs_without_a_share_add_nothing(n, dtype):
         rneg[1, n - 1] = math.nan
         loss, dpos, _ = check_prefer(pos, neg, torch.zeros_like(pos), rneg, temperature=1.0)
         assert bool(torch.isnan(loss)) and bool(torch.isnan(dpos[1]))
+
+
+def test_rows_of_no_pairs_are_not_read():
+    """With n_neg = 0 nothing is looked at: pos and neg may be NULL, and so may one of the references."""
+    import ctypes as C
+    from cuke_amd import _lib
+    L = _lib.lib()
+    for kind in range(3):
+        loss, dpos = torch.full((1,), -7.0, device=DEV), torch.full((3000,), -7.0, device=DEV)
+        d = _lib.Preference(0, kind, 3000, 0, None, None, 0, None, None, 0, None, 0, 1.0, 1.0, 0.0, 0.5)
+        need = L.kge_preference_workspace(C.byref(d))
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=DEV)
+        assert L.kge_preference_loss(C.byref(d), loss.data_ptr(), dpos.data_ptr(), None, ws.data_ptr(), need,
+                                     torch.cuda.current_stream().cuda_stream) == 0
+        assert loss.item() == 0 and not dpos.any()
