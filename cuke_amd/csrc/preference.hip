@@ -219,6 +219,7 @@ __global__ __launch_bounds__(1024) void preference_rows_kernel(PreferArgs a)
 // latency of each pass, a row's sums end before its gradients begin; of large batches by vector instructions and memory alike (2048 x 40943 so, 755 MB:
 // 325 us; with even weights and no mask, in one pass, 148).  Segments of 1024 pairs take 5 to 45 % longer there, of 4096 up to 35 % where rows are few.
 constexpr int kSegmentQuads = 2, kSegment = 256 * 4 * kSegmentQuads;
+constexpr int64_t kMostSegments = ((int64_t(1) << 32) - 1) / 256;  // a launch has fewer than 2^32 threads
 
 template <class T>
 __global__ __launch_bounds__(256) void preference_stats_kernel(PreferArgs a)
@@ -329,7 +330,7 @@ static int check(const kge_preference *p)
     if (!(p->smoothing >= 0.0f && p->smoothing <= 1.0f) || (p->smoothing != 0.0f && p->kind != KGE_PREFER_SIGMOID)) return KGE_EINVAL;
     if (p->batch < 0 || p->n_neg < 0) return KGE_ESHAPE;
     if (p->batch >= (int64_t)1 << 40 || p->n_neg >= (int64_t)1 << 40) return KGE_ESHAPE;
-    if (in_segments(p) && p->batch > (((int64_t)1 << 31) - 1) / segments_of(p)) return KGE_ESHAPE;  // (workgroups are counted in 31 bits)
+    if (in_segments(p) && p->batch > kMostSegments / segments_of(p)) return KGE_ESHAPE;
     if (p->neg_stride < p->n_neg || (p->ref_neg && p->ref_neg_stride < p->n_neg) || (p->mask && p->mask_stride < p->n_neg)) return KGE_ESHAPE;
     if ((p->ref_pos == nullptr) != (p->ref_neg == nullptr) && p->batch > 0 && p->n_neg > 0) return KGE_EINVAL;
     if (p->batch > 0 && p->n_neg > 0 && (!p->pos || !p->neg)) return KGE_EINVAL;
