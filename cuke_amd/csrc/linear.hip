@@ -190,6 +190,11 @@ using SmallF = Shape<64, 64, 32, 2, 2, 2>;
 using DeepF = Shape<64, 64, 64, 2, 2, 2, 2>;
 
 static int64_t tiles_of(int64_t a, int64_t b, int x) { return ceil_div(a, x) * ceil_div(b, x); }
+constexpr int64_t kMostThreads = (int64_t(1) << 32) - 1;  // of a launch
+template <class S>
+static bool launchable(int64_t blocks) { return blocks <= kMostThreads / S::kThreads; }
+template <class S>
+static bool tiles_launchable(int64_t a, int64_t b) { return launchable<S>(ceil_div(a, S::XA) * ceil_div(b, S::XB)); }
 
 template <class T, class S, bool WHOLE = true>
 static void launch_forward(TileArgs &t, hipStream_t st)
@@ -207,6 +212,7 @@ template <class S>
 static double forward_cost(const TileArgs &t, int64_t epilogue, int share, double pace, double epilogue_pace)
 {
     const int64_t tiles = ceil_div(t.a.extent, S::XA) * ceil_div(t.b.extent, S::XB), a_cu = ceil_div(tiles, 256);
+    if (!launchable<S>(tiles)) return INFINITY;
     const int64_t at_once = a_cu < share ? a_cu : share, rounds = ceil_div(tiles, 256 * (at_once > 0 ? at_once : 1));
     return (double)rounds * at_once * S::XA * S::XB * ((double)t.k / pace + epilogue / epilogue_pace) / (0.4 + 0.6 * at_once / share);
 }
@@ -265,8 +271,9 @@ static int64_t split_length(int64_t k, int splits) { return ceil_div(ceil_div(k,
 // -> 120 in one part of tiles of 64 17, in 6 of 128 22; fp32 9000 x 100 -> 1500 with dx's longer sums first 95, with dW's 105; 512 x 768 -> 400 in DeepF's
 // tiles 16, in SmallF's 20.
 struct GradPlan {
-    int tile, dw_splits;  // tile: 256, 128 or 64
+    int tile, dw_splits;  // tile: 256, 128 or 64; 0: no launch takes this many
     bool deep;            // DeepF
+    bool dx;              // whether the launch takes dx beside dW
 };
 // When n jobs of length a each, then m of length b, are done by `slots` workers.
 static double jobs_end(int64_t n, double a, int64_t m, double b, int64_t slots)
@@ -280,36 +287,44 @@ static double jobs_end(int64_t n, double a, int64_t m, double b, int64_t slots)
     t = ((double)m * b + (double)(slots - late) * first + (double)late * second) / (double)slots;
     return std::max(second, std::min(whole(first, t), whole(second, t)));
 }
-static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out)
+static GradPlan grad_plan(int type, int64_t rows, int64_t in, int64_t out, bool with_dx = true)
 {
     struct Pace {
-        int tile, slots;
+        int tile, threads, slots;
         double a_term, besides;  // us
         double alone;            // how much longer a long sum takes where nothing else hides its waits
         bool deep;
     };
-    static const Pace kHalf[] = {{64, 256, 0.0026, 1.0, 2.3, false}, {128, 256, 0.0066, 3.0, 1.4, false}, {256, 256, 0.0260, 8.1, 1.0, false}};
-    static const Pace kFloat[] = {{64, 512, 0.0268, 3.5, 1.0, false}, {128, 256, 0.0393, 6.7, 1.0, false}, {64, 256, 0.0165, 5.0, 1.0, true}};
+    static const Pace kHalf[] = {{64, Small::kThreads, 256, 0.0026, 1.0, 2.3, false}, {128, MiddleG::kThreads, 256, 0.0066, 3.0, 1.4, false},
+                                 {256, Large::kThreads, 256, 0.0260, 8.1, 1.0, false}};
+    static const Pace kFloat[] = {{64, SmallF::kThreads, 512, 0.0268, 3.5, 1.0, false}, {128, MiddleF::kThreads, 256, 0.0393, 6.7, 1.0, false},
+                                  {64, DeepF::kThreads, 256, 0.0165, 5.0, 1.0, true}};
     const bool f32 = type == KGE_F32;
     const Pace *paces = f32 ? kFloat : kHalf;
     const double parts_launch = f32 ? 7.0 : 5.0, part = (double)out * (double)in * 8.0 / (f32 ? 16e6 : 40e6);  // us
-    GradPlan best{64, 1, false};
+    GradPlan best{0, 1, false, with_dx};
     double best_end = INFINITY;
     for (int i = 0; i < 3; ++i) {
         const Pace &p = paces[i];
-        const int64_t dw = tiles_of(out, in, p.tile), dx = tiles_of(rows, in, p.tile);
+        const int64_t dw = tiles_of(out, in, p.tile), dx = with_dx ? tiles_of(rows, in, p.tile) : 0;
         const double b = (double)out * p.a_term + p.besides;
         for (int parts = 1; parts <= 64; parts += parts < 8 ? 1 : parts / 4) {
             const int64_t each = split_length(rows, parts), n = dw * ceil_div(rows, each > 0 ? each : 1);
-            if (parts > 1 && each < 128) break;
+            if (parts > 1 && (each < 128 || out * ceil_div(in, 4) > kMostThreads - 256)) break;  // (joining takes a thread a quad)
+            if (n + dx + ceil_div(out, 16) > kMostThreads / p.threads) continue;
             const double a = (double)each * p.a_term + p.besides;
             double end = out > each ? jobs_end(dx, b, n, a, p.slots) : jobs_end(n, a, dx, b, p.slots);
             end = std::max(end, p.alone * (double)std::max(each, out) * p.a_term);
             if (parts > 1) end += parts_launch + parts * part;
-            if (end < best_end) best_end = end, best = GradPlan{p.tile, parts, p.deep};
+            if (end < best_end) best_end = end, best = GradPlan{p.tile, parts, p.deep, with_dx};
         }
     }
     return best;
+}
+static GradPlan grad_plan(const kge_linear *l)
+{
+    const GradPlan g = grad_plan(l->type, l->rows, l->in, l->out);
+    return g.tile ? g : grad_plan(l->type, l->rows, l->in, l->out, false);
 }
 
 template <class T, class S, bool WHOLE = true>
@@ -378,9 +393,13 @@ static int check(const kge_linear *l)
     const int64_t most = (int64_t)1 << 31;
     if (l->rows < 0 || l->in < 0 || l->out < 0 || l->rows >= most || l->in >= most || l->out >= most) return KGE_ESHAPE;
     if (l->x_stride < l->in || l->weight_stride < l->in || (l->residual && l->residual_stride < l->out)) return KGE_ESHAPE;
-    // (every launch's workgroups are counted in 31 bits)
     if (ceil_div(l->rows, 32) * ceil_div(l->out, 32) >= most || ceil_div(l->rows, 32) * ceil_div(l->in, 32) >= most ||
         ceil_div(l->in, 32) * ceil_div(l->out, 32) >= most)
+        return KGE_ESHAPE;
+    const int64_t a = l->out, b = l->rows;  // (some shape's tiles have to fit a launch; the choices leave out those that do not)
+    if (l->type == KGE_F32 ? !tiles_launchable<MiddleF>(a, b) && !tiles_launchable<SmallF>(a, b) && !tiles_launchable<DeepF>(a, b)
+                           : !tiles_launchable<Large>(a, b) && !tiles_launchable<Middle>(a, b) && !tiles_launchable<Tall>(a, b) && !tiles_launchable<Lone>(a, b) &&
+                                 !tiles_launchable<Small>(a, b))
         return KGE_ESHAPE;
     if ((l->rows > 0 && l->in > 0 && !l->x) || (l->in > 0 && l->out > 0 && !l->weight)) return KGE_EINVAL;
     return KGE_OK;
@@ -520,7 +539,8 @@ int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_bac
 size_t kge_linear_bwd_workspace(const kge_linear *lin)
 {
     if (check(lin)) return 0;
-    return backward_bytes(lin, plan_of(lin), grad_plan(lin->type, lin->rows, lin->in, lin->out));
+    const GradPlan g = grad_plan(lin);
+    return g.tile ? backward_bytes(lin, plan_of(lin), g) : 0;
 }
 
 int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx, void *dweight,
@@ -530,7 +550,8 @@ int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, con
     if (dy_stride < lin->out) return KGE_ESHAPE;
     if (lin->rows > 0 && lin->out > 0 && !dy) return KGE_EINVAL;
     const Plan p = plan_of(lin);
-    const GradPlan g = grad_plan(lin->type, lin->rows, lin->in, lin->out);
+    const GradPlan g = grad_plan(lin);
+    if (!g.tile || (dx && !g.dx)) return KGE_ESHAPE;
     const size_t need_saved = p.slope + p.x + p.w, need = backward_bytes(lin, p, g);
     if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
