@@ -383,7 +383,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     const int64_t n0 = (int64_t)ta * S::XA, m0 = (int64_t)tb * S::XB;
     const int64_t k0 = split * t.k_each, k1 = k0 + t.k_each < t.k ? k0 + t.k_each : t.k;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int wa = (wave % WA) * (S::XA / WA), wb = (wave / WA % WB) * (S::XB / WB), part = SHARE > 1 ? wave / (WA * WB) : 0;  // of every tile's terms
+    const int wa = (wave % WA) * (S::XA / WA), wb = (SHARE > 1 ? wave / WA % WB : wave / WA) * (S::XB / WB), part = SHARE > 1 ? wave / (WA * WB) : 0;  // of every tile's terms
 
     floatx16 acc[FA][FB] = {}, low[kFloat ? FA : 1][kFloat ? FB : 1] = {};
     int64_t left = k1 - k0;  // terms not requested yet
