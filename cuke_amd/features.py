@@ -78,6 +78,8 @@ def _random(seed, step):
     if isinstance(step, torch.Tensor):
         if step.dtype != torch.int64 or not step.is_cuda or step.numel() != 1:
             raise TypeError("step must be an integer or one int64 on the GPU")
+        if step.device.index != torch.cuda.current_device():
+            raise KgeError(f"step must live on the current device (got {step.device}, current is cuda:{torch.cuda.current_device()})")
         return int(seed) & _U64, 0, step
     return int(seed) & _U64, int(step) & _U64, None
 

@@ -221,3 +221,14 @@ def test_rows_of_no_pairs_are_not_read():
         assert L.kge_preference_loss(C.byref(d), loss.data_ptr(), dpos.data_ptr(), None, ws.data_ptr(), need,
                                      torch.cuda.current_stream().cuda_stream) == 0
         assert loss.item() == 0 and not dpos.any()
+
+
+def test_a_step_on_another_device_is_refused(monkeypatch):
+    """The kernels read the word of the step: it has to be on the device that they run on."""
+    from cuke_amd import features
+    from cuke_amd.kge import KgeError
+    word = torch.zeros(1, dtype=torch.int64, device=DEV)
+    assert features._random(1, word)[2] is word
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(KgeError):
+        features._random(1, word)
