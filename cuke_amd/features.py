@@ -61,11 +61,15 @@ def _rows(x, name: str, dtype=None, ndim: int = 2, shape=None) -> torch.Tensor:
 
 
 def _apart(x, out) -> bool:
-    """Whether two blocks of equal rows are the very same one or do not overlap (as ranges of memory)."""
+    """Whether two blocks of equal rows are the very same one or do not overlap: as ranges of memory, or, with rows equally far apart, as ranges
+    of columns."""
     if x.data_ptr() == out.data_ptr() and (x.stride() == out.stride() or x.shape[0] <= 1):
         return True
     ends = [(t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _row_stride(t) + t.shape[1]) * t.element_size()) for t in (x, out)]
-    return x.numel() == 0 or ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]
+    if x.numel() == 0 or ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]:
+        return True
+    width, pitch = x.shape[1] * x.element_size(), _row_stride(x) * x.element_size()
+    return _row_stride(out) == _row_stride(x) and width <= (out.data_ptr() - x.data_ptr()) % pitch <= pitch - width
 
 
 def _row_stride(x: torch.Tensor) -> int:
@@ -219,7 +223,7 @@ def dropout(x, p, seed, step=0, out=None) -> torch.Tensor:
     elif _rows(out, "out", x.dtype, shape=x.shape) is not out:
         raise ValueError("out must have contiguous rows: it is written in place")
     elif not _apart(x, out):
-        raise ValueError("out must be x itself or share no memory with it")
+        raise ValueError("out must be x itself or lie apart from it: elsewhere, or in other columns of the same rows")
     _lib.check(_lib.lib().kge_dropout(_TYPES[x.dtype], _p(x), _row_stride(x), _p(out), _row_stride(out), x.shape[0], x.shape[1], p, seed,
                                       step, _p(word), _stream()), "kge_dropout")
     return out

@@ -232,3 +232,25 @@ def test_a_step_on_another_device_is_refused(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
     with pytest.raises(KgeError):
         features._random(1, word)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_dropout_into_the_other_columns_of_an_array(dtype):
+    """Two column ranges of one array share no element: one may be dropped into the other."""
+    from cuke_amd import features
+    g = torch.Generator().manual_seed(6)
+    for rows, cols, at in [(9, 8, 8), (64, 30, 37), (1, 5, 5), (300, 1, 2)]:
+        both = draw(g, (rows, cols + at + 3), dtype)
+        was = both.clone()
+        for x, out, rest in [(both[:, :cols], both[:, at:at + cols], [slice(0, at), slice(at + cols, None)]),
+                             (both[:, at:at + cols], both[:, :cols], [slice(cols, None)])]:
+            both.copy_(was)
+            want = features.dropout(x.clone(), 0.4, 3, 1)
+            assert features.dropout(x, 0.4, 3, 1, out=out) is out and torch.equal(out, want)
+            assert all(torch.equal(both[:, s], was[:, s]) for s in rest)
+    rows = torch.zeros(12, 16, device=DEV, dtype=dtype)
+    flat, nine = rows.view(-1), rows[:9]
+    for x, out in [(nine[:, :8], nine[:, 7:15]), (nine[:, 7:15], nine[:, :8]), (rows[:8, 8:], flat[20:148].view(8, 16)[:, :8]),
+                   (flat[:96].view(6, 16)[:, :9], flat[24:120].view(6, 16)[:, :9]), (nine[:, 4:12], flat[:72].view(9, 8))]:
+        with pytest.raises(ValueError):
+            features.dropout(x, 0.5, 1, out=out)
