@@ -81,10 +81,11 @@ struct Tile {
     static constexpr int kRounds = kChunks / THREADS;
     static constexpr int kRow = ACROSS ? X / 8 : K / 8;  // chunks a row
     static_assert(kChunks % THREADS == 0, "whole rounds");
+    static_assert(K == 32 || K == 64, "turn() knows these rows");
 
     __device__ __forceinline__ static int turn(int row)
     {
-        if (!ACROSS) return K == 128 ? row & 15 : (K == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
+        if (!ACROSS) return K == 64 ? (row >> 1) & 7 : (row >> 2) & 3;
         return X >= 256 ? 2 * (2 * (row & 3) + 8 * ((row >> 3) & 1)) : (X >= 128 ? 4 * (row & 3) : 2 * (row & 3));
     }
 
