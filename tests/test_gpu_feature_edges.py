@@ -254,3 +254,59 @@ def test_dropout_into_the_other_columns_of_an_array(dtype):
                    (flat[:96].view(6, 16)[:, :9], flat[24:120].view(6, 16)[:, :9]), (nine[:, 4:12], flat[:72].view(9, 8))]:
         with pytest.raises(ValueError):
             features.dropout(x, 0.5, 1, out=out)
+
+
+# ---- fp32 products as products of bf16 parts ---------------------------------------------------------
+# (rows, in, out): large enough that forward pass and gradients are made in tiles, on both sides of the rules that choose them
+PRODUCTS = [(2100, 72, 264), (2100, 136, 265), (2500, 520, 264), (851, 1968, 1016), (4090, 1021, 509), (8200, 520, 776)]
+
+
+def operand(gen, shape, values):
+    t = torch.randn(shape, generator=gen, dtype=torch.float64)
+    if values == "one sign":
+        t = t.abs() + 0.1
+    if values == "spread":
+        t = t * torch.exp2(torch.randint(-20, 21, shape, generator=gen).double())
+    return t.float().to(DEV)
+
+
+@pytest.mark.parametrize("values", ["normal", "one sign", "spread"])
+@pytest.mark.parametrize("shape", PRODUCTS, ids=lambda s: "%dx%dx%d" % s)
+def test_fp32_products_are_no_worse_than_fp32(shape, values):
+    """The error's 2-norm over the result's, of y, dx and dW, against that of fp32 sums of K products.
+
+    A chain of K fp32 additions leaves each partial sum off by a rounding of 2^-24 / sqrt(3) (root mean square) of it: of partial sums that grow as
+    sqrt(k) that comes to 2^-24 sqrt(K / 6), of those of one sign to less.  The result's own rounding is 2^-24 / sqrt(3).  Three of the six products of
+    parts, instead of all, leave 4e-6."""
+    from cuke_amd import features
+    rows, fin, fout = shape
+    g = torch.Generator().manual_seed(fin)
+    x, w, dy = operand(g, (rows, fin), values), operand(g, (fout, fin), values), operand(g, (rows, fout), values)
+    fw = features.linear_forward(x, w)
+    got = features.linear_backward(fw, dy)
+    for have, want, k, what in [(fw.y, x.double() @ w.double().T, fin, "y"), (got.x, dy.double() @ w.double(), fout, "dx"),
+                                (got.weight, dy.double().T.contiguous() @ x.double(), rows, "dw")]:
+        error = ((have.double() - want).norm() / want.norm()).item()
+        print(f"{what} {shape} {values}: {error:.2e} of {EPS * math.sqrt(k / 6 + 1 / 3):.2e}", flush=True)
+        assert error <= EPS * math.sqrt(k / 6 + 1 / 3), (what, error)
+
+
+def test_fp32_tiles_at_the_edge_of_the_range():
+    """Values whose leading bf16 part rounds to infinity, sums near the largest number, and very small ones, in sizes whose sums are made in tiles."""
+    from cuke_amd import features
+    rows, fin, fout = 2100, 136, 264
+    x = torch.full((rows, fin), 3.4e38, device=DEV)
+    w = torch.zeros(fout, fin, device=DEV)
+    w[:, 3], w[1, 4], w[2, 3], w[200, 135], w[263, 3] = 1.0, -1.0, 2.0, -0.5, -2.0
+    fw = features.linear_forward(x, w)
+    assert torch.equal(fw.y, (x.double() @ w.double().T).float())
+    dy = torch.zeros(rows, fout, device=DEV)
+    dy[7, 5], dy[8, 2], dy[2099, 263], dy[2099, 200] = 3.4e38, 3.4e38, -0.25, 3.3e38
+    dy[7, 6] = 1e36                                              # (of x, dy[7, 5] 3.4e38 passes the range, of w it does not)
+    got = features.linear_backward(fw, dy)
+    assert torch.equal(got.x, (dy.double() @ w.double()).float())
+    assert torch.equal(got.weight, (dy.double().T.contiguous() @ x.double()).float())
+    small, tiny = torch.full((rows, fin), 1e-30, device=DEV), torch.full((fout, fin), 1e-3, device=DEV)
+    y = features.linear(small, tiny)
+    want = small.double() @ tiny.double().T
+    assert bool(((y.double() - want).abs() <= (fin + 16) * EPS * want).all())
