@@ -128,7 +128,7 @@ __device__ __forceinline__ void activate(float (&z)[V], int act, float (&slope)[
 }
 
 // The derivative as it is kept for the backward pass of 16-bit layers: every one of them lies in [-0.13, 1.13], so 16 bits of fixed
-// point hold it to 1.02e-5 (0 and 1 exactly), where bf16 would add an error as large as that of the gradient's own rounding; 0, which no derivative
+// point hold it to 1.02e-5 (0 and 1 exactly; a nearly dead unit's below 1e-5, of gelu from about z = -5 down, becomes 0), where bf16 would add an error as large as that of the gradient's own rounding; 0, which no derivative
 // comes near, is NaN.  Layers in fp32 keep it in fp32.
 typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ us2 slopes_to_fixed(float a, float b)  // (one conversion to two unsigned normalised numbers; it makes 0 of NaN)

@@ -170,7 +170,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(JoinArgs j)
 // ---- products --------------------------------------------------------------------------------------
 // Larger tiles read less and multiply faster, smaller ones waste less at the edges and in the last round over the card, and where several share a
 // CU each hides the other's epilogue.  Forward passes by tile (us; Large, Middle, Tall, Lone, Small; what is chosen in brackets):
-//   32768 x 2048 -> 2048 bf16, gelu and drop   [349] 382  424  521  485       65536 x 512 -> 400, plain         [50] 50  56  75  62
+//   32768 x 2048 -> 2048 bf16, gelu and drop   [336] 382  424  521  485       65536 x 512 -> 400, plain         [50] 50  56  75  62
 //   65536 x 512 -> 400, fp32 residual            88 [75]  80  102   84        20000 x 304 -> 800, plain          36 [26] 29  37  30
 //   16384 x 768 -> 512, plain                    29 [20]  27   27   25         8192 x 768 -> 512, fp32 residual  37  19 [17] 20  20
 //    4096 x 1024 -> 512, gelu and drop           45  18   15  [12]  13         2500 x 520 -> 264, gelu and drop  36  19  12   9  [8]

@@ -355,7 +355,7 @@ __device__ __forceinline__ void lds_ready()
 // that the compiler sees that the one being read is none of those being written); STAGES - 1 are requested ahead, and one barrier a tile both
 // publishes the next and frees the last.  fp32: two stages, two more tiles in registers.  SHARE > 1: as many groups of WA x WB waves each multiply
 // their share of every tile's terms, and join their sums in LDS before the epilogue.
-// Bound by the matrix cores where sums are long: 32768 x 2048 -> 2048 bf16 plain 280 us (982 TFLOP/s; a large library product of this card 1383, both
+// Bound by the matrix cores where sums are long: 32768 x 2048 -> 2048 bf16 plain 277 us (992 TFLOP/s; a large library product of this card 1383, both
 // held by its power), its gradients 470 (1170); fp32 8192 x 1024 -> 1024 103 us (1.0 PFLOP/s of bf16 products).  Where they are short, by waits: a
 // CU's first tiles and its epilogues, which more workgroups a CU hide.
 template <int XA_, int XB_, int K_, int WA_, int WB_, int STAGES_, int SHARE_ = 1>
@@ -560,7 +560,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     }
 }
 
-// y = drop(act(x W^T + b)) + residual.  The epilogue is fused: with gelu, drop and act' kept 32768 x 2048 -> 2048 bf16 takes 333 us, 53 more than the
+// y = drop(act(x W^T + b)) + residual.  The epilogue is fused: with gelu, drop and act' kept 32768 x 2048 -> 2048 bf16 takes 336 us, 59 more than the
 // plain product, where a pass over memory of its own would take 100 or more.
 template <class T, class S, bool WHOLE>
 __global__ __launch_bounds__(S::kThreads) void linear_forward_kernel(TileArgs t)

@@ -183,7 +183,8 @@ __device__ __forceinline__ double block_total(double v)
 }
 
 // Rows of at most 1024 pairs, each read once and held in the registers of `lanes` lanes of a wave: bound by memory (16384 x 1024 fp32 with
-// reference, mask and weights: 218 MB in 48 us, 4.6 TB/s).  A workgroup leaves one partial loss; a single one writes the loss itself.
+// reference, mask and weights: 218 MB in 50 us, 4.4 TB/s), of 16-bit scores by vector instructions (the same in bf16, 151 MB: 51 us; with even weights and no
+// mask 44).  A workgroup leaves one partial loss; a single one writes the loss itself.
 template <class T, int C>
 __global__ __launch_bounds__(1024) void preference_rows_kernel(PreferArgs a)
 {
@@ -214,10 +215,11 @@ __global__ __launch_bounds__(1024) void preference_rows_kernel(PreferArgs a)
 }
 
 // Longer rows, in segments of kSegment pairs that a workgroup holds in its registers.  Their weights' sum is not known before all have been read:
-// one pass leaves every segment's largest exponent and sum (of mask bytes alone where weights are even; none at all without a mask), a second
-// joins them and reads the scores again, mostly from the caches (64 x 40943 bf16 with reference, mask and weights, 24 MB: 4.5 and 9.5 us).  Bound by the
+// one pass leaves every segment's largest score and its sum (there is none where weights are even and no pair is masked), a second
+// joins them and reads the scores again, mostly from the caches (64 x 40943 bf16 with reference and mask, 24 MB: 4.4 and 9.8 us; with weights 5.3 and
+// 10.2).  Bound by the
 // latency of each pass, a row's sums end before its gradients begin; of large batches by vector instructions and memory alike (2048 x 40943 so, 755 MB:
-// 325 us; with even weights and no mask, in one pass, 148).  Segments of 1024 pairs take 5 to 45 % longer there, of 4096 up to 35 % where rows are few.
+// 330 us, with weights 343; with neither, in one pass, 178).  Segments of 1024 pairs take 5 to 45 % longer there, of 4096 up to 35 % where rows are few.
 constexpr int kSegmentQuads = 2, kSegment = 256 * 4 * kSegmentQuads;
 constexpr int64_t kMostSegments = ((int64_t(1) << 32) - 1) / 256;  // a launch has fewer than 2^32 threads
 

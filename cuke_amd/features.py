@@ -183,7 +183,10 @@ def linear_forward(x, weight, bias=None, *, act="none", residual=None, out_dtype
 
 
 def linear_backward(fw: LinearForward, dy, need_x: bool = True, need_weight: bool = True, need_bias: bool = True) -> LinearGrads:
-    """Gradients of x, weight and bias from the gradient of y (of y's type)."""
+    """Gradients of x, weight and bias from the gradient of y (of y's type).
+
+    What enters the two products is rounded to the layer's type.  In float16 that makes 0 of values below 3e-8 and infinity of those above 65504: scale
+    the loss of a large batch up, and the gradients down again."""
     if not isinstance(fw, LinearForward):
         raise TypeError("fw must come from linear_forward()")
     x, _, bias = fw.tensors[:3]
@@ -210,7 +213,7 @@ def dropout(x, p, seed, step=0, out=None) -> torch.Tensor:
 
     Which elements go is a function of (seed, step, row, column) alone, defined at kge_dropout in the C header; nothing is stored.  step: an
     integer, or one int64 on the GPU that the kernel reads (a captured graph then draws a new mask at every replay).  out: where to, x
-    itself included."""
+    itself or other columns of the same array included."""
     if out is None:
         y = _lib.host().dropout(x, p, seed, step)
         if y is not None:
@@ -242,7 +245,8 @@ def preference_loss(pos, neg, ref_pos=None, ref_neg=None, *, beta=1.0, kind="sig
     With d = sign ((pos - ref_pos) - (neg - ref_neg)) a pair costs -(1 - smoothing) log sigma(beta d) - smoothing log sigma(-beta d)
     ("sigmoid"), max(0, 1 - beta d) ("hinge") or (d - 1 / (2 beta))^2 ("square").  A row's pairs are averaged, evenly or by
     softmax(temperature sign neg) (a constant to the gradient), rows evenly.  mask [B, N] (bool or uint8): False where there is no pair; what the
-    scores hold there is not looked at, and a row without a pair costs nothing.  Gradients and loss are float32."""
+    scores hold there is not looked at, and a row without a pair costs nothing.  Nor does a pair that takes no share of the softmax (an infinitely low
+    score, say); NaN stays NaN.  Gradients and loss are float32."""
     code = _lib.PREFERENCES.get(kind)
     if code is None:
         raise ValueError(f"kind must be one of {sorted(_lib.PREFERENCES)} (got {kind!r})")

@@ -563,7 +563,7 @@ typedef enum kge_act_t {
  * dropped (zero, whatever x holds) iff
  *   16 bits number j % 4 (the lowest first) of  splitmix64(base ^ ((i * ceil(cols / 4) + j / 4) * 0x9E3779B97F4A7C15))  are < T,
  *   base = splitmix64(splitmix64(seed ^ 0xD1B54A32D192ED03) ^ (step + (step_dev ? *step_dev : 0))),
- * and x * 65536 / (65536 - T) otherwise, rounded once.  step_dev is a word in device memory that the kernel reads, so that replays of a captured
+ * and x * 65536 / (65536 - T) otherwise, the factor and the product in fp32.  step_dev is a word in device memory that the kernel reads, so that replays of a captured
  * graph draw new masks.  The gradient of x is the same call on the gradient of y.  y == x is allowed; type: kge_type_t of x and y.
  */
 int kge_dropout(int32_t type, const void *x, int64_t x_stride, void *y, int64_t y_stride, int64_t rows, int64_t cols, double p,
@@ -576,7 +576,8 @@ int kge_dropout(int32_t type, const void *x, int64_t x_stride, void *y, int64_t 
  *   the [rows, out] block with p, seed, step, step_dev (p = 0: none).  16-bit products are summed in fp32 on the matrix cores, fp32 ones
  *   as three-part bf16 products or by fp32 instructions (few rows), with no larger an error against 64 bits than fp32 products;
  *   everything up to the last rounding is fp32.
- *   rows, in, out: 0 .. 2^31 - 1 (in = 0: an empty sum).
+ *   rows, in, out: 0 .. 2^31 - 1 (in = 0: an empty sum), as far as a launch of fewer than 2^32 threads covers the products in tiles
+ *   (some 2^39 elements of y in 16 bits, 2^37 in fp32; of few columns about 2^31 and 2^30 rows; dx likewise); KGE_ESHAPE beyond.
  */
 typedef struct kge_linear {
     int32_t type, out_type; /* kge_type_t */
@@ -597,7 +598,7 @@ typedef struct kge_linear {
 
 /*
  * saved: NULL for inference; else kge_linear_saved_bytes() bytes, 16-byte aligned, which kge_linear_fwd fills for kge_linear_bwd: act'(z)
- * (16-bit layers: in 16 bits of fixed point, to 1.02e-5), and copies of x and weight where the matrix cores cannot take them as they lie
+ * (16-bit layers: in 16 bits of fixed point, to 1.02e-5, so that derivatives below 1e-5 may become 0), and copies of x and weight where the matrix cores cannot take them as they lie
  * (16 bits, with rows that do not start on 16 bytes or whose width is no multiple of 8, or a large weight whose rows lie 4096 bytes apart).  x and weight have to be unchanged when kge_linear_bwd runs, and *step_dev too.
  * The byte counts depend on the types, sizes, strides, the low bits of addresses and whether there is an activation; a saved block of no bytes may be NULL.
  */
@@ -608,7 +609,8 @@ int kge_linear_fwd(const kge_linear *lin, void *y, int64_t y_stride, int for_bac
 
 /*
  * dx [rows, in], dweight [out, in], dbias [out]: contiguous, of type `type`; each may be NULL and is then not computed.  The gradient at the
- * products, dz = drop(dy) act'(z), enters them rounded to `type` (dbias sums it unrounded).  Sums over rows are split and joined in a fixed order:
+ * products, dz = drop(dy) act'(z), enters them rounded to `type`, whatever the type of dy (dbias sums it unrounded): in KGE_F16 what is below 3e-8
+ * becomes 0 and what is above 65504 infinite, so the loss of a large batch is scaled up first, as in other fp16 training.  Sums over rows are split and joined in a fixed order:
  * the same call gives the same bits.
  */
 size_t kge_linear_bwd_workspace(const kge_linear *lin);
@@ -618,13 +620,15 @@ int kge_linear_bwd(const kge_linear *lin, const void *dy, int64_t dy_stride, con
 /*
  * A preference loss over the positive and negative scores of a batch, against those a frozen reference gives the same triples:
  *   d[b][n] = sign * ((pos[b] - ref_pos[b]) - (neg[b][n] - ref_neg[b][n]))       (ref_* NULL: 0; both or neither)
- *   f(d):  KGE_PREFER_SIGMOID  (1 - smoothing) log(1 + exp(-beta d)) + smoothing log(1 + exp(beta d))
+ *   f(d):  KGE_PREFER_SIGMOID  (1 - smoothing) log(1 + exp(-beta d)) + smoothing log(1 + exp(beta d)), a term whose factor is 0 left out
  *          KGE_PREFER_HINGE    max(0, 1 - beta d)
  *          KGE_PREFER_SQUARE   (d - 1 / (2 beta))^2
  *   a[b][.] = softmax over the row's valid n of temperature * sign * neg[b][n]  (0: uniform); a constant to the gradient
  *   loss[0] = 1 / batch * sum_b sum_n a[b][n] f(d[b][n]),   dpos [batch], dneg [batch, n_neg]: its gradients, fp32, contiguous (NULL: not wanted)
  * mask: one byte per pair, 0 = the pair does not exist (what the score arrays hold there is not looked at, its gradient is 0), NULL = all
- * exist.  A row of no valid pair adds nothing, and its dpos is 0.  Scores and reference scores: kge_type_t `type`; sums and exponentials in fp32,
+ * exist.  A row of no valid pair adds nothing, and its dpos is 0.  With a temperature, a pair whose weight is 0 in fp32 adds nothing, also where its
+ * own f is infinite; a score infinitely low (sign * neg) has that weight, and a row of no others adds nothing.  NaN in a pair that exists stays NaN.
+ * batch * ceil(n_neg / 2048) is below 2^24 where n_neg > 1024 (KGE_ESHAPE beyond).  Scores and reference scores: kge_type_t `type`; sums and exponentials in fp32,
  * the loss over rows in 64 bits, joined in a fixed order.  sign: +1 where higher scores are better, -1 for distances.
  */
 typedef enum kge_prefer_t { KGE_PREFER_SIGMOID = 0, KGE_PREFER_HINGE = 1, KGE_PREFER_SQUARE = 2 } kge_prefer_t;
