@@ -106,6 +106,18 @@ class Preference(C.Structure):
                 ("sign", C.c_float), ("smoothing", C.c_float), ("temperature", C.c_float)]
 
 
+class Rows8(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("scale", C.c_void_p), ("scale_stride", C.c_int64)]
+
+
+E4M3 = 3  # KGE_E4M3, beside kge_type_t
+
+
+class RmsNorm(C.Structure):
+    _fields_ = [("type", C.c_int32), ("out_type", C.c_int32), ("rows", C.c_int64), ("cols", C.c_int64), ("x", C.c_void_p),
+                ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64), ("weight", C.c_void_p), ("eps", C.c_double)]
+
+
 EXPORTS = {
     # name: (restype, argtypes)
     "kge_strerror": (C.c_char_p, [C.c_int]),
@@ -172,6 +184,13 @@ EXPORTS = {
     "kge_preference_workspace": (C.c_size_t, [C.POINTER(Preference)]),
     "kge_preference_loss": (C.c_int, [C.POINTER(Preference), C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
                                       C.c_void_p]),
+    "kge_pack8": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.POINTER(Rows8), C.c_void_p]),
+    "kge_unpack8": (C.c_int, [C.POINTER(Rows8), C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
+    "kge_rms_norm_fwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p, C.c_int64, C.POINTER(Rows8), C.c_void_p, C.c_int64, C.c_void_p,
+                                   C.c_void_p]),
+    "kge_rms_norm_bwd_workspace": (C.c_size_t, [C.POINTER(RmsNorm)]),
+    "kge_rms_norm_bwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+                                   C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "kge_check_indices": (C.c_int, [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p]),
 }
 

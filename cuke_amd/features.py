@@ -276,6 +276,150 @@ def preference_loss(pos, neg, ref_pos=None, ref_neg=None, *, beta=1.0, kind="sig
     return loss, dpos, dneg
 
 
+# ---- rows in 8 bits --------------------------------------------------------------------------------
+E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+@dataclass(frozen=True)
+class Rows8:
+    """Rows of ``cols`` values in 8 bits: e4m3 numbers and one power of two for each 32 columns, a value being their product.
+
+    q [rows, 32 ceil(cols / 32)] (float8_e4m3fn), zero behind column cols; scale [rows, 4 ceil(cols / 128)] (float8_e8m0fnu), those behind the last
+    block anything but NaN.  :func:`pack8` and :func:`rms_norm` make them; arrays made elsewhere are taken as they are."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    cols: int
+
+    def __post_init__(self):
+        for t, name, dtype, width in ((self.q, "q", E4M3, 32 * (-(-self.cols // 32))), (self.scale, "scale", _E8M0, 4 * (-(-self.cols // 128)))):
+            if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+                raise TypeError(f"{name} must be a tensor of {dtype} (got {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__})")
+            if self.cols < 0 or t.dim() != 2 or t.shape[1] != width or t.shape[0] != self.q.shape[0]:
+                raise ValueError(f"rows of {self.cols} values need {name} of shape {(self.q.shape[0], width)} (got {tuple(t.shape)})")
+
+    @property
+    def shape(self):
+        return torch.Size((self.q.shape[0], self.cols))
+
+
+def _laid(t: torch.Tensor, unit: int) -> torch.Tensor:
+    """t with rows that start at multiples of `unit` bytes."""
+    ok = (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or (t.stride(0) >= t.shape[1] and t.stride(0) % unit == 0)) and t.data_ptr() % unit == 0
+    return t if ok else t.view(torch.uint8).clone(memory_format=torch.contiguous_format).view(t.dtype)
+
+
+def _rows8(r, name: str) -> Rows8:
+    if not isinstance(r, Rows8):
+        raise TypeError(f"{name} must be Rows8 (got {type(r).__name__})")
+    _tensor(r.q, f"{name}.q", 2), _tensor(r.scale, f"{name}.scale", 2)
+    q, scale = _laid(r.q, 16), _laid(r.scale, 4)
+    return r if q is r.q and scale is r.scale else Rows8(q, scale, r.cols)
+
+
+def _rows8_c(r: Rows8) -> _lib.Rows8:
+    one = r.q.shape[0] <= 1 or r.cols == 0  # (whose stride may be anything)
+    return _lib.Rows8(_p(r.q), r.q.shape[1] if one else r.q.stride(0), _p(r.scale), r.scale.shape[1] if one else r.scale.stride(0))
+
+
+def _new_rows8(rows: int, cols: int, device) -> Rows8:
+    return Rows8(torch.empty((rows, 32 * (-(-cols // 32))), dtype=E4M3, device=device),
+                 torch.empty((rows, 4 * (-(-cols // 128))), dtype=_E8M0, device=device), cols)
+
+
+def pack8(x) -> Rows8:
+    """x [rows, cols] in 8 bits: half the memory of 16 bits, each value within 2^-4 of itself (less than 2^-17 of its block's largest: within
+    2^-19 of that).  What is infinite becomes NaN."""
+    x = _rows(x, "x")
+    out = _new_rows8(x.shape[0], x.shape[1], x.device)
+    _lib.check(_lib.lib().kge_pack8(_TYPES[x.dtype], _p(x), _row_stride(x), x.shape[0], x.shape[1], C.byref(_rows8_c(out)), _stream()), "kge_pack8")
+    return out
+
+
+def unpack8(rows8, dtype=torch.bfloat16) -> torch.Tensor:
+    """What rows in 8 bits stand for, as bfloat16, float16 or float32 (exact, but for what float16 cannot hold)."""
+    r = _rows8(rows8, "rows8")
+    if dtype not in _TYPES:
+        raise TypeError(f"dtype must be float32, bfloat16 or float16 (got {dtype})")
+    y = torch.empty(tuple(r.shape), dtype=dtype, device=r.q.device)
+    _lib.check(_lib.lib().kge_unpack8(C.byref(_rows8_c(r)), r.shape[0], r.cols, _TYPES[dtype], _p(y), max(r.cols, 1), _stream()), "kge_unpack8")
+    return y
+
+
+# ---- norm ------------------------------------------------------------------------------------------
+@dataclass
+class NormForward:
+    """A norm's output, and what its backward pass needs (h and weight have to stay as they are until then)."""
+    y: torch.Tensor | Rows8
+    h: torch.Tensor     # x + residual; x itself where there is none
+    rstd: torch.Tensor  # float32 [rows]
+    weight: torch.Tensor | None
+
+
+@dataclass
+class NormGrads:
+    x: torch.Tensor | None       # of x, and of the residual
+    weight: torch.Tensor | None
+
+
+def _norm_call(x, weight, residual, eps, out_dtype, keep):
+    x = _rows(x, "x")
+    rows, cols = x.shape
+    if weight is not None:
+        weight = _rows(weight, "weight", x.dtype, ndim=1, shape=(cols,))
+    if residual is not None:
+        residual = _rows(residual, "residual", x.dtype, shape=x.shape)
+    eps = float(eps)
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"eps must be finite and not negative (got {eps})")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in _TYPES and out_dtype != E4M3:
+        raise TypeError(f"out_dtype must be float32, bfloat16, float16 or float8_e4m3fn (got {out_dtype})")
+    eight = out_dtype == E4M3
+    y = _new_rows8(rows, cols, x.device) if eight else torch.empty((rows, cols), dtype=out_dtype, device=x.device)
+    h = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if residual is not None else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
+    desc = _lib.RmsNorm(_TYPES[x.dtype], _lib.E4M3 if eight else _TYPES[out_dtype], rows, cols, _p(x), _row_stride(x), _p(residual),
+                        _row_stride(residual) if residual is not None else 0, _p(weight), eps)
+    _lib.check(_lib.lib().kge_rms_norm_fwd(C.byref(desc), None if eight else _p(y), cols, C.byref(_rows8_c(y)) if eight else None, _p(h), cols,
+                                           _p(rstd), _stream()), "kge_rms_norm_fwd")
+    return NormForward(y, x if h is None else h, rstd, weight)
+
+
+def rms_norm(x, weight=None, residual=None, *, eps=1e-6, out_dtype=None):
+    """``h / sqrt(mean(h^2) + eps) * weight`` of the rows of h = x + residual: x, residual [rows, cols] and weight [cols] of one type.
+
+    out_dtype: float32, bfloat16 or float16 (x's, unless said otherwise), or float8_e4m3fn: :class:`Rows8`, as the layers behind it take them.  Gives y, or (y, h) where
+    there is a residual; h is rounded to x's type, y is made of the sum before that."""
+    fw = _norm_call(x, weight, residual, eps, out_dtype, False)
+    return fw.y if residual is None else (fw.y, fw.h)
+
+
+def rms_norm_forward(x, weight=None, residual=None, *, eps=1e-6, out_dtype=None) -> NormForward:
+    """:func:`rms_norm`, with what :func:`rms_norm_backward` needs."""
+    return _norm_call(x, weight, residual, eps, out_dtype, True)
+
+
+def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_weight: bool = True) -> NormGrads:
+    """Gradients from that of y (float32, bfloat16 or float16, whatever y's own type) and, where h went on by itself, that of h (x's type).  The gradient of
+    the residual is that of x.  An 8-bit y's rounding counts as none."""
+    if not isinstance(fw, NormForward):
+        raise TypeError("fw must come from rms_norm_forward()")
+    h, weight = _tensor(fw.h, "h of the forward call", 2), fw.weight
+    dy = _rows(dy, "dy", shape=h.shape)
+    if dh is not None:
+        dh = _rows(dh, "dh", h.dtype, shape=h.shape)
+    rows, cols = h.shape
+    dx = torch.empty((rows, cols), dtype=h.dtype, device=h.device) if need_x else None
+    dw = torch.empty(cols, dtype=h.dtype, device=h.device) if need_weight and weight is not None else None
+    desc = _lib.RmsNorm(_TYPES[h.dtype], _TYPES[h.dtype], rows, cols, None, 0, None, 0, _p(weight), 0.0)
+    L = _lib.lib()
+    ws_bytes = int(L.kge_rms_norm_bwd_workspace(C.byref(desc))) if dw is not None else 0
+    ws = _bytes(ws_bytes, h.device)
+    _lib.check(L.kge_rms_norm_bwd(C.byref(desc), _p(h), _row_stride(h), _p(fw.rstd), _TYPES[dy.dtype], _p(dy), _row_stride(dy), _p(dh),
+                                  _row_stride(dh) if dh is not None else 0, _p(dx), cols, _p(dw), _p(ws), ws_bytes, _stream()), "kge_rms_norm_bwd")
+    return NormGrads(dx, dw)
+
+
 # ---- encoder ---------------------------------------------------------------------------------------
 @dataclass
 class EncoderForward:

@@ -650,6 +650,57 @@ size_t kge_preference_workspace(const kge_preference *pref);
 int kge_preference_loss(const kge_preference *pref, float *loss, float *dpos, float *dneg, void *workspace, size_t workspace_bytes,
                         void *stream);
 
+/* ---- rows in 8 bits, and what deeper encoders do with them -------------------------------------------------------------------
+ *
+ * Rows of `cols` values as e4m3 numbers (4 bits of exponent, 3 of mantissa, no infinity) with one power of two for each block of 32 consecutive
+ * columns, as the matrix cores take them:  value = q 2^(scale - 127), scale a byte (255: the block is NaN).
+ *   q      rows of 32 ceil(cols / 32) bytes, zero behind column cols; 16-byte aligned, rows a multiple of 16 bytes apart
+ *   scale  rows of 4 ceil(cols / 128) bytes, one a block, those behind the last block not 255; 4-byte aligned, rows a multiple of 4 bytes apart
+ * kge_pack8 writes such rows, the bytes behind the end among them (zeros).  A block's power is the least one, from 2^-127 up, that brings the largest of its finite values to
+ * 448 at most; values go to the nearest e4m3 number, ties to the even one.  An infinite value becomes NaN, as NaN does, and leaves the others as they are.
+ */
+typedef struct kge_rows8 {
+    void *q;
+    int64_t q_stride;     /* bytes between rows */
+    void *scale;
+    int64_t scale_stride; /* bytes between rows */
+} kge_rows8;
+#define KGE_E4M3 3 /* beside kge_type_t, where a call says so: rows in 8 bits */
+
+/* x [rows, cols] of kge_type_t `type` to 8 bits, and back.  Unpacking is exact but for what `type` cannot hold (fp16: from 65520 on
+   infinite; else a value that was rounded up to 2^128). */
+int kge_pack8(int32_t type, const void *x, int64_t x_stride, int64_t rows, int64_t cols, const kge_rows8 *out, void *stream);
+int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type, void *y, int64_t y_stride, void *stream);
+
+/*
+ * Root-mean-square norm of rows, a residual added in front of it:
+ *   h = x + residual,   r[i] = (mean_j h[i][j]^2 + eps)^-1/2,   y[i][j] = h[i][j] r[i] weight[j]            (residual, weight NULL: 0, 1)
+ * x, residual, weight and h have the type `type`; y any kge_type_t, or KGE_E4M3: rows in 8 bits (`y8`; else y, y_stride).  h (NULL: not wanted) is the sum
+ * rounded to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32.  Squares are summed in 64 bits, so that no value of a type
+ * overflows; a value in 8 bits is the one nearest to the 64-bit result.
+ * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
+ *   g = dy weight,   dx = dresidual = r (g - h r^2 mean_j(g h)) + dh,   dweight[j] = sum_i dy[i][j] h[i][j] r[i]
+ * h: what the forward call wrote there (x where there was no residual), rstd too.  dx [rows, cols] and dweight [cols] of type `type`, contiguous but for
+ * dx's stride; either may be NULL.  dx may be dy or dh where type and stride are the same.  The fields x and residual of the description are not looked at.  Sums over rows are joined
+ * in a fixed order.  rows, cols: 0 .. 2^31 - 1 (KGE_ESHAPE beyond).
+ */
+typedef struct kge_rms_norm {
+    int32_t type, out_type; /* kge_type_t; out_type also KGE_E4M3 */
+    int64_t rows, cols;
+    const void *x;
+    int64_t x_stride;
+    const void *residual;
+    int64_t residual_stride;
+    const void *weight;
+    double eps; /* >= 0 */
+} kge_rms_norm;
+int kge_rms_norm_fwd(const kge_rms_norm *norm, void *y, int64_t y_stride, const kge_rows8 *y8, void *h, int64_t h_stride, float *rstd,
+                     void *stream);
+size_t kge_rms_norm_bwd_workspace(const kge_rms_norm *norm);
+int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, const float *rstd, int32_t dy_type, const void *dy,
+                     int64_t dy_stride, const void *dh, int64_t dh_stride, void *dx, int64_t dx_stride, void *dweight, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
 /* Sets flag[0] (int32, caller-zeroed) to 1 if any idx[i] is outside [0, n_rows). */
 int kge_check_indices(const int64_t *idx, int64_t n, int64_t n_rows, int32_t *flag, void *stream);
 
