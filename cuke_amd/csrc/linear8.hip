@@ -1,0 +1,356 @@
+// Linear layers on rows in 8 bits: y = drop(act(x8 W^T + b)) + residual with a 16-bit weight or one in 8 bits too, and the gradients (kge_linear8_fwd,
+// kge_linear8_bwd).
+#include "linear_plan.hpp"
+
+namespace kge {
+
+// ---- few rows --------------------------------------------------------------------------------------
+// As linear_few_kernel, with rows in 8 bits (and the weight too: W8) widened on their way to the matrix cores: a step's 32 terms are a block, so that a lane's eight
+// numbers have one scale.
+template <class T>
+struct Line8 {
+    const uint8_t *q, *scale;
+    struct Raw {
+        u2 v;
+        int byte;
+        __device__ __forceinline__ typename Few<T>::piece widened() const { return widen(make_uint2(v[0], v[1]), __int_as_float(byte << 23), T{}); }
+    };
+    __device__ __forceinline__ Line8(const Rows8 &s, int64_t row, int k0) : q(s.q + row * s.q_stride + k0), scale(s.scale + row * s.scale_stride) {}
+    __device__ __forceinline__ Raw load(int64_t block) const { return Raw{*reinterpret_cast<const u2 *>(q + 32 * block), scale[block]}; }
+};
+
+template <class T, int MF, bool W8>
+__global__ __launch_bounds__(kFewWaves *kWave) void linear8_few_kernel(TileArgs t)
+{
+    using F = Few<T>;
+    using Raw = typename Line8<T>::Raw;
+    static_assert(F::kTerms == 32 && F::kEach == 8, "a block a step");
+    constexpr int kAhead = 4;  // steps whose loads are in flight together
+    __shared__ f4 sums[kFewWaves][MF][kWave];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, k0 = F::kEach * (lane >> 4);
+    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MF;
+    const int64_t n = n0 + r < t.a.extent ? n0 + r : t.a.extent - 1;  // (rows that do not exist: others, whose sums nobody asks for)
+    const T *a = static_cast<const T *>(t.a.p) + (W8 ? 0 : n * t.a.stride + k0);
+    const Line8<T> a8(t.a8, W8 ? n : 0, k0);
+    auto row = [&](int j) { return m0 + 16 * j + r < t.b.extent ? m0 + 16 * j + r : t.b.extent - 1; };
+    const Line8<T> first(t.b8, row(0), k0), second(t.b8, row(MF - 1), k0);
+    f4 acc[MF] = {};
+    const int64_t blocks = (t.k + 31) / 32, full = W8 ? blocks : t.k / 32;  // (numbers behind a row's end are zero; a 16-bit weight's row ends where it ends)
+    int64_t s = wave;
+    for (; s + (kAhead - 1) * kFewWaves < full; s += kAhead * kFewWaves) {
+        typename F::piece x[W8 ? 1 : kAhead];
+        Raw x8[W8 ? kAhead : 1], y[kAhead][MF];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int64_t at = s + u * kFewWaves;
+            if constexpr (W8) x8[u] = a8.load(at);
+            else x[u] = F::load(a + 32 * at);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) y[u][j] = (j ? second : first).load(at);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            typename F::piece p;
+            if constexpr (W8) p = x8[u].widened();
+            else p = x[u];
+#pragma unroll
+            for (int j = 0; j < MF; ++j) acc[j] = F::multiply(p, y[u][j].widened(), acc[j]);
+        }
+    }
+    for (; s < blocks; s += kFewWaves) {
+        typename F::piece p;
+        if constexpr (W8) {
+            p = a8.load(s).widened();
+        } else {
+            const int64_t left = t.k - 32 * s - k0;
+            p = F::load(a + 32 * s, left < 0 ? 0 : (int)(left < 8 ? left : 8));
+        }
+#pragma unroll
+        for (int j = 0; j < MF; ++j) acc[j] = F::multiply(p, (j ? second : first).load(s).widened(), acc[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < MF; ++j) sums[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= MF) return;
+    // wave j finishes rows 16 j ..: lane l holds columns 4 (l / 16) .. + 3 of row l % 16
+    f4 z = sums[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; ++w) z += sums[w][wave][lane];
+    const int64_t m = m0 + 16 * wave + r, col = n0 + 4 * (lane >> 4), left = t.e.cols - col;
+    if (m >= t.e.rows || left <= 0) return;
+    const int valid = (int)(left < 4 ? left : 4);
+    float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + col, valid);
+    float out[1][4] = {{z[0], z[1], z[2], z[3]}};
+    finish_quads<T, 1, true>(t.e, t.e.drop.base(), m, 1, col, valid, out, bias, nullptr);
+}
+
+template <class T>
+static void launch_few8(int few, bool w8, const TileArgs &t, hipStream_t st)
+{
+    const dim3 grid((unsigned)ceil_div(t.a.extent, 16), (unsigned)ceil_div(t.b.extent, 16 * few)), block(kFewWaves * kWave);
+    if (few == 1 && w8) hipLaunchKernelGGL((linear8_few_kernel<T, 1, true>), grid, block, 0, st, t);
+    else if (few == 1) hipLaunchKernelGGL((linear8_few_kernel<T, 1, false>), grid, block, 0, st, t);
+    else if (w8) hipLaunchKernelGGL((linear8_few_kernel<T, 2, true>), grid, block, 0, st, t);
+    else hipLaunchKernelGGL((linear8_few_kernel<T, 2, false>), grid, block, 0, st, t);
+}
+
+// ---- forward pass ----------------------------------------------------------------------------------
+// Both sides in 8 bits: tiles of 128 terms.
+using Large8 = Shape<256, 256, 64, 2, 4, 2>;
+using Middle8 = Shape<128, 128, 64, 2, 4, 2>;
+using Tall8 = Shape<64, 128, 64, 2, 2, 2>;
+using Small8 = Shape<64, 64, 64, 2, 2, 3>;
+
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads) void linear8_forward_kernel(TileArgs t)
+{
+    constexpr int kA = side_bytes<S, true>(), kB = side_bytes<S, false>(), k2 = S::STAGES > 2, k3 = S::STAGES > 3;
+    __shared__ __align__(16) char stage0[kA], stage1[kA], stage2[k2 ? kA : 16], stage3[k3 ? kA : 16];
+    __shared__ __align__(16) char wide0[kB], wide1[kB], wide2[k2 ? kB : 16], wide3[k3 ? kB : 16];
+    compute_tile<T, false, false, S, true, true, kSideB>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3, wide0, wide1, wide2, wide3);
+}
+// The matrix cores' own product of 8-bit sides, at twice the pace of the 16-bit one.  It sums eight neighbouring terms at a time and drops of each what lies below 2^-13
+// of the largest one's power (and adds such sums in fp32): some 2^-13 of a result, next to nothing beside its rounding to bf16 (2^-9) and too much for
+// fp16 and fp32, which are made of widened numbers.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads) void linear8_answer_kernel(TileArgs t)
+{
+    constexpr int kStage = stage_bytes8<S>();
+    __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
+    compute_tile<T, false, false, S, true, true, kBothSides>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
+}
+
+template <class T, class S, bool BOTH>
+static void launch_tiles(TileArgs &t, hipStream_t st)
+{
+    t.tiles_a = (int)ceil_div(t.a.extent, S::XA), t.tiles_b = (int)ceil_div(t.b.extent, S::XB);
+    const int64_t blocks = (int64_t)t.tiles_a * t.tiles_b;
+    if (!blocks) return;
+    if constexpr (BOTH && std::is_same<T, bf16_t>::value) hipLaunchKernelGGL((linear8_answer_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
+    else if constexpr (!BOTH) hipLaunchKernelGGL((linear8_forward_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
+}
+
+template <class T>
+static void launch_forward8(TileArgs &t, bool both, hipStream_t st)
+{
+    const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 1 : 0);
+    const int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
+    const double large = forward_cost<Large>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0), middle = forward_cost<Middle>(t, epilogue, 2, 0.73, 2.5);
+    const double tall = forward_cost<Tall>(t, epilogue, 3, 0.53, 2.3), small = forward_cost<Small>(t, epilogue, 3, 0.47, 0.9);
+    if (large <= middle && large <= tall && large <= small) both ? launch_tiles<T, Large8, true>(t, st) : launch_tiles<T, Large, false>(t, st);
+    else if (middle <= tall && middle <= small) both ? launch_tiles<T, Middle8, true>(t, st) : launch_tiles<T, Middle, false>(t, st);
+    else if (tall <= small) both ? launch_tiles<T, Tall8, true>(t, st) : launch_tiles<T, Tall, false>(t, st);
+    else both ? launch_tiles<T, Small8, true>(t, st) : launch_tiles<T, Small, false>(t, st);
+}
+
+// ---- gradients -------------------------------------------------------------------------------------
+// dW = dz^T x8, dx = dz W and the bias's gradient in one launch, as linear_grads_kernel.
+template <class T, class S>
+__global__ __launch_bounds__(S::kThreads) void linear8_grads_kernel(TileArgs dw, TileArgs dx, SumArgs db, int64_t dw_blocks, int64_t dx_blocks)
+{
+    constexpr int kA = side_bytes<S, true>(), kB = side_bytes<S, false>(), k2 = S::STAGES > 2, k3 = S::STAGES > 3;
+    __shared__ __align__(16) char stage0[kB], stage1[kB], stage2[k2 ? kB : 16], stage3[k3 ? kB : 16];
+    __shared__ __align__(16) char wide0[kA], wide1[kA], wide2[k2 ? kA : 16], wide3[k3 ? kA : 16];
+    const int64_t block = blockIdx.x, products = dw_blocks + dx_blocks, before = dx.k > dw.k_each ? dx_blocks : 0;
+    if (block >= products) join_sums<T, S::kThreads>(db, block - products, reinterpret_cast<float4 *>(stage0));
+    else if (block >= before && block < before + dw_blocks)
+        compute_tile<T, true, true, S, false, true, kSideA>(dw, block - before, dw_blocks, stage0, stage1, stage2, stage3, wide0, wide1, wide2, wide3);
+    else
+        compute_tile<T, true, false, S, false, true, kNoSideApart>(dx, before ? block : block - dw_blocks, dx_blocks, stage0, stage1, stage2, stage3, wide0, wide1, wide2,
+                                                                   wide3);
+}
+
+template <class T, class S>
+static void launch_grads8(TileArgs &dw, TileArgs &dx, const SumArgs &db, bool want_dw, bool want_dx, hipStream_t st)
+{
+    for (TileArgs *t : {&dw, &dx}) t->tiles_a = (int)ceil_div(t->a.extent, S::XA), t->tiles_b = (int)ceil_div(t->b.extent, S::XB);
+    const int64_t nw = want_dw ? (int64_t)dw.tiles_a * dw.tiles_b * dw.splits : 0, nx = want_dx ? (int64_t)dx.tiles_a * dx.tiles_b : 0;
+    const int64_t nb = db.out ? ceil_div(db.quads, 4) : 0;
+    if (nw + nx + nb) hipLaunchKernelGGL((linear8_grads_kernel<T, S>), dim3((unsigned)(nw + nx + nb)), dim3(S::kThreads), 0, st, dw, dx, db, nw, nx);
+}
+
+// ---- a layer's plan --------------------------------------------------------------------------------
+struct Plan8 {
+    bool pack_w;         // the weight is copied (one in 8 bits: widened) for the tiles
+    int few;             // few_rows() of the forward pass
+    size_t slope, w;     // bytes of each in a saved block, in this order
+    int64_t quads;
+    int sum_blocks;
+    int64_t sum_rows;
+};
+
+static Plan8 plan8_of(const kge_linear *l, bool w8 = false)
+{
+    Plan8 p;
+    p.quads = ceil_div(l->out, 4);
+    p.pack_w = w8 ? !(l->type == KGE_BF16 && l->out_type == KGE_BF16) : !lies_ready(l->type, l->weight, l->weight_stride, l->in);
+    // (a weight whose rows share a channel is worth copying where many rows are multiplied by it)
+    if (!w8 && l->weight_stride % 2048 == 0 && l->in >= 1024 && l->out >= 1024 && l->rows >= 8192) p.pack_w = true;
+    p.few = few_rows(l->type, l->rows, l->in, l->out, p.pack_w);
+    p.slope = l->act == KGE_ACT_NONE ? 0 : up256((size_t)l->rows * p.quads * 4);
+    p.w = p.pack_w ? packed_bytes(l->type, l->out, l->in) : 0;
+    sum_ranges(l->rows, l->out, &p.sum_blocks, &p.sum_rows);
+    return p;
+}
+
+// what kge_linear_fwd asks of a layer, with a weight that is read where `weight8` lies
+static int check8(const kge_linear *l, bool weight8)
+{
+    if (!l || l->type == KGE_F32) return KGE_EINVAL;
+    kge_linear as = *l;
+    as.x = &as, as.x_stride = as.in;
+    if (weight8) as.weight = &as, as.weight_stride = as.in;
+    return check(&as);
+}
+
+template <class T>
+static int forward8(const kge_linear *l, const kge_rows8 *x8, const kge_rows8 *w8, bool keep, void *y, int64_t y_stride, char *slope, char *pw, hipStream_t st)
+{
+    const Plan8 p = plan8_of(l, w8 != nullptr);
+    TileArgs t{};
+    t.splits = 1;
+    t.e = Ends{y, y_stride, l->bias, l->residual, l->residual_stride, slope, l->rows, l->out, p.quads,
+               make_drop(l->p, l->seed, l->step, l->step_dev, l->out), l->act, l->out_type == KGE_F32, passing(l, y, y_stride)};
+    t.b8 = rows8_of(x8), t.a8 = rows8_of(w8);
+    t.b.extent = l->rows;
+    t.k = l->in;
+    const bool both = w8 && !p.pack_w && !p.few;
+    if (both) {  // (elements of both sides: pairs of terms)
+        t.a = Side{w8->q, w8->q_stride / 2, l->out}, t.b = Side{x8->q, x8->q_stride / 2, l->rows};
+        t.k = q_width(l->in) / 2;
+    } else if (w8) {
+        if (!p.few) launch_unpack8(l->type, t.a8, l->out, up8(l->in), pw, pitch_of(l->type, l->in), st);
+        t.a = Side{pw, pitch_of(l->type, l->in), l->out};
+    } else {
+        if (p.pack_w && (keep || !p.few)) launch_pack(l, false, true, nullptr, pw, st);
+        t.a = side_of(l->weight, l->weight_stride, p.pack_w && !p.few, pw, l->type, l->in, l->out);
+    }
+    if (p.few) {
+        launch_few8<T>(p.few, w8 != nullptr, t, st);
+        KGE_CHECK_LAUNCH();
+        return KGE_OK;
+    }
+    t.k_each = split_length(t.k, 1);
+    launch_forward8<T>(t, both, st);
+    KGE_CHECK_LAUNCH();
+    return KGE_OK;
+}
+
+template <class T>
+static int backward8(const kge_linear *l, const kge_rows8 *x8, const Plan8 &p, const GradPlan &g, const void *dy, int64_t dy_stride, const char *saved, void *dx,
+                     void *dw, void *db, char *ws, hipStream_t st)
+{
+    const int64_t width8 = up8(l->out);
+    const bool ready = l->act == KGE_ACT_NONE && nearbyint(l->p * 65536.0) == 0.0 && l->out_type == l->type && lies_ready(l->type, dy, dy_stride, l->out);
+    char *dz = ws;
+    float *sums = reinterpret_cast<float *>(ws + packed_bytes(l->type, l->rows, l->out));
+    float *part = reinterpret_cast<float *>(reinterpret_cast<char *>(sums) + up256((size_t)p.sum_blocks * p.quads * 16));
+    const bool want_dz = !ready && (dx || dw);
+    if ((want_dz || db) && l->rows > 0 && l->out > 0) {
+        GradArgs a{dy, dy_stride, p.slope ? saved : nullptr, l->rows, l->out, p.quads, p.sum_rows,
+                   make_drop(l->p, l->seed, l->step, l->step_dev, l->out), want_dz ? dz : nullptr, width8, pitch_of(l->type, l->out), db ? sums : nullptr, 4};
+        while (a.lanes < 64 && 8 * a.lanes < width8) a.lanes *= 2;
+        const dim3 grid((unsigned)ceil_div(width8, 8 * a.lanes), (unsigned)p.sum_blocks);
+        if (l->out_type == KGE_F32) hipLaunchKernelGGL((linear_dz_kernel<T, float, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((linear_dz_kernel<T, T, true>), grid, dim3(256), 0, st, a);
+    }
+    const int64_t in_quads = ceil_div(l->in, 4);
+    TileArgs tx{}, tw{};
+    tx.a = side_of(l->weight, l->weight_stride, p.pack_w, saved + p.slope, l->type, l->in, l->in);
+    tx.b = side_of(dy, dy_stride, !ready, dz, l->type, l->out, l->rows);
+    tx.k = l->out, tx.splits = 1, tx.k_each = split_length(l->out, 1);
+    tx.e.y = dx, tx.e.y_stride = l->in, tx.e.rows = l->rows, tx.e.cols = l->in, tx.e.quads = in_quads;
+    tw.a.extent = l->in, tw.a8 = rows8_of(x8);
+    tw.b = tx.b, tw.b.extent = l->out;
+    tw.k = l->rows, tw.splits = g.dw_splits, tw.k_each = split_length(l->rows, tw.splits);
+    tw.partial = tw.splits > 1 ? part : nullptr;
+    tw.e.y = dw, tw.e.y_stride = l->in, tw.e.rows = l->out, tw.e.cols = l->in, tw.e.quads = in_quads;
+    const SumArgs sum{sums, p.sum_blocks, l->out, p.quads, db};
+    if (g.tile == 256) launch_grads8<T, Large>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
+    else if (g.tile == 128) launch_grads8<T, MiddleG>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
+    else launch_grads8<T, Small>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
+    if (dw && tw.partial) launch_join<T>(JoinArgs{part, l->out, l->in, in_quads, tw.splits, dw}, st);
+    KGE_CHECK_LAUNCH();
+    return KGE_OK;
+}
+
+}  // namespace kge
+
+using namespace kge;
+
+static size_t backward8_bytes(const kge_linear *l, const Plan8 &p, const GradPlan &g)
+{
+    return packed_bytes(l->type, l->rows, l->out) + up256((size_t)p.sum_blocks * p.quads * 16) +
+           (g.dw_splits > 1 ? (size_t)g.dw_splits * l->out * ceil_div(l->in, 4) * 16 : 0);
+}
+
+extern "C" {
+
+size_t kge_linear8_saved_bytes(const kge_linear *lin)
+{
+    if (check8(lin, false)) return 0;
+    const Plan8 p = plan8_of(lin);
+    return p.slope + p.w;
+}
+
+size_t kge_linear8_fwd_workspace(const kge_linear *lin, const kge_rows8 *weight8, int for_backward)
+{
+    if (check8(lin, weight8 != nullptr)) return 0;
+    const Plan8 p = plan8_of(lin, weight8 != nullptr);
+    return for_backward || p.few ? 0 : p.w;
+}
+
+int kge_linear8_fwd(const kge_linear *lin, const kge_rows8 *x8, const kge_rows8 *weight8, void *y, int64_t y_stride, int for_backward, void *saved,
+                    size_t saved_bytes, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (const int rc = check8(lin, weight8 != nullptr)) return rc;
+    if (const int rc = check_rows8(x8, lin->rows, lin->in)) return rc;
+    if (weight8) {
+        if (for_backward) return KGE_EINVAL;
+        if (const int rc = check_rows8(weight8, lin->out, lin->in)) return rc;
+    }
+    if (lin->rows == 0 || lin->out == 0) return KGE_OK;
+    if (!y) return KGE_EINVAL;
+    if (y_stride < lin->out) return KGE_ESHAPE;
+    const Plan8 p = plan8_of(lin, weight8 != nullptr);
+    const size_t need_saved = for_backward ? p.slope + p.w : 0, need = for_backward || p.few ? 0 : p.w;
+    if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
+    char *slope = for_backward && p.slope ? static_cast<char *>(saved) : nullptr;
+    char *pw = for_backward ? static_cast<char *>(saved) + p.slope : static_cast<char *>(workspace);
+    hipStream_t st = as_stream(stream);
+    KGE_CLEAR_LAUNCH_ERRORS();
+    if (lin->type == KGE_BF16) return forward8<bf16_t>(lin, x8, weight8, for_backward != 0, y, y_stride, slope, pw, st);
+    return forward8<half_t>(lin, x8, weight8, for_backward != 0, y, y_stride, slope, pw, st);
+}
+
+size_t kge_linear8_bwd_workspace(const kge_linear *lin)
+{
+    if (check8(lin, false)) return 0;
+    const GradPlan g = grad_plan(lin);
+    return g.tile ? backward8_bytes(lin, plan8_of(lin), g) : 0;
+}
+
+int kge_linear8_bwd(const kge_linear *lin, const kge_rows8 *x8, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx,
+                    void *dweight, void *dbias, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (const int rc = check8(lin, false)) return rc;
+    if (const int rc = check_rows8(x8, lin->rows, lin->in)) return rc;
+    if (dy_stride < lin->out) return KGE_ESHAPE;
+    if (lin->rows > 0 && lin->out > 0 && !dy) return KGE_EINVAL;
+    const Plan8 p = plan8_of(lin);
+    const GradPlan g = grad_plan(lin);
+    if (!g.tile || (dx && !g.dx)) return KGE_ESHAPE;
+    const size_t need_saved = p.slope + p.w, need = backward8_bytes(lin, p, g);
+    if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
+    hipStream_t st = as_stream(stream);
+    KGE_CLEAR_LAUNCH_ERRORS();
+    const char *s = static_cast<const char *>(saved);
+    char *ws = static_cast<char *>(workspace);
+    if (lin->type == KGE_BF16) return backward8<bf16_t>(lin, x8, p, g, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+    return backward8<half_t>(lin, x8, p, g, dy, dy_stride, s, dx, dweight, dbias, ws, st);
+}
+
+}  // extern "C"

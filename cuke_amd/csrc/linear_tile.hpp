@@ -4,11 +4,13 @@
 // over rows, the index inside).  y = x W^T has both sides along, dx = dz W one across, dW = dz^T x both: no operand is ever transposed in
 // memory.  A tile that lies across is turned by the transposing LDS reads on its way to the matrix cores.  16-bit tiles go to LDS 16 bytes a lane
 // without passing through registers; fp32 ones are taken through registers, where every value becomes three bf16 parts (mfma_split.hpp), of
-// whose nine products six are formed.
+// whose nine products six are formed.  Rows in 8 bits go through registers too, where they become 16-bit ones (every e4m3 number times a power of two is
+// one), or, where both sides are in 8 bits, to LDS as they lie: the matrix cores take them with their powers.
 #pragma once
 
 #include "features.hpp"
 #include "mfma_split.hpp"
+#include "rows8.hpp"
 
 namespace kge {
 
@@ -16,6 +18,8 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef int i8v __attribute__((ext_vector_type(8)));
 
 template <class E>
 struct Mfma;
@@ -56,13 +60,17 @@ struct Ends {
     int passing;  // y, in fp32 and its quads on 16 bytes, is written past the caches
 };
 
+// Which sides of a product are rows in 8 bits.  kNoSideApart: neither, but side a in the arrays that another product of the launch needs for such a side.
+enum Eight { kNoSide = 0, kSideA = 1, kSideB = 2, kBothSides = 3, kNoSideApart = 4 };
+
 struct TileArgs {
-    Side a, b;      // a: the columns of the output, b: its rows
+    Side a, b;      // a: the columns of the output, b: its rows (one in 8 bits: its extent, and what lies in memory is in a8 or b8)
     int64_t k;      // terms of every sum
     int64_t k_each; // per split, a multiple of 64
     int tiles_a, tiles_b, splits;
     float *partial; // where a sum is split: [splits][rows][quads * 4] in fp32, to be joined; else NULL
     Ends e;
+    Rows8 a8, b8;
 };
 
 static __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};  // what chunks outside a side read
@@ -70,6 +78,26 @@ static __device__ __align__(16) const uint32_t zero_chunk[4] = {0, 0, 0, 0};  //
 __device__ __forceinline__ void chunk_to_lds(const void *src, void *lds)
 {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+__device__ __forceinline__ void word_to_lds(const void *src, void *lds)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)lds, 4, 0, 0);
+}
+
+// eight e4m3 numbers times the power of two whose exponent byte is in bits 23 .. 30 of `power`, as 16-bit numbers
+__device__ __forceinline__ s16x8 widen(uint2 q, float power, bf16_t)
+{
+    typedef __bf16 pair __attribute__((ext_vector_type(2)));
+    const pair a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.x, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.x, power, true);
+    const pair c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.y, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q.y, power, true);
+    return __builtin_bit_cast(s16x8, __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7));
+}
+__device__ __forceinline__ s16x8 widen(uint2 q, float power, half_t)
+{
+    typedef _Float16 pair __attribute__((ext_vector_type(2)));
+    const pair a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q.x, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q.x, power, true);
+    const pair c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q.y, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(q.y, power, true);
+    return __builtin_bit_cast(s16x8, __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 // A tile of X indices by K (32 or 64) terms in LDS, as 16-byte chunks.  Along: K / 8 chunks a row, chunk j in slot j ^ (row / 2 % 8) (K = 32: j ^
@@ -193,6 +221,51 @@ struct Tile {
         }
     };
 
+    // The same of a side in 8 bits: a chunk's eight numbers and its block's scale wait in registers, two tiles' at a time, and go to LDS as 16-bit ones.
+    template <class E>
+    struct ByteFeed {
+        const uint8_t *q[kRounds], *scale[kRounds];
+        int64_t q_step, scale_step;
+        int term[kRounds];  // of the chunk, within the tile; above every other where its index does not exist
+        uint2 held[2][kRounds];
+        int byte[2][kRounds];
+
+        __device__ __forceinline__ void start(const Rows8 &s, int64_t extent, int64_t first, int64_t k)
+        {
+            q_step = ACROSS ? K * s.q_stride : K, scale_step = ACROSS ? K * s.scale_stride : K / 32;
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
+                const int64_t index = first + (ACROSS ? 8 * j : row), line = ACROSS ? k + row : index, col = ACROSS ? index : k + 8 * j;
+                term[r] = index < extent ? (ACROSS ? row : 8 * j) : 0x7FFFFFFF;
+                q[r] = s.q + line * s.q_stride + col, scale[r] = s.scale + line * s.scale_stride + (col >> 5);
+            }
+        }
+        // the next tile, of which `left` terms exist (none, behind the end)
+        __device__ __forceinline__ void fetch(int set, int64_t left)
+        {
+            typedef const __attribute__((address_space(1))) u2 *pair;
+            typedef const __attribute__((address_space(1))) uint8_t *single;
+            const uint64_t zero = reinterpret_cast<uint64_t>(zero_chunk);
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                // (an address that the compiler knows nothing of: it would branch around the load of what it knows to be zero, and loads are counted)
+                uint64_t at = term[r] < left ? reinterpret_cast<uint64_t>(q[r]) : zero, of = term[r] < left ? reinterpret_cast<uint64_t>(scale[r]) : zero;
+                asm("" : "+v"(at), "+v"(of));
+                const u2 v = *(pair)at;
+                held[set][r] = make_uint2(v[0], v[1]);
+                byte[set][r] = *(single)of;
+                q[r] += q_step, scale[r] += scale_step;
+            }
+        }
+        __device__ __forceinline__ void put(int set, char *lds)
+        {
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r)
+                *reinterpret_cast<s16x8 *>(lds + 16 * (r * THREADS + (int)threadIdx.x)) = widen(held[set][r], __int_as_float(byte[set][r] << 23), E{});
+        }
+    };
+
     // eight terms of an index for each lane: index at + lane % 32, terms 16 step + 8 (lane / 32) .. + 7
     __device__ __forceinline__ static s16x8 read(const char *lds, int at, int step, int lane)
     {
@@ -206,6 +279,41 @@ struct Tile {
         const char *q = lds + 16 * ((row + 4) * kRow + ((index >> 3) ^ turn(row + 4))) + 2 * (index & 7);
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)q);
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// 32 terms of 8 bits of an index for each lane (of a tile along rows whose elements are pairs of terms): index at + lane % 32, terms 64 step + 16 (lane / 32) .. + 15
+// and 32 on from there.  The instruction's first block of 32 terms is the first half of what all lanes hold; its scale is that of lane % 32, the second's that of
+// lane % 32 + 32.
+template <class TILE>
+__device__ __forceinline__ i8v read_eight(const char *lds, int at, int step, int lane)
+{
+    const int row = at + (lane & 31), j = 4 * step + (lane >> 5), turn = TILE::turn(row);
+    const s16x8 lo = *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + (j ^ turn)));
+    const s16x8 hi = *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + ((j + 2) ^ turn)));
+    return __builtin_bit_cast(i8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15));
+}
+
+// The scales of a tile of 128 terms of both sides, a word an index: XA of side a, then XB of side b, then what no index asks for.
+template <int XA, int XB, int THREADS>
+struct ScaleFeed {
+    static_assert(XA + XB <= THREADS, "a word a thread");
+    static constexpr int kBytes = 4 * THREADS;
+    const uint8_t *from;
+    int step;
+    __device__ __forceinline__ void start(const Rows8 &a, int64_t extent_a, int64_t n0, const Rows8 &b, int64_t extent_b, int64_t m0)
+    {
+        const int i = threadIdx.x;
+        const bool second = i >= XA;
+        const int64_t index = second ? m0 + i - XA : n0 + i;
+        const bool there = second ? i < XA + XB && index < extent_b : index < extent_a;
+        from = there ? (second ? b.scale + index * b.scale_stride : a.scale + index * a.scale_stride) : reinterpret_cast<const uint8_t *>(zero_chunk);
+        step = there ? 4 : 0;
+    }
+    __device__ __forceinline__ void load(bool more, char *lds)  // the next tile's (behind the end: zeros)
+    {
+        word_to_lds(more ? from : reinterpret_cast<const uint8_t *>(zero_chunk), lds + 4 * 64 * __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6));
+        from += step;
     }
 };
 
@@ -250,8 +358,9 @@ struct Raw4 {
 };
 
 // Four consecutive columns (`valid` of them exist) of R rows, `apart` rows from one to the next, through the layer's epilogue.  T: the layer's
-// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.  ahead: the rows' residuals, or NULL.
-template <class T, int R>
+// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.  ahead: the rows' residuals, or NULL.  KEEP8: act' is kept in
+// 8 bits.
+template <class T, int R, bool KEEP8 = false>
 __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64_t first, int apart, int64_t col, int valid, float (&z)[R][4], float4 bias,
                                              const Raw4 *ahead)
 {
@@ -285,7 +394,9 @@ __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64
             for (int r = 0; r < R; ++r) {
                 const int64_t row = first + r * apart, at = row * 4 * e.quads + col;
                 if (row >= e.rows) continue;
-                if (sizeof(T) == 4) {
+                if (KEEP8) {
+                    *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(e.slope) + at) = slopes_to_bytes(slope[4 * r], slope[4 * r + 1], slope[4 * r + 2], slope[4 * r + 3]);
+                } else if (sizeof(T) == 4) {
                     *reinterpret_cast<float4 *>(static_cast<float *>(e.slope) + at) = make_float4(slope[4 * r], slope[4 * r + 1], slope[4 * r + 2], slope[4 * r + 3]);
                 } else {
                     const us2 lo = slopes_to_fixed(slope[4 * r], slope[4 * r + 1]), hi = slopes_to_fixed(slope[4 * r + 2], slope[4 * r + 3]);
@@ -364,11 +475,17 @@ struct Shape {
 };
 template <class T, class S>
 constexpr int stage_bytes() { return (S::XA + S::XB) * S::K * 2 * (sizeof(T) == 4 ? kSplitParts : 1); }
+template <class S, bool A>
+constexpr int side_bytes() { return (A ? S::XA : S::XB) * S::K * 2; }
+template <class S>
+constexpr int stage_bytes8() { return (S::XA + S::XB) * S::K * 2 + 4 * S::kThreads; }  // (both sides in 8 bits: the scales lie behind them)
 
 // T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.  WHOLE: an fp32
-// side's rows are whole quads.
-template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER, bool WHOLE>
-__device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, int64_t blocks, char *stage0, char *stage1, char *stage2, char *stage3)
+// side's rows are whole quads.  EIGHT: the sides that are rows in 8 bits; one of them goes to arrays of its own (wide0 ..), so that its writes do not wait for the
+// other's loads; where both are, elements are pairs of terms (the stride of Side in pairs, TileArgs::k too).
+template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER, bool WHOLE, Eight EIGHT = kNoSide>
+__device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, int64_t blocks, char *stage0, char *stage1, char *stage2, char *stage3,
+                                             char *wide0 = nullptr, char *wide1 = nullptr, char *wide2 = nullptr, char *wide3 = nullptr)
 {
     constexpr bool kFloat = sizeof(T) == 4;
     using E = typename std::conditional<kFloat, bf16_t, T>::type;
@@ -376,9 +493,11 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     using A = Tile<S::XA, K, A_ACROSS, S::kThreads>;
     using B = Tile<S::XB, K, B_ACROSS, S::kThreads>;
     constexpr int kBytesA = S::XA * K * 2, kBytesB = S::XB * K * 2, kStage = stage_bytes<T, S>();
+    static_assert(EIGHT == kNoSide || (!kFloat && SHARE == 1 && (EIGHT != kBothSides || (K == 64 && !A_ACROSS && !B_ACROSS))), "sides in 8 bits");
     constexpr int FA = S::XA / WA / 32, FB = S::XB / WB / 32;
     static_assert(STAGES >= 2 && STAGES <= 4 && (!kFloat || STAGES == 2), "stages");
 
+    constexpr bool kWideA = EIGHT == kSideA || EIGHT == kNoSideApart, kApartSides = kWideA || EIGHT == kSideB;
     int ta, tb, split;
     tile_of(block, blocks, t, &ta, &tb, &split);
     const int64_t n0 = (int64_t)ta * S::XA, m0 = (int64_t)tb * S::XB;
@@ -390,7 +509,33 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     int64_t left = k1 - k0;  // terms not requested yet
     const int tiles = left > 0 ? (int)((left + K - 1) / K) : 0;
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
-    auto multiply = [&](const char *lds) {
+    auto wide = [&](int u) -> char * { return u == 0 ? wide0 : (u == 1 ? wide1 : (u == 2 ? wide2 : wide3)); };
+    auto multiply = [&](int u) {
+        const char *la = kWideA ? wide(u) : stage(u), *lb = kWideA ? stage(u) : (EIGHT == kSideB ? wide(u) : la + PLANES * kBytesA);
+        if constexpr (EIGHT == kBothSides) {
+            // (half a wave gives the first block's scales, the other the second's: its byte of a word is moved to where the instruction looks)
+            int sa[FA], sb[FB];
+            const char *scales = lb + kBytesB;
+#pragma unroll
+            for (int j = 0; j < FB; ++j) sb[j] = *reinterpret_cast<const int *>(scales + 4 * (S::XA + wb + 32 * j + (lane & 31))) >> 8 * (lane >> 5);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) sa[i] = *reinterpret_cast<const int *>(scales + 4 * (wa + 32 * i + (lane & 31))) >> 8 * (lane >> 5);
+#pragma unroll
+            for (int u = 0; u < K / 32; ++u) {
+                i8v a[FA], b[FB];
+#pragma unroll
+                for (int j = 0; j < FB; ++j) b[j] = read_eight<B>(lb, wb + 32 * j, u, lane);
+#pragma unroll
+                for (int i = 0; i < FA; ++i) a[i] = read_eight<A>(la, wa + 32 * i, u, lane);
+#pragma unroll
+                for (int i = 0; i < FA; ++i)
+#pragma unroll
+                    for (int j = 0; j < FB; ++j)
+                        acc[i][j] = u == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 0, sa[i], 0, sb[j])
+                                           : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 2, sa[i], 2, sb[j]);
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < K / 16 / SHARE; ++u) {
             const int step = part * (K / 16 / SHARE) + u;
@@ -398,9 +543,9 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
 #pragma unroll
             for (int p = 0; p < PLANES; ++p) {
 #pragma unroll
-                for (int j = 0; j < FB; ++j) b[j][p] = B::read(lds + PLANES * kBytesA + p * kBytesB, wb + 32 * j, step, lane);
+                for (int j = 0; j < FB; ++j) b[j][p] = B::read(lb + p * kBytesB, wb + 32 * j, step, lane);
 #pragma unroll
-                for (int i = 0; i < FA; ++i) a[i][p] = A::read(lds + p * kBytesA, wa + 32 * i, step, lane);
+                for (int i = 0; i < FA; ++i) a[i][p] = A::read(la + p * kBytesA, wa + 32 * i, step, lane);
             }
 #pragma unroll
             for (int i = 0; i < FA; ++i)
@@ -435,44 +580,103 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             lds_ready();
             put(1 - u, stage(1 - u));
             fetch(1 - u);
-            multiply(stage(u));
+            multiply(u);
         };
         int at = 0;
         for (; at + 2 <= tiles; at += 2) turn(0), turn(1);
         if (at < tiles) turn(0);
+    } else if constexpr (EIGHT == kSideA || EIGHT == kSideB) {
+        // The 16-bit side is requested STAGES - 1 tiles ahead; the other one's numbers come to registers three tiles ahead and to LDS one tile ahead.  Only what the
+        // turn before this one has requested may still be on its way at the barrier: the compiler, which cannot count loads to registers among those to LDS,
+        // would otherwise wait for all of them before it uses a register.
+        using Q = typename std::conditional<EIGHT == kSideA, A, B>::type;
+        using W = typename std::conditional<EIGHT == kSideA, B, A>::type;
+        constexpr int kOut = (STAGES > 2 ? W::kRounds : 0) + 2 * Q::kRounds;
+        typename Q::template ByteFeed<E> bytes;
+        typename W::template Feed<E> feed;
+        if constexpr (EIGHT == kSideA) bytes.start(t.a8, t.a.extent, n0, k0), feed.start(t.b, m0, k0);
+        else bytes.start(t.b8, t.b.extent, m0, k0), feed.start(t.a, n0, k0);
+        int64_t left8 = left;
+        auto fetch = [&](int set) { bytes.fetch(set, left8), left8 -= K; };
+        auto load = [&](char *lds) { feed.load(left, lds), left -= K; };
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        bytes.put(0, wide0);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+        auto in_order = [] {  // (what is still in flight is counted: no load moves in front of one that is written before it)
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        auto turn = [&](int u, int set) {
+            stage_ready<kOut>();
+            load(stage((u + STAGES - 1) % STAGES));
+            in_order();
+            bytes.put(1 - set, wide((u + 1) % STAGES));
+            in_order();
+            fetch(1 - set);
+            in_order();
+            multiply(u);
+        };
+        constexpr int kTurns = STAGES % 2 ? 2 * STAGES : STAGES;
+        int at = 0;
+        for (; at + kTurns <= tiles; at += kTurns)
+#pragma unroll
+            for (int u = 0; u < kTurns; ++u) turn(u % STAGES, u & 1);
+#pragma unroll
+        for (int u = 0; u < kTurns - 1; ++u) {
+            if (at + u >= tiles) break;
+            turn(u % STAGES, u & 1);
+        }
     } else {
         typename A::template Feed<E> feed_a;
         typename B::template Feed<E> feed_b;
-        constexpr int kLoads = A::kRounds + B::kRounds;  // per thread and tile
+        ScaleFeed<S::XA, S::XB, EIGHT == kBothSides ? S::kThreads : S::XA + S::XB> scales;
+        constexpr int kLoads = A::kRounds + B::kRounds + (EIGHT == kBothSides);  // per thread and tile
         feed_a.start(t.a, n0, k0), feed_b.start(t.b, m0, k0);
-        auto load = [&](char *lds) { feed_a.load(left, lds), feed_b.load(left, lds + kBytesA), left -= K; };
+        if constexpr (EIGHT == kBothSides) scales.start(t.a8, t.a.extent, n0, t.b8, t.b.extent, m0);
+        auto load = [&](int u) {
+            char *lds = stage(u);
+            if constexpr (EIGHT == kNoSideApart) feed_a.load(left, wide(u)), feed_b.load(left, lds);
+            else feed_a.load(left, lds), feed_b.load(left, lds + kBytesA);
+            if constexpr (EIGHT == kBothSides) scales.load(left > 0, lds + kBytesA + kBytesB);
+            left -= K;
+        };
         // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
 #pragma unroll
-        for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
+        for (int u = 0; u < STAGES - 1; ++u) load(u);
         int at = 0;
         for (; at + STAGES <= tiles; at += STAGES)
 #pragma unroll
             for (int u = 0; u < STAGES; ++u) {
                 stage_ready<kLoads * (STAGES - 2)>();
-                load(stage((u + STAGES - 1) % STAGES));
-                multiply(stage(u));
+                load((u + STAGES - 1) % STAGES);
+                multiply(u);
             }
 #pragma unroll
         for (int u = 0; u < STAGES - 1; ++u) {
             if (at + u >= tiles) break;
             stage_ready<kLoads * (STAGES - 2)>();
-            load(stage((u + STAGES - 1) % STAGES));
-            multiply(stage(u));
+            load((u + STAGES - 1) % STAGES);
+            multiply(u);
         }
     }
 
     // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows by 64 (or 32) of the wave's columns at a time, so that they
     // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.  A
     // strip's residuals are requested all at once and ahead of everything else that is done with it.
-    constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16, kPerStage = kStage / kStrip;
+    constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16;
+    constexpr int kPerStage = (kWideA ? kBytesB : (EIGHT == kSideB ? kBytesA : kStage)) / kStrip, kPerWide = (kWideA ? kBytesA : kBytesB) / kStrip;
     constexpr int kApart = 64 / kQuads, kRows = 4 / SHARE, kTurns = 32 / (kApart * kRows * SHARE);  // rows a read covers, reads a turn, turns of a wave in a strip
     constexpr int kStrips = FA / kGroup * FB;
-    static_assert(FA % kGroup == 0 && kPerStage >= 1 && (WA * WB + kPerStage - 1) / kPerStage <= STAGES, "a strip for every wave");
+    static_assert(FA % kGroup == 0 && kPerStage >= 1 && WA * WB <= STAGES * (kPerStage + (kApartSides ? kPerWide : 0)), "a strip for every wave");
     static_assert(SHARE == 1 || (kStrips == 1 && kPerStage >= SHARE * WA * WB), "waves that share a strip");
     const int quad = lane % kQuads, row0 = lane / kQuads + part * kTurns * kApart * kRows;
     const bool ahead = LAYER && t.e.residual && t.e.cols % 4 == 0;
@@ -490,6 +694,8 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     stage_ready<0>();
     auto skew = [](int row) { return kQuads == 16 ? row & 15 : (row >> 1) & 7; };
     char *lds = stage(wave / kPerStage) + wave % kPerStage * kStrip;
+    if constexpr (kApartSides)
+        if (wave >= STAGES * kPerStage) lds = wide((wave - STAGES * kPerStage) / kPerWide) + (wave - STAGES * kPerStage) % kPerWide * kStrip;
     uint64_t base = 0;
     if constexpr (LAYER) base = t.e.drop.base();
     // (one copy of what is done with a strip: unrolled, the epilogue alone would fill the instruction cache)
@@ -545,7 +751,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                 z[k][0] = v.x, z[k][1] = v.y, z[k][2] = v.z, z[k][3] = v.w;
             }
             if constexpr (LAYER) {
-                finish_quads<T, kRows>(t.e, base, first, kApart, col, valid, z, bias, ahead ? held[u] : nullptr);
+                finish_quads<T, kRows, (EIGHT != kNoSide)>(t.e, base, first, kApart, col, valid, z, bias, ahead ? held[u] : nullptr);
             } else {
 #pragma unroll
                 for (int k = 0; k < kRows; ++k) {

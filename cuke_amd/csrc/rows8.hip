@@ -72,15 +72,14 @@ static int pack(const void *x, int64_t x_stride, int64_t rows, int64_t cols, con
     KGE_CHECK_LAUNCH();
     return KGE_OK;
 }
-template <class T>
-static int unpack(const kge_rows8 *in, int64_t rows, int64_t cols, void *y, int64_t y_stride, hipStream_t st)
+void launch_unpack8(int type, const Rows8 &in, int64_t rows, int64_t cols, void *y, int64_t y_stride, hipStream_t st)
 {
     const int64_t each = ceil_div(cols, 8);
     const Places p{rows, cols, (uint32_t)each, rows * each};
-    KGE_CLEAR_LAUNCH_ERRORS();
-    hipLaunchKernelGGL(unpack8_kernel<T>, dim3(grid_for(p.total)), dim3(256), 0, st, rows8_of(in), static_cast<T *>(y), y_stride, p);
-    KGE_CHECK_LAUNCH();
-    return KGE_OK;
+    const dim3 grid(grid_for(p.total)), block(256);
+    if (type == KGE_F32) hipLaunchKernelGGL(unpack8_kernel<float>, grid, block, 0, st, in, static_cast<float *>(y), y_stride, p);
+    else if (type == KGE_BF16) hipLaunchKernelGGL(unpack8_kernel<bf16_t>, grid, block, 0, st, in, static_cast<bf16_t *>(y), y_stride, p);
+    else hipLaunchKernelGGL(unpack8_kernel<half_t>, grid, block, 0, st, in, static_cast<half_t *>(y), y_stride, p);
 }
 
 static bool too_large(int64_t rows, int64_t cols) { return rows < 0 || cols < 0 || rows >= (int64_t)1 << 31 || cols >= (int64_t)1 << 31; }
@@ -111,10 +110,10 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
     if (const int rc = check_rows8(rows8, rows, cols)) return rc;
     if (rows == 0 || cols == 0) return KGE_OK;
     if (!y) return KGE_EINVAL;
-    hipStream_t st = as_stream(stream);
-    if (type == KGE_F32) return unpack<float>(rows8, rows, cols, y, y_stride, st);
-    if (type == KGE_BF16) return unpack<bf16_t>(rows8, rows, cols, y, y_stride, st);
-    return unpack<half_t>(rows8, rows, cols, y, y_stride, st);
+    KGE_CLEAR_LAUNCH_ERRORS();
+    launch_unpack8(type, rows8_of(rows8), rows, cols, y, y_stride, as_stream(stream));
+    KGE_CHECK_LAUNCH();
+    return KGE_OK;
 }
 
 }  // extern "C"

@@ -29,6 +29,9 @@ inline int check_rows8(const kge_rows8 *r, int64_t rows, int64_t cols)
     return KGE_OK;
 }
 
+// kge_unpack8 of rows that have been checked; y [rows, cols] with any cols up to q_width() (what lies behind a row's end is zero)
+void launch_unpack8(int type, const Rows8 &in, int64_t rows, int64_t cols, void *y, int64_t y_stride, hipStream_t st);
+
 template <int CTRL>
 __device__ __forceinline__ int dpp(int v)
 {

@@ -5,7 +5,10 @@ The score functions of :mod:`cuke_amd.kge` look rows up.  The operators here sta
   linear / linear_forward / linear_backward   ``drop(act(x W^T + b)) + residual`` and its gradients
   dropout / dropout_backward                  rows dropped by a counter-based generator; no mask is kept
   preference_loss                             positive against negative scores, relative to a frozen reference's
+  Rows8, pack8, unpack8                       rows in 8 bits, with a power of two for each 32 columns: what deeper encoders keep
+  rms_norm / rms_norm_forward / rms_norm_backward   a residual's addition and the norm of the sum, to rows of a type or of 8 bits
   FeatureEncoder                              two linear layers that turn feature rows into entity rows
+  ResidualEncoder                             blocks of a norm and two layers on a residual stream, whose inputs are all kept in 8 bits
 
 Like the rest of the package they work on the current stream, allocate their outputs, give every gradient by an explicit call,
 and raise where an argument is not what the kernels take: there is no fallback.  The ordinary call goes through csrc/host.cpp, what that does
@@ -23,7 +26,8 @@ from . import _lib
 from ._lib import KgeError
 
 __all__ = ["linear", "linear_forward", "linear_backward", "LinearForward", "LinearGrads", "dropout", "dropout_backward",
-           "preference_loss", "FeatureEncoder", "EncoderForward", "EncoderGrads"]
+           "preference_loss", "Rows8", "pack8", "unpack8", "rms_norm", "rms_norm_forward", "rms_norm_backward", "NormForward", "NormGrads",
+           "FeatureEncoder", "EncoderForward", "EncoderGrads", "Block", "ResidualEncoder", "ResidualForward", "ResidualGrads"]
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # kge_type_t
 _U64 = (1 << 64) - 1
@@ -106,7 +110,8 @@ def _bytes(n: int, device):
 # ---- linear layers ---------------------------------------------------------------------------------
 @dataclass
 class LinearForward:
-    """A layer's output, and what its backward pass needs (x and weight have to stay as they are until then)."""
+    """A layer's output, and what its backward pass needs (x and weight have to stay as they are until then).  A layer on :class:`Rows8` does not need y: it may
+    be set to None."""
     y: torch.Tensor
     desc: bytes     # a kge_linear
     saved: torch.Tensor | None
@@ -160,11 +165,89 @@ def _act(act) -> int:
     return code
 
 
-def linear(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, drop=0.0, seed=0, step=0) -> torch.Tensor:
+def _describe8(x, weight, bias, act, drop, seed, step, residual, out_dtype, dtype):
+    x, weight8 = _rows8(x, "x"), None
+    if isinstance(weight, Rows8):
+        weight = weight8 = _rows8(weight, "weight")
+        if dtype is None:
+            dtype = bias.dtype if isinstance(bias, torch.Tensor) else (out_dtype if out_dtype in (torch.bfloat16, torch.float16) else torch.bfloat16)
+    else:
+        weight = _rows(weight, "weight")
+        if dtype not in (None, weight.dtype):
+            raise TypeError(f"dtype must be that of weight, {weight.dtype} (got {dtype})")
+        dtype = weight.dtype
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"layers on rows in 8 bits are bfloat16 or float16 (got {dtype})")
+    if weight.shape[1] != x.cols:
+        raise ValueError(f"weight must have as many columns as x (got {tuple(weight.shape)} for x {tuple(x.shape)})")
+    rows, out = x.shape[0], weight.shape[0]
+    if bias is not None:
+        bias = _rows(bias, "bias", dtype, ndim=1, shape=(out,))
+    if out_dtype is None:
+        out_dtype = dtype if residual is None else residual.dtype
+    if out_dtype not in (dtype, torch.float32):
+        raise TypeError(f"out_dtype must be {dtype} or float32 (got {out_dtype})")
+    if residual is not None:
+        residual = _rows(residual, "residual", out_dtype, shape=(rows, out))
+    seed, step, word = _random(seed, step)
+    desc = _lib.Linear(_TYPES[dtype], _TYPES[out_dtype], _act(act), 0, rows, x.cols, out, None, 0, None if weight8 else _p(weight),
+                       0 if weight8 else _row_stride(weight), _p(bias), _p(residual), _row_stride(residual) if residual is not None else 0,
+                       _probability(drop), seed, step, _p(word))
+    return desc, (x, weight, bias, residual, word), out_dtype, weight8
+
+
+def _linear8_call(desc, tensors, out_dtype, weight8, for_backward):
+    L, x = _lib.lib(), tensors[0]
+    if weight8 and for_backward:
+        raise TypeError("weight must be a tensor where there are gradients: a weight in 8 bits is for answering")
+    y = torch.empty((desc.rows, desc.out), dtype=out_dtype, device=x.q.device)
+    w8 = C.byref(_rows8_c(weight8)) if weight8 else None
+    saved_bytes = int(L.kge_linear8_saved_bytes(C.byref(desc))) if for_backward else 0
+    ws_bytes = int(L.kge_linear8_fwd_workspace(C.byref(desc), w8, int(for_backward)))
+    saved, ws = _bytes(saved_bytes, y.device), _bytes(ws_bytes, y.device)
+    _lib.check(L.kge_linear8_fwd(C.byref(desc), C.byref(_rows8_c(x)), w8, _p(y), max(desc.out, 1), int(for_backward), _p(saved), saved_bytes, _p(ws),
+                                 ws_bytes, _stream()), "kge_linear8_fwd")
+    return y, saved
+
+
+def _linear8_backward(fw, dy, need_x, need_weight, need_bias) -> LinearGrads:
+    x, weight, bias = fw.tensors[:3]
+    d = _lib.Linear.from_buffer_copy(fw.desc)
+    _tensor(x.q, "x of the forward call", 2)
+    dy = _rows(dy, "dy", torch.float32 if d.out_type == 0 else weight.dtype, shape=(d.rows, d.out))  # (fw.y may be gone)
+    dev = x.q.device
+    dx = torch.empty((d.rows, d.in_), dtype=weight.dtype, device=dev) if need_x else None
+    dw = torch.empty((d.out, d.in_), dtype=weight.dtype, device=dev) if need_weight else None
+    db = torch.empty(d.out, dtype=weight.dtype, device=dev) if need_bias and bias is not None else None
+    L = _lib.lib()
+    ws_bytes = int(L.kge_linear8_bwd_workspace(C.byref(d)))
+    ws = _bytes(ws_bytes, dev)
+    _lib.check(L.kge_linear8_bwd(C.byref(d), C.byref(_rows8_c(x)), _p(dy), _row_stride(dy), _p(fw.saved), fw.saved.numel() if fw.saved is not None else 0,
+                                 _p(dx), _p(dw), _p(db), _p(ws), ws_bytes, _stream()), "kge_linear8_bwd")
+    return LinearGrads(dx, dw, db)
+
+
+def _plain_dtype(x, weight, dtype):
+    """x's own type is the only one where x is a tensor."""
+    if isinstance(weight, Rows8):
+        raise TypeError("a weight in 8 bits goes with rows in 8 bits (pack8)")
+    if dtype is not None and isinstance(x, torch.Tensor) and dtype != x.dtype:
+        raise TypeError(f"dtype must be that of x, {x.dtype} (got {dtype})")
+
+
+def linear(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, drop=0.0, seed=0, step=0, dtype=None) -> torch.Tensor:
     """``drop(act(x weight^T + bias)) + residual``: x [rows, in], weight [out, in], bias [out], residual [rows, out].
 
     act: "none", "relu", "gelu" or "silu"; drop, seed, step as in :func:`dropout`.  The output has x's type, or float32 by out_dtype (or
-    because the residual is); 16-bit products are summed in fp32 and nothing is rounded before the end."""
+    because the residual is); 16-bit products are summed in fp32 and nothing is rounded before the end.
+
+    x may be :class:`Rows8`, with a weight in bfloat16 or float16, whose type the layer has, or in 8 bits too: then dtype is the layer's (that of the bias, or
+    bfloat16, unless said otherwise)."""
+    if isinstance(x, Rows8):
+        desc, tensors, out_dtype, weight8 = _describe8(x, weight, bias, act, drop, seed, step, residual, out_dtype, dtype)
+        return _linear8_call(desc, tensors, out_dtype, weight8, False)[0]
+    if dtype is not None or isinstance(weight, Rows8):
+        _plain_dtype(x, weight, dtype)
     y = _lib.host().linear(x, weight, bias, _act(act), residual, out_dtype, drop, seed, step, False)
     if y is not None:
         return y
@@ -172,7 +255,14 @@ def linear(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, d
 
 
 def linear_forward(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, drop=0.0, seed=0, step=0) -> LinearForward:
-    """:func:`linear`, with what :func:`linear_backward` needs."""
+    """:func:`linear`, with what :func:`linear_backward` needs.  Of a layer on :class:`Rows8` that is those rows and, in 8 bits too, the activation's
+    derivative (within 0.0025)."""
+    if isinstance(x, Rows8):
+        desc, tensors, out_dtype, weight8 = _describe8(x, weight, bias, act, drop, seed, step, residual, out_dtype, None)
+        y, saved = _linear8_call(desc, tensors, out_dtype, weight8, True)
+        return LinearForward(y, bytes(desc), saved, tensors)
+    if isinstance(weight, Rows8):
+        _plain_dtype(x, weight, None)
     got = _lib.host().linear(x, weight, bias, _act(act), residual, out_dtype, drop, seed, step, True)
     if got is not None:
         y, saved, desc = got
@@ -183,13 +273,15 @@ def linear_forward(x, weight, bias=None, *, act="none", residual=None, out_dtype
 
 
 def linear_backward(fw: LinearForward, dy, need_x: bool = True, need_weight: bool = True, need_bias: bool = True) -> LinearGrads:
-    """Gradients of x, weight and bias from the gradient of y (of y's type).
+    """Gradients of x, weight and bias from the gradient of y (of y's type).  That of x in 8 bits is the one at the values it stands for.
 
     What enters the two products is rounded to the layer's type.  In float16 that makes 0 of values below 3e-8 and infinity of those above 65504: scale
     the loss of a large batch up, and the gradients down again."""
     if not isinstance(fw, LinearForward):
         raise TypeError("fw must come from linear_forward()")
     x, _, bias = fw.tensors[:3]
+    if isinstance(x, Rows8):
+        return _linear8_backward(fw, dy, need_x, need_weight, need_bias)
     got = _lib.host().linear_backward(fw.desc, x, fw.saved, dy, need_x, need_weight, need_bias and bias is not None)
     if got is not None:
         return LinearGrads(*got)
@@ -466,3 +558,96 @@ class FeatureEncoder:
         d = drows if fw.drop is None else dropout_backward(drows, *fw.drop)
         last = linear_backward(fw.last, d)
         return EncoderGrads(linear_backward(fw.hidden, last.x, need_x=need_x), last, d)
+
+
+@dataclass
+class Block:
+    """A block's weights, or their gradients: norm [width], w1 [inner, width], b1 [inner], w2 [width, inner], b2 [width]."""
+    norm: torch.Tensor
+    w1: torch.Tensor | Rows8
+    b1: torch.Tensor
+    w2: torch.Tensor | Rows8
+    b2: torch.Tensor
+
+
+@dataclass
+class ResidualForward:
+    rows: torch.Tensor  # float32 [n, dim]
+    first: LinearForward
+    blocks: list        # (NormForward, LinearForward, LinearForward) of each
+    norm: NormForward
+    last: LinearForward
+
+
+@dataclass
+class ResidualGrads:
+    first: LinearGrads
+    blocks: list        # Block of each
+    norm: torch.Tensor
+    last: LinearGrads
+    base: torch.Tensor  # gradient of the free rows
+
+
+class ResidualEncoder:
+    """Entity rows from feature rows through a residual stream:  h = x W_in^T + b_in;  of each block
+    ``h += drop(act(norm(h) W1^T + b1)) W2^T + b2``;  rows = base + norm(h) W_out^T + b_out.
+
+    All weights are of one type (bfloat16 or float16), the stream too; the rows are float32.  What goes into a layer (the norms' outputs, the hidden rows) is made in 8 bits and
+    kept like that; x may be rows of the weights' type or :class:`Rows8`."""
+
+    def __init__(self, w_in, b_in, blocks, norm, w_out, b_out, act: str = "gelu", drop: float = 0.0, seed: int = 0, eps: float = 1e-6):
+        width = w_in.shape[0]
+        for i, b in enumerate(blocks):
+            if b.w1.shape[1] != width or b.w2.shape[0] != width or b.w2.shape[1] != b.w1.shape[0]:
+                raise ValueError(f"block {i} must take and give rows of {width} (got {tuple(b.w1.shape)} and {tuple(b.w2.shape)})")
+        if w_out.shape[1] != width:
+            raise ValueError(f"w_out must have {width} columns (got {tuple(w_out.shape)})")
+        self.w_in, self.b_in, self.blocks, self.norm, self.w_out, self.b_out = w_in, b_in, list(blocks), norm, w_out, b_out
+        self.act, self.drop, self.seed, self.eps = act, _probability(drop), int(seed), float(eps)
+
+    def packed(self) -> "ResidualEncoder":
+        """The same encoder for answering, its weights in 8 bits (those of w_in stay: they multiply rows that nobody has packed)."""
+        blocks = [Block(b.norm, pack8(b.w1), b.b1, pack8(b.w2), b.b2) for b in self.blocks]
+        return ResidualEncoder(self.w_in, self.b_in, blocks, self.norm, pack8(self.w_out), self.b_out, self.act, self.drop, self.seed, self.eps)
+
+    def encode(self, x, base=None) -> torch.Tensor:
+        """Rows for answering with: nothing is dropped, nothing is kept."""
+        h, more, dt = linear(x, self.w_in, self.b_in), None, self.b_in.dtype
+
+        def norm(weight):
+            nonlocal h
+            y = rms_norm(h if more is None else more, weight, None if more is None else h, eps=self.eps, out_dtype=E4M3)
+            if more is not None:
+                y, h = y
+            return y
+        for b in self.blocks:
+            more = linear(pack8(linear(norm(b.norm), b.w1, b.b1, act=self.act, dtype=dt)), b.w2, b.b2, dtype=dt)
+        return linear(norm(self.norm), self.w_out, self.b_out, residual=base, out_dtype=torch.float32, dtype=dt)
+
+    def forward(self, x, base=None, step=0) -> ResidualForward:
+        """Rows for a training step; step (an integer, or one int64 on the GPU) draws the masks."""
+        first = linear_forward(x, self.w_in, self.b_in)
+        h, more, kept = first.y, None, []
+        for i, b in enumerate(self.blocks):
+            n = rms_norm_forward(h if more is None else more, b.norm, None if more is None else h, eps=self.eps, out_dtype=E4M3)
+            hidden = linear_forward(n.y, b.w1, b.b1, act=self.act, drop=self.drop, seed=self.seed + i, step=step)
+            out = linear_forward(pack8(hidden.y), b.w2, b.b2)
+            kept.append((n, hidden, out))
+            h, more = n.h, out.y
+            hidden.y = out.y = None  # (the one is kept in 8 bits, the other is part of the stream)
+        n = rms_norm_forward(h if more is None else more, self.norm, None if more is None else h, eps=self.eps, out_dtype=E4M3)
+        last = linear_forward(n.y, self.w_out, self.b_out, residual=base, out_dtype=torch.float32)
+        return ResidualForward(last.y, first, kept, n, last)
+
+    def backward(self, fw: ResidualForward, drows, need_x: bool = False) -> ResidualGrads:
+        """Gradients from those of the rows."""
+        last = linear_backward(fw.last, drows)
+        g = rms_norm_backward(fw.norm, last.x)
+        norm, d, blocks = g.weight, g.x, []
+        for n, hidden, out in reversed(fw.blocks):  # d: the gradient of the stream behind the block, and of what the block adds to it
+            go = linear_backward(out, d)
+            gh = linear_backward(hidden, go.x)
+            g = rms_norm_backward(n, gh.x, d)
+            blocks.append(Block(g.weight, gh.weight, gh.bias, go.weight, go.bias))
+            d = g.x
+        return ResidualGrads(linear_backward(fw.first, d, need_x=need_x), blocks[::-1], norm, last, drows)

@@ -701,6 +701,22 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
                      int64_t dy_stride, const void *dh, int64_t dh_stride, void *dx, int64_t dx_stride, void *dweight, void *workspace,
                      size_t workspace_bytes, void *stream);
 
+/*
+ * Linear layers (kge_linear, whose x and x_stride are not looked at) on rows in 8 bits, x8 [rows, in]:  y = drop(act(x8 weight^T + bias)) + residual.
+ * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients; a value of x8 that KGE_F16 cannot hold is infinite.  Products are
+ * exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for answering:
+ * for_backward is 0 then (KGE_EINVAL).
+ * The backward pass reads x8 where the forward pass did, so that it is all that is kept of the layer's input; act'(z) is kept in 8 bits too (steps of 1/200
+ * from -0.135 up: within 0.0025).  dx is the gradient at the values that x8 stands for.  Otherwise as kge_linear_fwd and kge_linear_bwd.
+ */
+size_t kge_linear8_saved_bytes(const kge_linear *lin);
+size_t kge_linear8_fwd_workspace(const kge_linear *lin, const kge_rows8 *weight8, int for_backward);
+int kge_linear8_fwd(const kge_linear *lin, const kge_rows8 *x8, const kge_rows8 *weight8, void *y, int64_t y_stride, int for_backward, void *saved,
+                    size_t saved_bytes, void *workspace, size_t workspace_bytes, void *stream);
+size_t kge_linear8_bwd_workspace(const kge_linear *lin);
+int kge_linear8_bwd(const kge_linear *lin, const kge_rows8 *x8, const void *dy, int64_t dy_stride, const void *saved, size_t saved_bytes, void *dx,
+                    void *dweight, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Sets flag[0] (int32, caller-zeroed) to 1 if any idx[i] is outside [0, n_rows). */
 int kge_check_indices(const int64_t *idx, int64_t n, int64_t n_rows, int32_t *flag, void *stream);
 
