@@ -839,6 +839,229 @@ PyObject *py_preference_loss(PyObject *, PyObject *const *args, Py_ssize_t)
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rows in 8 bits, the norm, layers on such rows -------------------------------------------------
+int64_t q_width(int64_t cols) { return (cols + 31) / 32 * 32; }
+int64_t scale_width(int64_t cols) { return (cols + 127) / 128 * 4; }
+
+// arrays of rows in 8 bits this module can hand on
+bool rows8_of(PyObject *q, PyObject *scale, PyObject *columns, int dev, kge_rows8 *r, int64_t *rows, int64_t *cols)
+{
+    const at::Tensor *a = tensor(q), *b = tensor(scale);
+    if (!a || !b || !a->is_cuda() || !b->is_cuda() || a->device().index() != dev || b->device().index() != dev) return false;
+    if (a->scalar_type() != at::kFloat8_e4m3fn || b->scalar_type() != at::kFloat8_e8m0fnu || !PyLong_Check(columns)) return false;
+    *cols = PyLong_AsLongLong(columns);
+    if (a->dim() != 2 || b->dim() != 2 || *cols < 1) return false;
+    *rows = a->size(0);
+    if (b->size(0) != *rows || a->size(1) != q_width(*cols) || b->size(1) != scale_width(*cols) || a->stride(1) != 1 || b->stride(1) != 1) return false;
+    r->q = a->data_ptr(), r->q_stride = *rows > 1 ? a->stride(0) : a->size(1);
+    r->scale = b->data_ptr(), r->scale_stride = *rows > 1 ? b->stride(0) : b->size(1);
+    return r->q_stride >= a->size(1) && r->scale_stride >= b->size(1) && r->q_stride % 16 == 0 && r->scale_stride % 4 == 0 &&
+           reinterpret_cast<uintptr_t>(r->q) % 16 == 0 && reinterpret_cast<uintptr_t>(r->scale) % 4 == 0;
+}
+
+kge_rows8 new_rows8(int64_t rows, int64_t cols, const at::TensorOptions &opt, at::Tensor *q, at::Tensor *scale)
+{
+    *q = at::empty({rows, q_width(cols)}, opt.dtype(at::kFloat8_e4m3fn)), *scale = at::empty({rows, scale_width(cols)}, opt.dtype(at::kFloat8_e8m0fnu));
+    return kge_rows8{q->data_ptr(), q_width(cols), scale->data_ptr(), scale_width(cols)};
+}
+
+at::ScalarType scalar_of(int type) { return type == KGE_F32 ? at::kFloat : (type == KGE_BF16 ? at::kBFloat16 : at::kHalf); }
+// kge_type_t, or KGE_E4M3, of a torch type; -1: another one
+int type_of_dtype(PyObject *o)
+{
+    if (!THPDtype_Check(o)) return -1;
+    switch (reinterpret_cast<THPDtype *>(o)->scalar_type) {
+        case at::kFloat: return KGE_F32;
+        case at::kBFloat16: return KGE_BF16;
+        case at::kHalf: return KGE_F16;
+        case at::kFloat8_e4m3fn: return KGE_E4M3;
+        default: return -1;
+    }
+}
+
+// pack8(x) -> (q, scale), or None
+PyObject *py_pack8(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = tensor(args[0]);
+    if (!x || !x->is_cuda()) NOT_HERE;
+    const int dev = c10::hip::current_device(), type = type_of(x, dev);
+    int64_t stride;
+    if (type < 0 || x->dim() != 2 || !rows_of(x, type, x->size(0), x->size(1), dev, &stride)) NOT_HERE;
+    at::Tensor q, scale;
+    const kge_rows8 r = new_rows8(x->size(0), x->size(1), x->options().requires_grad(false), &q, &scale);
+    const void *from = x->data_ptr();
+    void *st = stream();
+    const int rc = nogil([&] { return kge_pack8(type, from, stride, x->size(0), x->size(1), &r, st); });
+    if (rc) return fail(rc, "kge_pack8"), nullptr;
+    return Py_BuildValue("(NN)", wrap(q), wrap(scale));
+    END_HANDLE_TH_ERRORS
+}
+
+// unpack8(q, scale, cols, dtype) -> y, or None
+PyObject *py_unpack8(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *q = tensor(args[0]);
+    if (!q || !q->is_cuda()) NOT_HERE;
+    const int dev = c10::hip::current_device(), type = type_of_dtype(args[3]);
+    kge_rows8 r;
+    int64_t rows, cols;
+    if (type < 0 || type == KGE_E4M3 || !rows8_of(args[0], args[1], args[2], dev, &r, &rows, &cols)) NOT_HERE;
+    at::Tensor y = at::empty({rows, cols}, q->options().requires_grad(false).dtype(scalar_of(type)));
+    void *to = y.data_ptr(), *st = stream();
+    const int rc = nogil([&] { return kge_unpack8(&r, rows, cols, type, to, cols, st); });
+    if (rc) return fail(rc, "kge_unpack8"), nullptr;
+    return wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm(x, weight, residual, eps, out_dtype or None, keep) -> (y, or q and None beside it; scale; h; rstd), or None
+PyObject *py_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = tensor(args[0]), *w = tensor(args[1]), *res = tensor(args[2]);
+    if (!x || !x->is_cuda()) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    kge_rms_norm n{};
+    n.type = type_of(x, dev);
+    if (n.type < 0 || x->dim() != 2) NOT_HERE;
+    n.rows = x->size(0), n.cols = x->size(1);
+    if (!rows_of(x, n.type, n.rows, n.cols, dev, &n.x_stride)) NOT_HERE;
+    if (args[1] != Py_None && !vector_of(w, n.type, n.cols, dev)) NOT_HERE;
+    if (args[2] != Py_None && !rows_of(res, n.type, n.rows, n.cols, dev, &n.residual_stride)) NOT_HERE;
+    if (!number(args[3], &n.eps) || !(n.eps >= 0.0 && n.eps < 1e300)) NOT_HERE;
+    n.out_type = args[4] == Py_None ? n.type : type_of_dtype(args[4]);
+    if (n.out_type < 0) NOT_HERE;
+    const bool keep = PyObject_IsTrue(args[5]), eight = n.out_type == KGE_E4M3;
+    n.x = x->data_ptr(), n.weight = args[1] != Py_None ? w->data_ptr() : nullptr, n.residual = args[2] != Py_None ? res->data_ptr() : nullptr;
+    const auto opt = x->options().requires_grad(false);
+    at::Tensor y, scale, h, rstd;
+    kge_rows8 y8{};
+    if (eight) y8 = new_rows8(n.rows, n.cols, opt, &y, &scale);
+    else y = at::empty({n.rows, n.cols}, opt.dtype(scalar_of(n.out_type)));
+    if (n.residual) h = at::empty({n.rows, n.cols}, opt);
+    if (keep) rstd = at::empty({n.rows}, opt.dtype(at::kFloat));
+    void *st = stream(), *to = eight ? nullptr : y.data_ptr(), *ph = h.defined() ? h.data_ptr() : nullptr;
+    float *pr = keep ? rstd.data_ptr<float>() : nullptr;
+    const int rc = nogil([&] { return kge_rms_norm_fwd(&n, to, n.cols, eight ? &y8 : nullptr, ph, n.cols, pr, st); });
+    if (rc) return fail(rc, "kge_rms_norm_fwd"), nullptr;
+    return Py_BuildValue("(NNNN)", wrap(y), wrap(scale), wrap(h), wrap(rstd));
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_backward(h, rstd, weight, dy, dh, need x, need weight) -> (dx, dweight), or None.  h, rstd and weight are those of the forward call.
+PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *h = tensor(args[0]), *rstd = tensor(args[1]), *w = tensor(args[2]), *dy = tensor(args[3]), *dh = tensor(args[4]);
+    if (!h || !h->is_cuda() || !rstd || !dy) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    kge_rms_norm n{};
+    n.type = n.out_type = type_of(h, dev);
+    if (n.type < 0 || h->dim() != 2) NOT_HERE;
+    n.rows = h->size(0), n.cols = h->size(1);
+    int64_t h_stride, dy_stride, dh_stride = 0;
+    const int dy_type = type_of(dy, dev);
+    if (!rows_of(h, n.type, n.rows, n.cols, dev, &h_stride) || dy_type < 0 || !rows_of(dy, dy_type, n.rows, n.cols, dev, &dy_stride)) NOT_HERE;
+    if (!vector_of(rstd, KGE_F32, n.rows, dev) || (args[2] != Py_None && !vector_of(w, n.type, n.cols, dev))) NOT_HERE;
+    if (args[4] != Py_None && !rows_of(dh, n.type, n.rows, n.cols, dev, &dh_stride)) NOT_HERE;
+    n.weight = args[2] != Py_None ? w->data_ptr() : nullptr;
+    const auto opt = h->options().requires_grad(false);
+    at::Tensor dx, dw;
+    if (PyObject_IsTrue(args[5])) dx = at::empty({n.rows, n.cols}, opt);
+    if (PyObject_IsTrue(args[6]) && n.weight) dw = at::empty({n.cols}, opt);
+    const size_t ws_bytes = dw.defined() ? kge_rms_norm_bwd_workspace(&n) : 0;
+    c10::DataPtr ws;
+    if (ws_bytes) ws = scratch(ws_bytes);
+    const void *from = h->data_ptr(), *pdy = dy->data_ptr(), *pdh = args[4] != Py_None ? dh->data_ptr() : nullptr;
+    const float *pr = rstd->data_ptr<float>();
+    void *px = dx.defined() ? dx.data_ptr() : nullptr, *pw = dw.defined() ? dw.data_ptr() : nullptr, *st = stream();
+    const int rc = nogil([&] { return kge_rms_norm_bwd(&n, from, h_stride, pr, dy_type, pdy, dy_stride, pdh, dh_stride, px, n.cols, pw, ws.get(), ws_bytes, st); });
+    if (rc) return fail(rc, "kge_rms_norm_bwd"), nullptr;
+    return Py_BuildValue("(NN)", wrap(dx), wrap(dw));
+    END_HANDLE_TH_ERRORS
+}
+
+// linear8(q, scale, cols, weight (or its q), its scale or None, bias, act, residual, out_dtype, dtype, drop, seed, step, for_backward) -> y, or (y, saved,
+// kge_linear as bytes), or None
+PyObject *py_linear8(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    const at::Tensor *q = tensor(args[0]), *w = tensor(args[3]), *b = tensor(args[5]), *res = tensor(args[7]);
+    if (!q || !q->is_cuda() || !w) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    kge_linear l{};
+    kge_rows8 x8, w8;
+    if (!rows8_of(args[0], args[1], args[2], dev, &x8, &l.rows, &l.in)) NOT_HERE;
+    const bool eight = args[4] != Py_None, keep = PyObject_IsTrue(args[13]);
+    if (eight) {
+        int64_t cols;
+        if (keep || !rows8_of(args[3], args[4], args[2], dev, &w8, &l.out, &cols)) NOT_HERE;
+        l.type = args[9] != Py_None ? type_of_dtype(args[9]) : (args[5] != Py_None ? type_of(b, dev) : KGE_BF16);
+        if (args[9] == Py_None && args[5] == Py_None && args[8] != Py_None && type_of_dtype(args[8]) == KGE_F16) l.type = KGE_F16;
+    } else {
+        l.type = type_of(w, dev);
+        if (l.type < 0 || w->dim() != 2 || !rows_of(w, l.type, w->size(0), l.in, dev, &l.weight_stride)) NOT_HERE;
+        if (args[9] != Py_None && type_of_dtype(args[9]) != l.type) NOT_HERE;
+        l.out = w->size(0), l.weight = w->data_ptr();
+    }
+    if (l.type != KGE_BF16 && l.type != KGE_F16) NOT_HERE;
+    if (args[5] != Py_None && !vector_of(b, l.type, l.out, dev)) NOT_HERE;
+    if (!PyLong_Check(args[6])) NOT_HERE;
+    l.act = (int32_t)PyLong_AsLong(args[6]);
+    l.out_type = args[8] != Py_None ? type_of_dtype(args[8]) : (args[7] != Py_None ? type_of(res, dev) : l.type);
+    if (l.out_type != l.type && l.out_type != KGE_F32) NOT_HERE;
+    if (args[7] != Py_None && !rows_of(res, l.out_type, l.rows, l.out, dev, &l.residual_stride)) NOT_HERE;
+    if (!number(args[10], &l.p) || !word(args[11], &l.seed) || !word(args[12], &l.step) || !(l.p >= 0.0 && l.p <= 1.0)) NOT_HERE;
+    l.bias = args[5] != Py_None ? b->data_ptr() : nullptr, l.residual = args[7] != Py_None ? res->data_ptr() : nullptr;
+    const auto opt = q->options().requires_grad(false);
+    at::Tensor y = at::empty({l.rows, l.out}, opt.dtype(scalar_of(l.out_type))), saved;
+    const kge_rows8 *weight8 = eight ? &w8 : nullptr;
+    const size_t saved_bytes = keep ? kge_linear8_saved_bytes(&l) : 0, ws_bytes = kge_linear8_fwd_workspace(&l, weight8, keep);
+    if (saved_bytes) saved = at::empty({(int64_t)saved_bytes}, opt.dtype(at::kByte));
+    c10::DataPtr ws;
+    if (ws_bytes) ws = scratch(ws_bytes);
+    void *st = stream(), *to = y.data_ptr(), *kept = saved_bytes ? saved.data_ptr() : nullptr;
+    const int rc = nogil([&] { return kge_linear8_fwd(&l, &x8, weight8, to, std::max<int64_t>(l.out, 1), keep, kept, saved_bytes, ws.get(), ws_bytes, st); });
+    if (rc) return fail(rc, "kge_linear8_fwd"), nullptr;
+    if (!keep) return wrap(y);
+    return Py_BuildValue("(NNy#)", wrap(y), wrap(saved), reinterpret_cast<const char *>(&l), (Py_ssize_t)sizeof(l));
+    END_HANDLE_TH_ERRORS
+}
+
+// linear8_backward(kge_linear as bytes, q, scale, cols, weight, saved, dy, need x, need weight, need bias) -> (dx, dweight, dbias), or None.  All but dy are those
+// of the forward call.
+PyObject *py_linear8_backward(PyObject *, PyObject *const *args, Py_ssize_t)
+{
+    HANDLE_TH_ERRORS
+    kge_linear l;
+    if (!PyBytes_Check(args[0]) || PyBytes_GET_SIZE(args[0]) != (Py_ssize_t)sizeof(l)) NOT_HERE;
+    std::memcpy(&l, PyBytes_AS_STRING(args[0]), sizeof(l));
+    const at::Tensor *q = tensor(args[1]), *w = tensor(args[4]), *saved = tensor(args[5]), *dy = tensor(args[6]);
+    if (!q || !q->is_cuda() || !w || !dy) NOT_HERE;
+    const int dev = c10::hip::current_device();
+    kge_rows8 x8;
+    int64_t dy_stride, rows, cols;
+    if (!rows8_of(args[1], args[2], args[3], dev, &x8, &rows, &cols) || rows != l.rows || cols != l.in) NOT_HERE;
+    if (type_of(w, dev) != l.type || !rows_of(dy, l.out_type, l.rows, l.out, dev, &dy_stride)) NOT_HERE;
+    const auto opt = w->options().requires_grad(false);
+    at::Tensor dx, dw, db;
+    if (PyObject_IsTrue(args[7])) dx = at::empty({l.rows, l.in}, opt);
+    if (PyObject_IsTrue(args[8])) dw = at::empty({l.out, l.in}, opt);
+    if (PyObject_IsTrue(args[9])) db = at::empty({l.out}, opt);
+    const size_t ws_bytes = kge_linear8_bwd_workspace(&l);
+    const c10::DataPtr ws = scratch(ws_bytes);
+    auto at = [](const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; };
+    void *st = stream(), *px = at(dx), *pw = at(dw), *pb = at(db);
+    const void *kept = saved ? saved->data_ptr() : nullptr, *from = dy->data_ptr();
+    const size_t kept_bytes = saved ? saved->numel() : 0;
+    const int rc = nogil([&] { return kge_linear8_bwd(&l, &x8, from, dy_stride, kept, kept_bytes, px, pw, pb, ws.get(), ws_bytes, st); });
+    if (rc) return fail(rc, "kge_linear8_bwd"), nullptr;
+    return Py_BuildValue("(NNN)", wrap(dx), wrap(dw), wrap(db));
+    END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"set_error", py_set_error, METH_O, nullptr},
                          FAST(inspect),
@@ -853,6 +1076,12 @@ PyMethodDef methods[] = {{"set_error", py_set_error, METH_O, nullptr},
                          FAST(linear_backward),
                          FAST(dropout),
                          FAST(preference_loss),
+                         FAST(pack8),
+                         FAST(unpack8),
+                         FAST(rms_norm),
+                         FAST(rms_norm_backward),
+                         FAST(linear8),
+                         FAST(linear8_backward),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

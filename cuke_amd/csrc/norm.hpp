@@ -1,0 +1,67 @@
+// What the two passes of the root-mean-square norm share: how lanes hold a row, sums over them.
+#pragma once
+
+#include "rows8.hpp"
+
+namespace kge {
+
+// sum over `lanes` neighbouring lanes (a power of two, 64 at most), the same in each of them
+template <class V>
+__device__ __forceinline__ V lanes_sum(V v, int lanes)
+{
+    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+// sum over 128 or 256 neighbouring threads of a workgroup of 256, the same in each of them; `part` may be written again behind the next barrier
+template <class V>
+__device__ __forceinline__ V waves_sum(V v, int lanes, V *part)
+{
+    v = lanes_sum(v, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    const int pair = threadIdx.x >> 7 << 1;
+    return lanes == 128 ? part[pair] + part[pair + 1] : (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+// How a row is held in registers: `pieces` of eight columns a lane (1, 2 or 4; 0: it is too long for that), by `lanes` lanes: a power of two from 4 to 64, or
+// 128 or 256, which are several waves.  Two pieces where that still makes `enough` waves, so that they share what a row costs besides; one where it does not; four
+// only where rows are too long for fewer.  Forward passes with one, two and four pieces (us): 65536 x 2048 bf16 188, 186, 204, to 8 bits 184, 192, 253;
+// 30000 x 300 to 8 bits 32, 25, 25; 65536 x 128 13.0, 11.4, 11.7; 4096 x 1024 to 8 bits 10.0, 11, 14.1.
+struct Hold {
+    int pieces, lanes;
+};
+inline Hold hold_of(int64_t rows, int64_t cols, int64_t enough)
+{
+    const int64_t need = ceil_div(cols, 8);
+    if (need > 256 * 4) return Hold{0, 256};
+    int pieces = need > 4 && rows * need / 128 >= enough ? 2 : 1, lanes = 4;
+    while ((int64_t)lanes * pieces < need && lanes < 256) lanes *= 2;
+    while ((int64_t)lanes * pieces < need) pieces *= 2;
+    return Hold{pieces, lanes};
+}
+
+// calls f with (pieces, whether several waves hold a row) as compile-time values; not for pieces == 0
+template <class F>
+inline void with_hold(const Hold &h, F &&f)
+{
+    using std::integral_constant;
+    auto waves = [&](auto pieces) {
+        if (h.lanes > 64) f(pieces, std::true_type{});
+        else f(pieces, std::false_type{});
+    };
+    if (h.pieces == 1) waves(integral_constant<int, 1>{});
+    else if (h.pieces == 2) waves(integral_constant<int, 2>{});
+    else waves(integral_constant<int, 4>{});
+}
+
+inline int check_norm(const kge_rms_norm *n)
+{
+    if (!n) return KGE_EINVAL;
+    if (!known_type(n->type) || !(known_type(n->out_type) || n->out_type == KGE_E4M3) || !(n->eps >= 0.0) || n->eps > 1.7976931348623157e308) return KGE_EINVAL;
+    const int64_t most = (int64_t)1 << 31;
+    if (n->rows < 0 || n->cols < 0 || n->rows >= most || n->cols >= most) return KGE_ESHAPE;
+    return KGE_OK;
+}
+
+}  // namespace kge

@@ -1,0 +1,309 @@
+// Gradients of the root-mean-square norm (kge_rms_norm_bwd).  With n = h r and g = dy weight:
+//   dx = r (g - n mean(g n)) + dh,   dweight = sum over rows of dy n
+#include <type_traits>
+
+#include "linear_tile.hpp"
+#include "norm.hpp"
+
+namespace kge {
+
+struct NormGradArgs {
+    const void *h, *dy, *dh, *weight;
+    int64_t h_stride, dy_stride, dh_stride;
+    const float *rstd;
+    int64_t rows, cols, quads, rows_each;
+    void *dx;     // or NULL
+    int64_t dx_stride;
+    float *sums;  // [ranges][4 quads]: dweight's over a range of rows, or NULL
+    int lanes;
+};
+
+// Eight elements as they lie in memory, requested ahead of their use.  A row's last piece is moved back to end with the row (rows of at least eight columns), so that
+// no load needs a branch; the first `skip` elements belong to the piece before it too.
+template <class E>
+struct Held {
+    typename Pack<E, 8>::type v;
+    __device__ __forceinline__ void fetch(const void *row, int at) { v = Pack<E, 8>::load(static_cast<const E *>(row) + at).v; }
+    __device__ __forceinline__ void values(float (&f)[8]) const
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)v[e];
+    }
+};
+
+// A workgroup takes a range of rows, each held by `lanes` lanes (WAVES: by two or four waves); what the next row needs is requested while the present one is worked on.  A lane's
+// columns are the same in all rows, so dweight's sums wait in registers until the range's end.
+// Bound by memory: 65536 x 2048 bf16 with dh (1.07 GB) GRAD_US.
+template <class T, class D, int C, bool WAVES, bool DH>
+__global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
+{
+    __shared__ float part[4];
+    __shared__ float s_sum[256][8];
+    const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
+    const int64_t first = (int64_t)blockIdx.x * a.rows_each, last = first + a.rows_each < a.rows ? first + a.rows_each : a.rows;
+    const float share = 1.0f / (float)a.cols;
+    const int cols = (int)a.cols;
+    int at[C], skip[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int col = 8 * (c * lanes + lane);
+        at[c] = col < cols - 8 ? col : cols - 8, skip[c] = col - at[c];
+    }
+    float sum[C][8] = {};
+    Held<T> h[C], dh[DH ? C : 1], w[C];
+    Held<D> dy[C];
+    float r;
+    if (a.weight) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) w[c].fetch(a.weight, at[c]);
+    }
+    auto fetch = [&](int64_t row) {
+        row = row < last ? row : last - 1;
+        r = a.rstd[row];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            h[c].fetch(static_cast<const T *>(a.h) + row * a.h_stride, at[c]);
+            dy[c].fetch(static_cast<const D *>(a.dy) + row * a.dy_stride, at[c]);
+            if constexpr (DH) dh[c].fetch(static_cast<const T *>(a.dh) + row * a.dh_stride, at[c]);
+        }
+    };
+    fetch(first + group);
+    for (int64_t row0 = first; row0 < last; row0 += groups) {
+        const int64_t row = row0 + group;
+        const bool there = row < last;
+        float n[C][8], g[C][8], dot = 0.0f;
+        const float rr = r;
+        Held<T> more[DH ? C : 1];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            h[c].values(n[c]), dy[c].values(g[c]);
+            if constexpr (DH) more[c] = dh[c];
+            if (skip[c] > 0) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < skip[c]) g[c][e] = 0.0f;  // (counted by the piece before)
+            }
+        }
+        fetch(row + groups);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                n[c][e] *= rr;
+                if (there) sum[c][e] = fmaf(g[c][e], n[c][e], sum[c][e]);
+            }
+            if (a.weight) {
+                float v[8];
+                w[c].values(v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) g[c][e] *= v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot = fmaf(g[c][e], n[c][e], dot);
+        }
+        if (!a.dx) continue;
+        const float mean = (WAVES ? waves_sum(dot, lanes, part) : lanes_sum(dot, lanes)) * share;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float d[8] = {};
+            if constexpr (DH) more[c].values(d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmaf(rr, g[c][e] - n[c][e] * mean, d[e]);
+            if (!there || skip[c] >= 8) continue;
+            T *to = static_cast<T *>(a.dx) + row * a.dx_stride + at[c];
+            if (skip[c] == 0) {
+                store8(to, d, 8);
+            } else {
+#pragma unroll
+                for (int e = 1; e < 8; ++e)
+                    if (e >= skip[c]) to[e] = (T)d[e];
+            }
+        }
+    }
+    if (!a.sums) return;
+    float *to = a.sums + (int64_t)blockIdx.x * a.quads * 4;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        if (groups > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s_sum[threadIdx.x][e] = sum[c][e];
+            __syncthreads();
+            if (group) continue;
+            for (int k = 1; k < groups; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[c][e] += s_sum[k * lanes + lane][e];
+        }
+        if (skip[c] == 0) {
+            Pack<float, 4> lo, hi;
+            lo.v[0] = sum[c][0], lo.v[1] = sum[c][1], lo.v[2] = sum[c][2], lo.v[3] = sum[c][3];
+            hi.v[0] = sum[c][4], hi.v[1] = sum[c][5], hi.v[2] = sum[c][6], hi.v[3] = sum[c][7];
+            lo.store(to + at[c]), hi.store(to + at[c] + 4);
+        } else {
+#pragma unroll
+            for (int e = 1; e < 8; ++e)
+                if (e >= skip[c]) to[at[c] + e] = sum[c][e];
+        }
+    }
+}
+
+// Rows that registers do not hold, and those of fewer than eight columns: dx by a workgroup that goes over a row twice.
+template <class T, class D>
+__global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
+{
+    __shared__ float part[4];
+    auto load = [&](int64_t row, int64_t col, float r, float(&n)[8], float(&g)[8]) {
+        const int64_t left = a.cols - col;
+        const int valid = (int)(left < 8 ? left : 8);
+        load8(static_cast<const T *>(a.h) + row * a.h_stride + col, valid, n);
+        load8(static_cast<const D *>(a.dy) + row * a.dy_stride + col, valid, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n[e] *= r;
+        if (!a.weight) return valid;
+        float w[8];
+        load8(static_cast<const T *>(a.weight) + col, valid, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] *= w[e];
+        return valid;
+    };
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float r = a.rstd[row];
+        float dot = 0.0f;
+        for (int64_t col = 8 * threadIdx.x; col < a.cols; col += 8 * 256) {
+            float n[8], g[8];
+            load(row, col, r, n, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dot = fmaf(g[e], n[e], dot);
+        }
+        const float mean = waves_sum(dot, 256, part) * (1.0f / (float)a.cols);
+        for (int64_t col = 8 * threadIdx.x; col < a.cols; col += 8 * 256) {
+            float n[8], g[8], d[8] = {};
+            const int valid = load(row, col, r, n, g);
+            if (a.dh) load8(static_cast<const T *>(a.dh) + row * a.dh_stride + col, valid, d);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmaf(r, g[e] - n[e] * mean, d[e]);
+            store8(static_cast<T *>(a.dx) + row * a.dx_stride + col, d, valid);
+        }
+    }
+}
+// dweight's sums over ranges of rows, of such rows: eight columns a thread
+template <class T, class D>
+__global__ __launch_bounds__(256) void rms_norm_long_sums_kernel(NormGradArgs a)
+{
+    const int64_t first = (int64_t)blockIdx.y * a.rows_each, last = first + a.rows_each < a.rows ? first + a.rows_each : a.rows;
+    const int64_t col = 8 * ((int64_t)blockIdx.x * 256 + threadIdx.x), left = a.cols - col;
+    if (left <= 0) return;
+    const int valid = (int)(left < 8 ? left : 8);
+    float sum[8] = {};
+    for (int64_t row = first; row < last; ++row) {
+        const float r = a.rstd[row];
+        float n[8], g[8];
+        load8(static_cast<const T *>(a.h) + row * a.h_stride + col, valid, n);
+        load8(static_cast<const D *>(a.dy) + row * a.dy_stride + col, valid, g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum[e] = fmaf(g[e], n[e] * r, sum[e]);
+    }
+    float *to = a.sums + (int64_t)blockIdx.y * a.quads * 4 + col;
+    *reinterpret_cast<float4 *>(to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    if (valid > 4) *reinterpret_cast<float4 *>(to + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void norm_join_kernel(SumArgs j)
+{
+    __shared__ float4 lds[256];
+    join_sums<T, 256>(j, blockIdx.x, lds);
+}
+
+// ---- launches --------------------------------------------------------------------------------------
+static Hold grad_hold(int64_t rows, int64_t cols)
+{
+    return cols < 8 ? Hold{0, 256} : hold_of(rows, cols, 4096);
+}
+
+// Ranges of rows, one a workgroup, that dweight is summed over: 512 of them (us with 512, 1024 and 2048: 65536 x 2048 bf16 211, 219, 221; 4096 x 1024 12.7, 15.2, 15.0;
+// 30000 x 300 20.6, 22.2, 24.6).
+struct Ranges {
+    int64_t rows_each;
+    int count;
+};
+static Ranges ranges_of(int64_t rows, int64_t cols)
+{
+    const Hold hold = grad_hold(rows, cols);
+    const int64_t turn = hold.pieces ? 256 / hold.lanes : 8, turns = ceil_div(rows, turn);
+    const int64_t across = hold.pieces ? 1 : ceil_div(cols, 2048), most = 512, want = across < most ? most / across : 1;
+    const int64_t each = turn * ceil_div(turns, want);
+    return Ranges{each > 0 ? each : 1, (int)ceil_div(rows, each > 0 ? each : 1)};
+}
+
+template <class T, class D>
+static void launch_grads(const NormGradArgs &args, const Ranges &ranges, void *dweight, hipStream_t st)
+{
+    NormGradArgs a = args;
+    const Hold hold = grad_hold(a.rows, a.cols);
+    a.lanes = hold.lanes;
+    const dim3 grid((unsigned)ranges.count), block(256);
+    if (hold.pieces == 0) {
+        // (the sums first: dx may take the place of dy)
+        if (a.sums) hipLaunchKernelGGL((rms_norm_long_sums_kernel<T, D>), dim3((unsigned)ceil_div(a.cols, 2048), (unsigned)ranges.count), block, 0, st, a);
+        if (a.dx) hipLaunchKernelGGL((rms_norm_grad_long_kernel<T, D>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), block, 0, st, a);
+    } else {
+        with_hold(hold, [&](auto pieces, auto waves) {
+            if (a.dh) hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, decltype(pieces)::value, decltype(waves)::value, true>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, decltype(pieces)::value, decltype(waves)::value, false>), grid, block, 0, st, a);
+        });
+    }
+    if (a.sums) hipLaunchKernelGGL(norm_join_kernel<T>, dim3((unsigned)ceil_div(a.quads, 4)), block, 0, st, SumArgs{a.sums, ranges.count, a.cols, a.quads, dweight});
+}
+template <class T>
+static void launch_grads(const NormGradArgs &a, const Ranges &ranges, int dy_type, void *dweight, hipStream_t st)
+{
+    if (dy_type == KGE_F32) launch_grads<T, float>(a, ranges, dweight, st);
+    else if (dy_type == KGE_BF16) launch_grads<T, bf16_t>(a, ranges, dweight, st);
+    else launch_grads<T, half_t>(a, ranges, dweight, st);
+}
+
+}  // namespace kge
+
+using namespace kge;
+
+extern "C" {
+
+size_t kge_rms_norm_bwd_workspace(const kge_rms_norm *norm)
+{
+    if (check_norm(norm) || norm->rows == 0 || norm->cols == 0) return 0;
+    return (size_t)ranges_of(norm->rows, norm->cols).count * ceil_div(norm->cols, 4) * 16;
+}
+
+int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, const float *rstd, int32_t dy_type, const void *dy,
+                     int64_t dy_stride, const void *dh, int64_t dh_stride, void *dx, int64_t dx_stride, void *dweight, void *workspace,
+                     size_t workspace_bytes, void *stream)
+{
+    if (const int rc = check_norm(norm)) return rc;
+    if (!known_type(dy_type)) return KGE_EINVAL;
+    if (h_stride < norm->cols || dy_stride < norm->cols || (dh && dh_stride < norm->cols) || (dx && dx_stride < norm->cols)) return KGE_ESHAPE;
+    if (norm->cols == 0 || (!dx && !dweight)) return KGE_OK;
+    if (norm->rows > 0 && (!h || !rstd || !dy)) return KGE_EINVAL;
+    const size_t need = dweight ? kge_rms_norm_bwd_workspace(norm) : 0;
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
+    const Ranges ranges = norm->rows ? ranges_of(norm->rows, norm->cols) : Ranges{1, 0};
+    const NormGradArgs a{h, dy, dh, norm->weight, h_stride, dy_stride, dh_stride, rstd, norm->rows, norm->cols, ceil_div(norm->cols, 4), ranges.rows_each,
+                         dx, dx_stride, dweight ? static_cast<float *>(workspace) : nullptr, 0};
+    hipStream_t st = as_stream(stream);
+    KGE_CLEAR_LAUNCH_ERRORS();
+    if (norm->rows == 0) {  // (dweight is an empty sum)
+        if (dweight) {
+            const SumArgs none{nullptr, 0, norm->cols, a.quads, dweight};
+            const dim3 grid((unsigned)ceil_div(a.quads, 4)), block(256);
+            if (norm->type == KGE_F32) hipLaunchKernelGGL(norm_join_kernel<float>, grid, block, 0, st, none);
+            else if (norm->type == KGE_BF16) hipLaunchKernelGGL(norm_join_kernel<bf16_t>, grid, block, 0, st, none);
+            else hipLaunchKernelGGL(norm_join_kernel<half_t>, grid, block, 0, st, none);
+        }
+    } else if (norm->type == KGE_F32) launch_grads<float>(a, ranges, dy_type, dweight, st);
+    else if (norm->type == KGE_BF16) launch_grads<bf16_t>(a, ranges, dy_type, dweight, st);
+    else launch_grads<half_t>(a, ranges, dy_type, dweight, st);
+    KGE_CHECK_LAUNCH();
+    return KGE_OK;
+}
+
+}  // extern "C"

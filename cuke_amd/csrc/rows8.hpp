@@ -56,17 +56,14 @@ __device__ __forceinline__ float scale_value(int byte)
 }
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
-// eight values, each 448 at most or not finite (NaN then), to e4m3
+// eight values, each 448 at most or not finite (NaN then, by the instruction too), to e4m3
 __device__ __forceinline__ uint2 to_e4m3(const float (&v)[8])
 {
-    float u[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) u[e] = finite(v[e]) ? v[e] : __builtin_nanf("");
     int lo = 0, hi = 0;
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[0], u[1], lo, false);
-    lo = __builtin_amdgcn_cvt_pk_fp8_f32(u[2], u[3], lo, true);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(u[4], u[5], hi, false);
-    hi = __builtin_amdgcn_cvt_pk_fp8_f32(u[6], u[7], hi, true);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], lo, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], hi, false);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
     return make_uint2((uint32_t)lo, (uint32_t)hi);
 }
 __device__ __forceinline__ void from_e4m3(uint2 q, float scale, float (&v)[8])
@@ -78,12 +75,17 @@ __device__ __forceinline__ void from_e4m3(uint2 q, float scale, float (&v)[8])
     v[4] = c[0] * scale, v[5] = c[1] * scale, v[6] = d[0] * scale, v[7] = d[1] * scale;
 }
 
-// the largest of eight values that is finite
+// the largest of eight values that is finite (a maximum passes NaN over; infinities are rare enough to be looked for afterwards)
 __device__ __forceinline__ float top_of(const float (&v)[8])
 {
     float top = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) top = fmaxf(top, finite(v[e]) ? fabsf(v[e]) : 0.0f);
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+    if (!finite(top)) {
+        top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, finite(v[e]) ? fabsf(v[e]) : 0.0f);
+    }
     return top;
 }
 

@@ -210,8 +210,22 @@ def _linear8_call(desc, tensors, out_dtype, weight8, for_backward):
     return y, saved
 
 
+def _host8(x, weight, bias, act, residual, out_dtype, dtype, drop, seed, step, keep):
+    """The native call, or None."""
+    if isinstance(weight, Rows8):
+        if weight.cols != x.cols:
+            return None
+        w, scale = weight.q, weight.scale
+    else:
+        w, scale = weight, None
+    return _lib.host().linear8(x.q, x.scale, x.cols, w, scale, bias, _act(act), residual, out_dtype, dtype, drop, seed, step, keep)
+
+
 def _linear8_backward(fw, dy, need_x, need_weight, need_bias) -> LinearGrads:
     x, weight, bias = fw.tensors[:3]
+    got = _lib.host().linear8_backward(fw.desc, x.q, x.scale, x.cols, weight, fw.saved, dy, need_x, need_weight, need_bias and bias is not None)
+    if got is not None:
+        return LinearGrads(*got)
     d = _lib.Linear.from_buffer_copy(fw.desc)
     _tensor(x.q, "x of the forward call", 2)
     dy = _rows(dy, "dy", torch.float32 if d.out_type == 0 else weight.dtype, shape=(d.rows, d.out))  # (fw.y may be gone)
@@ -244,6 +258,9 @@ def linear(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, d
     x may be :class:`Rows8`, with a weight in bfloat16 or float16, whose type the layer has, or in 8 bits too: then dtype is the layer's (that of the bias, or
     bfloat16, unless said otherwise)."""
     if isinstance(x, Rows8):
+        y = _host8(x, weight, bias, act, residual, out_dtype, dtype, drop, seed, step, False)
+        if y is not None:
+            return y
         desc, tensors, out_dtype, weight8 = _describe8(x, weight, bias, act, drop, seed, step, residual, out_dtype, dtype)
         return _linear8_call(desc, tensors, out_dtype, weight8, False)[0]
     if dtype is not None or isinstance(weight, Rows8):
@@ -258,6 +275,10 @@ def linear_forward(x, weight, bias=None, *, act="none", residual=None, out_dtype
     """:func:`linear`, with what :func:`linear_backward` needs.  Of a layer on :class:`Rows8` that is those rows and, in 8 bits too, the activation's
     derivative (within 0.0025)."""
     if isinstance(x, Rows8):
+        got = _host8(x, weight, bias, act, residual, out_dtype, None, drop, seed, step, True)
+        if got is not None:
+            y, saved, desc = got
+            return LinearForward(y, desc, saved, (x, weight, bias, residual, None))
         desc, tensors, out_dtype, weight8 = _describe8(x, weight, bias, act, drop, seed, step, residual, out_dtype, None)
         y, saved = _linear8_call(desc, tensors, out_dtype, weight8, True)
         return LinearForward(y, bytes(desc), saved, tensors)
@@ -372,26 +393,34 @@ def preference_loss(pos, neg, ref_pos=None, ref_neg=None, *, beta=1.0, kind="sig
 E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
-@dataclass(frozen=True)
 class Rows8:
     """Rows of ``cols`` values in 8 bits: e4m3 numbers and one power of two for each 32 columns, a value being their product.
 
     q [rows, 32 ceil(cols / 32)] (float8_e4m3fn), zero behind column cols; scale [rows, 4 ceil(cols / 128)] (float8_e8m0fnu), those behind the last
     block anything but NaN.  :func:`pack8` and :func:`rms_norm` make them; arrays made elsewhere are taken as they are."""
-    q: torch.Tensor
-    scale: torch.Tensor
-    cols: int
+    __slots__ = ("q", "scale", "cols")
 
-    def __post_init__(self):
-        for t, name, dtype, width in ((self.q, "q", E4M3, 32 * (-(-self.cols // 32))), (self.scale, "scale", _E8M0, 4 * (-(-self.cols // 128)))):
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, cols: int):
+        for t, name, dtype, width in ((q, "q", E4M3, -(-cols // 32) * 32), (scale, "scale", _E8M0, -(-cols // 128) * 4)):
             if not isinstance(t, torch.Tensor) or t.dtype != dtype:
                 raise TypeError(f"{name} must be a tensor of {dtype} (got {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__})")
-            if self.cols < 0 or t.dim() != 2 or t.shape[1] != width or t.shape[0] != self.q.shape[0]:
-                raise ValueError(f"rows of {self.cols} values need {name} of shape {(self.q.shape[0], width)} (got {tuple(t.shape)})")
+            if cols < 0 or t.dim() != 2 or t.shape[1] != width or t.shape[0] != q.shape[0]:
+                raise ValueError(f"rows of {cols} values need {name} of shape {(q.shape[0] if q.dim() else 0, width)} (got {tuple(t.shape)})")
+        self.q, self.scale, self.cols = q, scale, int(cols)
 
     @property
     def shape(self):
         return torch.Size((self.q.shape[0], self.cols))
+
+    def __repr__(self):
+        return f"Rows8(rows={self.q.shape[0]}, cols={self.cols}, device={self.q.device})"
+
+
+def _made8(q, scale, cols) -> Rows8:
+    """Rows8 of arrays that were made here."""
+    r = Rows8.__new__(Rows8)
+    r.q, r.scale, r.cols = q, scale, cols
+    return r
 
 
 def _laid(t: torch.Tensor, unit: int) -> torch.Tensor:
@@ -421,6 +450,9 @@ def _new_rows8(rows: int, cols: int, device) -> Rows8:
 def pack8(x) -> Rows8:
     """x [rows, cols] in 8 bits: half the memory of 16 bits, each value within 2^-4 of itself (less than 2^-17 of its block's largest: within
     2^-19 of that).  What is infinite becomes NaN."""
+    got = _lib.host().pack8(x)
+    if got is not None:
+        return _made8(*got, x.shape[1])
     x = _rows(x, "x")
     out = _new_rows8(x.shape[0], x.shape[1], x.device)
     _lib.check(_lib.lib().kge_pack8(_TYPES[x.dtype], _p(x), _row_stride(x), x.shape[0], x.shape[1], C.byref(_rows8_c(out)), _stream()), "kge_pack8")
@@ -429,6 +461,10 @@ def pack8(x) -> Rows8:
 
 def unpack8(rows8, dtype=torch.bfloat16) -> torch.Tensor:
     """What rows in 8 bits stand for, as bfloat16, float16 or float32 (exact, but for what float16 cannot hold)."""
+    if isinstance(rows8, Rows8):
+        y = _lib.host().unpack8(rows8.q, rows8.scale, rows8.cols, dtype)
+        if y is not None:
+            return y
     r = _rows8(rows8, "rows8")
     if dtype not in _TYPES:
         raise TypeError(f"dtype must be float32, bfloat16 or float16 (got {dtype})")
@@ -454,6 +490,10 @@ class NormGrads:
 
 
 def _norm_call(x, weight, residual, eps, out_dtype, keep):
+    got = _lib.host().rms_norm(x, weight, residual, eps, out_dtype, keep)
+    if got is not None:
+        y, scale, h, rstd = got
+        return NormForward(y if scale is None else _made8(y, scale, x.shape[1]), x if h is None else h, rstd, weight)
     x = _rows(x, "x")
     rows, cols = x.shape
     if weight is not None:
@@ -496,6 +536,9 @@ def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_we
     the residual is that of x.  An 8-bit y's rounding counts as none."""
     if not isinstance(fw, NormForward):
         raise TypeError("fw must come from rms_norm_forward()")
+    got = _lib.host().rms_norm_backward(fw.h, fw.rstd, fw.weight, dy, dh, need_x, need_weight)
+    if got is not None:
+        return NormGrads(*got)
     h, weight = _tensor(fw.h, "h of the forward call", 2), fw.weight
     dy = _rows(dy, "dy", shape=h.shape)
     if dh is not None:
