@@ -96,19 +96,25 @@ static void launch_few8(int few, bool w8, const TileArgs &t, hipStream_t st)
 }
 
 // ---- forward pass ----------------------------------------------------------------------------------
-// Both sides in 8 bits: tiles of 128 terms.
-using Large8 = Shape<256, 256, 64, 2, 4, 2>;
+// The shapes of linear_plan.hpp with the stages that rows in 8 bits leave room for; those that are other ones where both sides are in 8 bits (a stage's terms are
+// then twice as many).
+using LargeB = Shape<256, 256, 64, 2, 4, 3>;
+using MiddleB = Shape<128, 128, 64, 2, 4, 3>;
+using TallB = Shape<64, 128, 64, 2, 2, 3>;
+using LoneB = Shape<64, 128, 64, 2, 4, 4>;
+using SmallB = Shape<64, 64, 64, 2, 2, 3>;
+using Large8 = Shape<256, 256, 32, 2, 4, 4>;
 using Middle8 = Shape<128, 128, 64, 2, 4, 2>;
 using Tall8 = Shape<64, 128, 64, 2, 2, 2>;
-using Small8 = Shape<64, 64, 64, 2, 2, 3>;
 
+// The weight in 16 bits, rows widened as they leave LDS.  A workgroup of eight waves whose tile lets two of them share a CU holds itself to 128 registers (65536 x 512 -> 400:
+// 78 us with 136).
 template <class T, class S>
-__global__ __launch_bounds__(S::kThreads) void linear8_forward_kernel(TileArgs t)
+__global__ __launch_bounds__(S::kThreads, S::kThreads == 512 && S::XA * S::XB <= 128 * 128 ? 4 : 1) void linear8_forward_kernel(TileArgs t)
 {
-    constexpr int kA = side_bytes<S, true>(), kB = side_bytes<S, false>(), k2 = S::STAGES > 2, k3 = S::STAGES > 3;
-    __shared__ __align__(16) char stage0[kA], stage1[kA], stage2[k2 ? kA : 16], stage3[k3 ? kA : 16];
-    __shared__ __align__(16) char wide0[kB], wide1[kB], wide2[k2 ? kB : 16], wide3[k3 ? kB : 16];
-    compute_tile<T, false, false, S, true, true, kSideB>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3, wide0, wide1, wide2, wide3);
+    constexpr int kStage = stage_bytes8<S, kSideB>();
+    __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
+    compute_tile<T, false, false, S, true, true, kSideB>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
 }
 // The matrix cores' own product of 8-bit sides, at twice the pace of the 16-bit one.  It sums eight neighbouring terms at a time and drops of each what lies below 2^-13
 // of the largest one's power (and adds such sums in fp32): some 2^-13 of a result, next to nothing beside its rounding to bf16 (2^-9) and too much for
@@ -116,7 +122,7 @@ __global__ __launch_bounds__(S::kThreads) void linear8_forward_kernel(TileArgs t
 template <class T, class S>
 __global__ __launch_bounds__(S::kThreads) void linear8_answer_kernel(TileArgs t)
 {
-    constexpr int kStage = stage_bytes8<S>();
+    constexpr int kStage = stage_bytes8<S, kBothSides>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
     compute_tile<T, false, false, S, true, true, kBothSides>(t, blockIdx.x, gridDim.x, stage0, stage1, stage2, stage3);
 }
@@ -131,17 +137,31 @@ static void launch_tiles(TileArgs &t, hipStream_t st)
     else if constexpr (!BOTH) hipLaunchKernelGGL((linear8_forward_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
+// By forward_cost(), whose paces hold for these kernels too (a pair of terms of both sides in 8 bits takes as long as one and a half of 16-bit ones).  Over twelve sizes the shape
+// chosen takes 0.1 % longer than the best one on average with a 16-bit weight, 0.3 % with one in 8 bits.  Some of them (us; Large, Middle, Tall, Lone, Small; what is chosen
+// in brackets), with a 16-bit weight:
+//   32768 x 2048 -> 2048, gelu, drop, act' kept  [329] 370 405 435 474       65536 x 512 -> 400, fp32 residual  79 [76] 76  82 88
+//    4096 x 1024 -> 512, gelu, drop, act' kept    47   18  15 [13] 14         2500 x 520 -> 264, gelu           38  21  12  10 [8]
+// and with one in 8 bits:
+//   32768 x 2048 -> 2048, gelu                   [222] 225 298 344 280       16384 x 768 -> 512, plain          23 [15] 20  24 20
+//    1000 x 2048 -> 2048, gelu                    44   20  19 [12] 13         4096 x 4096 -> 1024, gelu  75 [30; 37 in two stages] 37 40 40
 template <class T>
 static void launch_forward8(TileArgs &t, bool both, hipStream_t st)
 {
     const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 1 : 0);
-    const int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
-    const double large = forward_cost<Large>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0), middle = forward_cost<Middle>(t, epilogue, 2, 0.73, 2.5);
-    const double tall = forward_cost<Tall>(t, epilogue, 3, 0.53, 2.3), small = forward_cost<Small>(t, epilogue, 3, 0.47, 0.9);
-    if (large <= middle && large <= tall && large <= small) both ? launch_tiles<T, Large8, true>(t, st) : launch_tiles<T, Large, false>(t, st);
-    else if (middle <= tall && middle <= small) both ? launch_tiles<T, Middle8, true>(t, st) : launch_tiles<T, Middle, false>(t, st);
-    else if (tall <= small) both ? launch_tiles<T, Tall8, true>(t, st) : launch_tiles<T, Tall, false>(t, st);
-    else both ? launch_tiles<T, Small8, true>(t, st) : launch_tiles<T, Small, false>(t, st);
+    int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
+    if (both) epilogue = epilogue * 7 / 10;
+    const double large = forward_cost<LargeB>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0), middle = forward_cost<MiddleB>(t, epilogue, 2, 0.73, 2.5);
+    const double tall = forward_cost<TallB>(t, epilogue, 3, 0.5, 2.3), small = forward_cost<SmallB>(t, epilogue, 3, 0.45, 0.9);
+    const double lone = forward_cost<LoneB>(t, epilogue, 1, 0.4, 0.9);
+    if (lone < large && lone < middle && lone < tall && lone < small) both ? launch_tiles<T, LoneB, true>(t, st) : launch_tiles<T, LoneB, false>(t, st);
+    else if (large <= middle && large <= tall && large <= small) both ? launch_tiles<T, Large8, true>(t, st) : launch_tiles<T, LargeB, false>(t, st);
+    else if (middle <= tall && middle <= small) {
+        // (a tile a CU at most: nothing but its own stages hides its waits)
+        if (both) tiles_of(t.a.extent, t.b.extent, 128) <= 256 ? launch_tiles<T, MiddleB, true>(t, st) : launch_tiles<T, Middle8, true>(t, st);
+        else launch_tiles<T, MiddleB, false>(t, st);
+    } else if (tall <= small) both ? launch_tiles<T, Tall8, true>(t, st) : launch_tiles<T, TallB, false>(t, st);
+    else both ? launch_tiles<T, SmallB, true>(t, st) : launch_tiles<T, SmallB, false>(t, st);
 }
 
 // ---- gradients -------------------------------------------------------------------------------------
@@ -213,12 +233,12 @@ static int forward8(const kge_linear *l, const kge_rows8 *x8, const kge_rows8 *w
     t.e = Ends{y, y_stride, l->bias, l->residual, l->residual_stride, slope, l->rows, l->out, p.quads,
                make_drop(l->p, l->seed, l->step, l->step_dev, l->out), l->act, l->out_type == KGE_F32, passing(l, y, y_stride)};
     t.b8 = rows8_of(x8), t.a8 = rows8_of(w8);
-    t.b.extent = l->rows;
-    t.k = l->in;
+    t.b = Side{x8->q, x8->q_stride / 2, l->rows};
+    t.k = l->in, t.k8 = q_width(l->in) / 2;
     const bool both = w8 && !p.pack_w && !p.few;
     if (both) {  // (elements of both sides: pairs of terms)
-        t.a = Side{w8->q, w8->q_stride / 2, l->out}, t.b = Side{x8->q, x8->q_stride / 2, l->rows};
-        t.k = q_width(l->in) / 2;
+        t.a = Side{w8->q, w8->q_stride / 2, l->out};
+        t.k = t.k8;
     } else if (w8) {
         if (!p.few) launch_unpack8(l->type, t.a8, l->out, up8(l->in), pw, pitch_of(l->type, l->in), st);
         t.a = Side{pw, pitch_of(l->type, l->in), l->out};

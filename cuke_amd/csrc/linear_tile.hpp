@@ -66,6 +66,7 @@ enum Eight { kNoSide = 0, kSideA = 1, kSideB = 2, kBothSides = 3, kNoSideApart =
 struct TileArgs {
     Side a, b;      // a: the columns of the output, b: its rows (one in 8 bits: its extent, and what lies in memory is in a8 or b8)
     int64_t k;      // terms of every sum
+    int64_t k8;     // side b in 8 bits: pairs of terms that its rows hold, zeros behind their end among them
     int64_t k_each; // per split, a multiple of 64
     int tiles_a, tiles_b, splits;
     float *partial; // where a sum is split: [splits][rows][quads * 4] in fp32, to be joined; else NULL
@@ -294,27 +295,44 @@ __device__ __forceinline__ i8v read_eight(const char *lds, int at, int step, int
     return __builtin_bit_cast(i8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15));
 }
 
-// The scales of a tile of 128 terms of both sides, a word an index: XA of side a, then XB of side b, then what no index asks for.
-template <int XA, int XB, int THREADS>
+// 16 terms of 8 bits of an index for each lane (of such a tile): index at + lane % 32, terms 32 block + 16 (lane / 32) .. + 15; and eight of 16 bits of a tile whose
+// elements are terms: chunk `chunk`.
+template <class TILE>
+__device__ __forceinline__ uint4 read_sixteen(const char *lds, int at, int block, int lane)
+{
+    const int row = at + (lane & 31), j = 2 * block + (lane >> 5);
+    return *reinterpret_cast<const uint4 *>(lds + 16 * (row * TILE::kRow + (j ^ TILE::turn(row))));
+}
+template <class TILE>
+__device__ __forceinline__ s16x8 read_chunk(const char *lds, int at, int chunk, int lane)
+{
+    const int row = at + (lane & 31);
+    return *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + (chunk ^ TILE::turn(row))));
+}
+
+// The scales of a tile, a word (four blocks: 128 terms, of which a tile has all or half) an index: XA of side a, then XB of side b, then what no index asks for.
+// Every thread brings in one, so that all waves have as many loads on their way.
+template <int XA, int XB, int THREADS, int BLOCKS>
 struct ScaleFeed {
-    static_assert(XA + XB <= THREADS, "a word a thread");
-    static constexpr int kBytes = 4 * THREADS;
+    static_assert(XA + XB <= THREADS && (BLOCKS == 2 || BLOCKS == 4), "a word a thread");
     const uint8_t *from;
-    int step;
+    int there;  // all ones, or 0
     __device__ __forceinline__ void start(const Rows8 &a, int64_t extent_a, int64_t n0, const Rows8 &b, int64_t extent_b, int64_t m0)
     {
         const int i = threadIdx.x;
         const bool second = i >= XA;
         const int64_t index = second ? m0 + i - XA : n0 + i;
-        const bool there = second ? i < XA + XB && index < extent_b : index < extent_a;
-        from = there ? (second ? b.scale + index * b.scale_stride : a.scale + index * a.scale_stride) : reinterpret_cast<const uint8_t *>(zero_chunk);
-        step = there ? 4 : 0;
+        const bool yes = second ? i < XA + XB && index < extent_b : index < extent_a;
+        from = yes ? (second ? b.scale + index * b.scale_stride : a.scale + index * a.scale_stride) : reinterpret_cast<const uint8_t *>(zero_chunk);
+        there = yes ? -1 : 0;
     }
-    __device__ __forceinline__ void load(bool more, char *lds)  // the next tile's (behind the end: zeros)
+    __device__ __forceinline__ void load(int tile, bool more, char *lds)  // (behind the end: zeros)
     {
-        word_to_lds(more ? from : reinterpret_cast<const uint8_t *>(zero_chunk), lds + 4 * 64 * __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6));
-        from += step;
+        const uint8_t *p = more ? from + (tile * BLOCKS & ~3 & there) : reinterpret_cast<const uint8_t *>(zero_chunk);
+        word_to_lds(p, lds + 4 * 64 * __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6));
     }
+    // where a tile's first block is in a word
+    __device__ __forceinline__ static int shift(int tile) { return BLOCKS == 4 ? 0 : 16 * (tile & 1); }
 };
 
 // The sums of four (`valid`) output elements of a row by fp32 instructions, for fp32 sides.  Not for speed: it runs where a sum is not finite.
@@ -477,12 +495,14 @@ template <class T, class S>
 constexpr int stage_bytes() { return (S::XA + S::XB) * S::K * 2 * (sizeof(T) == 4 ? kSplitParts : 1); }
 template <class S, bool A>
 constexpr int side_bytes() { return (A ? S::XA : S::XB) * S::K * 2; }
-template <class S>
-constexpr int stage_bytes8() { return (S::XA + S::XB) * S::K * 2 + 4 * S::kThreads; }  // (both sides in 8 bits: the scales lie behind them)
+// Side b in 8 bits, or both (whose tiles have twice as many terms as S::K says); the scales lie behind them.
+template <class S, Eight E>
+constexpr int stage_bytes8() { return S::XA * S::K * 2 + S::XB * S::K * (E == kSideB ? 1 : 2) + 4 * S::kThreads; }
 
 // T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.  WHOLE: an fp32
-// side's rows are whole quads.  EIGHT: the sides that are rows in 8 bits; one of them goes to arrays of its own (wide0 ..), so that its writes do not wait for the
-// other's loads; where both are, elements are pairs of terms (the stride of Side in pairs, TileArgs::k too).
+// side's rows are whole quads.  EIGHT: the sides that are rows in 8 bits.  Side a goes through registers to arrays of its own (wide0 ..), so that its writes do not
+// wait for the other's loads; side b goes to LDS as it lies, in elements that are pairs of terms (the stride of Side in pairs), and so do both (TileArgs::k in
+// pairs too).
 template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER, bool WHOLE, Eight EIGHT = kNoSide>
 __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, int64_t blocks, char *stage0, char *stage1, char *stage2, char *stage3,
                                              char *wide0 = nullptr, char *wide1 = nullptr, char *wide2 = nullptr, char *wide3 = nullptr)
@@ -491,13 +511,14 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     using E = typename std::conditional<kFloat, bf16_t, T>::type;
     constexpr int PLANES = kFloat ? kSplitParts : 1, K = S::K, STAGES = S::STAGES, WA = S::WA, WB = S::WB, SHARE = S::SHARE;
     using A = Tile<S::XA, K, A_ACROSS, S::kThreads>;
-    using B = Tile<S::XB, K, B_ACROSS, S::kThreads>;
-    constexpr int kBytesA = S::XA * K * 2, kBytesB = S::XB * K * 2, kStage = stage_bytes<T, S>();
-    static_assert(EIGHT == kNoSide || (!kFloat && SHARE == 1 && (EIGHT != kBothSides || (K == 64 && !A_ACROSS && !B_ACROSS))), "sides in 8 bits");
+    using B = Tile<S::XB, EIGHT == kSideB ? K / 2 : K, B_ACROSS, S::kThreads>;  // (of a side in 8 bits that goes to LDS as it lies: elements are pairs of terms)
+    constexpr int kBytesA = S::XA * K * 2, kBytesB = S::XB * K * (EIGHT == kSideB ? 1 : 2), kStage = EIGHT == kSideB ? kBytesA + kBytesB : stage_bytes<T, S>();
+    constexpr bool kScales = EIGHT == kSideB || EIGHT == kBothSides;
+    static_assert(EIGHT == kNoSide || (!kFloat && SHARE == 1 && (!kScales || (!A_ACROSS && !B_ACROSS)) && (EIGHT != kSideB || K == 64)), "sides in 8 bits");
     constexpr int FA = S::XA / WA / 32, FB = S::XB / WB / 32;
     static_assert(STAGES >= 2 && STAGES <= 4 && (!kFloat || STAGES == 2), "stages");
 
-    constexpr bool kWideA = EIGHT == kSideA || EIGHT == kNoSideApart, kApartSides = kWideA || EIGHT == kSideB;
+    constexpr bool kWideA = EIGHT == kSideA || EIGHT == kNoSideApart;
     int ta, tb, split;
     tile_of(block, blocks, t, &ta, &tb, &split);
     const int64_t n0 = (int64_t)ta * S::XA, m0 = (int64_t)tb * S::XB;
@@ -510,16 +531,58 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     const int tiles = left > 0 ? (int)((left + K - 1) / K) : 0;
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
     auto wide = [&](int u) -> char * { return u == 0 ? wide0 : (u == 1 ? wide1 : (u == 2 ? wide2 : wide3)); };
-    auto multiply = [&](int u) {
-        const char *la = kWideA ? wide(u) : stage(u), *lb = kWideA ? stage(u) : (EIGHT == kSideB ? wide(u) : la + PLANES * kBytesA);
+    using Scales = ScaleFeed<EIGHT == kBothSides ? S::XA : 0, S::XB, kScales ? S::kThreads : S::XA + S::XB, EIGHT == kBothSides && K == 64 ? 4 : 2>;
+    auto multiply = [&](int u, int tile) {
+        const char *la = kWideA ? wide(u) : stage(u), *lb = kWideA ? stage(u) : la + PLANES * kBytesA;
+        if constexpr (EIGHT == kSideB) {
+            // (32 terms at a time: a lane's sixteen of side b are half a block, which one scale widens; side a's are read to match)
+            int sb[FB];
+#pragma unroll
+            for (int j = 0; j < FB; ++j) sb[j] = *reinterpret_cast<const int *>(lb + kBytesB + 4 * (wb + 32 * j + (lane & 31))) >> Scales::shift(tile);
+            // (where a wave has one product or two, all of a tile is read before the first of it is widened: little else hides the reads' latency)
+            constexpr int kAhead = FA * FB <= 2 ? K / 32 : 1;
+            static_assert(K / 32 % kAhead == 0, "whole turns");
+#pragma unroll
+            for (int u = 0; u < K / 32; u += kAhead) {
+                s16x8 a[kAhead][FA][2];
+                uint4 q[kAhead][FB];
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+#pragma unroll
+                    for (int j = 0; j < FB; ++j) q[k][j] = read_sixteen<B>(lb, wb + 32 * j, u + k, lane);
+#pragma unroll
+                    for (int i = 0; i < FA; ++i)
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) a[k][i][v] = read_chunk<A>(la, wa + 32 * i, 4 * (u + k) + 2 * (lane >> 5) + v, lane);
+                }
+                if (kAhead > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < kAhead; ++k) {
+                    s16x8 b[FB][2];
+#pragma unroll
+                    for (int j = 0; j < FB; ++j) {
+                        const float power = __int_as_float((sb[j] >> 8 * (u + k) & 0xFF) << 23);
+                        b[j][0] = widen(make_uint2(q[k][j].x, q[k][j].y), power, E{}), b[j][1] = widen(make_uint2(q[k][j].z, q[k][j].w), power, E{});
+                    }
+#pragma unroll
+                    for (int v = 0; v < 2; ++v)
+#pragma unroll
+                        for (int i = 0; i < FA; ++i)
+#pragma unroll
+                            for (int j = 0; j < FB; ++j) acc[i][j] = Mfma<E>::go(a[k][i][v], b[j][v], acc[i][j]);
+                }
+            }
+            return;
+        }
         if constexpr (EIGHT == kBothSides) {
             // (half a wave gives the first block's scales, the other the second's: its byte of a word is moved to where the instruction looks)
             int sa[FA], sb[FB];
             const char *scales = lb + kBytesB;
+            const int shift = Scales::shift(tile) + 8 * (lane >> 5);
 #pragma unroll
-            for (int j = 0; j < FB; ++j) sb[j] = *reinterpret_cast<const int *>(scales + 4 * (S::XA + wb + 32 * j + (lane & 31))) >> 8 * (lane >> 5);
+            for (int j = 0; j < FB; ++j) sb[j] = *reinterpret_cast<const int *>(scales + 4 * (S::XA + wb + 32 * j + (lane & 31))) >> shift;
 #pragma unroll
-            for (int i = 0; i < FA; ++i) sa[i] = *reinterpret_cast<const int *>(scales + 4 * (wa + 32 * i + (lane & 31))) >> 8 * (lane >> 5);
+            for (int i = 0; i < FA; ++i) sa[i] = *reinterpret_cast<const int *>(scales + 4 * (wa + 32 * i + (lane & 31))) >> shift;
 #pragma unroll
             for (int u = 0; u < K / 32; ++u) {
                 i8v a[FA], b[FB];
@@ -580,22 +643,19 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             lds_ready();
             put(1 - u, stage(1 - u));
             fetch(1 - u);
-            multiply(u);
+            multiply(u, 0);
         };
         int at = 0;
         for (; at + 2 <= tiles; at += 2) turn(0), turn(1);
         if (at < tiles) turn(0);
-    } else if constexpr (EIGHT == kSideA || EIGHT == kSideB) {
+    } else if constexpr (EIGHT == kSideA) {
         // The 16-bit side is requested STAGES - 1 tiles ahead; the other one's numbers come to registers three tiles ahead and to LDS one tile ahead.  Only what the
         // turn before this one has requested may still be on its way at the barrier: the compiler, which cannot count loads to registers among those to LDS,
         // would otherwise wait for all of them before it uses a register.
-        using Q = typename std::conditional<EIGHT == kSideA, A, B>::type;
-        using W = typename std::conditional<EIGHT == kSideA, B, A>::type;
-        constexpr int kOut = (STAGES > 2 ? W::kRounds : 0) + 2 * Q::kRounds;
-        typename Q::template ByteFeed<E> bytes;
-        typename W::template Feed<E> feed;
-        if constexpr (EIGHT == kSideA) bytes.start(t.a8, t.a.extent, n0, k0), feed.start(t.b, m0, k0);
-        else bytes.start(t.b8, t.b.extent, m0, k0), feed.start(t.a, n0, k0);
+        constexpr int kOut = (STAGES > 2 ? B::kRounds : 0) + 2 * A::kRounds;
+        typename A::template ByteFeed<E> bytes;
+        typename B::template Feed<E> feed;
+        bytes.start(t.a8, t.a.extent, n0, k0), feed.start(t.b, m0, k0);
         int64_t left8 = left;
         auto fetch = [&](int set) { bytes.fetch(set, left8), left8 -= K; };
         auto load = [&](char *lds) { feed.load(left, lds), left -= K; };
@@ -623,7 +683,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             in_order();
             fetch(1 - set);
             in_order();
-            multiply(u);
+            multiply(u, 0);
         };
         constexpr int kTurns = STAGES % 2 ? 2 * STAGES : STAGES;
         int at = 0;
@@ -638,15 +698,17 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     } else {
         typename A::template Feed<E> feed_a;
         typename B::template Feed<E> feed_b;
-        ScaleFeed<S::XA, S::XB, EIGHT == kBothSides ? S::kThreads : S::XA + S::XB> scales;
-        constexpr int kLoads = A::kRounds + B::kRounds + (EIGHT == kBothSides);  // per thread and tile
+        Scales scales;
+        constexpr int kLoads = A::kRounds + B::kRounds + kScales;  // per thread and tile
         feed_a.start(t.a, n0, k0), feed_b.start(t.b, m0, k0);
-        if constexpr (EIGHT == kBothSides) scales.start(t.a8, t.a.extent, n0, t.b8, t.b.extent, m0);
+        if constexpr (kScales) scales.start(t.a8, t.a.extent, n0, t.b8, t.b.extent, m0);
+        int64_t left8 = t.k8;  // (side b in 8 bits: pairs of terms, of which zeros behind the row's end are some)
+        int loaded = 0;
         auto load = [&](int u) {
             char *lds = stage(u);
             if constexpr (EIGHT == kNoSideApart) feed_a.load(left, wide(u)), feed_b.load(left, lds);
-            else feed_a.load(left, lds), feed_b.load(left, lds + kBytesA);
-            if constexpr (EIGHT == kBothSides) scales.load(left > 0, lds + kBytesA + kBytesB);
+            else feed_a.load(left, lds), feed_b.load(EIGHT == kSideB ? left8 : left, lds + kBytesA);
+            if constexpr (kScales) scales.load(loaded, left > 0, lds + kBytesA + kBytesB), ++loaded, left8 -= K / 2;
             left -= K;
         };
         // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
@@ -658,14 +720,14 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             for (int u = 0; u < STAGES; ++u) {
                 stage_ready<kLoads * (STAGES - 2)>();
                 load((u + STAGES - 1) % STAGES);
-                multiply(u);
+                multiply(u, at + u);
             }
 #pragma unroll
         for (int u = 0; u < STAGES - 1; ++u) {
             if (at + u >= tiles) break;
             stage_ready<kLoads * (STAGES - 2)>();
             load((u + STAGES - 1) % STAGES);
-            multiply(u);
+            multiply(u, at + u);
         }
     }
 
@@ -673,10 +735,10 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.  A
     // strip's residuals are requested all at once and ahead of everything else that is done with it.
     constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16;
-    constexpr int kPerStage = (kWideA ? kBytesB : (EIGHT == kSideB ? kBytesA : kStage)) / kStrip, kPerWide = (kWideA ? kBytesA : kBytesB) / kStrip;
+    constexpr int kPerStage = (kWideA ? kBytesB : kStage) / kStrip, kPerWide = kBytesA / kStrip;
     constexpr int kApart = 64 / kQuads, kRows = 4 / SHARE, kTurns = 32 / (kApart * kRows * SHARE);  // rows a read covers, reads a turn, turns of a wave in a strip
     constexpr int kStrips = FA / kGroup * FB;
-    static_assert(FA % kGroup == 0 && kPerStage >= 1 && WA * WB <= STAGES * (kPerStage + (kApartSides ? kPerWide : 0)), "a strip for every wave");
+    static_assert(FA % kGroup == 0 && kPerStage >= 1 && WA * WB <= STAGES * (kPerStage + (kWideA ? kPerWide : 0)), "a strip for every wave");
     static_assert(SHARE == 1 || (kStrips == 1 && kPerStage >= SHARE * WA * WB), "waves that share a strip");
     const int quad = lane % kQuads, row0 = lane / kQuads + part * kTurns * kApart * kRows;
     const bool ahead = LAYER && t.e.residual && t.e.cols % 4 == 0;
@@ -694,7 +756,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     stage_ready<0>();
     auto skew = [](int row) { return kQuads == 16 ? row & 15 : (row >> 1) & 7; };
     char *lds = stage(wave / kPerStage) + wave % kPerStage * kStrip;
-    if constexpr (kApartSides)
+    if constexpr (kWideA)
         if (wave >= STAGES * kPerStage) lds = wide((wave - STAGES * kPerStage) / kPerWide) + (wave - STAGES * kPerStage) % kPerWide * kStrip;
     uint64_t base = 0;
     if constexpr (LAYER) base = t.e.drop.base();
