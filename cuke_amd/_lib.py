@@ -187,9 +187,9 @@ EXPORTS = {
     "kge_pack8": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.POINTER(Rows8), C.c_void_p]),
     "kge_unpack8": (C.c_int, [C.POINTER(Rows8), C.c_int64, C.c_int64, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "kge_rms_norm_fwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p, C.c_int64, C.POINTER(Rows8), C.c_void_p, C.c_int64, C.c_void_p,
-                                   C.c_void_p]),
+                                   C.c_void_p, C.c_void_p]),
     "kge_rms_norm_bwd_workspace": (C.c_size_t, [C.POINTER(RmsNorm)]),
-    "kge_rms_norm_bwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
+    "kge_rms_norm_bwd": (C.c_int, [C.POINTER(RmsNorm), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p,
                                    C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
     "kge_linear8_saved_bytes": (C.c_size_t, [C.POINTER(Linear)]),
     "kge_linear8_fwd_workspace": (C.c_size_t, [C.POINTER(Linear), C.POINTER(Rows8), C.c_int]),

@@ -916,7 +916,7 @@ PyObject *py_unpack8(PyObject *, PyObject *const *args, Py_ssize_t)
     END_HANDLE_TH_ERRORS
 }
 
-// rms_norm(x, weight, residual, eps, out_dtype or None, keep) -> (y, or q and None beside it; scale; h; rstd), or None
+// rms_norm(x, weight, residual, eps, out_dtype or None, keep) -> (y or q, scale or None, h or None, rstd or None, rest or None), or None
 PyObject *py_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t)
 {
     HANDLE_TH_ERRORS
@@ -936,25 +936,26 @@ PyObject *py_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t)
     const bool keep = PyObject_IsTrue(args[5]), eight = n.out_type == KGE_E4M3;
     n.x = x->data_ptr(), n.weight = args[1] != Py_None ? w->data_ptr() : nullptr, n.residual = args[2] != Py_None ? res->data_ptr() : nullptr;
     const auto opt = x->options().requires_grad(false);
-    at::Tensor y, scale, h, rstd;
+    at::Tensor y, scale, h, rstd, rest;
     kge_rows8 y8{};
     if (eight) y8 = new_rows8(n.rows, n.cols, opt, &y, &scale);
     else y = at::empty({n.rows, n.cols}, opt.dtype(scalar_of(n.out_type)));
     if (n.residual) h = at::empty({n.rows, n.cols}, opt);
     if (keep) rstd = at::empty({n.rows}, opt.dtype(at::kFloat));
-    void *st = stream(), *to = eight ? nullptr : y.data_ptr(), *ph = h.defined() ? h.data_ptr() : nullptr;
+    if (keep && n.residual && n.type != KGE_F32) rest = at::empty({n.rows, (n.cols + 7) / 8}, opt.dtype(at::kInt));
+    void *st = stream(), *to = eight ? nullptr : y.data_ptr(), *ph = h.defined() ? h.data_ptr() : nullptr, *pt = rest.defined() ? rest.data_ptr() : nullptr;
     float *pr = keep ? rstd.data_ptr<float>() : nullptr;
-    const int rc = nogil([&] { return kge_rms_norm_fwd(&n, to, n.cols, eight ? &y8 : nullptr, ph, n.cols, pr, st); });
+    const int rc = nogil([&] { return kge_rms_norm_fwd(&n, to, n.cols, eight ? &y8 : nullptr, ph, n.cols, pr, pt, st); });
     if (rc) return fail(rc, "kge_rms_norm_fwd"), nullptr;
-    return Py_BuildValue("(NNNN)", wrap(y), wrap(scale), wrap(h), wrap(rstd));
+    return Py_BuildValue("(NNNNN)", wrap(y), wrap(scale), wrap(h), wrap(rstd), wrap(rest));
     END_HANDLE_TH_ERRORS
 }
 
-// rms_norm_backward(h, rstd, weight, dy, dh, need x, need weight) -> (dx, dweight), or None.  h, rstd and weight are those of the forward call.
+// rms_norm_backward(h, rstd, rest, weight, dy, dh, need x, need weight) -> (dx, dweight), or None.  h, rstd, rest and weight are those of the forward call.
 PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t)
 {
     HANDLE_TH_ERRORS
-    const at::Tensor *h = tensor(args[0]), *rstd = tensor(args[1]), *w = tensor(args[2]), *dy = tensor(args[3]), *dh = tensor(args[4]);
+    const at::Tensor *h = tensor(args[0]), *rstd = tensor(args[1]), *rest = tensor(args[2]), *w = tensor(args[3]), *dy = tensor(args[4]), *dh = tensor(args[5]);
     if (!h || !h->is_cuda() || !rstd || !dy) NOT_HERE;
     const int dev = c10::hip::current_device();
     kge_rms_norm n{};
@@ -964,20 +965,21 @@ PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t)
     int64_t h_stride, dy_stride, dh_stride = 0;
     const int dy_type = type_of(dy, dev);
     if (!rows_of(h, n.type, n.rows, n.cols, dev, &h_stride) || dy_type < 0 || !rows_of(dy, dy_type, n.rows, n.cols, dev, &dy_stride)) NOT_HERE;
-    if (!vector_of(rstd, KGE_F32, n.rows, dev) || (args[2] != Py_None && !vector_of(w, n.type, n.cols, dev))) NOT_HERE;
-    if (args[4] != Py_None && !rows_of(dh, n.type, n.rows, n.cols, dev, &dh_stride)) NOT_HERE;
-    n.weight = args[2] != Py_None ? w->data_ptr() : nullptr;
+    if (!vector_of(rstd, KGE_F32, n.rows, dev) || (args[3] != Py_None && !vector_of(w, n.type, n.cols, dev))) NOT_HERE;
+    if (args[5] != Py_None && !rows_of(dh, n.type, n.rows, n.cols, dev, &dh_stride)) NOT_HERE;
+    n.weight = args[3] != Py_None ? w->data_ptr() : nullptr;
     const auto opt = h->options().requires_grad(false);
     at::Tensor dx, dw;
-    if (PyObject_IsTrue(args[5])) dx = at::empty({n.rows, n.cols}, opt);
-    if (PyObject_IsTrue(args[6]) && n.weight) dw = at::empty({n.cols}, opt);
+    if (PyObject_IsTrue(args[6])) dx = at::empty({n.rows, n.cols}, opt);
+    if (PyObject_IsTrue(args[7]) && n.weight) dw = at::empty({n.cols}, opt);
     const size_t ws_bytes = dw.defined() ? kge_rms_norm_bwd_workspace(&n) : 0;
     c10::DataPtr ws;
     if (ws_bytes) ws = scratch(ws_bytes);
-    const void *from = h->data_ptr(), *pdy = dy->data_ptr(), *pdh = args[4] != Py_None ? dh->data_ptr() : nullptr;
+    const void *from = h->data_ptr(), *pdy = dy->data_ptr(), *pdh = args[5] != Py_None ? dh->data_ptr() : nullptr;
     const float *pr = rstd->data_ptr<float>();
+    const void *pt = rest ? rest->data_ptr() : nullptr;
     void *px = dx.defined() ? dx.data_ptr() : nullptr, *pw = dw.defined() ? dw.data_ptr() : nullptr, *st = stream();
-    const int rc = nogil([&] { return kge_rms_norm_bwd(&n, from, h_stride, pr, dy_type, pdy, dy_stride, pdh, dh_stride, px, n.cols, pw, ws.get(), ws_bytes, st); });
+    const int rc = nogil([&] { return kge_rms_norm_bwd(&n, from, h_stride, pr, pt, dy_type, pdy, dy_stride, pdh, dh_stride, px, n.cols, pw, ws.get(), ws_bytes, st); });
     if (rc) return fail(rc, "kge_rms_norm_bwd"), nullptr;
     return Py_BuildValue("(NN)", wrap(dx), wrap(dw));
     END_HANDLE_TH_ERRORS

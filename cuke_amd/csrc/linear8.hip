@@ -107,10 +107,14 @@ using Large8 = Shape<256, 256, 32, 2, 4, 4>;
 using Middle8 = Shape<128, 128, 64, 2, 4, 2>;
 using Tall8 = Shape<64, 128, 64, 2, 2, 2>;
 
-// The weight in 16 bits, rows widened as they leave LDS.  A workgroup of eight waves whose tile lets two of them share a CU holds itself to 128 registers (65536 x 512 -> 400:
+// Waves a SIMD that the registers have to leave room for: a workgroup of eight whose LDS lets two of them share a CU holds itself to 128 registers (65536 x 512 -> 400:
 // 78 us with 136).
+template <class S, Eight E>
+constexpr int waves_for() { return S::kThreads == 512 && 2 * S::STAGES * stage_bytes8<S, E>() <= 160 << 10 ? 4 : 1; }
+
+// The weight in 16 bits, rows widened as they leave LDS.
 template <class T, class S>
-__global__ __launch_bounds__(S::kThreads, S::kThreads == 512 && S::XA * S::XB <= 128 * 128 ? 4 : 1) void linear8_forward_kernel(TileArgs t)
+__global__ __launch_bounds__(S::kThreads, (waves_for<S, kSideB>())) void linear8_forward_kernel(TileArgs t)
 {
     constexpr int kStage = stage_bytes8<S, kSideB>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads == 512 && S::XA * S::XB <=
 // of the largest one's power (and adds such sums in fp32): some 2^-13 of a result, next to nothing beside its rounding to bf16 (2^-9) and too much for
 // fp16 and fp32, which are made of widened numbers.
 template <class T, class S>
-__global__ __launch_bounds__(S::kThreads) void linear8_answer_kernel(TileArgs t)
+__global__ __launch_bounds__(S::kThreads, (waves_for<S, kBothSides>())) void linear8_answer_kernel(TileArgs t)
 {
     constexpr int kStage = stage_bytes8<S, kBothSides>();
     __shared__ __align__(16) char stage0[kStage], stage1[kStage], stage2[S::STAGES > 2 ? kStage : 16], stage3[S::STAGES > 3 ? kStage : 16];
@@ -165,29 +169,33 @@ static void launch_forward8(TileArgs &t, bool both, hipStream_t st)
 }
 
 // ---- gradients -------------------------------------------------------------------------------------
-// dW = dz^T x8, dx = dz W and the bias's gradient in one launch, as linear_grads_kernel.
-template <class T, class S>
-__global__ __launch_bounds__(S::kThreads) void linear8_grads_kernel(TileArgs dw, TileArgs dx, SumArgs db, int64_t dw_blocks, int64_t dx_blocks)
+// dW = dz^T x8, dx = dz W and the bias's gradient in one launch, as linear_grads_kernel; W and X: the shapes of the two products.
+using MiddleA = Shape<128, 128, 32, 4, 2, 4>;
+using SmallA = Shape<64, 64, 32, 2, 2, 4>;
+template <class T, class W, class X>
+__global__ __launch_bounds__(W::kThreads, W::kThreads == 512 && W::XA * W::XB <= 128 * 128 ? 4 : 1) void linear8_grads_kernel(TileArgs dw, TileArgs dx, SumArgs db, int64_t dw_blocks, int64_t dx_blocks)
 {
-    constexpr int kA = side_bytes<S, true>(), kB = side_bytes<S, false>(), k2 = S::STAGES > 2, k3 = S::STAGES > 3;
-    __shared__ __align__(16) char stage0[kB], stage1[kB], stage2[k2 ? kB : 16], stage3[k3 ? kB : 16];
-    __shared__ __align__(16) char wide0[kA], wide1[kA], wide2[k2 ? kA : 16], wide3[k3 ? kA : 16];
+    static_assert(W::kThreads == X::kThreads && W::XA == X::XA && W::XB == X::XB && W::STAGES >= X::STAGES, "one grid, and arrays of the larger one");
+    constexpr int kA = side_bytes<W, true>() > side_bytes<X, true>() ? side_bytes<W, true>() : side_bytes<X, true>();
+    constexpr int kB = side_bytes<W, false>() > side_bytes<X, false>() ? side_bytes<W, false>() : side_bytes<X, false>();
+    __shared__ __align__(16) char stage0[kB], stage1[kB], stage2[W::STAGES > 2 ? kB : 16], stage3[W::STAGES > 3 ? kB : 16];
+    __shared__ __align__(16) char wide0[kA], wide1[kA], wide2[X::STAGES > 2 ? kA : 16], wide3[X::STAGES > 3 ? kA : 16];
     const int64_t block = blockIdx.x, products = dw_blocks + dx_blocks, before = dx.k > dw.k_each ? dx_blocks : 0;
-    if (block >= products) join_sums<T, S::kThreads>(db, block - products, reinterpret_cast<float4 *>(stage0));
+    if (block >= products) join_sums<T, W::kThreads>(db, block - products, reinterpret_cast<float4 *>(stage0));
     else if (block >= before && block < before + dw_blocks)
-        compute_tile<T, true, true, S, false, true, kSideA>(dw, block - before, dw_blocks, stage0, stage1, stage2, stage3, wide0, wide1, wide2, wide3);
+        compute_tile<T, true, true, W, false, true, kSideA>(dw, block - before, dw_blocks, stage0, stage1, stage2, stage3, wide0, wide1);
     else
-        compute_tile<T, true, false, S, false, true, kNoSideApart>(dx, before ? block : block - dw_blocks, dx_blocks, stage0, stage1, stage2, stage3, wide0, wide1, wide2,
+        compute_tile<T, true, false, X, false, true, kNoSideApart>(dx, before ? block : block - dw_blocks, dx_blocks, stage0, stage1, stage2, stage3, wide0, wide1, wide2,
                                                                    wide3);
 }
 
-template <class T, class S>
+template <class T, class W, class X>
 static void launch_grads8(TileArgs &dw, TileArgs &dx, const SumArgs &db, bool want_dw, bool want_dx, hipStream_t st)
 {
-    for (TileArgs *t : {&dw, &dx}) t->tiles_a = (int)ceil_div(t->a.extent, S::XA), t->tiles_b = (int)ceil_div(t->b.extent, S::XB);
+    for (TileArgs *t : {&dw, &dx}) t->tiles_a = (int)ceil_div(t->a.extent, W::XA), t->tiles_b = (int)ceil_div(t->b.extent, W::XB);
     const int64_t nw = want_dw ? (int64_t)dw.tiles_a * dw.tiles_b * dw.splits : 0, nx = want_dx ? (int64_t)dx.tiles_a * dx.tiles_b : 0;
     const int64_t nb = db.out ? ceil_div(db.quads, 4) : 0;
-    if (nw + nx + nb) hipLaunchKernelGGL((linear8_grads_kernel<T, S>), dim3((unsigned)(nw + nx + nb)), dim3(S::kThreads), 0, st, dw, dx, db, nw, nx);
+    if (nw + nx + nb) hipLaunchKernelGGL((linear8_grads_kernel<T, W, X>), dim3((unsigned)(nw + nx + nb)), dim3(W::kThreads), 0, st, dw, dx, db, nw, nx);
 }
 
 // ---- a layer's plan --------------------------------------------------------------------------------
@@ -287,9 +295,9 @@ static int backward8(const kge_linear *l, const kge_rows8 *x8, const Plan8 &p, c
     tw.partial = tw.splits > 1 ? part : nullptr;
     tw.e.y = dw, tw.e.y_stride = l->in, tw.e.rows = l->out, tw.e.cols = l->in, tw.e.quads = in_quads;
     const SumArgs sum{sums, p.sum_blocks, l->out, p.quads, db};
-    if (g.tile == 256) launch_grads8<T, Large>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
-    else if (g.tile == 128) launch_grads8<T, MiddleG>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
-    else launch_grads8<T, Small>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
+    if (g.tile == 256) launch_grads8<T, Large, Large>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
+    else if (g.tile == 128) launch_grads8<T, MiddleA, MiddleA>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
+    else launch_grads8<T, SmallA, SmallA>(tw, tx, sum, dw != nullptr, dx != nullptr, st);
     if (dw && tw.partial) launch_join<T>(JoinArgs{part, l->out, l->in, in_quads, tw.splits, dw}, st);
     KGE_CHECK_LAUNCH();
     return KGE_OK;

@@ -139,6 +139,16 @@ struct Tile {
                 step[r] = there ? (ACROSS ? K * s.stride : K) * (int64_t)sizeof(E) : 0;
             }
         }
+        // the next tile, all of whose terms exist
+        __device__ __forceinline__ void load_whole(char *lds)
+        {
+            const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                chunk_to_lds(from[r], lds + 16 * (r * THREADS + wave * 64));
+                from[r] += step[r];
+            }
+        }
         // the next tile, of which `left` terms exist (none, behind the end)
         __device__ __forceinline__ void load(int64_t left, char *lds)
         {
@@ -222,42 +232,46 @@ struct Tile {
         }
     };
 
-    // The same of a side in 8 bits: a chunk's eight numbers and its block's scale wait in registers, two tiles' at a time, and go to LDS as 16-bit ones.
+    // The same of a side in 8 bits across rows: a chunk's eight numbers and its block's scale wait in registers, two tiles' at a time, and go to LDS as 16-bit ones.
+    // Read through buffers that end with the tile's rows: what lies behind comes back as zeros, so that every load is made and none needs an address of its own.
+    // (An index that does not exist may be another row's: its sums go nowhere.)
     template <class E>
     struct ByteFeed {
-        const uint8_t *q[kRounds], *scale[kRounds];
-        int64_t q_step, scale_step;
-        int term[kRounds];  // of the chunk, within the tile; above every other where its index does not exist
+        static constexpr int kTurnRows = THREADS / kRow;  // rows a round covers: turn() is the same in all of them
+        static_assert(ACROSS && kTurnRows % 16 == 0, "chunk j of a row is the same in every round");
+        const uint8_t *q, *scale;       // of the next tile's first row
+        int64_t q_step, scale_step;     // bytes of a tile's rows
+        int q_whole, q_last, scale_whole, scale_last;  // bytes from there to the end of a tile's rows: of whole tiles, and of the last one
+        int left;                       // tiles not requested yet
+        uint32_t q_at, scale_at, q_round, scale_round;  // the lane's chunk, and how far those of its rounds are apart
         uint2 held[2][kRounds];
         int byte[2][kRounds];
 
-        __device__ __forceinline__ void start(const Rows8 &s, int64_t extent, int64_t first, int64_t k)
+        // terms: rows from k on, more than none
+        __device__ __forceinline__ void start(const Rows8 &s, int64_t extent, int64_t first, int64_t k, int64_t terms, int tiles)
         {
-            q_step = ACROSS ? K * s.q_stride : K, scale_step = ACROSS ? K * s.scale_stride : K / 32;
-#pragma unroll
-            for (int r = 0; r < kRounds; ++r) {
-                const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
-                const int64_t index = first + (ACROSS ? 8 * j : row), line = ACROSS ? k + row : index, col = ACROSS ? index : k + 8 * j;
-                term[r] = index < extent ? (ACROSS ? row : 8 * j) : 0x7FFFFFFF;
-                q[r] = s.q + line * s.q_stride + col, scale[r] = s.scale + line * s.scale_stride + (col >> 5);
-            }
+            const int row = threadIdx.x / kRow, j = (threadIdx.x % kRow) ^ turn(row);
+            q = s.q + k * s.q_stride + first, scale = s.scale + k * s.scale_stride + (first >> 5);
+            q_step = K * s.q_stride, scale_step = K * s.scale_stride, left = tiles;
+            const int width = (int)((extent + 31) / 32 * 32 - first), q_row = (int)s.q_stride, scale_row = (int)s.scale_stride;  // (K rows are less than 2^31)
+            const int last = (int)((terms - 1) % K);
+            q_whole = (K - 1) * q_row + width, q_last = last * q_row + width;
+            scale_whole = (K - 1) * scale_row + width / 32, scale_last = last * scale_row + width / 32;
+            q_at = row * q_row + 8 * j, scale_at = row * scale_row + (j >> 2);
+            q_round = kTurnRows * q_row, scale_round = kTurnRows * scale_row;
         }
-        // the next tile, of which `left` terms exist (none, behind the end)
-        __device__ __forceinline__ void fetch(int set, int64_t left)
+        __device__ __forceinline__ void fetch(int set)  // the next tile; behind the last one zeros
         {
-            typedef const __attribute__((address_space(1))) u2 *pair;
-            typedef const __attribute__((address_space(1))) uint8_t *single;
-            const uint64_t zero = reinterpret_cast<uint64_t>(zero_chunk);
+            constexpr int kFormat = 0x00020000;  // raw, 32 bits an element
+            const auto from = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(q), 0, left > 1 ? q_whole : (left == 1 ? q_last : 0), kFormat);
+            const auto of = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(scale), 0, left > 1 ? scale_whole : (left == 1 ? scale_last : 0), kFormat);
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
-                // (an address that the compiler knows nothing of: it would branch around the load of what it knows to be zero, and loads are counted)
-                uint64_t at = term[r] < left ? reinterpret_cast<uint64_t>(q[r]) : zero, of = term[r] < left ? reinterpret_cast<uint64_t>(scale[r]) : zero;
-                asm("" : "+v"(at), "+v"(of));
-                const u2 v = *(pair)at;
+                const u2 v = __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(from, q_at + r * q_round, 0, 0));
                 held[set][r] = make_uint2(v[0], v[1]);
-                byte[set][r] = *(single)of;
-                q[r] += q_step, scale[r] += scale_step;
+                byte[set][r] = __builtin_amdgcn_raw_buffer_load_b8(of, scale_at + r * scale_round, 0, 0);
             }
+            q += q_step, scale += scale_step, --left;
         }
         __device__ __forceinline__ void put(int set, char *lds)
         {
@@ -500,8 +514,8 @@ template <class S, Eight E>
 constexpr int stage_bytes8() { return S::XA * S::K * 2 + S::XB * S::K * (E == kSideB ? 1 : 2) + 4 * S::kThreads; }
 
 // T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.  WHOLE: an fp32
-// side's rows are whole quads.  EIGHT: the sides that are rows in 8 bits.  Side a goes through registers to arrays of its own (wide0 ..), so that its writes do not
-// wait for the other's loads; side b goes to LDS as it lies, in elements that are pairs of terms (the stride of Side in pairs), and so do both (TileArgs::k in
+// side's rows are whole quads.  EIGHT: the sides that are rows in 8 bits.  Side a goes through registers to two arrays of its own (wide0, wide1), so that its writes do
+// not wait for the other's loads; side b goes to LDS as it lies, in elements that are pairs of terms (the stride of Side in pairs), and so do both (TileArgs::k in
 // pairs too).
 template <class T, bool A_ACROSS, bool B_ACROSS, class S, bool LAYER, bool WHOLE, Eight EIGHT = kNoSide>
 __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, int64_t blocks, char *stage0, char *stage1, char *stage2, char *stage3,
@@ -532,8 +546,8 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
     auto wide = [&](int u) -> char * { return u == 0 ? wide0 : (u == 1 ? wide1 : (u == 2 ? wide2 : wide3)); };
     using Scales = ScaleFeed<EIGHT == kBothSides ? S::XA : 0, S::XB, kScales ? S::kThreads : S::XA + S::XB, EIGHT == kBothSides && K == 64 ? 4 : 2>;
-    auto multiply = [&](int u, int tile) {
-        const char *la = kWideA ? wide(u) : stage(u), *lb = kWideA ? stage(u) : la + PLANES * kBytesA;
+    auto multiply_steps = [&](int u, int tile, int first, int last) {
+        const char *la = EIGHT == kSideA ? wide(tile & 1) : (kWideA ? wide(u) : stage(u)), *lb = kWideA ? stage(u) : la + PLANES * kBytesA;
         if constexpr (EIGHT == kSideB) {
             // (32 terms at a time: a lane's sixteen of side b are half a block, which one scale widens; side a's are read to match)
             int sb[FB];
@@ -600,7 +614,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             return;
         }
 #pragma unroll
-        for (int u = 0; u < K / 16 / SHARE; ++u) {
+        for (int u = first; u < last; ++u) {
             const int step = part * (K / 16 / SHARE) + u;
             s16x8 a[FA][PLANES], b[FB][PLANES];
 #pragma unroll
@@ -624,6 +638,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                 }
         }
     };
+    auto multiply = [&](int u, int tile) { multiply_steps(u, tile, 0, K / 16 / SHARE); };
     if constexpr (kFloat) {
         typename A::template FloatFeed<WHOLE> feed_a;
         typename B::template FloatFeed<WHOLE> feed_b;
@@ -655,45 +670,55 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
         constexpr int kOut = (STAGES > 2 ? B::kRounds : 0) + 2 * A::kRounds;
         typename A::template ByteFeed<E> bytes;
         typename B::template Feed<E> feed;
-        bytes.start(t.a8, t.a.extent, n0, k0), feed.start(t.b, m0, k0);
-        int64_t left8 = left;
-        auto fetch = [&](int set) { bytes.fetch(set, left8), left8 -= K; };
-        auto load = [&](char *lds) { feed.load(left, lds), left -= K; };
+        bytes.start(t.a8, t.a.extent, n0, k0, k1 - k0, tiles), feed.start(t.b, m0, k0);
+        auto fetch = [&](int set) { bytes.fetch(set); };
+        auto load = [&](char *lds, auto whole) {
+            if constexpr (decltype(whole)::value) feed.load_whole(lds);
+            else feed.load(left, lds);
+            left -= K;
+        };
         fetch(0);
         __builtin_amdgcn_sched_barrier(0);
         fetch(1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < STAGES - 1; ++u) load(stage(u));
+        for (int u = 0; u < STAGES - 1; ++u) load(stage(u), std::false_type{});
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
         bytes.put(0, wide0);
         __builtin_amdgcn_sched_barrier(0);
         fetch(0);
         __builtin_amdgcn_sched_barrier(0);
-        auto in_order = [] {  // (what is still in flight is counted: no load moves in front of one that is written before it)
+        auto in_order = [] {  // (what is still in flight is counted: no load moves in front of one that is written before it; all else may)
             asm volatile("" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0x38F);
         };
-        auto turn = [&](int u, int set) {
+        // (the next tile is widened between the products, which it hides behind: in front of them it would keep the matrix cores waiting)
+        auto turn = [&](int u, int set, auto whole) {
+            __builtin_amdgcn_sched_barrier(0);
             stage_ready<kOut>();
-            load(stage((u + STAGES - 1) % STAGES));
+            __builtin_amdgcn_sched_barrier(0);
+            load(stage((u + STAGES - 1) % STAGES), whole);
             in_order();
-            bytes.put(1 - set, wide((u + 1) % STAGES));
+            multiply_steps(u, set, 0, K / 32);
+            bytes.put(1 - set, wide(1 - set));
             in_order();
             fetch(1 - set);
             in_order();
-            multiply(u, 0);
+            multiply_steps(u, set, K / 32, K / 16);
         };
         constexpr int kTurns = STAGES % 2 ? 2 * STAGES : STAGES;
         int at = 0;
+        for (const int whole = (int)((k1 - k0) / K); at + kTurns + STAGES - 1 <= whole; at += kTurns)  // (what is requested here are whole tiles)
+#pragma unroll
+            for (int u = 0; u < kTurns; ++u) turn(u % STAGES, u & 1, std::true_type{});
         for (; at + kTurns <= tiles; at += kTurns)
 #pragma unroll
-            for (int u = 0; u < kTurns; ++u) turn(u % STAGES, u & 1);
+            for (int u = 0; u < kTurns; ++u) turn(u % STAGES, u & 1, std::false_type{});
 #pragma unroll
         for (int u = 0; u < kTurns - 1; ++u) {
             if (at + u >= tiles) break;
-            turn(u % STAGES, u & 1);
+            turn(u % STAGES, u & 1, std::false_type{});
         }
     } else {
         typename A::template Feed<E> feed_a;
@@ -704,29 +729,38 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
         if constexpr (kScales) scales.start(t.a8, t.a.extent, n0, t.b8, t.b.extent, m0);
         int64_t left8 = t.k8;  // (side b in 8 bits: pairs of terms, of which zeros behind the row's end are some)
         int loaded = 0;
-        auto load = [&](int u) {
-            char *lds = stage(u);
-            if constexpr (EIGHT == kNoSideApart) feed_a.load(left, wide(u)), feed_b.load(left, lds);
-            else feed_a.load(left, lds), feed_b.load(EIGHT == kSideB ? left8 : left, lds + kBytesA);
-            if constexpr (kScales) scales.load(loaded, left > 0, lds + kBytesA + kBytesB), ++loaded, left8 -= K / 2;
+        auto load = [&](int u, auto whole) {
+            char *to_a = EIGHT == kNoSideApart ? wide(u) : stage(u), *to_b = EIGHT == kNoSideApart ? stage(u) : stage(u) + kBytesA;
+            if constexpr (decltype(whole)::value) feed_a.load_whole(to_a), feed_b.load_whole(to_b);
+            else feed_a.load(left, to_a), feed_b.load(EIGHT == kSideB ? left8 : left, to_b);
+            if constexpr (kScales) scales.load(loaded, loaded < tiles, stage(u) + kBytesA + kBytesB);
+            if constexpr (EIGHT != kNoSide) ++loaded, left8 -= K / 2;
             left -= K;
         };
         // (tiles behind the end are requested too, as zeros: the number of loads in flight is then always the same)
 #pragma unroll
-        for (int u = 0; u < STAGES - 1; ++u) load(u);
+        for (int u = 0; u < STAGES - 1; ++u) load(u, std::false_type{});
         int at = 0;
+        if constexpr (EIGHT != kNoSide)
+            for (const int whole = (int)((k1 - k0) / K); at + 2 * STAGES - 1 <= whole; at += STAGES)  // (what is requested here are whole tiles)
+#pragma unroll
+                for (int u = 0; u < STAGES; ++u) {
+                    stage_ready<kLoads * (STAGES - 2)>();
+                    load((u + STAGES - 1) % STAGES, std::true_type{});
+                    multiply(u, at + u);
+                }
         for (; at + STAGES <= tiles; at += STAGES)
 #pragma unroll
             for (int u = 0; u < STAGES; ++u) {
                 stage_ready<kLoads * (STAGES - 2)>();
-                load((u + STAGES - 1) % STAGES);
+                load((u + STAGES - 1) % STAGES, std::false_type{});
                 multiply(u, at + u);
             }
 #pragma unroll
         for (int u = 0; u < STAGES - 1; ++u) {
             if (at + u >= tiles) break;
             stage_ready<kLoads * (STAGES - 2)>();
-            load((u + STAGES - 1) % STAGES);
+            load((u + STAGES - 1) % STAGES, std::false_type{});
             multiply(u, at + u);
         }
     }
@@ -734,11 +768,12 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     // No load may still be on its way to LDS: the sums go there next, a strip of 32 rows by 64 (or 32) of the wave's columns at a time, so that they
     // come back row by row and memory is written (and a residual read) in whole lines.  Quads are permuted within a row as chunks are above.  A
     // strip's residuals are requested all at once and ahead of everything else that is done with it.
-    constexpr int kGroup = FA < 2 ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16;
+    constexpr bool kRoom = EIGHT != kSideA || WA * WB <= STAGES * (kBytesB / 8192) + 2 * (kBytesA / 8192);  // for strips of 64 columns
+    constexpr int kGroup = FA < 2 || !kRoom ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16;
     constexpr int kPerStage = (kWideA ? kBytesB : kStage) / kStrip, kPerWide = kBytesA / kStrip;
     constexpr int kApart = 64 / kQuads, kRows = 4 / SHARE, kTurns = 32 / (kApart * kRows * SHARE);  // rows a read covers, reads a turn, turns of a wave in a strip
     constexpr int kStrips = FA / kGroup * FB;
-    static_assert(FA % kGroup == 0 && kPerStage >= 1 && WA * WB <= STAGES * (kPerStage + (kWideA ? kPerWide : 0)), "a strip for every wave");
+    static_assert(FA % kGroup == 0 && kPerStage >= 1 && WA * WB <= STAGES * kPerStage + (EIGHT == kSideA ? 2 : (kWideA ? STAGES : 0)) * kPerWide, "a strip for every wave");
     static_assert(SHARE == 1 || (kStrips == 1 && kPerStage >= SHARE * WA * WB), "waves that share a strip");
     const int quad = lane % kQuads, row0 = lane / kQuads + part * kTurns * kApart * kRows;
     const bool ahead = LAYER && t.e.residual && t.e.cols % 4 == 0;

@@ -21,7 +21,8 @@ struct NormArgs {
     void *h;
     int64_t h_stride;
     float *rstd;
-    int lanes;  // of a row
+    uint32_t *rest;  // [rows][ceil(cols / 8)], or NULL
+    int lanes;       // of a row
 };
 
 template <class T>
@@ -162,6 +163,8 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             if (a.h && there) store8(static_cast<T *>(a.h) + row * a.h_stride + column(c), h[c], FULL && valid(c) > 0 ? 8 : valid(c));
+            if constexpr (sizeof(T) == 2)
+                if (a.rest && there && valid(c) > 0) a.rest[row * ((a.cols + 7) / 8) + column(c) / 8] = rest_of<T>(h[c]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fma((double)h[c][e], (double)h[c][e], sum);
         }
@@ -220,6 +223,8 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormArgs a)
             float h[8];
             const int valid = load(row, col, h);
             if (a.h) store8(static_cast<T *>(a.h) + row * a.h_stride + col, h, valid);
+            if constexpr (sizeof(T) == 2)
+                if (a.rest && valid > 0) a.rest[row * ((a.cols + 7) / 8) + col / 8] = rest_of<T>(h);
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] *= r;
             if (a.weight) {
@@ -268,7 +273,7 @@ using namespace kge;
 extern "C" {
 
 int kge_rms_norm_fwd(const kge_rms_norm *norm, void *y, int64_t y_stride, const kge_rows8 *y8, void *h, int64_t h_stride, float *rstd,
-                     void *stream)
+                     void *rest, void *stream)
 {
     if (const int rc = check_norm(norm)) return rc;
     if (norm->x_stride < norm->cols || (norm->residual && norm->residual_stride < norm->cols) || (h && h_stride < norm->cols)) return KGE_ESHAPE;
@@ -279,9 +284,9 @@ int kge_rms_norm_fwd(const kge_rms_norm *norm, void *y, int64_t y_stride, const 
         return KGE_ESHAPE;
     }
     if (norm->rows == 0 || norm->cols == 0) return KGE_OK;
-    if (!norm->x || (!eight && !y)) return KGE_EINVAL;
+    if (!norm->x || (!eight && !y) || reinterpret_cast<uintptr_t>(rest) % 4 != 0) return KGE_EINVAL;
     const NormArgs a{norm->x, norm->residual, norm->weight, norm->x_stride, norm->residual_stride, norm->rows, norm->cols, norm->eps,
-                     y, y_stride, rows8_of(eight ? y8 : nullptr), h, h_stride, rstd, 0};
+                     y, y_stride, rows8_of(eight ? y8 : nullptr), h, h_stride, rstd, static_cast<uint32_t *>(rest), 0};
     hipStream_t st = as_stream(stream);
     KGE_CLEAR_LAUNCH_ERRORS();
     if (norm->type == KGE_F32) launch_norm<float>(a, norm->out_type, st);

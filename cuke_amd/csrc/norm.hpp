@@ -1,6 +1,8 @@
 // What the two passes of the root-mean-square norm share: how lanes hold a row, sums over them.
 #pragma once
 
+#include <type_traits>
+
 #include "rows8.hpp"
 
 namespace kge {
@@ -39,6 +41,37 @@ inline Hold hold_of(int64_t rows, int64_t cols, int64_t enough)
     while ((int64_t)lanes * pieces < need && lanes < 256) lanes *= 2;
     while ((int64_t)lanes * pieces < need) pieces *= 2;
     return Hold{pieces, lanes};
+}
+
+// What a sum loses when it is rounded to 16 bits, in sixteenths of a step of the result there, -8 .. 7: four bits an element, eight of a row in a word.  With it the
+// gradients are those of the sum itself, to 2^-13: from the rounded one alone dweight would be off by 1.4 times its own rounding, and dx of short rows,
+// where g - n mean(g n) cancels, by several times.
+template <class T>
+__device__ __forceinline__ int step_exponent(float h)  // of 1/16 of a step of T at h
+{
+    const int e = (int)(__float_as_uint(h) >> 23 & 0xFF), least = std::is_same<T, bf16_t>::value ? 1 : 113;
+    return (e > least ? e : least) - 127 - (std::is_same<T, bf16_t>::value ? 11 : 14);
+}
+template <class T>
+__device__ __forceinline__ uint32_t rest_of(const float (&sum)[8])
+{
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float h = (float)(T)sum[e];
+        const float q = rintf(__builtin_amdgcn_ldexpf(sum[e] - h, -step_exponent<T>(h)));  // (NaN of what is not finite: 0 below)
+        word |= ((uint32_t)(int)fminf(fmaxf(q, -8.0f), 7.0f) & 15u) << (4 * e);
+    }
+    return word;
+}
+template <class T>
+__device__ __forceinline__ void add_rest(float (&h)[8], uint32_t word)
+{
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int q = (int)(word << (28 - 4 * e)) >> 28;
+        h[e] += __builtin_amdgcn_ldexpf((float)q, step_exponent<T>(h[e]));
+    }
 }
 
 // calls f with (pieces, whether several waves hold a row) as compile-time values; not for pieces == 0

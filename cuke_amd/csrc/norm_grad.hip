@@ -11,6 +11,7 @@ struct NormGradArgs {
     const void *h, *dy, *dh, *weight;
     int64_t h_stride, dy_stride, dh_stride;
     const float *rstd;
+    const uint32_t *rest;  // or NULL
     int64_t rows, cols, quads, rows_each;
     void *dx;     // or NULL
     int64_t dx_stride;
@@ -34,7 +35,7 @@ struct Held {
 // A workgroup takes a range of rows, each held by `lanes` lanes (WAVES: by two or four waves); what the next row needs is requested while the present one is worked on.  A lane's
 // columns are the same in all rows, so dweight's sums wait in registers until the range's end.
 // Bound by memory: 65536 x 2048 bf16 with dh (1.07 GB) GRAD_US.
-template <class T, class D, int C, bool WAVES, bool DH>
+template <class T, class D, int C, bool WAVES, bool DH, bool REST>
 __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 {
     __shared__ float part[4];
@@ -52,7 +53,9 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
     float sum[C][8] = {};
     Held<T> h[C], dh[DH ? C : 1], w[C];
     Held<D> dy[C];
+    uint32_t rest[REST ? C : 1], rest_end[REST ? C : 1];
     float r;
+    const int words = (cols + 7) / 8;
     if (a.weight) {
 #pragma unroll
         for (int c = 0; c < C; ++c) w[c].fetch(a.weight, at[c]);
@@ -65,6 +68,10 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
             h[c].fetch(static_cast<const T *>(a.h) + row * a.h_stride, at[c]);
             dy[c].fetch(static_cast<const D *>(a.dy) + row * a.dy_stride, at[c]);
             if constexpr (DH) dh[c].fetch(static_cast<const T *>(a.dh) + row * a.dh_stride, at[c]);
+            if constexpr (REST) {  // (a piece that was moved back begins inside a word)
+                const uint32_t *p = a.rest + row * words;
+                rest[c] = p[at[c] >> 3], rest_end[c] = p[(at[c] + 7) >> 3];
+            }
         }
     };
     fetch(first + group);
@@ -77,6 +84,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             h[c].values(n[c]), dy[c].values(g[c]);
+            if constexpr (REST) add_rest<T>(n[c], __builtin_amdgcn_alignbit(rest_end[c], rest[c], 4 * (at[c] & 7)));
             if constexpr (DH) more[c] = dh[c];
             if (skip[c] > 0) {
 #pragma unroll
@@ -157,6 +165,8 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
         const int valid = (int)(left < 8 ? left : 8);
         load8(static_cast<const T *>(a.h) + row * a.h_stride + col, valid, n);
         load8(static_cast<const D *>(a.dy) + row * a.dy_stride + col, valid, g);
+        if constexpr (sizeof(T) == 2)
+            if (a.rest) add_rest<T>(n, a.rest[row * ((a.cols + 7) / 8) + col / 8]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) n[e] *= r;
         if (!a.weight) return valid;
@@ -200,6 +210,8 @@ __global__ __launch_bounds__(256) void rms_norm_long_sums_kernel(NormGradArgs a)
         float n[8], g[8];
         load8(static_cast<const T *>(a.h) + row * a.h_stride + col, valid, n);
         load8(static_cast<const D *>(a.dy) + row * a.dy_stride + col, valid, g);
+        if constexpr (sizeof(T) == 2)
+            if (a.rest) add_rest<T>(n, a.rest[row * ((a.cols + 7) / 8) + col / 8]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum[e] = fmaf(g[e], n[e] * r, sum[e]);
     }
@@ -249,8 +261,15 @@ static void launch_grads(const NormGradArgs &args, const Ranges &ranges, void *d
         if (a.dx) hipLaunchKernelGGL((rms_norm_grad_long_kernel<T, D>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), block, 0, st, a);
     } else {
         with_hold(hold, [&](auto pieces, auto waves) {
-            if (a.dh) hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, decltype(pieces)::value, decltype(waves)::value, true>), grid, block, 0, st, a);
-            else hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, decltype(pieces)::value, decltype(waves)::value, false>), grid, block, 0, st, a);
+            constexpr int kPieces = decltype(pieces)::value;
+            constexpr bool kWaves = decltype(waves)::value;
+            if constexpr (sizeof(T) == 2) {
+                if (a.rest && a.dh) hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, kPieces, kWaves, true, true>), grid, block, 0, st, a);
+                else if (a.rest) hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, kPieces, kWaves, false, true>), grid, block, 0, st, a);
+                if (a.rest) return;
+            }
+            if (a.dh) hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, kPieces, kWaves, true, false>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((rms_norm_grad_kernel<T, D, kPieces, kWaves, false, false>), grid, block, 0, st, a);
         });
     }
     if (a.sums) hipLaunchKernelGGL(norm_join_kernel<T>, dim3((unsigned)ceil_div(a.quads, 4)), block, 0, st, SumArgs{a.sums, ranges.count, a.cols, a.quads, dweight});
@@ -275,7 +294,7 @@ size_t kge_rms_norm_bwd_workspace(const kge_rms_norm *norm)
     return (size_t)ranges_of(norm->rows, norm->cols).count * ceil_div(norm->cols, 4) * 16;
 }
 
-int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, const float *rstd, int32_t dy_type, const void *dy,
+int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, const float *rstd, const void *rest, int32_t dy_type, const void *dy,
                      int64_t dy_stride, const void *dh, int64_t dh_stride, void *dx, int64_t dx_stride, void *dweight, void *workspace,
                      size_t workspace_bytes, void *stream)
 {
@@ -283,11 +302,11 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
     if (!known_type(dy_type)) return KGE_EINVAL;
     if (h_stride < norm->cols || dy_stride < norm->cols || (dh && dh_stride < norm->cols) || (dx && dx_stride < norm->cols)) return KGE_ESHAPE;
     if (norm->cols == 0 || (!dx && !dweight)) return KGE_OK;
-    if (norm->rows > 0 && (!h || !rstd || !dy)) return KGE_EINVAL;
+    if (norm->rows > 0 && (!h || !rstd || !dy || reinterpret_cast<uintptr_t>(rest) % 4 != 0)) return KGE_EINVAL;
     const size_t need = dweight ? kge_rms_norm_bwd_workspace(norm) : 0;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
     const Ranges ranges = norm->rows ? ranges_of(norm->rows, norm->cols) : Ranges{1, 0};
-    const NormGradArgs a{h, dy, dh, norm->weight, h_stride, dy_stride, dh_stride, rstd, norm->rows, norm->cols, ceil_div(norm->cols, 4), ranges.rows_each,
+    const NormGradArgs a{h, dy, dh, norm->weight, h_stride, dy_stride, dh_stride, rstd, static_cast<const uint32_t *>(rest), norm->rows, norm->cols, ceil_div(norm->cols, 4), ranges.rows_each,
                          dx, dx_stride, dweight ? static_cast<float *>(workspace) : nullptr, 0};
     hipStream_t st = as_stream(stream);
     KGE_CLEAR_LAUNCH_ERRORS();

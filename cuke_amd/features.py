@@ -481,6 +481,7 @@ class NormForward:
     h: torch.Tensor     # x + residual; x itself where there is none
     rstd: torch.Tensor  # float32 [rows]
     weight: torch.Tensor | None
+    rest: torch.Tensor | None = None  # int32 [rows, ceil(cols / 8)]: what h lost when it was rounded to 16 bits, in four bits an element
 
 
 @dataclass
@@ -492,8 +493,8 @@ class NormGrads:
 def _norm_call(x, weight, residual, eps, out_dtype, keep):
     got = _lib.host().rms_norm(x, weight, residual, eps, out_dtype, keep)
     if got is not None:
-        y, scale, h, rstd = got
-        return NormForward(y if scale is None else _made8(y, scale, x.shape[1]), x if h is None else h, rstd, weight)
+        y, scale, h, rstd, rest = got
+        return NormForward(y if scale is None else _made8(y, scale, x.shape[1]), x if h is None else h, rstd, weight, rest)
     x = _rows(x, "x")
     rows, cols = x.shape
     if weight is not None:
@@ -510,11 +511,12 @@ def _norm_call(x, weight, residual, eps, out_dtype, keep):
     y = _new_rows8(rows, cols, x.device) if eight else torch.empty((rows, cols), dtype=out_dtype, device=x.device)
     h = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if residual is not None else None
     rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if keep else None
+    rest = torch.empty((rows, -(-cols // 8)), dtype=torch.int32, device=x.device) if keep and h is not None and x.dtype != torch.float32 else None
     desc = _lib.RmsNorm(_TYPES[x.dtype], _lib.E4M3 if eight else _TYPES[out_dtype], rows, cols, _p(x), _row_stride(x), _p(residual),
                         _row_stride(residual) if residual is not None else 0, _p(weight), eps)
     _lib.check(_lib.lib().kge_rms_norm_fwd(C.byref(desc), None if eight else _p(y), cols, C.byref(_rows8_c(y)) if eight else None, _p(h), cols,
-                                           _p(rstd), _stream()), "kge_rms_norm_fwd")
-    return NormForward(y, x if h is None else h, rstd, weight)
+                                           _p(rstd), _p(rest), _stream()), "kge_rms_norm_fwd")
+    return NormForward(y, x if h is None else h, rstd, weight, rest)
 
 
 def rms_norm(x, weight=None, residual=None, *, eps=1e-6, out_dtype=None):
@@ -536,7 +538,7 @@ def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_we
     the residual is that of x.  An 8-bit y's rounding counts as none."""
     if not isinstance(fw, NormForward):
         raise TypeError("fw must come from rms_norm_forward()")
-    got = _lib.host().rms_norm_backward(fw.h, fw.rstd, fw.weight, dy, dh, need_x, need_weight)
+    got = _lib.host().rms_norm_backward(fw.h, fw.rstd, fw.rest, fw.weight, dy, dh, need_x, need_weight)
     if got is not None:
         return NormGrads(*got)
     h, weight = _tensor(fw.h, "h of the forward call", 2), fw.weight
@@ -550,7 +552,7 @@ def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_we
     L = _lib.lib()
     ws_bytes = int(L.kge_rms_norm_bwd_workspace(C.byref(desc))) if dw is not None else 0
     ws = _bytes(ws_bytes, h.device)
-    _lib.check(L.kge_rms_norm_bwd(C.byref(desc), _p(h), _row_stride(h), _p(fw.rstd), _TYPES[dy.dtype], _p(dy), _row_stride(dy), _p(dh),
+    _lib.check(L.kge_rms_norm_bwd(C.byref(desc), _p(h), _row_stride(h), _p(fw.rstd), _p(fw.rest), _TYPES[dy.dtype], _p(dy), _row_stride(dy), _p(dh),
                                   _row_stride(dh) if dh is not None else 0, _p(dx), cols, _p(dw), _p(ws), ws_bytes, _stream()), "kge_rms_norm_bwd")
     return NormGrads(dx, dw)
 

@@ -677,10 +677,11 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
  *   h = x + residual,   r[i] = (mean_j h[i][j]^2 + eps)^-1/2,   y[i][j] = h[i][j] r[i] weight[j]            (residual, weight NULL: 0, 1)
  * x, residual, weight and h have the type `type`; y any kge_type_t, or KGE_E4M3: rows in 8 bits (`y8`; else y, y_stride).  h (NULL: not wanted) is the sum
  * rounded to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32.  Squares are summed in 64 bits, so that no value of a type
- * overflows; a value in 8 bits is the one nearest to the 64-bit result.
+ * overflows; a value in 8 bits is the one nearest to the 64-bit result.  rest (NULL: not wanted; KGE_F32: not looked at): 4 ceil(cols / 8) bytes a row, 4-byte
+ * aligned, what rounding took from h, in 16ths of a step of `type`: four bits an element.
  * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
  *   g = dy weight,   dx = dresidual = r (g - h r^2 mean_j(g h)) + dh,   dweight[j] = sum_i dy[i][j] h[i][j] r[i]
- * h: what the forward call wrote there (x where there was no residual), rstd too.  dx [rows, cols] and dweight [cols] of type `type`, contiguous but for
+ * h: what the forward call wrote there (x where there was no residual), rstd and rest too (NULL: the gradients are those of h as it was rounded).  dx [rows, cols] and dweight [cols] of type `type`, contiguous but for
  * dx's stride; either may be NULL.  dx may be dy or dh where type and stride are the same.  The fields x and residual of the description are not looked at.  Sums over rows are joined
  * in a fixed order.  rows, cols: 0 .. 2^31 - 1 (KGE_ESHAPE beyond).
  */
@@ -695,9 +696,9 @@ typedef struct kge_rms_norm {
     double eps; /* >= 0 */
 } kge_rms_norm;
 int kge_rms_norm_fwd(const kge_rms_norm *norm, void *y, int64_t y_stride, const kge_rows8 *y8, void *h, int64_t h_stride, float *rstd,
-                     void *stream);
+                     void *rest, void *stream);
 size_t kge_rms_norm_bwd_workspace(const kge_rms_norm *norm);
-int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, const float *rstd, int32_t dy_type, const void *dy,
+int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, const float *rstd, const void *rest, int32_t dy_type, const void *dy,
                      int64_t dy_stride, const void *dh, int64_t dh_stride, void *dx, int64_t dx_stride, void *dweight, void *workspace,
                      size_t workspace_bytes, void *stream);
 

@@ -4,7 +4,8 @@ What is in 8 bits has to be equal: a power of two and the e4m3 number nearest to
 element, from the roundings a result goes through (u: half a step of a type, eps = 2^-24):
   y      h = x + residual eps, r eps (from 64 bits), two products eps each: 4 eps |y|, doubled, and u |y|
   h      u |h| + eps |h|
-  dx     a sum of K products in fp32 in any order: (K + 8) eps sum |g n|; its share of the row, and 8 eps of every other term; then u |dx|
+  dx     a sum of K products in fp32 in any order: (K + 8) eps sum |g n|; its share of the row, and 8 eps of every other term; h of 16 bits with a residual is the
+         sum to a 16th of a step; then u |dx|
   dweight  (M + 8) eps sum |dy n| and u |dweight|
 """
 import ctypes as C
@@ -186,18 +187,21 @@ class Norm:
 
     def check_backward(self, fw, grads, what):
         M, K = self.h.shape
-        n = fw.h.double() * self.r                       # (h as it was kept)
+        n = self.h * self.r                              # (of the sum itself: what h's rounding dropped is kept to a 32nd of a step, a 16th where it is a half)
         dy = self.dy.double()
         g = dy * self.w64
         mean = (g * n).mean(1, keepdim=True)
         dx = self.r * (g - n * mean)
+        # h's own error: of 16-bit sums a 16th of a step (2 u |h|, or 2 TINY where the type's numbers are evenly spaced), else its rounding to 32 bits
+        off = EPS * n.abs() + ((2 * U[self.dtype] * n.abs() + 2 * TINY[self.dtype] * self.r) / 16 if self.res is not None and self.dtype != torch.float32 else 0.0)
         tol = self.r * (8 * EPS * (g.abs() + (n * mean).abs()) + n.abs() * (K + 8) * EPS * (g * n).abs().mean(1, keepdim=True))
+        tol = tol + self.r * (off * mean.abs() + (n.abs() + off) * (g.abs() * off).mean(1, keepdim=True))
         if self.dh is not None:
             dx = dx + self.dh.double()
             tol = tol + 2 * EPS * self.dh.double().abs()
         within(grads.x, dx, tol + U[self.dtype] * (dx.abs() + tol) + TINY[self.dtype], (what, "dx"))
         if self.w is not None:
-            dw, tol = (dy * n).sum(0), (M + 8) * EPS * (dy * n).abs().sum(0)
+            dw, tol = (dy * n).sum(0), (M + 8) * EPS * (dy * n).abs().sum(0) + (dy.abs() * off).sum(0)
             within(grads.weight, dw, tol + U[self.dtype] * (dw.abs() + tol) + TINY[self.dtype], (what, "dweight"))
         else:
             assert grads.weight is None
@@ -299,9 +303,34 @@ def test_norm_gradient_into_the_place_of_dy_or_dh():
         for place in ("dy", "dh"):
             t = {"dy": c.dy.clone(), "dh": c.dh.clone()}
             dw = torch.empty(cols, device=DEV)
-            rc = L.kge_rms_norm_bwd(C.byref(d), fw.h.data_ptr(), cols, fw.rstd.data_ptr(), 0, t["dy"].data_ptr(), cols, t["dh"].data_ptr(), cols,
+            rc = L.kge_rms_norm_bwd(C.byref(d), fw.h.data_ptr(), cols, fw.rstd.data_ptr(), None, 0, t["dy"].data_ptr(), cols, t["dh"].data_ptr(), cols,
                                     t[place].data_ptr(), cols, dw.data_ptr(), ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
             assert rc == 0 and torch.equal(t[place], want.x) and torch.equal(dw, want.weight), (cols, place)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+def test_what_a_sum_loses_is_kept(dtype):
+    """h and rest together are the sum to a 16th of a step, for all sizes of numbers; without rest the gradients are those of h."""
+    from cuke_amd import _lib, features
+    g = torch.Generator().manual_seed(4)
+    for cols in (1, 5, 8, 100, 9001):
+        size = torch.exp2(torch.randint(-30 if dtype == torch.float16 else -120, 12, (40, cols), generator=g).float())
+        x, res = (torch.randn((40, cols), generator=g) * size).to(DEV).to(dtype), (torch.randn((40, cols), generator=g) * size * 1.7).to(DEV).to(dtype)
+        fw = features.rms_norm_forward(x, None, res)
+        assert fw.rest.shape == (40, -(-cols // 8))
+        bits = (fw.rest.view(40, -1, 1) << torch.arange(28, -4, -4, device=DEV, dtype=torch.int32)) >> 28
+        bits = bits.view(40, -1)[:, :cols].double()
+        step = torch.exp2(torch.floor(torch.log2(fw.h.double().abs().clamp(min=2.0 ** -140)))) * 2 * U[dtype] * (1 if dtype == torch.float16 else 1)
+        if dtype == torch.float16:
+            step = step.clamp(min=2.0 ** -24)
+        want = x.double() + res.double()
+        assert bool(((fw.h.double() + bits * step / 16 - want).abs() <= step / 16 * 1.001 + EPS * want.abs() + 2.0 ** -130).all()), (dtype, cols)
+    c = Norm(33, 70, dtype)
+    fw = c.forward()
+    fw.rest = None
+    got = features.rms_norm_backward(fw, c.dy, c.dh)
+    c.h, c.res = fw.h.double(), None                             # (r stays that of the sum)
+    c.check_backward(fw, got, "rounded")
 
 
 def test_norm_refuses():

@@ -67,7 +67,7 @@ def test_rows_in_8_bits_are_checked(bad, rc):
     r, n = rows8(**bad), norm(out=3)
     assert L.kge_pack8(0, FAKE, 40, 4, 40, C.byref(r), None) == rc
     assert L.kge_unpack8(C.byref(r), 4, 40, 0, FAKE, 40, None) == rc
-    assert L.kge_rms_norm_fwd(C.byref(n), None, 0, C.byref(r), None, 0, None, None) == rc
+    assert L.kge_rms_norm_fwd(C.byref(n), None, 0, C.byref(r), None, 0, None, None, None) == rc
 
 
 @pytest.mark.parametrize("args,rc", [
@@ -88,26 +88,26 @@ def test_pack_refusals(args, rc):
 def test_norm_refusals(bad, rc):
     _, L = lib()
     d = norm(**bad)
-    assert L.kge_rms_norm_fwd(C.byref(d), FAKE, 1 << 31, None, None, 0, None, None) == rc
+    assert L.kge_rms_norm_fwd(C.byref(d), FAKE, 1 << 31, None, None, 0, None, None, None) == rc
 
 
 def test_norm_outputs_and_workspaces_are_checked():
     _, L = lib()
     d = norm()
-    fwd = lambda **k: L.kge_rms_norm_fwd(C.byref(k.get("d", d)), k.get("y", FAKE), k.get("ys", 40), None, k.get("h"), k.get("hs", 0), None, None)
-    assert L.kge_rms_norm_fwd(None, FAKE, 40, None, None, 0, None, None) == EINVAL
-    assert fwd(y=None) == EINVAL and fwd(ys=39) == ESHAPE and fwd(h=FAKE, hs=39) == ESHAPE
-    assert L.kge_rms_norm_fwd(C.byref(norm(out=3)), FAKE, 40, None, None, 0, None, None) == EINVAL        # no y8
+    fwd = lambda **k: L.kge_rms_norm_fwd(C.byref(k.get("d", d)), k.get("y", FAKE), k.get("ys", 40), None, k.get("h"), k.get("hs", 0), None, k.get("rest"), None)
+    assert L.kge_rms_norm_fwd(None, FAKE, 40, None, None, 0, None, None, None) == EINVAL
+    assert fwd(y=None) == EINVAL and fwd(rest=FAKE + 2) == EINVAL and fwd(ys=39) == ESHAPE and fwd(h=FAKE, hs=39) == ESHAPE
+    assert L.kge_rms_norm_fwd(C.byref(norm(out=3)), FAKE, 40, None, None, 0, None, None, None) == EINVAL        # no y8
     assert fwd(d=norm(rows=0, x=None), y=None) == 0 and fwd(d=norm(cols=0, x=None), y=None) == 0
     need = L.kge_rms_norm_bwd_workspace(C.byref(d))
     assert need >= 40 * 4 and L.kge_rms_norm_bwd_workspace(None) == 0 and L.kge_rms_norm_bwd_workspace(C.byref(norm(type=9))) == 0
-    ok = dict(h=FAKE, hs=40, rstd=FAKE, t=1, dy=FAKE, dys=40, dh=None, dhs=0, dx=FAKE, dxs=40, dw=FAKE, ws=FAKE, n=need)
+    ok = dict(h=FAKE, hs=40, rstd=FAKE, rest=None, t=1, dy=FAKE, dys=40, dh=None, dhs=0, dx=FAKE, dxs=40, dw=FAKE, ws=FAKE, n=need)
 
     def bwd(d=d, **k):
         a = dict(ok, **k)
-        return L.kge_rms_norm_bwd(C.byref(d), a["h"], a["hs"], a["rstd"], a["t"], a["dy"], a["dys"], a["dh"], a["dhs"], a["dx"], a["dxs"], a["dw"],
+        return L.kge_rms_norm_bwd(C.byref(d), a["h"], a["hs"], a["rstd"], a["rest"], a["t"], a["dy"], a["dys"], a["dh"], a["dhs"], a["dx"], a["dxs"], a["dw"],
                                   a["ws"], a["n"], None)
-    assert bwd(t=3) == EINVAL and bwd(h=None) == EINVAL and bwd(rstd=None) == EINVAL and bwd(dy=None) == EINVAL
+    assert bwd(t=3) == EINVAL and bwd(rest=FAKE + 1) == EINVAL and bwd(h=None) == EINVAL and bwd(rstd=None) == EINVAL and bwd(dy=None) == EINVAL
     assert bwd(hs=39) == ESHAPE and bwd(dys=39) == ESHAPE and bwd(dh=FAKE, dhs=39) == ESHAPE and bwd(dxs=39) == ESHAPE
     assert bwd(n=need - 1) == EWORKSPACE and bwd(ws=None) == EWORKSPACE and bwd(ws=FAKE + 8) == EWORKSPACE
     assert bwd(dx=None, dw=None, ws=None, n=0) == 0 and bwd(d=norm(cols=0), ws=None, n=0) == 0
