@@ -5,68 +5,109 @@
 namespace kge {
 
 // ---- few rows --------------------------------------------------------------------------------------
-// As linear_few_kernel, with rows in 8 bits (and the weight too: W8) widened on their way to the matrix cores: a step's 32 terms are a block, so that a lane's eight
-// numbers have one scale.
+// As linear_few_kernel, with rows in 8 bits (and the weight too: W8) widened on their way to the matrix cores.  A wave takes every eighth group of four blocks, a quarter of
+// its lanes a block each: 32 numbers in two loads and one scale.  (A step multiplies eight terms of each of the four: which terms meet in it does not matter.)
 template <class T>
 struct Line8 {
-    const uint8_t *q, *scale;
-    struct Raw {
-        u2 v;
+    const uint8_t *q, *scale;  // of the lane's block in the first group
+    struct Group {
+        uint4 lo, hi;
         int byte;
-        __device__ __forceinline__ typename Few<T>::piece widened() const { return widen(make_uint2(v[0], v[1]), __int_as_float(byte << 23), T{}); }
+        __device__ __forceinline__ typename Few<T>::piece widened(int step) const
+        {
+            const uint4 v = step < 2 ? lo : hi;
+            return widen(step & 1 ? make_uint2(v.z, v.w) : make_uint2(v.x, v.y), __int_as_float(byte << 23), T{});
+        }
     };
-    __device__ __forceinline__ Line8(const Rows8 &s, int64_t row, int k0) : q(s.q + row * s.q_stride + k0), scale(s.scale + row * s.scale_stride) {}
-    __device__ __forceinline__ Raw load(int64_t block) const { return Raw{*reinterpret_cast<const u2 *>(q + 32 * block), scale[block]}; }
+    __device__ __forceinline__ Line8(const Rows8 &s, int64_t row, int quarter) : q(s.q + row * s.q_stride + 32 * quarter), scale(s.scale + row * s.scale_stride + quarter) {}
+    __device__ __forceinline__ Group load(int64_t group) const
+    {
+        const uint4 *p = reinterpret_cast<const uint4 *>(q + 128 * group);
+        return Group{p[0], p[1], scale[4 * group]};
+    }
+};
+// 32 terms of a 16-bit weight's row
+template <class T>
+struct Line16 {
+    typedef typename Few<T>::piece piece;
+    const T *p;
+    struct Group {
+        piece v[4];
+        __device__ __forceinline__ piece widened(int step) const { return v[step]; }
+    };
+    __device__ __forceinline__ Line16(const Side &s, int64_t row, int quarter) : p(static_cast<const T *>(s.p) + row * s.stride + 32 * quarter) {}
+    __device__ __forceinline__ Group load(int64_t group) const
+    {
+        Group g;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) g.v[u] = Few<T>::load(p + 128 * group + 8 * u);
+        return g;
+    }
+    __device__ __forceinline__ Group load(int64_t group, int64_t left) const  // `left` terms of the 32 exist
+    {
+        Group g;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int64_t rest = left - 8 * u;
+            g.v[u] = Few<T>::load(p + 128 * group + 8 * u, rest < 0 ? 0 : (int)(rest < 8 ? rest : 8));
+        }
+        return g;
+    }
 };
 
 template <class T, int MF, bool W8>
 __global__ __launch_bounds__(kFewWaves *kWave) void linear8_few_kernel(TileArgs t)
 {
     using F = Few<T>;
-    using Raw = typename Line8<T>::Raw;
-    static_assert(F::kTerms == 32 && F::kEach == 8, "a block a step");
-    constexpr int kAhead = 4;  // steps whose loads are in flight together
+    using Rows = Line8<T>;
+    using Weight = typename std::conditional<W8, Line8<T>, Line16<T>>::type;
+    static_assert(F::kTerms == 32 && F::kEach == 8, "a step");
+    constexpr int kAhead = 2;  // groups whose loads are in flight together
     __shared__ f4 sums[kFewWaves][MF][kWave];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, k0 = F::kEach * (lane >> 4);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), r = lane & 15, quarter = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16 * MF;
     const int64_t n = n0 + r < t.a.extent ? n0 + r : t.a.extent - 1;  // (rows that do not exist: others, whose sums nobody asks for)
-    const T *a = static_cast<const T *>(t.a.p) + (W8 ? 0 : n * t.a.stride + k0);
-    const Line8<T> a8(t.a8, W8 ? n : 0, k0);
+    auto weight = [&] {
+        if constexpr (W8) return Weight(t.a8, n, quarter);
+        else return Weight(t.a, n, quarter);
+    };
+    const Weight a = weight();
     auto row = [&](int j) { return m0 + 16 * j + r < t.b.extent ? m0 + 16 * j + r : t.b.extent - 1; };
-    const Line8<T> first(t.b8, row(0), k0), second(t.b8, row(MF - 1), k0);
+    const Rows first(t.b8, row(0), quarter), second(t.b8, row(MF - 1), quarter);
     f4 acc[MF] = {};
-    const int64_t blocks = (t.k + 31) / 32, full = W8 ? blocks : t.k / 32;  // (numbers behind a row's end are zero; a 16-bit weight's row ends where it ends)
-    int64_t s = wave;
-    for (; s + (kAhead - 1) * kFewWaves < full; s += kAhead * kFewWaves) {
-        typename F::piece x[W8 ? 1 : kAhead];
-        Raw x8[W8 ? kAhead : 1], y[kAhead][MF];
+    const int64_t blocks = (t.k + 31) / 32, full = t.k / 128;  // full: groups all of whose terms exist
+    auto multiply = [&](const typename Weight::Group &x, const typename Rows::Group (&y)[MF]) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int64_t at = s + u * kFewWaves;
-            if constexpr (W8) x8[u] = a8.load(at);
-            else x[u] = F::load(a + 32 * at);
+        for (int u = 0; u < 4; ++u) {
+            const typename F::piece p = x.widened(u);
 #pragma unroll
-            for (int j = 0; j < MF; ++j) y[u][j] = (j ? second : first).load(at);
+            for (int j = 0; j < MF; ++j) acc[j] = F::multiply(p, y[j].widened(u), acc[j]);
+        }
+    };
+    int64_t g = wave;
+    for (; g + (kAhead - 1) * kFewWaves < full; g += kAhead * kFewWaves) {
+        typename Weight::Group x[kAhead];
+        typename Rows::Group y[kAhead][MF];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            x[k] = a.load(g + k * kFewWaves);
+#pragma unroll
+            for (int j = 0; j < MF; ++j) y[k][j] = (j ? second : first).load(g + k * kFewWaves);
         }
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            typename F::piece p;
-            if constexpr (W8) p = x8[u].widened();
-            else p = x[u];
-#pragma unroll
-            for (int j = 0; j < MF; ++j) acc[j] = F::multiply(p, y[u][j].widened(), acc[j]);
-        }
+        for (int k = 0; k < kAhead; ++k) multiply(x[k], y[k]);
     }
-    for (; s < blocks; s += kFewWaves) {
-        typename F::piece p;
-        if constexpr (W8) {
-            p = a8.load(s).widened();
-        } else {
-            const int64_t left = t.k - 32 * s - k0;
-            p = F::load(a + 32 * s, left < 0 ? 0 : (int)(left < 8 ? left : 8));
-        }
+    for (; 4 * g < blocks; g += kFewWaves) {  // (numbers behind a row's end are zero, to the end of its last block; a 16-bit weight's row ends where it ends)
+        typename Weight::Group x{};
+        typename Rows::Group y[MF]{};
+        if (4 * g + quarter < blocks) {
+            if constexpr (W8) x = a.load(g);
+            else if (g < full) x = a.load(g);
+            else x = a.load(g, t.k - 128 * g - 32 * quarter);
 #pragma unroll
-        for (int j = 0; j < MF; ++j) acc[j] = F::multiply(p, (j ? second : first).load(s).widened(), acc[j]);
+            for (int j = 0; j < MF; ++j) y[j] = (j ? second : first).load(g);
+        }
+        multiply(x, y);
     }
 #pragma unroll
     for (int j = 0; j < MF; ++j) sums[wave][j][lane] = acc[j];

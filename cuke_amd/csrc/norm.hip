@@ -14,7 +14,7 @@ struct NormArgs {
     const void *x, *residual, *weight;
     int64_t x_stride, residual_stride;
     int64_t rows, cols;
-    double eps;
+    double eps, share;  // share: 1 / cols
     void *y;
     int64_t y_stride;
     Rows8 y8;
@@ -32,11 +32,18 @@ __device__ __forceinline__ double sum_at(const NormArgs &a, int64_t row, int64_t
     if (a.residual) h += (double)(float)static_cast<const T *>(a.residual)[row * a.residual_stride + col];
     return h;
 }
-// an element of the result in 64 bits, from memory
-template <class T>
-__device__ __forceinline__ double result_at(const NormArgs &a, int64_t row, int64_t col, double r)
+// r of a row, to half a unit of its last place and 2^-40: the instruction's 2^-23 and a step of Newton's method
+__device__ __forceinline__ float root(const NormArgs &a, double sum)
 {
-    const double y = sum_at<T>(a, row, col) * r;
+    const double m = fma(sum, a.share, a.eps), r = __builtin_amdgcn_rsq(m);
+    const double better = r * fma(-0.5 * m * r, r, 1.5);
+    return (float)(r > 0.0 && r < 1e300 ? better : r);  // (of 0 and infinity the step would make NaN)
+}
+// an element of the result in 64 bits, from memory and the row's sum of squares
+template <class T>
+__device__ __forceinline__ double result_at(const NormArgs &a, int64_t row, int64_t col, double sum)
+{
+    const double y = sum_at<T>(a, row, col) * (1.0 / sqrt(sum / (double)a.cols + a.eps));
     return a.weight ? y * (double)(float)static_cast<const T *>(a.weight)[col] : y;
 }
 // to 32 bits towards zero, the last bit set where that was not exact: what is rounded further from there lands where the 64-bit value does
@@ -49,25 +56,25 @@ __device__ __forceinline__ float to_odd(double d)
     return __uint_as_float(b | 1u);
 }
 template <class T>
-__device__ __forceinline__ float top_in_64(const NormArgs &a, int64_t row, int64_t col, double r)
+__device__ __forceinline__ float top_in_64(const NormArgs &a, int64_t row, int64_t col, double sum)
 {
     float top = 0.0f;
 #pragma unroll 1
     for (int e = 0; e < 8 && col + e < a.cols; ++e) {
-        const float v = fabsf(to_odd(result_at<T>(a, row, col + e, r)));
+        const float v = fabsf(to_odd(result_at<T>(a, row, col + e, sum)));
         top = fmaxf(top, finite(v) ? v : 0.0f);
     }
     return top;
 }
 // the bytes of q that differ from `other` formed again
 template <class T>
-__device__ __forceinline__ uint2 settle(const NormArgs &a, int64_t row, int64_t col, double r, float inverse, uint2 q, uint2 other)
+__device__ __forceinline__ uint2 settle(const NormArgs &a, int64_t row, int64_t col, double sum, float inverse, uint2 q, uint2 other)
 {
 #pragma unroll 1
     for (int e = 0; e < 8 && col + e < a.cols; ++e) {
         const uint32_t mask = 0xFFu << (8 * (e & 3)), differ = e < 4 ? q.x ^ other.x : q.y ^ other.y;
         if (!(differ & mask)) continue;
-        const float v = to_odd(result_at<T>(a, row, col + e, r) * (double)inverse);
+        const float v = to_odd(result_at<T>(a, row, col + e, sum) * (double)inverse);
         const uint32_t byte = ((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xFFu) << (8 * (e & 3));
         if (e < 4) q.x = (q.x & ~mask) | byte;
         else q.y = (q.y & ~mask) | byte;
@@ -75,24 +82,24 @@ __device__ __forceinline__ uint2 settle(const NormArgs &a, int64_t row, int64_t 
     return q;
 }
 
-// Eight consecutive results (fp32, each within 4 units of its last place; zero behind the row's end) to 8 bits; the lanes of a block come together.  A value that another
+// Eight consecutive results (fp32, each within 6 units of its last place; zero behind the row's end) to 8 bits; the lanes of a block come together.  A value that another
 // rounding of fp32 would put on the other side of a border of e4m3, one in 40000, is formed again in 64 bits, and so is a block's largest value at the border
 // of two powers: to see that, every value is rounded twice, 16 units apart.
 constexpr float kUp = 1.0f + 0x1p-20f, kDown = 1.0f - 0x1p-20f;
 template <class T>
-__device__ __forceinline__ void store_e4m3(const NormArgs &a, int64_t row, int64_t col, double r, const float (&y)[8], bool there)
+__device__ __forceinline__ void store_e4m3(const NormArgs &a, int64_t row, int64_t col, double sum, const float (&y)[8], bool there)
 {
     const int64_t width = (a.cols + 31) / 32 * 32;
     const float top = quad_max(top_of(y));
     int byte = scale_byte(top * kDown);
-    if (byte != scale_byte(top * kUp)) byte = scale_byte(quad_max(top_in_64<T>(a, row, col, r)));
+    if (byte != scale_byte(top * kUp)) byte = scale_byte(quad_max(top_in_64<T>(a, row, col, sum)));
     const float inverse = scale_inverse(byte), down = inverse * kDown, up = inverse * kUp;
     float low[8], high[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) low[e] = y[e] * down, high[e] = y[e] * up;
     uint2 q = to_e4m3(low);
     const uint2 other = to_e4m3(high);
-    if (q.x != other.x || q.y != other.y) q = settle<T>(a, row, col, r, inverse, q, other);
+    if (q.x != other.x || q.y != other.y) q = settle<T>(a, row, col, sum, inverse, q, other);
     if (there && col < width) {
         *reinterpret_cast<uint2 *>(a.y8.q + row * a.y8.q_stride + col) = q;
         if ((col & 31) == 0) a.y8.scale[row * a.y8.scale_stride + col / 32] = (uint8_t)byte;
@@ -110,7 +117,8 @@ __device__ __forceinline__ void finish_scales(const NormArgs &a, int64_t row, in
 template <class T, class O, int C, bool WAVES, bool FULL>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 {
-    __shared__ double part[4];
+    __shared__ double part[2][4];
+    int turn = 0;
     const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
     auto column = [&](int c) { return 8 * (c * lanes + lane); };
     auto valid = [&](int c) { return (int)a.cols - column(c); };
@@ -168,9 +176,8 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fma((double)h[c][e], (double)h[c][e], sum);
         }
-        sum = WAVES ? waves_sum(sum, lanes, part) : lanes_sum(sum, lanes);
-        const double r64 = 1.0 / sqrt(sum / (double)a.cols + a.eps);
-        const float r = (float)r64;
+        sum = WAVES ? waves_sum(sum, lanes, part, turn++) : lanes_sum(sum, lanes);
+        const float r = root(a, sum);
         if (a.rstd && there && lane == 0) a.rstd[row] = r;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
@@ -182,7 +189,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[c][e] *= w[e];
             }
-            if constexpr (std::is_same<O, e4m3_t>::value) store_e4m3<T>(a, row, column(c), r64, h[c], there);
+            if constexpr (std::is_same<O, e4m3_t>::value) store_e4m3<T>(a, row, column(c), sum, h[c], there);
             else if (there) store8(static_cast<O *>(a.y) + row * a.y_stride + column(c), h[c], FULL && valid(c) > 0 ? 8 : valid(c));
         }
         if constexpr (std::is_same<O, e4m3_t>::value)
@@ -194,7 +201,8 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 template <class T, class O>
 __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormArgs a)
 {
-    __shared__ double part[4];
+    __shared__ double part[2][4];
+    int turn = 0;
     auto load = [&](int64_t row, int64_t col, float(&h)[8]) {
         const int64_t left = a.cols - col;
         const int valid = (int)(left < 8 ? left : 8);
@@ -214,9 +222,8 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormArgs a)
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum = fma((double)h[e], (double)h[e], sum);
         }
-        sum = waves_sum(sum, 256, part);
-        const double r64 = 1.0 / sqrt(sum / (double)a.cols + a.eps);
-        const float r = (float)r64;
+        sum = waves_sum(sum, 256, part, turn++);
+        const float r = root(a, sum);
         if (a.rstd && threadIdx.x == 0) a.rstd[row] = r;
         for (int64_t col0 = 0; col0 < a.cols; col0 += 8 * 256) {  // (all lanes come along)
             const int64_t col = col0 + 8 * threadIdx.x;
@@ -233,7 +240,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormArgs a)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[e] *= w[e];
             }
-            if constexpr (std::is_same<O, e4m3_t>::value) store_e4m3<T>(a, row, col, r64, h, true);
+            if constexpr (std::is_same<O, e4m3_t>::value) store_e4m3<T>(a, row, col, sum, h, true);
             else store8(static_cast<O *>(a.y) + row * a.y_stride + col, h, valid);
         }
         if constexpr (std::is_same<O, e4m3_t>::value) finish_scales(a, row, threadIdx.x);
@@ -285,7 +292,7 @@ int kge_rms_norm_fwd(const kge_rms_norm *norm, void *y, int64_t y_stride, const 
     }
     if (norm->rows == 0 || norm->cols == 0) return KGE_OK;
     if (!norm->x || (!eight && !y) || reinterpret_cast<uintptr_t>(rest) % 4 != 0) return KGE_EINVAL;
-    const NormArgs a{norm->x, norm->residual, norm->weight, norm->x_stride, norm->residual_stride, norm->rows, norm->cols, norm->eps,
+    const NormArgs a{norm->x, norm->residual, norm->weight, norm->x_stride, norm->residual_stride, norm->rows, norm->cols, norm->eps, 1.0 / (double)norm->cols,
                      y, y_stride, rows8_of(eight ? y8 : nullptr), h, h_stride, rstd, static_cast<uint32_t *>(rest), 0};
     hipStream_t st = as_stream(stream);
     KGE_CLEAR_LAUNCH_ERRORS();

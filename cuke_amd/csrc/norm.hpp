@@ -7,23 +7,58 @@
 
 namespace kge {
 
-// sum over `lanes` neighbouring lanes (a power of two, 64 at most), the same in each of them
+// A value as another lane of a group of 2 * WIDTH has it, the sum so far being the same in WIDTH lanes (or as it is in them: the swaps give both halves).
+__device__ __forceinline__ float other_half(float v, int width)
+{
+    const int b = __float_as_int(v);
+    if (width == 1) return __int_as_float(dpp<0xB1>(b));    // quad_perm 1 0 3 2
+    if (width == 2) return __int_as_float(dpp<0x4E>(b));    // quad_perm 2 3 0 1
+    if (width == 4) return __int_as_float(dpp<0x141>(b));   // row_half_mirror
+    return __int_as_float(dpp<0x140>(b));                   // row_mirror
+}
+__device__ __forceinline__ double other_half(double v, int width)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const float lo = other_half(__int_as_float((int)b), width), hi = other_half(__int_as_float((int)(b >> 32)), width);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__float_as_int(hi) << 32 | (uint32_t)__float_as_int(lo));
+}
+__device__ __forceinline__ float both_halves(float v, bool wide)  // the sum over two rows of sixteen lanes, or (wide) over two halves of the wave
+{
+    const uint32_t b = __float_as_uint(v);
+    const auto r = wide ? __builtin_amdgcn_permlane32_swap(b, b, false, false) : __builtin_amdgcn_permlane16_swap(b, b, false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ double both_halves(double v, bool wide)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t x = (uint32_t)b, y = (uint32_t)(b >> 32);
+    const auto lo = wide ? __builtin_amdgcn_permlane32_swap(x, x, false, false) : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const auto hi = wide ? __builtin_amdgcn_permlane32_swap(y, y, false, false) : __builtin_amdgcn_permlane16_swap(y, y, false, false);
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+// sum over `lanes` neighbouring lanes (a power of two from 4 to 64), the same in each of them.  No step goes through LDS.
 template <class V>
 __device__ __forceinline__ V lanes_sum(V v, int lanes)
 {
-    for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor(v, o, kWave);
+    v += other_half(v, 1);
+    v += other_half(v, 2);
+    if (lanes > 4) v += other_half(v, 4);
+    if (lanes > 8) v += other_half(v, 8);
+    if (lanes > 16) v = both_halves(v, false);
+    if (lanes > 32) v = both_halves(v, true);
     return v;
 }
-// sum over 128 or 256 neighbouring threads of a workgroup of 256, the same in each of them; `part` may be written again behind the next barrier
+// sum over 128 or 256 neighbouring threads of a workgroup of 256, the same in each of them; `turn` changes from one call to the next, so that one barrier a call
+// is enough
 template <class V>
-__device__ __forceinline__ V waves_sum(V v, int lanes, V *part)
+__device__ __forceinline__ V waves_sum(V v, int lanes, V (&part)[2][4], int turn)
 {
     v = lanes_sum(v, 64);
+    if ((threadIdx.x & 63) == 0) part[turn & 1][threadIdx.x >> 6] = v;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
+    const V *p = part[turn & 1];
     const int pair = threadIdx.x >> 7 << 1;
-    return lanes == 128 ? part[pair] + part[pair + 1] : (part[0] + part[1]) + (part[2] + part[3]);
+    return lanes == 128 ? p[pair] + p[pair + 1] : (p[0] + p[1]) + (p[2] + p[3]);
 }
 
 // How a row is held in registers: `pieces` of eight columns a lane (1, 2 or 4; 0: it is too long for that), by `lanes` lanes: a power of two from 4 to 64, or
@@ -59,7 +94,7 @@ __device__ __forceinline__ uint32_t rest_of(const float (&sum)[8])
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float h = (float)(T)sum[e];
-        const float q = rintf(__builtin_amdgcn_ldexpf(sum[e] - h, -step_exponent<T>(h)));  // (NaN of what is not finite: 0 below)
+        const float q = rintf(__builtin_amdgcn_ldexpf(sum[e] - h, -step_exponent<T>(h)));  // (of what is not finite NaN, and -8 below, which changes neither)
         word |= ((uint32_t)(int)fminf(fmaxf(q, -8.0f), 7.0f) & 15u) << (4 * e);
     }
     return word;

@@ -38,7 +38,8 @@ struct Held {
 template <class T, class D, int C, bool WAVES, bool DH, bool REST>
 __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 {
-    __shared__ float part[4];
+    __shared__ float part[2][4];
+    int turn = 0;
     __shared__ float s_sum[256][8];
     const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
     const int64_t first = (int64_t)blockIdx.x * a.rows_each, last = first + a.rows_each < a.rows ? first + a.rows_each : a.rows;
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
             for (int e = 0; e < 8; ++e) dot = fmaf(g[c][e], n[c][e], dot);
         }
         if (!a.dx) continue;
-        const float mean = (WAVES ? waves_sum(dot, lanes, part) : lanes_sum(dot, lanes)) * share;
+        const float mean = (WAVES ? waves_sum(dot, lanes, part, turn++) : lanes_sum(dot, lanes)) * share;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             float d[8] = {};
@@ -159,7 +160,8 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 template <class T, class D>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
 {
-    __shared__ float part[4];
+    __shared__ float part[2][4];
+    int turn = 0;
     auto load = [&](int64_t row, int64_t col, float r, float(&n)[8], float(&g)[8]) {
         const int64_t left = a.cols - col;
         const int valid = (int)(left < 8 ? left : 8);
@@ -185,7 +187,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot = fmaf(g[e], n[e], dot);
         }
-        const float mean = waves_sum(dot, 256, part) * (1.0f / (float)a.cols);
+        const float mean = waves_sum(dot, 256, part, turn++) * (1.0f / (float)a.cols);
         for (int64_t col = 8 * threadIdx.x; col < a.cols; col += 8 * 256) {
             float n[8], g[8], d[8] = {};
             const int valid = load(row, col, r, n, g);
