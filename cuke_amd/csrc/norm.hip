@@ -39,11 +39,12 @@ __device__ __forceinline__ float root(const NormArgs &a, double sum)
     const double better = r * fma(-0.5 * m * r, r, 1.5);
     return (float)(r > 0.0 && r < 1e300 ? better : r);  // (of 0 and infinity the step would make NaN)
 }
-// an element of the result in 64 bits, from memory and the row's sum of squares
+// r in 64 bits, and an element of the result, from memory
+__device__ __forceinline__ double root64(const NormArgs &a, double sum) { return 1.0 / sqrt(sum / (double)a.cols + a.eps); }
 template <class T>
-__device__ __forceinline__ double result_at(const NormArgs &a, int64_t row, int64_t col, double sum)
+__device__ __forceinline__ double result_at(const NormArgs &a, int64_t row, int64_t col, double r)
 {
-    const double y = sum_at<T>(a, row, col) * (1.0 / sqrt(sum / (double)a.cols + a.eps));
+    const double y = sum_at<T>(a, row, col) * r;
     return a.weight ? y * (double)(float)static_cast<const T *>(a.weight)[col] : y;
 }
 // to 32 bits towards zero, the last bit set where that was not exact: what is rounded further from there lands where the 64-bit value does
@@ -58,34 +59,37 @@ __device__ __forceinline__ float to_odd(double d)
 template <class T>
 __device__ __forceinline__ float top_in_64(const NormArgs &a, int64_t row, int64_t col, double sum)
 {
+    const double r = root64(a, sum);
     float top = 0.0f;
 #pragma unroll 1
     for (int e = 0; e < 8 && col + e < a.cols; ++e) {
-        const float v = fabsf(to_odd(result_at<T>(a, row, col + e, sum)));
+        const float v = fabsf(to_odd(result_at<T>(a, row, col + e, r)));
         top = fmaxf(top, finite(v) ? v : 0.0f);
     }
     return top;
 }
-// the bytes of q that differ from `other` formed again
+// the bytes of q that differ from `other` formed again (one, as a rule)
 template <class T>
 __device__ __forceinline__ uint2 settle(const NormArgs &a, int64_t row, int64_t col, double sum, float inverse, uint2 q, uint2 other)
 {
+    uint64_t all = (uint64_t)q.y << 32 | q.x, differ = all ^ ((uint64_t)other.y << 32 | other.x);
+    const double r = root64(a, sum);
 #pragma unroll 1
-    for (int e = 0; e < 8 && col + e < a.cols; ++e) {
-        const uint32_t mask = 0xFFu << (8 * (e & 3)), differ = e < 4 ? q.x ^ other.x : q.y ^ other.y;
-        if (!(differ & mask)) continue;
-        const float v = to_odd(result_at<T>(a, row, col + e, sum) * (double)inverse);
-        const uint32_t byte = ((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xFFu) << (8 * (e & 3));
-        if (e < 4) q.x = (q.x & ~mask) | byte;
-        else q.y = (q.y & ~mask) | byte;
+    while (differ) {
+        const int shift = __builtin_ctzll(differ) & ~7;
+        const uint64_t mask = 0xFFull << shift;
+        differ &= ~mask;
+        if (col + shift / 8 >= a.cols) continue;
+        const float v = to_odd(result_at<T>(a, row, col + shift / 8, r) * (double)inverse);
+        all = (all & ~mask) | (uint64_t)((uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xFFu) << shift;
     }
-    return q;
+    return make_uint2((uint32_t)all, (uint32_t)(all >> 32));
 }
 
 // Eight consecutive results (fp32, each within 6 units of its last place; zero behind the row's end) to 8 bits; the lanes of a block come together.  A value that another
-// rounding of fp32 would put on the other side of a border of e4m3, one in 40000, is formed again in 64 bits, and so is a block's largest value at the border
+// rounding of fp32 would put on the other side of a border of e4m3, one in 100000, is formed again in 64 bits, and so is a block's largest value at the border
 // of two powers: to see that, every value is rounded twice, 16 units apart.
-constexpr float kUp = 1.0f + 0x1p-20f, kDown = 1.0f - 0x1p-20f;
+constexpr float kUp = 1.0f + 0x1p-21f, kDown = 1.0f - 0x1p-21f;
 template <class T>
 __device__ __forceinline__ void store_e4m3(const NormArgs &a, int64_t row, int64_t col, double sum, const float (&y)[8], bool there)
 {
