@@ -123,7 +123,7 @@ __global__ __launch_bounds__(kFewWaves *kWave) void linear8_few_kernel(TileArgs 
     float4 bias = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (t.e.bias) bias = load4(static_cast<const T *>(t.e.bias) + col, valid);
     float out[1][4] = {{z[0], z[1], z[2], z[3]}};
-    finish_quads<T, 1, true>(t.e, t.e.drop.base(), m, 1, col, valid, out, bias, nullptr);
+    finish_quads<T, 1, W8 ? 0 : 8>(t.e, t.e.drop.base(), m, 1, col, valid, out, bias, nullptr);
 }
 
 template <class T>

@@ -8,6 +8,8 @@
 // one), or, where both sides are in 8 bits, to LDS as they lie: the matrix cores take them with their powers.
 #pragma once
 
+#include <type_traits>
+
 #include "features.hpp"
 #include "mfma_split.hpp"
 #include "rows8.hpp"
@@ -122,8 +124,10 @@ struct Tile {
     template <class E>
     struct Feed {
         const char *from[kRounds];
-        int64_t step[kRounds];
-        int term[kRounds];  // of the chunk, within the tile
+        typename std::conditional<ACROSS, int64_t, int>::type step[kRounds];
+        int term;  // of the first chunk, within the tile (along rows of all of them: rounds are whole turns of turn())
+        static_assert(ACROSS || THREADS / kRow % 16 == 0, "one term for all rounds");
+        __device__ __forceinline__ int term_of(int r) const { return ACROSS ? term + r * (THREADS / kRow) : term; }
 
         __device__ __forceinline__ void start(const Side &s, int64_t first, int64_t k)
         {
@@ -132,11 +136,12 @@ struct Tile {
             for (int r = 0; r < kRounds; ++r) {
                 const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
                 const int64_t index = first + (ACROSS ? 8 * j : row);
-                term[r] = ACROSS ? row : 8 * j;
+                if (r == 0) term = ACROSS ? row : 8 * j;
                 const bool there = index < s.extent;
                 from[r] = there ? reinterpret_cast<const char *>(p + (ACROSS ? (k + row) * s.stride + index : index * s.stride + k + 8 * j))
                                 : reinterpret_cast<const char *>(zero_chunk);
-                step[r] = there ? (ACROSS ? K * s.stride : K) * (int64_t)sizeof(E) : 0;
+                if constexpr (ACROSS) step[r] = there ? K * s.stride * (int64_t)sizeof(E) : 0;
+                else step[r] = there ? K * (int)sizeof(E) : 0;
             }
         }
         // the next tile, all of whose terms exist
@@ -155,7 +160,7 @@ struct Tile {
             const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
 #pragma unroll
             for (int r = 0; r < kRounds; ++r) {
-                chunk_to_lds(term[r] < left ? from[r] : reinterpret_cast<const char *>(zero_chunk), lds + 16 * (r * THREADS + wave * 64));
+                chunk_to_lds(term_of(r) < left ? from[r] : reinterpret_cast<const char *>(zero_chunk), lds + 16 * (r * THREADS + wave * 64));
                 from[r] += step[r];
             }
         }
@@ -390,9 +395,9 @@ struct Raw4 {
 };
 
 // Four consecutive columns (`valid` of them exist) of R rows, `apart` rows from one to the next, through the layer's epilogue.  T: the layer's
-// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.  ahead: the rows' residuals, or NULL.  KEEP8: act' is kept in
-// 8 bits.
-template <class T, int R, bool KEEP8 = false>
+// type.  R rows at a time, so that one's arithmetic hides another's latencies where few waves run.  ahead: the rows' residuals, or NULL.  KEEP: the bits that act' is
+// kept in (16: those of the type; 0: it is not kept).
+template <class T, int R, int KEEP = 16>
 __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64_t first, int apart, int64_t col, int valid, float (&z)[R][4], float4 bias,
                                              const Raw4 *ahead)
 {
@@ -421,12 +426,12 @@ __device__ __forceinline__ void finish_quads(const Ends &e, uint64_t base, int64
         activate(flat, e.act, slope);
 #pragma unroll
         for (int i = 0; i < 4 * R; ++i) z[i / 4][i % 4] = flat[i];
-        if (e.slope) {  // (rows of whole quads)
+        if (KEEP > 0 && e.slope) {  // (rows of whole quads)
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 const int64_t row = first + r * apart, at = row * 4 * e.quads + col;
                 if (row >= e.rows) continue;
-                if (KEEP8) {
+                if (KEEP == 8) {
                     *reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(e.slope) + at) = slopes_to_bytes(slope[4 * r], slope[4 * r + 1], slope[4 * r + 2], slope[4 * r + 3]);
                 } else if (sizeof(T) == 4) {
                     *reinterpret_cast<float4 *>(static_cast<float *>(e.slope) + at) = make_float4(slope[4 * r], slope[4 * r + 1], slope[4 * r + 2], slope[4 * r + 3]);
@@ -733,7 +738,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             char *to_a = EIGHT == kNoSideApart ? wide(u) : stage(u), *to_b = EIGHT == kNoSideApart ? stage(u) : stage(u) + kBytesA;
             if constexpr (decltype(whole)::value) feed_a.load_whole(to_a), feed_b.load_whole(to_b);
             else feed_a.load(left, to_a), feed_b.load(EIGHT == kSideB ? left8 : left, to_b);
-            if constexpr (kScales) scales.load(loaded, loaded < tiles, stage(u) + kBytesA + kBytesB);
+            if constexpr (kScales) scales.load(loaded, decltype(whole)::value || loaded < tiles, stage(u) + kBytesA + kBytesB);
             if constexpr (EIGHT != kNoSide) ++loaded, left8 -= K / 2;
             left -= K;
         };
@@ -749,11 +754,18 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                     load((u + STAGES - 1) % STAGES, std::true_type{});
                     multiply(u, at + u);
                 }
+        // (both sides in 8 bits: nothing moves over these lines, which in the largest tiles would cost a register more than there are)
+        auto keep_order = [] {
+            if constexpr (EIGHT == kBothSides) __builtin_amdgcn_sched_barrier(0);
+        };
+        keep_order();
         for (; at + STAGES <= tiles; at += STAGES)
 #pragma unroll
             for (int u = 0; u < STAGES; ++u) {
                 stage_ready<kLoads * (STAGES - 2)>();
+                keep_order();
                 load((u + STAGES - 1) % STAGES, std::false_type{});
+                keep_order();
                 multiply(u, at + u);
             }
 #pragma unroll
@@ -771,7 +783,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     constexpr bool kRoom = EIGHT != kSideA || WA * WB <= STAGES * (kBytesB / 8192) + 2 * (kBytesA / 8192);  // for strips of 64 columns
     constexpr int kGroup = FA < 2 || !kRoom ? 1 : 2, kQuads = 8 * kGroup, kStrip = 32 * kQuads * 16;
     constexpr int kPerStage = (kWideA ? kBytesB : kStage) / kStrip, kPerWide = kBytesA / kStrip;
-    constexpr int kApart = 64 / kQuads, kRows = 4 / SHARE, kTurns = 32 / (kApart * kRows * SHARE);  // rows a read covers, reads a turn, turns of a wave in a strip
+    constexpr int kApart = 64 / kQuads, kRows = EIGHT == kSideB && FA * FB == 8 ? 2 : 4 / SHARE, kTurns = 32 / (kApart * kRows * SHARE);  // rows a read covers, reads a turn, turns of a wave in a strip
     constexpr int kStrips = FA / kGroup * FB;
     static_assert(FA % kGroup == 0 && kPerStage >= 1 && WA * WB <= STAGES * kPerStage + (EIGHT == kSideA ? 2 : (kWideA ? STAGES : 0)) * kPerWide, "a strip for every wave");
     static_assert(SHARE == 1 || (kStrips == 1 && kPerStage >= SHARE * WA * WB), "waves that share a strip");
@@ -848,7 +860,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                 z[k][0] = v.x, z[k][1] = v.y, z[k][2] = v.z, z[k][3] = v.w;
             }
             if constexpr (LAYER) {
-                finish_quads<T, kRows, (EIGHT != kNoSide)>(t.e, base, first, kApart, col, valid, z, bias, ahead ? held[u] : nullptr);
+                finish_quads<T, kRows, EIGHT == kNoSide ? 16 : (EIGHT == kBothSides ? 0 : 8)>(t.e, base, first, kApart, col, valid, z, bias, ahead ? held[u] : nullptr);
             } else {
 #pragma unroll
                 for (int k = 0; k < kRows; ++k) {

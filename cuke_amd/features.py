@@ -661,7 +661,7 @@ class ResidualEncoder:
 
     def encode(self, x, base=None) -> torch.Tensor:
         """Rows for answering with: nothing is dropped, nothing is kept."""
-        h, more, dt = linear(x, self.w_in, self.b_in), None, self.b_in.dtype
+        h, more, dt = linear(x, self.w_in, self.b_in), None, self.w_in.dtype
 
         def norm(weight):
             nonlocal h
