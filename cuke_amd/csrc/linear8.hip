@@ -182,23 +182,22 @@ static void launch_tiles(TileArgs &t, hipStream_t st)
     else if constexpr (!BOTH) hipLaunchKernelGGL((linear8_forward_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
-// By forward_cost(), whose paces hold for these kernels too (a pair of terms of both sides in 8 bits takes as long as one and a half of 16-bit ones).  Over twelve sizes the shape
-// chosen takes 0.1 % longer than the best one on average with a 16-bit weight, 0.3 % with one in 8 bits.  Some of them (us; Large, Middle, Tall, Lone, Small; what is chosen
-// in brackets), with a 16-bit weight:
+// By forward_cost(); terms of both sides in 8 bits count in pairs.  The shape chosen takes 1.1 % longer than the best one on average over seventeen sizes with a 16-bit weight,
+// 0.9 % over fifteen with one in 8 bits.  Some of them (us; Large, Middle, Tall, Lone, Small; what is chosen in brackets), with a 16-bit weight:
 //   32768 x 2048 -> 2048, gelu, drop, act' kept  [329] 370 405 435 474       65536 x 512 -> 400, fp32 residual  79 [76] 76  82 88
 //    4096 x 1024 -> 512, gelu, drop, act' kept    47   18  15 [13] 14         2500 x 520 -> 264, gelu           38  21  12  10 [8]
 // and with one in 8 bits:
-//   32768 x 2048 -> 2048, gelu                   [222] 225 298 344 280       16384 x 768 -> 512, plain          23 [15] 20  24 20
-//    1000 x 2048 -> 2048, gelu                    44   20  19 [12] 13         4096 x 4096 -> 1024, gelu  75 [30; 37 in two stages] 37 40 40
+//   32768 x 2048 -> 2048, gelu                   [222] 225 298 344 280       30198 x 488 -> 1392, plain         59 [51]
+//    1000 x 2048 -> 2048, gelu                    44   20  19 [12] 13         4096 x 4096 -> 1024, gelu         75 [30; 37 in two stages] 37 40 40
 template <class T>
 static void launch_forward8(TileArgs &t, bool both, hipStream_t st)
 {
     const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 1 : 0);
     int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
-    if (both) epilogue = epilogue * 7 / 10;
-    const double large = forward_cost<LargeB>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0), middle = forward_cost<MiddleB>(t, epilogue, 2, 0.73, 2.5);
-    const double tall = forward_cost<TallB>(t, epilogue, 3, 0.5, 2.3), small = forward_cost<SmallB>(t, epilogue, 3, 0.45, 0.9);
-    const double lone = forward_cost<LoneB>(t, epilogue, 1, 0.4, 0.9);
+    if (both) epilogue = epilogue * 13 / 10;
+    const double large = forward_cost<LargeB>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0);
+    const double middle = forward_cost<MiddleB>(t, epilogue, 2, both ? 0.7 : 0.73, both ? 3.5 : 2.5), tall = forward_cost<TallB>(t, epilogue, 3, both ? 0.45 : 0.5, 2.3);
+    const double small = forward_cost<SmallB>(t, epilogue, 3, both ? 0.4 : 0.45, 0.9), lone = forward_cost<LoneB>(t, epilogue, 1, both ? 0.35 : 0.4, 0.9);
     if (lone < large && lone < middle && lone < tall && lone < small) both ? launch_tiles<T, LoneB, true>(t, st) : launch_tiles<T, LoneB, false>(t, st);
     else if (large <= middle && large <= tall && large <= small) both ? launch_tiles<T, Large8, true>(t, st) : launch_tiles<T, LargeB, false>(t, st);
     else if (middle <= tall && middle <= small) {
