@@ -216,6 +216,7 @@ template <class T, class W, class X>
 __global__ __launch_bounds__(W::kThreads, W::kThreads == 512 && W::XA * W::XB <= 128 * 128 ? 4 : 1) void linear8_grads_kernel(TileArgs dw, TileArgs dx, SumArgs db, int64_t dw_blocks, int64_t dx_blocks)
 {
     static_assert(W::kThreads == X::kThreads && W::XA == X::XA && W::XB == X::XB && W::STAGES >= X::STAGES, "one grid, and arrays of the larger one");
+    static_assert(W::K == 32, "kFarthest");
     constexpr int kA = side_bytes<W, true>() > side_bytes<X, true>() ? side_bytes<W, true>() : side_bytes<X, true>();
     constexpr int kB = side_bytes<W, false>() > side_bytes<X, false>() ? side_bytes<W, false>() : side_bytes<X, false>();
     __shared__ __align__(16) char stage0[kB], stage1[kB], stage2[W::STAGES > 2 ? kB : 16], stage3[W::STAGES > 3 ? kB : 16];
@@ -347,6 +348,9 @@ static int backward8(const kge_linear *l, const kge_rows8 *x8, const Plan8 &p, c
 
 using namespace kge;
 
+// Bytes between rows of x8 that the backward pass takes: a stage's 32 rows are addressed with 32 bits.
+constexpr int64_t kFarthest = (int64_t)1 << 26;
+
 static size_t backward8_bytes(const kge_linear *l, const Plan8 &p, const GradPlan &g)
 {
     return packed_bytes(l->type, l->rows, l->out) + up256((size_t)p.sum_blocks * p.quads * 16) +
@@ -405,7 +409,7 @@ int kge_linear8_bwd(const kge_linear *lin, const kge_rows8 *x8, const void *dy, 
 {
     if (const int rc = check8(lin, false)) return rc;
     if (const int rc = check_rows8(x8, lin->rows, lin->in)) return rc;
-    if (dy_stride < lin->out) return KGE_ESHAPE;
+    if (dy_stride < lin->out || x8->q_stride >= kFarthest || x8->scale_stride >= kFarthest) return KGE_ESHAPE;
     if (lin->rows > 0 && lin->out > 0 && !dy) return KGE_EINVAL;
     const Plan8 p = plan8_of(lin);
     const GradPlan g = grad_plan(lin);

@@ -681,9 +681,10 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
  * aligned, what rounding took from h, in 16ths of a step of `type`: four bits an element.
  * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
  *   g = dy weight,   dx = dresidual = r (g - h r^2 mean_j(g h)) + dh,   dweight[j] = sum_i dy[i][j] h[i][j] r[i]
- * h: what the forward call wrote there (x where there was no residual), rstd and rest too (NULL: the gradients are those of h as it was rounded).  dx [rows, cols] and dweight [cols] of type `type`, contiguous but for
- * dx's stride; either may be NULL.  dx may be dy or dh where type and stride are the same.  The fields x and residual of the description are not looked at.  Sums over rows are joined
- * in a fixed order.  rows, cols: 0 .. 2^31 - 1 (KGE_ESHAPE beyond).
+ * h: what the forward call wrote there (x where there was no residual), rstd and rest too (NULL: the gradients are those of h as it was rounded).  dx [rows, cols]
+ * and dweight [cols] of type `type`, contiguous but for dx's stride; either may be NULL.  The fields x and residual of the description are not looked at.
+ * Sums over rows are joined in a fixed order.  rows, cols: 0 .. 2^31 - 1 (KGE_ESHAPE beyond).
+ * Outputs overlap no input, but that dx may be dy or dh where type and stride are the same.
  */
 typedef struct kge_rms_norm {
     int32_t type, out_type; /* kge_type_t; out_type also KGE_E4M3 */
@@ -704,11 +705,13 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
 
 /*
  * Linear layers (kge_linear, whose x and x_stride are not looked at) on rows in 8 bits, x8 [rows, in]:  y = drop(act(x8 weight^T + bias)) + residual.
- * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients; a value of x8 that KGE_F16 cannot hold is infinite.  Products are
- * exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for answering:
- * for_backward is 0 then (KGE_EINVAL).
- * The backward pass reads x8 where the forward pass did, so that it is all that is kept of the layer's input; act'(z) is kept in 8 bits too (steps of 1/200
- * from -0.135 up: within 0.0025).  dx is the gradient at the values that x8 stands for.  Otherwise as kge_linear_fwd and kge_linear_bwd.
+ * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients; a value of x8 or weight8 that KGE_F16 cannot hold is infinite.
+ * Products are exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for
+ * answering: for_backward is 0 then (KGE_EINVAL).  Where all of x8, weight8 and a KGE_BF16 y meet, the matrix cores' product of 8-bit sides may be taken, which drops
+ * from each sum of eight neighbouring terms what lies below 2^-13 of the largest one's power.
+ * The backward pass reads x8 where the forward pass did, so that it is all that is kept of the layer's input (its rows less than 2^26 bytes apart: KGE_ESHAPE);
+ * act'(z) is kept in 8 bits too (steps of 1/200 from -0.135 up: within 0.0025).  dx is the gradient at the values that x8 stands for.  Otherwise as kge_linear_fwd and
+ * kge_linear_bwd.
  */
 size_t kge_linear8_saved_bytes(const kge_linear *lin);
 size_t kge_linear8_fwd_workspace(const kge_linear *lin, const kge_rows8 *weight8, int for_backward);

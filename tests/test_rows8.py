@@ -113,6 +113,61 @@ def test_norm_outputs_and_workspaces_are_checked():
     assert bwd(dx=None, dw=None, ws=None, n=0) == 0 and bwd(d=norm(cols=0), ws=None, n=0) == 0
 
 
+def layer(type=1, out_type=None, rows=4, inn=40, out=24, weight=FAKE, ws=40, act=2, p=0.0):
+    from cuke_amd import _lib
+    return _lib.Linear(type, type if out_type is None else out_type, act, 0, rows, inn, out, None, 0, weight, ws, None, None, 0, p, 0, 0, None)
+
+
+@pytest.mark.parametrize("bad,rc", [
+    (dict(type=0), EINVAL), (dict(type=3), EINVAL), (dict(out_type=2), EINVAL), (dict(act=9), EINVAL), (dict(p=1.5), EINVAL), (dict(weight=None), EINVAL),
+    (dict(rows=-1), ESHAPE), (dict(inn=-1), ESHAPE), (dict(ws=39), ESHAPE), (dict(rows=1 << 31), ESHAPE)])
+def test_layers_of_rows_in_8_bits_refuse(bad, rc):
+    _, L = lib()
+    d, x = layer(**bad), rows8()
+    assert L.kge_linear8_fwd(C.byref(d), C.byref(x), None, FAKE, 1 << 31, 0, None, 0, FAKE, 1 << 40, None) == rc
+    assert L.kge_linear8_bwd(C.byref(d), C.byref(x), FAKE, 1 << 31, FAKE, 1 << 40, FAKE, FAKE, None, FAKE, 1 << 40, None) == rc
+    assert L.kge_linear8_saved_bytes(C.byref(d)) == 0 and L.kge_linear8_fwd_workspace(C.byref(d), None, 0) == 0 and L.kge_linear8_bwd_workspace(C.byref(d)) == 0
+
+
+@pytest.mark.parametrize("bad,rc", [
+    (dict(q=None), EINVAL), (dict(scale=None), EINVAL), (dict(q=FAKE + 8), EINVAL), (dict(scale=FAKE + 2), EINVAL), (dict(qs=32), ESHAPE),
+    (dict(qs=72), ESHAPE), (dict(ss=0), ESHAPE), (dict(ss=6), ESHAPE)])
+def test_layers_check_their_rows_in_8_bits(bad, rc):
+    _, L = lib()
+    d, good, x = layer(), rows8(), rows8(**bad)
+    fwd = lambda a, b: L.kge_linear8_fwd(C.byref(d), C.byref(a) if a else None, C.byref(b) if b else None, FAKE, 24, 0, None, 0, FAKE, 1 << 40, None)
+    assert fwd(x, None) == rc and fwd(good, x) == rc and fwd(None, None) == EINVAL
+    assert L.kge_linear8_bwd(C.byref(d), C.byref(x), FAKE, 24, FAKE, 1 << 40, FAKE, FAKE, None, FAKE, 1 << 40, None) == rc
+    assert L.kge_linear8_bwd(C.byref(d), None, FAKE, 24, FAKE, 1 << 40, FAKE, FAKE, None, FAKE, 1 << 40, None) == EINVAL
+
+
+def test_layers_check_outputs_blocks_and_workspaces():
+    _, L = lib()
+    d, x = layer(rows=300), rows8()
+    saved, wide = L.kge_linear8_saved_bytes(C.byref(d)), L.kge_linear8_bwd_workspace(C.byref(d))
+    assert saved >= 300 * 24 and wide >= 300 * 24 * 2
+    for name in ("kge_linear8_saved_bytes", "kge_linear8_bwd_workspace"):
+        assert getattr(L, name)(None) == 0
+    assert L.kge_linear8_fwd_workspace(None, None, 0) == 0
+
+    def fwd(d=d, y=FAKE, ys=24, keep=1, s=FAKE, sn=saved, w8=None):
+        return L.kge_linear8_fwd(C.byref(d), C.byref(x), C.byref(w8) if w8 else None, y, ys, keep, s, sn, FAKE, 1 << 40, None)
+    assert fwd(y=None) == EINVAL and fwd(ys=23) == ESHAPE and fwd(w8=rows8()) == EINVAL
+    assert fwd(s=None) == EWORKSPACE and fwd(s=FAKE + 8) == EWORKSPACE and fwd(sn=saved - 1) == EWORKSPACE
+    assert fwd(d=layer(rows=0), y=None) == 0 and fwd(d=layer(out=0), y=None, ys=0) == 0
+    half = layer(type=2, rows=3000, weight=None, ws=0)           # fp16 with the weight in 8 bits: widened into the workspace
+    need = L.kge_linear8_fwd_workspace(C.byref(half), C.byref(rows8()), 0)
+    assert need >= 24 * 40 * 2
+    for ws, n in ((None, need), (FAKE + 8, need), (FAKE, need - 1)):
+        assert L.kge_linear8_fwd(C.byref(half), C.byref(x), C.byref(rows8()), FAKE, 24, 0, None, 0, ws, n, None) == EWORKSPACE
+
+    def bwd(d=d, x=x, dy=FAKE, dys=24, s=FAKE, sn=saved, ws=FAKE, n=wide):
+        return L.kge_linear8_bwd(C.byref(d), C.byref(x), dy, dys, s, sn, FAKE, FAKE, None, ws, n, None)
+    assert bwd(dy=None) == EINVAL and bwd(dys=23) == ESHAPE
+    assert bwd(x=rows8(qs=1 << 26)) == ESHAPE and bwd(x=rows8(ss=1 << 26)) == ESHAPE           # (a stage's rows are addressed with 32 bits)
+    assert bwd(s=None) == EWORKSPACE and bwd(sn=saved - 1) == EWORKSPACE and bwd(ws=None) == EWORKSPACE and bwd(n=wide - 1) == EWORKSPACE and bwd(ws=FAKE + 8) == EWORKSPACE
+
+
 def test_rows8_says_what_it_takes():
     from cuke_amd import features
     q, s = torch.zeros((3, 64), dtype=torch.float8_e4m3fn), torch.zeros((3, 4), dtype=torch.uint8).view(torch.float8_e8m0fnu)
