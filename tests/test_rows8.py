@@ -155,11 +155,11 @@ def test_layers_check_outputs_blocks_and_workspaces():
     assert fwd(y=None) == EINVAL and fwd(ys=23) == ESHAPE and fwd(w8=rows8()) == EINVAL
     assert fwd(s=None) == EWORKSPACE and fwd(s=FAKE + 8) == EWORKSPACE and fwd(sn=saved - 1) == EWORKSPACE
     assert fwd(d=layer(rows=0), y=None) == 0 and fwd(d=layer(out=0), y=None, ys=0) == 0
-    half = layer(type=2, rows=3000, weight=None, ws=0)           # fp16 with the weight in 8 bits: widened into the workspace
+    half = layer(type=2, rows=3000, out=1000, weight=None, ws=0)           # fp16 with the weight in 8 bits: widened into the workspace
     need = L.kge_linear8_fwd_workspace(C.byref(half), C.byref(rows8()), 0)
-    assert need >= 24 * 40 * 2
+    assert need >= 1000 * 40 * 2
     for ws, n in ((None, need), (FAKE + 8, need), (FAKE, need - 1)):
-        assert L.kge_linear8_fwd(C.byref(half), C.byref(x), C.byref(rows8()), FAKE, 24, 0, None, 0, ws, n, None) == EWORKSPACE
+        assert L.kge_linear8_fwd(C.byref(half), C.byref(x), C.byref(rows8()), FAKE, 1000, 0, None, 0, ws, n, None) == EWORKSPACE
 
     def bwd(d=d, x=x, dy=FAKE, dys=24, s=FAKE, sn=saved, ws=FAKE, n=wide):
         return L.kge_linear8_bwd(C.byref(d), C.byref(x), dy, dys, s, sn, FAKE, FAKE, None, ws, n, None)
