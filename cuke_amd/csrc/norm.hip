@@ -123,7 +123,10 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 {
     __shared__ double part[2][4];
     int turn = 0;
-    const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
+    int lane;
+    uint32_t group;
+    place_in_rows<WAVES>(a.lanes, &lane, &group);
+    const int lanes = a.lanes, groups = 256 >> (31 - __builtin_clz(lanes));
     auto column = [&](int c) { return 8 * (c * lanes + lane); };
     auto valid = [&](int c) { return (int)a.cols - column(c); };
     auto load = [&](const void *from, int64_t at, int c, float(&v)[8]) {
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
     };
     for (int64_t row0 = (int64_t)blockIdx.x * groups; row0 < a.rows; row0 += (int64_t)gridDim.x * groups) {
         const bool there = row0 + group < a.rows;
-        const int64_t row = there ? row0 + group : a.rows - 1;  // (lanes without a row of their own go along)
+        const int64_t row = (uint32_t)row0 + (there ? group : 0u);  // (lanes without a row of their own go along)
         float h[C][8];
         double sum = 0.0;
 #pragma unroll

@@ -78,6 +78,15 @@ inline Hold hold_of(int64_t rows, int64_t cols, int64_t enough)
     return Hold{pieces, lanes};
 }
 
+// A thread's place among the 256 of a workgroup, `lanes` of which hold a row (WAVES: whole waves, all of whose lanes then know that they work on the same one).
+template <bool WAVES>
+__device__ __forceinline__ void place_in_rows(int lanes, int *lane, uint32_t *group)
+{
+    *lane = threadIdx.x & (lanes - 1);
+    *group = threadIdx.x >> (31 - __builtin_clz(lanes));
+    if (WAVES) *group = (uint32_t)__builtin_amdgcn_readfirstlane((int)*group);
+}
+
 // What a sum loses when it is rounded to 16 bits, in sixteenths of a step of the result there, -8 .. 7: four bits an element, eight of a row in a word.  With it the
 // gradients are those of the sum itself, to 2^-13: from the rounded one alone dweight would be off by 1.4 times its own rounding, and dx of short rows,
 // where g - n mean(g n) cancels, by several times.

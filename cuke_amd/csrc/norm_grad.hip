@@ -41,7 +41,10 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
     __shared__ float part[2][4];
     int turn = 0;
     __shared__ float s_sum[256][8];
-    const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), group = threadIdx.x / lanes, groups = 256 / lanes;
+    int lane;
+    uint32_t group;
+    place_in_rows<WAVES>(a.lanes, &lane, &group);
+    const int lanes = a.lanes, groups = 256 >> (31 - __builtin_clz(lanes));
     const int64_t first = (int64_t)blockIdx.x * a.rows_each, last = first + a.rows_each < a.rows ? first + a.rows_each : a.rows;
     const float share = 1.0f / (float)a.cols;
     const int cols = (int)a.cols;
@@ -61,21 +64,26 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 #pragma unroll
         for (int c = 0; c < C; ++c) w[c].fetch(a.weight, at[c]);
     }
-    auto fetch = [&](int64_t row) {
-        row = row < last ? row : last - 1;
-        r = a.rstd[row];
+    // the lane's present row, and the one requested ahead (behind the range's end: a row that is there)
+    const int64_t mine = first + (first + group < last ? group : 0u);
+    const T *row_h = static_cast<const T *>(a.h) + mine * a.h_stride, *row_dh = static_cast<const T *>(a.dh) + (DH ? mine * a.dh_stride : 0);
+    const D *row_dy = static_cast<const D *>(a.dy) + mine * a.dy_stride;
+    const uint32_t *row_rest = a.rest + (REST ? mine * words : 0);
+    const float *row_r = a.rstd + mine;
+    T *row_dx = static_cast<T *>(a.dx) + mine * a.dx_stride;
+    const int64_t step_h = groups * a.h_stride, step_dy = groups * a.dy_stride, step_dh = groups * a.dh_stride, step_dx = groups * a.dx_stride;
+    auto fetch = [&] {
+        r = *row_r;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            h[c].fetch(static_cast<const T *>(a.h) + row * a.h_stride, at[c]);
-            dy[c].fetch(static_cast<const D *>(a.dy) + row * a.dy_stride, at[c]);
-            if constexpr (DH) dh[c].fetch(static_cast<const T *>(a.dh) + row * a.dh_stride, at[c]);
-            if constexpr (REST) {  // (a piece that was moved back begins inside a word)
-                const uint32_t *p = a.rest + row * words;
-                rest[c] = p[at[c] >> 3], rest_end[c] = p[(at[c] + 7) >> 3];
-            }
+            h[c].fetch(row_h, at[c]);
+            dy[c].fetch(row_dy, at[c]);
+            if constexpr (DH) dh[c].fetch(row_dh, at[c]);
+            if constexpr (REST)  // (a piece that was moved back begins inside a word)
+                rest[c] = row_rest[at[c] >> 3], rest_end[c] = row_rest[(at[c] + 7) >> 3];
         }
     };
-    fetch(first + group);
+    fetch();
     for (int64_t row0 = first; row0 < last; row0 += groups) {
         const int64_t row = row0 + group;
         const bool there = row < last;
@@ -93,7 +101,12 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
                     if (e < skip[c]) g[c][e] = 0.0f;  // (counted by the piece before)
             }
         }
-        fetch(row + groups);
+        if (row + groups < last) {
+            row_r += groups, row_h += step_h, row_dy += step_dy;
+            if constexpr (DH) row_dh += step_dh;
+            if constexpr (REST) row_rest += groups * words;
+        }
+        fetch();
 #pragma unroll
         for (int c = 0; c < C; ++c) {
 #pragma unroll
@@ -119,7 +132,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e] = fmaf(rr, g[c][e] - n[c][e] * mean, d[e]);
             if (!there || skip[c] >= 8) continue;
-            T *to = static_cast<T *>(a.dx) + row * a.dx_stride + at[c];
+            T *to = row_dx + at[c];
             if (skip[c] == 0) {
                 store8(to, d, 8);
             } else {
@@ -128,6 +141,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
                     if (e >= skip[c]) to[e] = (T)d[e];
             }
         }
+        row_dx += step_dx;
     }
     if (!a.sums) return;
     float *to = a.sums + (int64_t)blockIdx.x * a.quads * 4;
