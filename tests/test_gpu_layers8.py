@@ -261,6 +261,67 @@ def test_rows_behind_the_last_are_left_alone():
     assert bool((big[70:] == 7).all()) and bool((big[:70, 90:] == 7).all())
 
 
+@pytest.mark.parametrize("shape", [(100, 1000, 24), (40, 520, 264), (3, 96, 50)])
+def test_rows_that_lie_far_apart(shape):
+    """x in 8 bits with the most bytes between its rows that the backward pass takes (the last of a hundred begins 6 GiB from the first)."""
+    from cuke_amd import features
+    from cuke_amd.kge import KgeError
+    c = Layer8(*shape, torch.bfloat16, "gelu", drop=0.1)
+    fw = features.linear_forward(c.x, c.w, c.b, **c.kw())
+    g = features.linear_backward(fw, c.dy)
+
+    def moved(stride):
+        def one(t, unit):
+            base = torch.empty((shape[0] - 1) * (stride - unit) + t.shape[1], dtype=torch.uint8, device=DEV)
+            v = base.as_strided(t.shape, (stride - unit, 1))
+            v.copy_(t.view(torch.uint8))
+            return v.view(t.dtype)
+        return features.Rows8(one(c.x.q, 16), one(c.x.scale, 4), c.x.cols)
+    x = moved(1 << 26)
+    again = features.linear_forward(x, c.w, c.b, **c.kw())
+    got = features.linear_backward(again, c.dy)
+    assert torch.equal(again.y, fw.y) and torch.equal(got.x, g.x) and torch.equal(got.weight, g.weight) and torch.equal(got.bias, g.bias)
+    again = features.linear_forward(moved((1 << 26) + 16), c.w, c.b, **c.kw())
+    assert torch.equal(again.y, fw.y)
+    with pytest.raises(KgeError):
+        features.linear_backward(again, c.dy)
+
+
+def test_on_another_stream_and_in_two_graphs():
+    from cuke_amd import features
+    small, large = Layer8(300, 200, 136, torch.float16, "silu", drop=0.2, residual=True), Layer8(2100, 520, 264, torch.bfloat16, "gelu", drop=0.1, residual=True)
+
+    def run(c):
+        fw = features.linear_forward(c.x, c.w, c.b, **c.kw())
+        g = features.linear_backward(fw, c.dy)
+        return [fw.y, g.x, g.weight, g.bias, features.linear(c.x, features.pack8(c.w), c.b, dtype=c.dtype, **c.kw())]
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))
+    want = [run(small), run(large)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s, c in zip(streams, (small, large)):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append(run(c))
+    torch.cuda.synchronize()
+    assert same(got[0], want[0]) and same(got[1], want[1])
+    graphs, got = [], []
+    for c in (small, large):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(run(c))
+    for turn in range(3):
+        for c in (small, large):
+            c.dy.mul_(0.5)
+        eager = [run(small), run(large)]
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert same(got[0], eager[0]) and same(got[1], eager[1])
+
+
 def test_refusals():
     from cuke_amd import features
     from cuke_amd.kge import KgeError

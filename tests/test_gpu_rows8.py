@@ -383,3 +383,30 @@ def test_on_another_stream_and_in_a_graph():
         assert torch.equal(g.x, eager_g.x) and torch.equal(g.weight, eager_g.weight)
         assert torch.equal(y, features.unpack8(eager.y)) and torch.equal(features.unpack8(again), y)
     assert not torch.equal(back, y)
+
+
+def far(rows, cols, dtype, stride):
+    """Rows `stride` elements apart, in memory that nobody has written."""
+    base = torch.empty((rows - 1) * stride + cols, dtype=dtype, device=DEV)
+    return base.as_strided((rows, cols), (stride, 1))
+
+
+@pytest.mark.parametrize("cols", [40, 1027, 9000])
+def test_rows_that_lie_more_than_32_bits_apart(cols):
+    from cuke_amd import features
+    c = Norm(5, cols, torch.bfloat16, out=E4M3)
+    want = c.forward()
+    want_g = features.rms_norm_backward(want, c.dy, c.dh)
+    for name in ("x", "res", "dy", "dh"):
+        t = far(5, cols, torch.bfloat16, 3 << 28)                # (the last row begins 6 GiB from the first)
+        t.copy_(getattr(c, name))
+        setattr(c, name, t)
+    fw = c.forward()
+    g = features.rms_norm_backward(fw, c.dy, c.dh)
+    assert torch.equal(fw.y.q.view(torch.uint8), want.y.q.view(torch.uint8)) and torch.equal(fw.h, want.h)
+    assert torch.equal(g.x, want_g.x) and torch.equal(g.weight, want_g.weight)
+    q = far(5, want.y.q.shape[1], torch.uint8, 3 << 29)
+    scale = far(5, want.y.scale.shape[1], torch.uint8, 3 << 28)
+    q.copy_(want.y.q.view(torch.uint8)), scale.copy_(want.y.scale.view(torch.uint8))
+    r = features.Rows8(q.view(E4M3), scale.view(torch.float8_e8m0fnu), cols)
+    assert torch.equal(features.unpack8(r), features.unpack8(want.y))
