@@ -166,6 +166,45 @@ struct Tile {
         }
     };
 
+    // The same along rows, addressed with 32 bits from where the tile begins (its rows less than 2^32 bytes): an index that does not exist is another one, whose sums go
+    // nowhere.
+    struct NearFeed {
+        const char *from;
+        uint32_t at[kRounds];
+        int term;
+        __device__ __forceinline__ void start(const Side &s, int64_t first, int64_t k)  // (elements of 16 bits)
+        {
+            from = static_cast<const char *>(s.p) + 2 * (first * s.stride + k);
+            const int last = (int)(s.extent - first < X ? s.extent - first : X) - 1;
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) {
+                const int c = r * THREADS + (int)threadIdx.x, row = c / kRow, j = (c % kRow) ^ turn(row);
+                if (r == 0) term = 8 * j;
+                at[r] = (uint32_t)(row < last ? row : last) * (2 * (uint32_t)s.stride) + 16 * j;
+            }
+        }
+        __device__ __forceinline__ uint32_t offset(int r) const
+        {
+            uint32_t v = at[r];
+            asm volatile("" : "+v"(v));  // (the compiler would hold an address of 64 bits for each)
+            return v;
+        }
+        __device__ __forceinline__ void load_whole(char *lds)
+        {
+            const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) chunk_to_lds(from + offset(r), lds + 16 * (r * THREADS + wave * 64));
+            from += 2 * K;
+        }
+        __device__ __forceinline__ void load(int64_t left, char *lds)
+        {
+            const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+#pragma unroll
+            for (int r = 0; r < kRounds; ++r) chunk_to_lds(term < left ? from + at[r] : reinterpret_cast<const char *>(zero_chunk), lds + 16 * (r * THREADS + wave * 64));
+            from += 2 * K;
+        }
+    };
+
     // The same of an fp32 side: a chunk's eight values wait in registers (two tiles' at a time) until they go to LDS as parts.  A quad that
     // exists as a whole or not at all needs no branch, behind which its load would be waited for; only where rows are no whole quads (not WHOLE) and
     // a tile holds their end are values taken one at a time.
@@ -308,7 +347,7 @@ struct Tile {
 template <class TILE>
 __device__ __forceinline__ i8v read_eight(const char *lds, int at, int step, int lane)
 {
-    const int row = at + (lane & 31), j = 4 * step + (lane >> 5), turn = TILE::turn(row);
+    const int row = at + (lane & 31), j = 4 * step + (lane >> 5), turn = TILE::turn(lane & 31);
     const s16x8 lo = *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + (j ^ turn)));
     const s16x8 hi = *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + ((j + 2) ^ turn)));
     return __builtin_bit_cast(i8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15));
@@ -320,13 +359,13 @@ template <class TILE>
 __device__ __forceinline__ uint4 read_sixteen(const char *lds, int at, int block, int lane)
 {
     const int row = at + (lane & 31), j = 2 * block + (lane >> 5);
-    return *reinterpret_cast<const uint4 *>(lds + 16 * (row * TILE::kRow + (j ^ TILE::turn(row))));
+    return *reinterpret_cast<const uint4 *>(lds + 16 * (row * TILE::kRow + (j ^ TILE::turn(lane & 31))));
 }
 template <class TILE>
 __device__ __forceinline__ s16x8 read_chunk(const char *lds, int at, int chunk, int lane)
 {
     const int row = at + (lane & 31);
-    return *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + (chunk ^ TILE::turn(row))));
+    return *reinterpret_cast<const s16x8 *>(lds + 16 * (row * TILE::kRow + (chunk ^ TILE::turn(lane & 31))));
 }
 
 // The scales of a tile, a word (four blocks: 128 terms, of which a tile has all or half) an index: XA of side a, then XB of side b, then what no index asks for.
@@ -352,6 +391,42 @@ struct ScaleFeed {
     }
     // where a tile's first block is in a word
     __device__ __forceinline__ static int shift(int tile) { return BLOCKS == 4 ? 0 : 16 * (tile & 1); }
+};
+
+// The scales of both sides for tiles of 128 terms in two stages: 16 bytes (512 terms, four tiles') an index at a time, a quarter of the indices with each of the four tiles before,
+// so that four lanes read one line.
+template <int XA, int XB, int THREADS>
+struct ScaleGroups {
+    static constexpr int kIndices = XA + XB, kBytes = 16 * kIndices, kOnce = kIndices < THREADS ? kIndices : THREADS;  // kOnce: words that a load brings in
+    static_assert(kIndices % kOnce == 0 && XA % (kOnce / 4) == 0 && (kIndices / 4) % (kOnce / 4) == 0, "the indices of a load are all of one side");
+    const uint8_t *a, *b;
+    int64_t a_stride, b_stride;
+    int a_last, b_last, last;  // indices and words there are, less one: what does not exist is another one, whose sums nobody asks for or whose numbers are zero
+    __device__ __forceinline__ ScaleGroups(const TileArgs &t, int64_t n0, int64_t m0)
+        : a(t.a8.scale + n0 * t.a8.scale_stride), b(t.b8.scale + m0 * t.b8.scale_stride), a_stride(t.a8.scale_stride), b_stride(t.b8.scale_stride),
+          a_last((int)(t.a.extent - n0 < XA ? t.a.extent - n0 : XA) - 1), b_last((int)(t.b.extent - m0 < XB ? t.b.extent - m0 : XB) - 1), last((int)((t.k + 63) / 64) - 1)
+    {
+    }
+    // part `quarter` % 4 of group `quarter` / 4, to the one of two buffers that belongs to it
+    __device__ __forceinline__ void load(int quarter, char *buffers) const
+    {
+        const int group = quarter >> 2, part = quarter & 3, i = (int)threadIdx.x % kOnce, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6) % (kOnce / 64);
+        const int word = 4 * group + (i & 3);
+#pragma unroll
+        for (int first = 0; first < kIndices; first += kOnce) {
+            const int index0 = part * (kIndices / 4) + first / 4;
+            const bool second = index0 >= XA;
+            const uint8_t *from = second ? b : a;
+            const int64_t stride = second ? b_stride : a_stride;
+            const int most = second ? b_last : a_last, index = index0 - (second ? XA : 0) + (i >> 2);
+            word_to_lds(from + (uint32_t)(index < most ? index : most) * stride + 4 * (word < last ? word : last),
+                        buffers + (group & 1) * kBytes + 4 * (part * kIndices + first + 64 * wave));
+        }
+    }
+    __device__ __forceinline__ static int word(const char *buffers, int index, int tile)
+    {
+        return *reinterpret_cast<const int *>(buffers + (tile >> 2 & 1) * kBytes + 16 * index + 4 * (tile & 3));
+    }
 };
 
 // The sums of four (`valid`) output elements of a row by fp32 instructions, for fp32 sides.  Not for speed: it runs where a sum is not finite.
@@ -515,8 +590,12 @@ constexpr int stage_bytes() { return (S::XA + S::XB) * S::K * 2 * (sizeof(T) == 
 template <class S, bool A>
 constexpr int side_bytes() { return (A ? S::XA : S::XB) * S::K * 2; }
 // Side b in 8 bits, or both (whose tiles have twice as many terms as S::K says); the scales lie behind them.
+// Whether both sides' scales come in by groups (ScaleGroups): where tiles are large enough for a word an index and tile to be as many lines as the numbers are (32768 x 2048 -> 2048
+// 186 us with words, 160 with groups; 65536 x 512 -> 2048 with gelu, of 128 x 128 tiles, 213 and 200).  The rows of a tile's side have to be less than 2^32 bytes, which is for the launch to see.
+template <class S>
+constexpr bool grouped_scales() { return S::K == 64 && S::STAGES == 2 && S::XA * S::XB >= 128 * 128; }
 template <class S, Eight E>
-constexpr int stage_bytes8() { return S::XA * S::K * 2 + S::XB * S::K * (E == kSideB ? 1 : 2) + 4 * S::kThreads; }
+constexpr int stage_bytes8() { return S::XA * S::K * 2 + S::XB * S::K * (E == kSideB ? 1 : 2) + (E == kBothSides && grouped_scales<S>() ? 0 : 4 * S::kThreads); }
 
 // T: the layer's type.  LAYER: sums go through the layer's epilogue; else they are stored in its type, or as parts of split sums.  WHOLE: an fp32
 // side's rows are whole quads.  EIGHT: the sides that are rows in 8 bits.  Side a goes through registers to two arrays of its own (wide0, wide1), so that its writes do
@@ -537,6 +616,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     constexpr int FA = S::XA / WA / 32, FB = S::XB / WB / 32;
     static_assert(STAGES >= 2 && STAGES <= 4 && (!kFloat || STAGES == 2), "stages");
 
+    constexpr bool kGrouped = EIGHT == kBothSides && grouped_scales<S>();
     constexpr bool kWideA = EIGHT == kSideA || EIGHT == kNoSideApart;
     int ta, tb, split;
     tile_of(block, blocks, t, &ta, &tb, &split);
@@ -550,7 +630,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     const int tiles = left > 0 ? (int)((left + K - 1) / K) : 0;
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
     auto wide = [&](int u) -> char * { return u == 0 ? wide0 : (u == 1 ? wide1 : (u == 2 ? wide2 : wide3)); };
-    using Scales = ScaleFeed<EIGHT == kBothSides ? S::XA : 0, S::XB, kScales ? S::kThreads : S::XA + S::XB, EIGHT == kBothSides && K == 64 ? 4 : 2>;
+    using Scales = ScaleFeed<EIGHT == kBothSides && !kGrouped ? S::XA : 0, S::XB, kScales ? S::kThreads : S::XA + S::XB, EIGHT == kBothSides && K == 64 ? 4 : 2>;
     auto multiply_steps = [&](int u, int tile, int first, int last) {
         const char *la = EIGHT == kSideA ? wide(tile & 1) : (kWideA ? wide(u) : stage(u)), *lb = kWideA ? stage(u) : la + PLANES * kBytesA;
         if constexpr (EIGHT == kSideB) {
@@ -725,6 +805,57 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
             if (at + u >= tiles) break;
             turn(u % STAGES, u & 1, std::false_type{});
         }
+    } else if constexpr (kGrouped) {
+        typename A::NearFeed feed_a;
+        typename B::NearFeed feed_b;
+        ScaleGroups<S::XA, S::XB, S::kThreads> scales(t, n0, m0);
+        feed_a.start(t.a, n0, k0), feed_b.start(t.b, m0, k0);
+        auto load = [&](int u, auto whole) {
+            if constexpr (decltype(whole)::value) feed_a.load_whole(stage(u)), feed_b.load_whole(stage(u) + kBytesA);
+            else feed_a.load(left, stage(u)), feed_b.load(left, stage(u) + kBytesA);
+            left -= K;
+        };
+        int sa[FA], sb[FB];
+        // (half a wave gives the first block's scales, the other the second's: its byte of a word is moved to where the instruction looks)
+        auto multiply_eight = [&](int u, auto step) {
+            constexpr int kStep = decltype(step)::value, kByte = 2 * kStep;
+            i8v a[FA], b[FB];
+#pragma unroll
+            for (int j = 0; j < FB; ++j) b[j] = read_eight<B>(stage(u) + kBytesA, wb + 32 * j, kStep, lane);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) a[i] = read_eight<A>(stage(u), wa + 32 * i, kStep, lane);
+            if constexpr (kStep == 0) {
+#pragma unroll
+                for (int j = 0; j < FB; ++j) sb[j] >>= 8 * (lane >> 5);
+#pragma unroll
+                for (int i = 0; i < FA; ++i) sa[i] >>= 8 * (lane >> 5);
+            }
+#pragma unroll
+            for (int i = 0; i < FA; ++i)
+#pragma unroll
+                for (int j = 0; j < FB; ++j) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i], b[j], acc[i][j], 0, 0, kByte, sa[i], kByte, sb[j]);
+        };
+        if (tiles > 0)  // (a side of no terms has no scales)
+            for (int q = 0; q < 4; ++q) scales.load(q, wide0);
+        load(0, std::false_type{});
+        // (a tile's scales are read in front of what is requested: behind it, the compiler would wait for that)
+        auto turn = [&](int u, int tile, auto whole) {
+            stage_ready<0>();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < FB; ++j) sb[j] = scales.word(wide0, S::XA + wb + 32 * j + (lane & 31), tile);
+#pragma unroll
+            for (int i = 0; i < FA; ++i) sa[i] = scales.word(wide0, wa + 32 * i + (lane & 31), tile);
+            __builtin_amdgcn_sched_barrier(0);
+            load(1 - u, whole);
+            scales.load(tile + 4, wide0);
+            multiply_eight(u, std::integral_constant<int, 0>{});
+            multiply_eight(u, std::integral_constant<int, 1>{});
+        };
+        int at = 0;
+        for (const int whole = (int)((k1 - k0) / K); at + 3 <= whole; at += 2) turn(0, at, std::true_type{}), turn(1, at + 1, std::true_type{});
+        for (; at + 2 <= tiles; at += 2) turn(0, at, std::false_type{}), turn(1, at + 1, std::false_type{});
+        if (at < tiles) turn(0, at, std::false_type{});
     } else {
         typename A::template Feed<E> feed_a;
         typename B::template Feed<E> feed_b;

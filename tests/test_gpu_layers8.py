@@ -287,6 +287,19 @@ def test_rows_that_lie_far_apart(shape):
         features.linear_backward(again, c.dy)
 
 
+@pytest.mark.parametrize("side", ["x", "w"])
+def test_both_sides_in_8_bits_far_apart(side):
+    """More bytes between rows than the largest tiles address with 32 bits."""
+    from cuke_amd import features
+    c = Layer8(8200 if side == "w" else 900, 520, 776 if side == "w" else 8200, torch.bfloat16, "gelu", eight=True)
+    old = getattr(c, side)
+    base = torch.empty((old.q.shape[0] - 1) * (1 << 24) + old.q.shape[1], dtype=torch.uint8, device=DEV)
+    q = base.as_strided(old.q.shape, (1 << 24, 1))
+    q.copy_(old.q.view(torch.uint8))
+    setattr(c, side, features.Rows8(q.view(E4M3), old.scale, old.cols))
+    within(features.linear(c.x, c.w, c.b, dtype=c.dtype, **c.kw()), c.y, c.y_tol, side)
+
+
 def test_on_another_stream_and_in_two_graphs():
     from cuke_amd import features
     small, large = Layer8(300, 200, 136, torch.float16, "silu", drop=0.2, residual=True), Layer8(2100, 520, 264, torch.bfloat16, "gelu", drop=0.1, residual=True)
