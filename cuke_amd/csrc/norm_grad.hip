@@ -34,7 +34,7 @@ struct Held {
 
 // A workgroup takes a range of rows, each held by `lanes` lanes (WAVES: by two or four waves); what the next row needs is requested while the present one is worked on.  A lane's
 // columns are the same in all rows, so dweight's sums wait in registers until the range's end.
-// Bound by memory: 65536 x 2048 bf16 with dh (1.07 GB) GRAD_US.
+// Bound by memory: 65536 x 2048 bf16 with dh and rest (1.14 GB) 230 us, 5.0 TB/s; 4096 x 1024 (36 MB, in the caches) 8, and 2.4 for the joining of dweight's sums.
 template <class T, class D, int C, bool WAVES, bool DH, bool REST>
 __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 {
