@@ -967,6 +967,9 @@ PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t)
     if (!rows_of(h, n.type, n.rows, n.cols, dev, &h_stride) || dy_type < 0 || !rows_of(dy, dy_type, n.rows, n.cols, dev, &dy_stride)) NOT_HERE;
     if (!vector_of(rstd, KGE_F32, n.rows, dev) || (args[3] != Py_None && !vector_of(w, n.type, n.cols, dev))) NOT_HERE;
     if (args[5] != Py_None && !rows_of(dh, n.type, n.rows, n.cols, dev, &dh_stride)) NOT_HERE;
+    if (rest && (!rest->is_cuda() || rest->device().index() != dev || rest->scalar_type() != at::kInt || !rest->is_contiguous() || rest->dim() != 2 ||
+                 rest->size(0) != n.rows || rest->size(1) != (n.cols + 7) / 8))
+        NOT_HERE;
     n.weight = args[3] != Py_None ? w->data_ptr() : nullptr;
     const auto opt = h->options().requires_grad(false);
     at::Tensor dx, dw;

@@ -295,7 +295,7 @@ static int forward8(const kge_linear *l, const kge_rows8 *x8, const kge_rows8 *w
         t.a = Side{w8->q, w8->q_stride / 2, l->out};
         t.k = t.k8;
     } else if (w8) {
-        if (!p.few) launch_unpack8(l->type, t.a8, l->out, up8(l->in), pw, pitch_of(l->type, l->in), st);
+        if (!p.few && l->in > 0) launch_unpack8(l->type, t.a8, l->out, up8(l->in), pw, pitch_of(l->type, l->in), st);
         t.a = Side{pw, pitch_of(l->type, l->in), l->out};
     } else {
         if (p.pack_w && (keep || !p.few)) launch_pack(l, false, true, nullptr, pw, st);

@@ -545,18 +545,23 @@ def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_we
     got = _lib.host().rms_norm_backward(fw.h, fw.rstd, fw.rest, fw.weight, dy, dh, need_x, need_weight)
     if got is not None:
         return NormGrads(*got)
-    h, weight = _tensor(fw.h, "h of the forward call", 2), fw.weight
+    h, weight, rest = _rows(fw.h, "h of the forward call"), fw.weight, fw.rest
     dy = _rows(dy, "dy", shape=h.shape)
     if dh is not None:
         dh = _rows(dh, "dh", h.dtype, shape=h.shape)
     rows, cols = h.shape
+    rstd = _rows(fw.rstd, "rstd of the forward call", torch.float32, ndim=1, shape=(rows,))
+    if weight is not None:
+        weight = _rows(weight, "weight of the forward call", h.dtype, ndim=1, shape=(cols,))
+    if rest is not None:
+        rest = _rows(rest, "rest of the forward call", torch.int32, shape=(rows, -(-cols // 8))).contiguous()
     dx = torch.empty((rows, cols), dtype=h.dtype, device=h.device) if need_x else None
     dw = torch.empty(cols, dtype=h.dtype, device=h.device) if need_weight and weight is not None else None
     desc = _lib.RmsNorm(_TYPES[h.dtype], _TYPES[h.dtype], rows, cols, None, 0, None, 0, _p(weight), 0.0)
     L = _lib.lib()
     ws_bytes = int(L.kge_rms_norm_bwd_workspace(C.byref(desc))) if dw is not None else 0
     ws = _bytes(ws_bytes, h.device)
-    _lib.check(L.kge_rms_norm_bwd(C.byref(desc), _p(h), _row_stride(h), _p(fw.rstd), _p(fw.rest), _TYPES[dy.dtype], _p(dy), _row_stride(dy), _p(dh),
+    _lib.check(L.kge_rms_norm_bwd(C.byref(desc), _p(h), _row_stride(h), _p(rstd), _p(rest), _TYPES[dy.dtype], _p(dy), _row_stride(dy), _p(dh),
                                   _row_stride(dh) if dh is not None else 0, _p(dx), cols, _p(dw), _p(ws), ws_bytes, _stream()), "kge_rms_norm_bwd")
     return NormGrads(dx, dw)
 

@@ -211,7 +211,7 @@ def test_derivatives_reach_their_ends():
 @pytest.mark.parametrize("dtype", HALF)
 def test_layers_of_nothing(dtype):
     from cuke_amd import features
-    for rows, fin, fout in [(0, 8, 8), (5, 0, 8), (5, 8, 0), (0, 0, 0), (0, 8, 0)]:
+    for rows, fin, fout in [(0, 8, 8), (5, 0, 8), (5, 8, 0), (0, 0, 0), (0, 8, 0), (2000, 0, 1000), (9000, 0, 800)]:
         x, w = features.pack8(torch.randn(rows, fin, device=DEV)), torch.randn(fout, fin, device=DEV).to(dtype)
         b = torch.randn(fout, device=DEV).to(dtype)
         want = torch.nn.functional.silu(b.double()).expand(rows, fout)
@@ -403,6 +403,21 @@ def test_encoder_against_its_own_operators(dtype, given8):
         assert torch.equal(b.norm, gn.weight) and torch.equal(b.w1, ga.weight) and torch.equal(b.b1, ga.bias) and torch.equal(b.w2, go.weight) and torch.equal(b.b2, go.bias)
         d = gn.x
     assert back.first.x.shape == (301, 60) and back.first.weight.shape == enc.w_in.shape
+
+
+def test_encoder_without_blocks():
+    from cuke_amd import features as f
+    enc = encoder(torch.bfloat16)
+    enc = f.ResidualEncoder(enc.w_in, enc.b_in, [], enc.norm, enc.w_out, enc.b_out)
+    g = torch.Generator().manual_seed(6)
+    x, drows = torch.randn(301, 60, generator=g).to(DEV).bfloat16(), torch.randn(301, 50, generator=g).to(DEV)
+    fw = enc.forward(x)
+    assert torch.equal(enc.encode(x), fw.rows)
+    n = f.rms_norm_forward(f.linear(x, enc.w_in, enc.b_in), enc.norm, out_dtype=E4M3)
+    last = f.linear_forward(n.y, enc.w_out, enc.b_out, out_dtype=torch.float32)
+    back, gl = enc.backward(fw, drows), f.linear_backward(last, drows)
+    assert torch.equal(last.y, fw.rows) and back.blocks == [] and torch.equal(back.last.weight, gl.weight)
+    assert torch.equal(back.norm, f.rms_norm_backward(n, gl.x).weight) and enc.packed().encode(x).shape == (301, 50)
 
 
 def test_encoder_against_64_bits():

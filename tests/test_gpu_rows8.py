@@ -9,6 +9,7 @@ element, from the roundings a result goes through (u: half a step of a type, eps
   dweight  (M + 8) eps sum |dy n| and u |dweight|
 """
 import ctypes as C
+import dataclasses
 
 import numpy as np
 import pytest
@@ -350,6 +351,11 @@ def test_norm_refuses():
     for dy, dh, error in ((x[:3], None, ValueError), (x.int(), None, TypeError), (x, x.half(), TypeError), (x, x[:, :7], ValueError)):
         with pytest.raises(error):
             features.rms_norm_backward(fw, dy, dh)
+    fw = features.rms_norm_forward(x.bfloat16(), w.bfloat16(), x.bfloat16())
+    for name, bad, error in (("rest", fw.rest[:3], ValueError), ("rest", fw.rest.float(), TypeError), ("rstd", fw.rstd[:3], ValueError),
+                             ("rstd", fw.rstd.double(), TypeError), ("rest", fw.rest.cpu(), KgeError), ("weight", fw.weight[:7], ValueError), ("h", fw.h[:, :7], ValueError)):
+        with pytest.raises(error):
+            features.rms_norm_backward(dataclasses.replace(fw, **{name: bad}), x)
 
 
 def test_on_another_stream_and_in_a_graph():
