@@ -87,23 +87,31 @@ __device__ __forceinline__ void place_in_rows(int lanes, int *lane, uint32_t *gr
     if (WAVES) *group = (uint32_t)__builtin_amdgcn_readfirstlane((int)*group);
 }
 
-// What a sum loses when it is rounded to 16 bits, in sixteenths of a step of the result there, -8 .. 7: four bits an element, eight of a row in a word.  With it the
-// gradients are those of the sum itself, to 2^-13: from the rounded one alone dweight would be off by 1.4 times its own rounding, and dx of short rows,
-// where g - n mean(g n) cancels, by several times.
-template <class T>
-__device__ __forceinline__ int step_exponent(float h)  // of 1/16 of a step of T at h
+// What a sum loses when it is rounded to 16 bits, in sixteenths of a step, -8 .. 7: four bits an element, eight of a row in a word.  bf16: the difference of the two numbers'
+// bits, in units of 2^12 (a step at the sum: below a power of two that it was rounded up to, half of the step there); fp16, whose small numbers are evenly spaced: in sixteenths
+// of the step at the result.  With it the gradients are those of the sum itself, to 2^-13: from the rounded one alone dweight would be off by 1.4 times its own rounding, and dx of short
+// rows, where g - n mean(g n) cancels, by several times.
+__device__ __forceinline__ int step_exponent(float h)  // of 1/16 of a step of fp16 at h
 {
-    const int e = (int)(__float_as_uint(h) >> 23 & 0xFF), least = std::is_same<T, bf16_t>::value ? 1 : 113;
-    return (e > least ? e : least) - 127 - (std::is_same<T, bf16_t>::value ? 11 : 14);
+    const int e = (int)(__float_as_uint(h) >> 23 & 0xFF);
+    return (e > 113 ? e : 113) - 127 - 14;
 }
 template <class T>
 __device__ __forceinline__ uint32_t rest_of(const float (&sum)[8])
 {
     uint32_t word = 0;
+    if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t lost = __float_as_uint(sum[e]) - __float_as_uint((float)(T)sum[e]), q = (lost + 0x8800u) >> 12;  // (rounded, and 8 more; of a tie downwards 16)
+            word |= (q < 15u ? q : 15u) << (4 * e);
+        }
+        return word ^ 0x88888888u;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const float h = (float)(T)sum[e];
-        const float q = rintf(__builtin_amdgcn_ldexpf(sum[e] - h, -step_exponent<T>(h)));  // (of what is not finite NaN, and -8 below, which changes neither)
+        const float q = rintf(__builtin_amdgcn_ldexpf(sum[e] - h, -step_exponent(h)));  // (of what is not finite NaN, and -8 below, which changes neither)
         word |= ((uint32_t)(int)fminf(fmaxf(q, -8.0f), 7.0f) & 15u) << (4 * e);
     }
     return word;
@@ -111,10 +119,16 @@ __device__ __forceinline__ uint32_t rest_of(const float (&sum)[8])
 template <class T>
 __device__ __forceinline__ void add_rest(float (&h)[8], uint32_t word)
 {
+    if constexpr (std::is_same<T, bf16_t>::value) {
+        word ^= 0x88888888u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = __uint_as_float(__float_as_uint(h[e]) - 0x8000u + ((word >> (4 * e) & 15u) << 12));  // (NaN stays NaN)
+        return;
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int q = (int)(word << (28 - 4 * e)) >> 28;
-        h[e] += __builtin_amdgcn_ldexpf((float)q, step_exponent<T>(h[e]));
+        h[e] += __builtin_amdgcn_ldexpf((float)q, step_exponent(h[e]));
     }
 }
 

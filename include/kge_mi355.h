@@ -678,7 +678,8 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
  * x, residual, weight and h have the type `type`; y any kge_type_t, or KGE_E4M3: rows in 8 bits (`y8`; else y, y_stride).  h (NULL: not wanted) is the sum
  * rounded to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32.  Squares are summed in 64 bits, so that no value of a type
  * overflows; a value in 8 bits is the one nearest to the 64-bit result.  rest (NULL: not wanted; KGE_F32: not looked at): 4 ceil(cols / 8) bytes a row, 4-byte
- * aligned, what rounding took from h, in 16ths of a step of `type`: four bits an element.
+ * aligned, what rounding took from h, four bits an element, from -8 to 7: KGE_BF16: the fp32 bits of the sum less those of h, in units of 2^12; KGE_F16: in
+ * 16ths of a step at h.
  * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
  *   g = dy weight,   dx = dresidual = r (g - h r^2 mean_j(g h)) + dh,   dweight[j] = sum_i dy[i][j] h[i][j] r[i]
  * h: what the forward call wrote there (x where there was no residual), rstd and rest too (NULL: the gradients are those of h as it was rounded).  dx [rows, cols]

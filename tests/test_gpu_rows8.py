@@ -321,17 +321,73 @@ def test_what_a_sum_loses_is_kept(dtype):
         assert fw.rest.shape == (40, -(-cols // 8))
         bits = (fw.rest.view(40, -1, 1) << torch.arange(28, -4, -4, device=DEV, dtype=torch.int32)) >> 28
         bits = bits.view(40, -1)[:, :cols].double()
-        step = torch.exp2(torch.floor(torch.log2(fw.h.double().abs().clamp(min=2.0 ** -140)))) * 2 * U[dtype] * (1 if dtype == torch.float16 else 1)
-        if dtype == torch.float16:
-            step = step.clamp(min=2.0 ** -24)
         want = x.double() + res.double()
-        assert bool(((fw.h.double() + bits * step / 16 - want).abs() <= step / 16 * 1.001 + EPS * want.abs() + 2.0 ** -130).all()), (dtype, cols)
+        step = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=2.0 ** -140)))) * 2 * U[dtype]
+        if dtype == torch.float16:
+            step = torch.exp2(torch.floor(torch.log2(fw.h.double().abs().clamp(min=2.0 ** -140)))) * 2 * U[dtype]
+            step = step.clamp(min=2.0 ** -24)
+            got = fw.h.double() + bits * step / 16
+        else:
+            got = (fw.h.float().view(torch.int32) + bits.int() * 4096).view(torch.float32).double()
+        assert bool(((got - want).abs() <= step / 16 * 1.001 + EPS * want.abs() + 2.0 ** -130).all()), (dtype, cols)
     c = Norm(33, 70, dtype)
     fw = c.forward()
     fw.rest = None
     got = features.rms_norm_backward(fw, c.dy, c.dh)
     c.h, c.res = fw.h.double(), None                             # (r stays that of the sum)
     c.check_backward(fw, got, "rounded")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_nothing_is_written_beside_rows(dtype):
+    """Columns behind a row's end, rows behind the last one: left as they were, by every array of the C calls."""
+    from cuke_amd import _lib, features
+    L, st, code = _lib.lib(), torch.cuda.current_stream().cuda_stream, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]
+    for rows, cols in ((5, 77), (3, 1027), (2, 9001), (4, 64)):
+        c = Norm(rows, cols, dtype)
+        want = features.rms_norm_forward(c.x, c.w, c.res)
+        e = features.rms_norm(c.x, c.w, out_dtype=E4M3)
+        canary = lambda r, n, t: torch.full((r, n), 0x5A, dtype=torch.uint8, device=DEV).view(t)
+        size = c.x.element_size()
+        y, h = canary(rows + 2, (cols + 9) * size, dtype), canary(rows + 2, (cols + 11) * size, dtype)
+        rstd, rest = canary(1, 4 * (rows + 2), torch.float32), canary(rows + 2, 4 * (-(-cols // 8)), torch.int32)
+        q, scale = canary(rows + 2, e.q.shape[1] + 32, torch.uint8), canary(rows + 2, e.scale.shape[1] + 8, torch.uint8)
+        d = _lib.RmsNorm(code, code, rows, cols, c.x.data_ptr(), cols, c.res.data_ptr(), cols, c.w.data_ptr(), 1e-6)
+        assert L.kge_rms_norm_fwd(C.byref(d), y.data_ptr(), cols + 9, None, h.data_ptr(), cols + 11, rstd.data_ptr(), rest.data_ptr(), st) == 0
+        assert torch.equal(y[:rows, :cols], want.y) and torch.equal(h[:rows, :cols], want.h) and torch.equal(rstd[0, :rows], want.rstd)
+        untouched = lambda t, keep: bool((t.view(torch.uint8)[keep(t.view(torch.uint8))] == 0x5A).all())
+
+        def beside(width):
+            def keep(t):
+                m = torch.ones_like(t, dtype=torch.bool)
+                m[:rows, :width] = False
+                return m
+            return keep
+        assert untouched(y, beside(cols * size)) and untouched(h, beside(cols * size)) and bool((rstd[0, rows:].view(torch.uint8) == 0x5A).all())
+        assert untouched(rest, beside(rest.shape[1] * 4 if dtype != torch.float32 else 0))
+        r8 = _lib.Rows8(q.data_ptr(), q.shape[1], scale.data_ptr(), scale.shape[1])
+        for call in ("norm", "pack"):
+            q.fill_(0x5A), scale.fill_(0x5A)
+            if call == "norm":
+                d = _lib.RmsNorm(code, _lib.E4M3, rows, cols, c.x.data_ptr(), cols, None, 0, c.w.data_ptr(), 1e-6)
+                assert L.kge_rms_norm_fwd(C.byref(d), None, 0, C.byref(r8), None, 0, None, None, st) == 0
+                same = e
+            else:
+                assert L.kge_pack8(code, c.x.data_ptr(), cols, rows, cols, C.byref(r8), st) == 0
+                same = features.pack8(c.x)
+            assert torch.equal(q[:rows, :e.q.shape[1]], same.q.view(torch.uint8)) and torch.equal(scale[:rows, :e.scale.shape[1]], same.scale.view(torch.uint8))
+            assert untouched(q, beside(e.q.shape[1])) and untouched(scale, beside(e.scale.shape[1]))
+        assert L.kge_unpack8(C.byref(r8), rows, cols, code, y.fill_(7).data_ptr(), cols + 9, st) == 0
+        assert torch.equal(y[:rows, :cols], features.unpack8(features.pack8(c.x), dtype)) and bool((y[rows:] == 7).all()) and bool((y[:, cols:] == 7).all())
+        g = features.rms_norm_backward(want, c.dy, c.dh)
+        d = _lib.RmsNorm(code, code, rows, cols, None, 0, None, 0, c.w.data_ptr(), 0.0)
+        n = L.kge_rms_norm_bwd_workspace(C.byref(d))
+        ws, dw = canary(1, n + 64, torch.uint8), canary(1, (cols + 5) * size, dtype)
+        y.fill_(7)
+        assert L.kge_rms_norm_bwd(C.byref(d), want.h.data_ptr(), cols, want.rstd.data_ptr(), want.rest.data_ptr() if want.rest is not None else None, code, c.dy.data_ptr(), cols,
+                                  c.dh.data_ptr(), cols, y.data_ptr(), cols + 9, dw.data_ptr(), ws.data_ptr(), n, st) == 0
+        assert torch.equal(y[:rows, :cols], g.x) and bool((y[rows:] == 7).all()) and bool((y[:, cols:] == 7).all())
+        assert torch.equal(dw[0, :cols], g.weight) and bool((dw.view(torch.uint8)[0, cols * size:] == 0x5A).all()) and bool((ws[0, n:] == 0x5A).all())
 
 
 def test_norm_refuses():
