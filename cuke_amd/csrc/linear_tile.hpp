@@ -612,7 +612,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     using B = Tile<S::XB, EIGHT == kSideB ? K / 2 : K, B_ACROSS, S::kThreads>;  // (of a side in 8 bits that goes to LDS as it lies: elements are pairs of terms)
     constexpr int kBytesA = S::XA * K * 2, kBytesB = S::XB * K * (EIGHT == kSideB ? 1 : 2), kStage = EIGHT == kSideB ? kBytesA + kBytesB : stage_bytes<T, S>();
     constexpr bool kScales = EIGHT == kSideB || EIGHT == kBothSides;
-    static_assert(EIGHT == kNoSide || (!kFloat && SHARE == 1 && (!kScales || (!A_ACROSS && !B_ACROSS)) && (EIGHT != kSideB || K == 64)), "sides in 8 bits");
+    static_assert(EIGHT == kNoSide || (!kFloat && SHARE == 1 && (!kScales || (!A_ACROSS && !B_ACROSS)) && (!kScales || K == 64)), "sides in 8 bits");
     constexpr int FA = S::XA / WA / 32, FB = S::XB / WB / 32;
     static_assert(STAGES >= 2 && STAGES <= 4 && (!kFloat || STAGES == 2), "stages");
 
@@ -630,7 +630,7 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
     const int tiles = left > 0 ? (int)((left + K - 1) / K) : 0;
     auto stage = [&](int u) -> char * { return u == 0 ? stage0 : (u == 1 ? stage1 : (u == 2 ? stage2 : stage3)); };
     auto wide = [&](int u) -> char * { return u == 0 ? wide0 : (u == 1 ? wide1 : (u == 2 ? wide2 : wide3)); };
-    using Scales = ScaleFeed<EIGHT == kBothSides && !kGrouped ? S::XA : 0, S::XB, kScales ? S::kThreads : S::XA + S::XB, EIGHT == kBothSides && K == 64 ? 4 : 2>;
+    using Scales = ScaleFeed<EIGHT == kBothSides && !kGrouped ? S::XA : 0, S::XB, kScales ? S::kThreads : S::XA + S::XB, EIGHT == kBothSides ? 4 : 2>;
     auto multiply_steps = [&](int u, int tile, int first, int last) {
         const char *la = EIGHT == kSideA ? wide(tile & 1) : (kWideA ? wide(u) : stage(u)), *lb = kWideA ? stage(u) : la + PLANES * kBytesA;
         if constexpr (EIGHT == kSideB) {
@@ -885,18 +885,11 @@ __device__ __forceinline__ void compute_tile(const TileArgs &t, int64_t block, i
                     load((u + STAGES - 1) % STAGES, std::true_type{});
                     multiply(u, at + u);
                 }
-        // (both sides in 8 bits: nothing moves over these lines, which in the largest tiles would cost a register more than there are)
-        auto keep_order = [] {
-            if constexpr (EIGHT == kBothSides) __builtin_amdgcn_sched_barrier(0);
-        };
-        keep_order();
         for (; at + STAGES <= tiles; at += STAGES)
 #pragma unroll
             for (int u = 0; u < STAGES; ++u) {
                 stage_ready<kLoads * (STAGES - 2)>();
-                keep_order();
                 load((u + STAGES - 1) % STAGES, std::false_type{});
-                keep_order();
                 multiply(u, at + u);
             }
 #pragma unroll
