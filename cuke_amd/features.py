@@ -393,6 +393,21 @@ def preference_loss(pos, neg, ref_pos=None, ref_neg=None, *, beta=1.0, kind="sig
 E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
+def _fits8(q, scale, cols) -> bool:
+    if not (isinstance(q, torch.Tensor) and isinstance(scale, torch.Tensor) and q.dtype is E4M3 and scale.dtype is _E8M0 and cols >= 0):
+        return False
+    shape = q.shape
+    return len(shape) == 2 and shape[1] == -(-cols // 32) * 32 and scale.shape == (shape[0], -(-cols // 128) * 4)
+
+
+def _refuse8(q, scale, cols):
+    for t, name, dtype, width in ((q, "q", E4M3, -(-cols // 32) * 32), (scale, "scale", _E8M0, -(-cols // 128) * 4)):
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+            raise TypeError(f"{name} must be a tensor of {dtype} (got {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__})")
+        if cols < 0 or t.dim() != 2 or t.shape[1] != width or t.shape[0] != q.shape[0]:
+            raise ValueError(f"rows of {cols} values need {name} of shape {(q.shape[0] if q.dim() else 0, width)} (got {tuple(t.shape)})")
+
+
 class Rows8:
     """Rows of ``cols`` values in 8 bits: e4m3 numbers and one power of two for each 32 columns, a value being their product.
 
@@ -401,11 +416,8 @@ class Rows8:
     __slots__ = ("q", "scale", "cols")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, cols: int):
-        for t, name, dtype, width in ((q, "q", E4M3, -(-cols // 32) * 32), (scale, "scale", _E8M0, -(-cols // 128) * 4)):
-            if not isinstance(t, torch.Tensor) or t.dtype != dtype:
-                raise TypeError(f"{name} must be a tensor of {dtype} (got {t.dtype if isinstance(t, torch.Tensor) else type(t).__name__})")
-            if cols < 0 or t.dim() != 2 or t.shape[1] != width or t.shape[0] != q.shape[0]:
-                raise ValueError(f"rows of {cols} values need {name} of shape {(q.shape[0] if q.dim() else 0, width)} (got {tuple(t.shape)})")
+        if not _fits8(q, scale, cols):
+            _refuse8(q, scale, cols)
         self.q, self.scale, self.cols = q, scale, int(cols)
 
     @property
