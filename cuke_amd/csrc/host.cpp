@@ -958,7 +958,7 @@ PyObject *py_rms_norm(PyObject *, PyObject *const *args, Py_ssize_t)
     END_HANDLE_TH_ERRORS
 }
 
-// rms_norm_backward(h, rstd, rest, weight, dy, dh, need x, need weight) -> (dx, dweight), or None.  h, rstd, rest and weight are those of the forward call.
+// rms_norm_backward(h, rstd, rest, weight, dy, dh, need x, need weight, eps) -> (dx, dweight), or None.  All but dy and dh are of the forward call.
 PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t)
 {
     HANDLE_TH_ERRORS
@@ -977,6 +977,7 @@ PyObject *py_rms_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t)
     if (rest && (!rest->is_cuda() || rest->device().index() != dev || rest->scalar_type() != at::kInt || !rest->is_contiguous() || rest->dim() != 2 ||
                  rest->size(0) != n.rows || rest->size(1) != (n.cols + 7) / 8))
         NOT_HERE;
+    if (!number(args[8], &n.eps) || !(n.eps >= 0.0 && n.eps < 1e300)) NOT_HERE;
     n.weight = args[3] != Py_None ? w->data_ptr() : nullptr;
     at::Tensor dx, dw;
     if (PyObject_IsTrue(args[6])) dx = fresh({n.rows, n.cols}, h->scalar_type());

@@ -1,5 +1,6 @@
 // Gradients of the root-mean-square norm (kge_rms_norm_bwd).  With n = h r and g = dy weight:
 //   dx = r (g - n mean(g n)) + dh,   dweight = sum over rows of dy n
+#include <algorithm>
 #include <type_traits>
 
 #include "linear_tile.hpp"
@@ -17,6 +18,7 @@ struct NormGradArgs {
     int64_t dx_stride;
     float *sums;  // [ranges][4 quads]: dweight's over a range of rows, or NULL
     int lanes;
+    double eps;
 };
 
 // Eight elements as they lie in memory, requested ahead of their use.  A row's last piece is moved back to end with the row (rows of at least eight columns), so that
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
     }
 }
 
-// Rows that registers do not hold, and those of fewer than eight columns: dx by a workgroup that goes over a row twice.
+// Rows that registers do not hold, and those of two to seven columns: dx by a workgroup that goes over a row twice.
 template <class T, class D>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
 {
@@ -210,6 +212,20 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
             for (int e = 0; e < 8; ++e) d[e] = fmaf(r, g[e] - n[e] * mean, d[e]);
             store8(static_cast<T *>(a.dx) + row * a.dx_stride + col, d, valid);
         }
+    }
+}
+// dx of rows of one column, where g - n mean(g n) = g (1 - n^2) = g eps r^2: the difference of two nearly equal numbers (eps 1e-6: of fp32's digits one or two are left), the
+// product of what is known.  A thread a row.
+template <class T, class D>
+__global__ __launch_bounds__(256) void rms_norm_grad_one_kernel(NormGradArgs a)
+{
+    const double w = a.weight ? (double)(float)*static_cast<const T *>(a.weight) : 1.0;
+    for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
+        const double h = (double)(float)static_cast<const T *>(a.h)[row * a.h_stride], r = (double)a.rstd[row];
+        double d = a.eps * r * r * r * w * (double)(float)static_cast<const D *>(a.dy)[row * a.dy_stride];
+        d += 0.0 * h;  // (of what is not finite NaN, as the difference would be)
+        if (a.dh) d += (double)(float)static_cast<const T *>(a.dh)[row * a.dh_stride];
+        static_cast<T *>(a.dx)[row * a.dx_stride] = (T)(float)d;
     }
 }
 // dweight's sums over ranges of rows, of such rows: eight columns a thread
@@ -274,7 +290,8 @@ static void launch_grads(const NormGradArgs &args, const Ranges &ranges, void *d
     if (hold.pieces == 0) {
         // (the sums first: dx may take the place of dy)
         if (a.sums) hipLaunchKernelGGL((rms_norm_long_sums_kernel<T, D>), dim3((unsigned)ceil_div(a.cols, 2048), (unsigned)ranges.count), block, 0, st, a);
-        if (a.dx) hipLaunchKernelGGL((rms_norm_grad_long_kernel<T, D>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), block, 0, st, a);
+        if (a.dx && a.cols == 1) hipLaunchKernelGGL((rms_norm_grad_one_kernel<T, D>), dim3((unsigned)std::min<int64_t>(ceil_div(a.rows, 256), 1 << 20)), block, 0, st, a);
+        else if (a.dx) hipLaunchKernelGGL((rms_norm_grad_long_kernel<T, D>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), block, 0, st, a);
     } else {
         with_hold(hold, [&](auto pieces, auto waves) {
             constexpr int kPieces = decltype(pieces)::value;
@@ -323,7 +340,7 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;
     const Ranges ranges = norm->rows ? ranges_of(norm->rows, norm->cols) : Ranges{1, 0};
     const NormGradArgs a{h, dy, dh, norm->weight, h_stride, dy_stride, dh_stride, rstd, static_cast<const uint32_t *>(rest), norm->rows, norm->cols, ceil_div(norm->cols, 4), ranges.rows_each,
-                         dx, dx_stride, dweight ? static_cast<float *>(workspace) : nullptr, 0};
+                         dx, dx_stride, dweight ? static_cast<float *>(workspace) : nullptr, 0, norm->eps};
     hipStream_t st = as_stream(stream);
     KGE_CLEAR_LAUNCH_ERRORS();
     if (norm->rows == 0) {  // (dweight is an empty sum)

@@ -494,6 +494,7 @@ class NormForward:
     rstd: torch.Tensor  # float32 [rows]
     weight: torch.Tensor | None
     rest: torch.Tensor | None = None  # int32 [rows, ceil(cols / 8)]: what h lost when it was rounded to 16 bits, in four bits an element
+    eps: float = 1e-6
 
 
 @dataclass
@@ -506,7 +507,7 @@ def _norm_call(x, weight, residual, eps, out_dtype, keep):
     got = _lib.host().rms_norm(x, weight, residual, eps, out_dtype, keep)
     if got is not None:
         y, scale, h, rstd, rest = got
-        return NormForward(y if scale is None else _made8(y, scale, x.shape[1]), x if h is None else h, rstd, weight, rest)
+        return NormForward(y if scale is None else _made8(y, scale, x.shape[1]), x if h is None else h, rstd, weight, rest, float(eps))
     x = _rows(x, "x")
     rows, cols = x.shape
     if weight is not None:
@@ -528,7 +529,7 @@ def _norm_call(x, weight, residual, eps, out_dtype, keep):
                         _row_stride(residual) if residual is not None else 0, _p(weight), eps)
     _lib.check(_lib.lib().kge_rms_norm_fwd(C.byref(desc), None if eight else _p(y), cols, C.byref(_rows8_c(y)) if eight else None, _p(h), cols,
                                            _p(rstd), _p(rest), _stream()), "kge_rms_norm_fwd")
-    return NormForward(y, x if h is None else h, rstd, weight, rest)
+    return NormForward(y, x if h is None else h, rstd, weight, rest, eps)
 
 
 def rms_norm(x, weight=None, residual=None, *, eps=1e-6, out_dtype=None):
@@ -554,7 +555,7 @@ def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_we
     the residual is that of x.  An 8-bit y's rounding counts as none."""
     if not isinstance(fw, NormForward):
         raise TypeError("fw must come from rms_norm_forward()")
-    got = _lib.host().rms_norm_backward(fw.h, fw.rstd, fw.rest, fw.weight, dy, dh, need_x, need_weight)
+    got = _lib.host().rms_norm_backward(fw.h, fw.rstd, fw.rest, fw.weight, dy, dh, need_x, need_weight, fw.eps)
     if got is not None:
         return NormGrads(*got)
     h, weight, rest = _rows(fw.h, "h of the forward call"), fw.weight, fw.rest
@@ -569,7 +570,7 @@ def rms_norm_backward(fw: NormForward, dy, dh=None, need_x: bool = True, need_we
         rest = _rows(rest, "rest of the forward call", torch.int32, shape=(rows, -(-cols // 8))).contiguous()
     dx = torch.empty((rows, cols), dtype=h.dtype, device=h.device) if need_x else None
     dw = torch.empty(cols, dtype=h.dtype, device=h.device) if need_weight and weight is not None else None
-    desc = _lib.RmsNorm(_TYPES[h.dtype], _TYPES[h.dtype], rows, cols, None, 0, None, 0, _p(weight), 0.0)
+    desc = _lib.RmsNorm(_TYPES[h.dtype], _TYPES[h.dtype], rows, cols, None, 0, None, 0, _p(weight), fw.eps)
     L = _lib.lib()
     ws_bytes = int(L.kge_rms_norm_bwd_workspace(C.byref(desc))) if dw is not None else 0
     ws = _bytes(ws_bytes, h.device)

@@ -683,7 +683,8 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
  * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
  *   g = dy weight,   dx = dresidual = r (g - h r^2 mean_j(g h)) + dh,   dweight[j] = sum_i dy[i][j] h[i][j] r[i]
  * h: what the forward call wrote there (x where there was no residual), rstd and rest too (NULL: the gradients are those of h as it was rounded).  dx [rows, cols]
- * and dweight [cols] of type `type`, contiguous but for dx's stride; either may be NULL.  The fields x and residual of the description are not looked at.
+ * and dweight [cols] of type `type`, contiguous but for dx's stride; either may be NULL.  The fields x and residual of the description are not looked at; eps is
+ * that of the forward call (of one column dx = eps r^3 g + dh, which is what the difference comes to).
  * Sums over rows are joined in a fixed order.  rows, cols: 0 .. 2^31 - 1 (KGE_ESHAPE beyond).
  * Outputs overlap no input, but that dx may be dy or dh where type and stride are the same.
  */

@@ -1,0 +1,105 @@
+"""The root-mean-square norm where a formula loses its digits or a number its range: rows of one column, rows of the smallest numbers.
+
+Tolerances as in test_gpu_rows8.py (u: half a step of a type, eps = 2^-24, r to 2 eps).  Of one column dx is eps_norm r^3 g, a product whose only error is that of
+r: 6 eps, and its rounding.
+"""
+import ctypes as C
+import dataclasses
+
+import pytest
+import torch
+
+from test_gpu_rows8 import DEV, E4M3, EPS, TINY, TYPES, U, Norm, laid, within
+
+pytestmark = pytest.mark.gpu
+
+CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def one_column(c):
+    """(dx, its tolerance) of a Norm of one column."""
+    dx = c.eps * c.r ** 3 * c.dy.double() * c.w64
+    tol = 8 * EPS * dx.abs()
+    if c.dh is not None:
+        dx, tol = dx + c.dh.double(), tol + 2 * EPS * c.dh.double().abs()
+    return dx, tol + U[c.dtype] * (dx.abs() + tol) + TINY[c.dtype]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dy", TYPES)
+@pytest.mark.parametrize("weight", [False, True])
+def test_gradients_of_one_column(dtype, dy, weight):
+    """Two nearly equal terms leave some 1e-6 of themselves: of each row as exact as of longer ones."""
+    from cuke_amd import features
+    for rows in (1, 10, 257, 5000):
+        for eps in (1e-6, 1e-2, 0.0, 7.0):
+            for layout in ("plain", "apart"):
+                c = Norm(rows, 1, dtype, residual=False, weight=weight, dy=dy, layout=layout, eps=eps)
+                print("one column", dtype, dy, rows, eps, layout, flush=True)
+                c.x.masked_fill_(c.x == 0, 1.0)
+                c.h = c.x.double()
+                c.r = (c.h.square() + eps).rsqrt()
+                fw = c.forward()
+                g = features.rms_norm_backward(fw, c.dy)
+                within(g.x, *one_column(c), "dx")
+                if weight:
+                    n = c.dy.double() * c.h * c.r
+                    tol = (rows + 8) * EPS * n.abs().sum(0)
+                    within(g.weight, n.sum(0), tol + U[dtype] * (n.sum(0).abs() + tol) + TINY[dtype], "dweight")
+                c.dh = (c.dy.double() * 1e-6).to(dtype)
+                within(features.rms_norm_backward(fw, c.dy, c.dh, need_weight=False).x, *one_column(c), "dx with dh")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradients_of_one_column_of_a_sum(dtype):
+    from cuke_amd import features
+    c = Norm(300, 1, dtype, eps=1e-4)
+    fw = c.forward()
+    assert fw.eps == 1e-4
+    c.dh = None
+    within(features.rms_norm_backward(fw, c.dy).x, *one_column(c), "dx")
+
+
+def test_gradients_of_one_column_against_differences():
+    from cuke_amd import features
+    c = Norm(50, 1, torch.float32, residual=False, eps=0.5)
+    g = features.rms_norm_backward(c.forward(), c.dy)
+    value = lambda t: (c.dy.double() * c.w64 * (c.h + t) * ((c.h + t).square() + c.eps).rsqrt())
+    t = 1e-4
+    slope = (value(t) - value(-t)) / (2 * t)                                          # off by t^2 / 6 times a third derivative, |dy w| 30 at most
+    within(g.x, slope, 5 * t * t * (c.dy.double() * c.w64).abs() + 8 * EPS * slope.abs() + 1e-12, "dx")
+
+
+def test_one_column_that_is_not_a_number():
+    from cuke_amd import features
+    inf, nan = float("inf"), float("nan")
+    for eps in (0.0, 1e-6):
+        x = torch.tensor([[0.0], [inf], [-inf], [nan], [2.0]], device=DEV)
+        fw = features.rms_norm_forward(x, eps=eps)
+        dx = features.rms_norm_backward(fw, torch.ones_like(x)).x
+        assert torch.isnan(dx[1:4]).all() and not torch.isnan(dx[4])
+        assert torch.isnan(dx[0]) if eps == 0 else abs(dx[0].item() - 1e3) < 1e-3            # (0 / 0, as the formula says)
+        dx = features.rms_norm_backward(fw, torch.tensor([[1.0], [1.0], [1.0], [1.0], [nan]], device=DEV)).x
+        assert torch.isnan(dx[4])
+
+
+def test_one_column_by_the_c_call():
+    """In the place of dy and of dh, with nothing written beside the rows."""
+    from cuke_amd import _lib, features
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for dtype in TYPES:
+        c = Norm(300, 1, dtype, eps=1e-3)
+        fw = c.forward()
+        want = features.rms_norm_backward(fw, c.dy, c.dh)
+        d = _lib.RmsNorm(CODE[dtype], CODE[dtype], 300, 1, None, 0, None, 0, c.w.data_ptr(), 1e-3)
+        n = L.kge_rms_norm_bwd_workspace(C.byref(d))
+        ws = torch.empty(n, dtype=torch.uint8, device=DEV)
+        for place in ("dy", "dh", "apart"):
+            wide = {k: torch.full((303, 4), 7.0, dtype=dtype, device=DEV) for k in ("dy", "dh", "apart")}
+            wide["dy"][:300, :1], wide["dh"][:300, :1] = c.dy, c.dh
+            dw = torch.empty(1, dtype=dtype, device=DEV)
+            rest = fw.rest.data_ptr() if fw.rest is not None else None
+            assert L.kge_rms_norm_bwd(C.byref(d), fw.h.data_ptr(), 1, fw.rstd.data_ptr(), rest, CODE[dtype], wide["dy"].data_ptr(), 4, wide["dh"].data_ptr(), 4,
+                                      wide[place].data_ptr(), 4, dw.data_ptr(), ws.data_ptr(), n, st) == 0
+            assert torch.equal(wide[place][:300, :1], want.x) and torch.equal(dw, want.weight), (dtype, place)
+            assert all(bool((t[300:] == 7).all()) and bool((t[:, 1:] == 7).all()) for t in wide.values())
