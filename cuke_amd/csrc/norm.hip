@@ -32,12 +32,13 @@ __device__ __forceinline__ double sum_at(const NormArgs &a, int64_t row, int64_t
     if (a.residual) h += (double)(float)static_cast<const T *>(a.residual)[row * a.residual_stride + col];
     return h;
 }
-// r of a row, to half a unit of its last place and 2^-40: the instruction's 2^-23 and a step of Newton's method
+// r of a row as it is kept (to_reach()), to half a unit of its last place and 2^-40: the instruction's 2^-23 and a step of Newton's method
 __device__ __forceinline__ float root(const NormArgs &a, double sum)
 {
     const double m = fma(sum, a.share, a.eps), r = __builtin_amdgcn_rsq(m);
-    const double better = r * fma(-0.5 * m * r, r, 1.5);
-    return (float)(r > 0.0 && r < 1e300 ? better : r);  // (of 0 and infinity the step would make NaN)
+    const double better = r * fma(-0.5 * m * r, r, 1.5), v = r > 0.0 && r < 1e300 ? better : r;  // (of 0 and infinity the step would make NaN)
+    const float f = (float)v;
+    return finite(f) || !(v < 1e300) ? f : -(float)fmin(v * 0x1p-64, 0x1.fffffep127);  // (beyond that rows are zeros)
 }
 // r in 64 bits, and an element of the result, from memory
 __device__ __forceinline__ double root64(const NormArgs &a, double sum) { return 1.0 / sqrt(sum / (double)a.cols + a.eps); }
@@ -185,10 +186,11 @@ __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
             for (int e = 0; e < 8; ++e) sum = fma((double)h[c][e], (double)h[c][e], sum);
         }
         sum = WAVES ? waves_sum(sum, lanes, part, turn++) : lanes_sum(sum, lanes);
-        const float r = root(a, sum);
-        if (a.rstd && there && lane == 0) a.rstd[row] = r;
+        const float kept = root(a, sum), r = fabsf(kept);
+        if (a.rstd && there && lane == 0) a.rstd[row] = kept;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
+            to_reach(kept, h[c]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[c][e] *= r;
             if (a.weight) {
@@ -231,8 +233,8 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormArgs a)
             for (int e = 0; e < 8; ++e) sum = fma((double)h[e], (double)h[e], sum);
         }
         sum = waves_sum(sum, 256, part, turn++);
-        const float r = root(a, sum);
-        if (a.rstd && threadIdx.x == 0) a.rstd[row] = r;
+        const float kept = root(a, sum), r = fabsf(kept);
+        if (a.rstd && threadIdx.x == 0) a.rstd[row] = kept;
         for (int64_t col0 = 0; col0 < a.cols; col0 += 8 * 256) {  // (all lanes come along)
             const int64_t col = col0 + 8 * threadIdx.x;
             float h[8];
@@ -240,6 +242,7 @@ __global__ __launch_bounds__(256) void rms_norm_long_kernel(NormArgs a)
             if (a.h) store8(static_cast<T *>(a.h) + row * a.h_stride + col, h, valid);
             if constexpr (sizeof(T) == 2)
                 if (a.rest && valid > 0) a.rest[row * ((a.cols + 7) / 8) + col / 8] = rest_of<T>(h);
+            to_reach(kept, h);
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] *= r;
             if (a.weight) {

@@ -87,6 +87,15 @@ __device__ __forceinline__ void place_in_rows(int lanes, int *lane, uint32_t *gr
     if (WAVES) *group = (uint32_t)__builtin_amdgcn_readfirstlane((int)*group);
 }
 
+// How r is kept in 32 bits: as it is, or where it does not fit (2^128 and more: rows whose root mean square is below 2^-128, which only an eps below 2^-256 leaves so) as
+// -r 2^-64.  The row's numbers are then taken times 2^64, which rounds none of them, and so is what is multiplied by r again.
+__device__ __forceinline__ void to_reach(float kept, float (&v)[8])
+{
+    if (kept < 0.0f)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= 0x1p64f;
+}
+
 // What a sum loses when it is rounded to 16 bits, in sixteenths of a step, -8 .. 7: four bits an element, eight of a row in a word.  bf16: the difference of the two numbers'
 // bits, in units of 2^12 (a step at the sum: below a power of two that it was rounded up to, half of the step there); fp16, whose small numbers are evenly spaced: in sixteenths
 // of the step at the result.  With it the gradients are those of the sum itself, to 2^-13: from the rounded one alone dweight would be off by 1.4 times its own rounding, and dx of short

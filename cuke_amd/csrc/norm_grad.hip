@@ -90,12 +90,13 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
         const int64_t row = row0 + group;
         const bool there = row < last;
         float n[C][8], g[C][8], dot = 0.0f;
-        const float rr = r;
+        const float kept = r, rr = fabsf(kept);
         Held<T> more[DH ? C : 1];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
             h[c].values(n[c]), dy[c].values(g[c]);
             if constexpr (REST) add_rest<T>(n[c], __builtin_amdgcn_alignbit(rest_end[c], rest[c], 4 * (at[c] & 7)));
+            to_reach(kept, n[c]);
             if constexpr (DH) more[c] = dh[c];
             if (skip[c] > 0) {
 #pragma unroll
@@ -132,7 +133,10 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
             float d[8] = {};
             if constexpr (DH) more[c].values(d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = fmaf(rr, g[c][e] - n[c][e] * mean, d[e]);
+            for (int e = 0; e < 8; ++e) g[c][e] -= n[c][e] * mean;
+            to_reach(kept, g[c]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmaf(rr, g[c][e], d[e]);
             if (!there || skip[c] >= 8) continue;
             T *to = row_dx + at[c];
             if (skip[c] == 0) {
@@ -178,15 +182,16 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
 {
     __shared__ float part[2][4];
     int turn = 0;
-    auto load = [&](int64_t row, int64_t col, float r, float(&n)[8], float(&g)[8]) {
+    auto load = [&](int64_t row, int64_t col, float kept, float(&n)[8], float(&g)[8]) {
         const int64_t left = a.cols - col;
         const int valid = (int)(left < 8 ? left : 8);
         load8(static_cast<const T *>(a.h) + row * a.h_stride + col, valid, n);
         load8(static_cast<const D *>(a.dy) + row * a.dy_stride + col, valid, g);
         if constexpr (sizeof(T) == 2)
             if (a.rest) add_rest<T>(n, a.rest[row * ((a.cols + 7) / 8) + col / 8]);
+        to_reach(kept, n);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) n[e] *= r;
+        for (int e = 0; e < 8; ++e) n[e] *= fabsf(kept);
         if (!a.weight) return valid;
         float w[8];
         load8(static_cast<const T *>(a.weight) + col, valid, w);
@@ -195,21 +200,24 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
         return valid;
     };
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        const float r = a.rstd[row];
+        const float kept = a.rstd[row];
         float dot = 0.0f;
         for (int64_t col = 8 * threadIdx.x; col < a.cols; col += 8 * 256) {
             float n[8], g[8];
-            load(row, col, r, n, g);
+            load(row, col, kept, n, g);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dot = fmaf(g[e], n[e], dot);
         }
         const float mean = waves_sum(dot, 256, part, turn++) * (1.0f / (float)a.cols);
         for (int64_t col = 8 * threadIdx.x; col < a.cols; col += 8 * 256) {
             float n[8], g[8], d[8] = {};
-            const int valid = load(row, col, r, n, g);
+            const int valid = load(row, col, kept, n, g);
             if (a.dh) load8(static_cast<const T *>(a.dh) + row * a.dh_stride + col, valid, d);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) d[e] = fmaf(r, g[e] - n[e] * mean, d[e]);
+            for (int e = 0; e < 8; ++e) g[e] -= n[e] * mean;
+            to_reach(kept, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmaf(fabsf(kept), g[e], d[e]);
             store8(static_cast<T *>(a.dx) + row * a.dx_stride + col, d, valid);
         }
     }
@@ -221,7 +229,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_one_kernel(NormGradArgs a)
 {
     const double w = a.weight ? (double)(float)*static_cast<const T *>(a.weight) : 1.0;
     for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
-        const double h = (double)(float)static_cast<const T *>(a.h)[row * a.h_stride], r = (double)a.rstd[row];
+        const double h = (double)(float)static_cast<const T *>(a.h)[row * a.h_stride], r = (double)a.rstd[row] * (a.rstd[row] < 0.0f ? -0x1p64 : 1.0);
         double d = a.eps * r * r * r * w * (double)(float)static_cast<const D *>(a.dy)[row * a.dy_stride];
         d += 0.0 * h;  // (of what is not finite NaN, as the difference would be)
         if (a.dh) d += (double)(float)static_cast<const T *>(a.dh)[row * a.dh_stride];
@@ -238,14 +246,15 @@ __global__ __launch_bounds__(256) void rms_norm_long_sums_kernel(NormGradArgs a)
     const int valid = (int)(left < 8 ? left : 8);
     float sum[8] = {};
     for (int64_t row = first; row < last; ++row) {
-        const float r = a.rstd[row];
+        const float kept = a.rstd[row];
         float n[8], g[8];
         load8(static_cast<const T *>(a.h) + row * a.h_stride + col, valid, n);
         load8(static_cast<const D *>(a.dy) + row * a.dy_stride + col, valid, g);
         if constexpr (sizeof(T) == 2)
             if (a.rest) add_rest<T>(n, a.rest[row * ((a.cols + 7) / 8) + col / 8]);
+        to_reach(kept, n);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum[e] = fmaf(g[e], n[e] * r, sum[e]);
+        for (int e = 0; e < 8; ++e) sum[e] = fmaf(g[e], n[e] * fabsf(kept), sum[e]);
     }
     float *to = a.sums + (int64_t)blockIdx.y * a.quads * 4 + col;
     *reinterpret_cast<float4 *>(to) = make_float4(sum[0], sum[1], sum[2], sum[3]);

@@ -491,7 +491,7 @@ class NormForward:
     """A norm's output, and what its backward pass needs (h and weight have to stay as they are until then)."""
     y: torch.Tensor | Rows8
     h: torch.Tensor     # x + residual; x itself where there is none
-    rstd: torch.Tensor  # float32 [rows]
+    rstd: torch.Tensor  # float32 [rows]; -r 2^-64 where r is 2^128 or more
     weight: torch.Tensor | None
     rest: torch.Tensor | None = None  # int32 [rows, ceil(cols / 8)]: what h lost when it was rounded to 16 bits, in four bits an element
     eps: float = 1e-6

@@ -676,8 +676,9 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
  * Root-mean-square norm of rows, a residual added in front of it:
  *   h = x + residual,   r[i] = (mean_j h[i][j]^2 + eps)^-1/2,   y[i][j] = h[i][j] r[i] weight[j]            (residual, weight NULL: 0, 1)
  * x, residual, weight and h have the type `type`; y any kge_type_t, or KGE_E4M3: rows in 8 bits (`y8`; else y, y_stride).  h (NULL: not wanted) is the sum
- * rounded to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32.  Squares are summed in 64 bits, so that no value of a type
- * overflows; a value in 8 bits is the one nearest to the 64-bit result.  rest (NULL: not wanted; KGE_F32: not looked at): 4 ceil(cols / 8) bytes a row, 4-byte
+ * rounded to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32, or, of rows whose r is
+ * 2^128 or more (a root mean square below 2^-128, with an eps below 2^-256), -r 2^-64.  Squares are summed in 64 bits, so that no value of a type
+ * overflows; a value in 8 bits is the one nearest to the 64-bit result (of numbers 2^126 times smaller than their row's root mean square h r is a multiple of 2^-149 first).  rest (NULL: not wanted; KGE_F32: not looked at): 4 ceil(cols / 8) bytes a row, 4-byte
  * aligned, what rounding took from h, four bits an element, from -8 to 7: KGE_BF16: the fp32 bits of the sum less those of h, in units of 2^12; KGE_F16: in
  * 16ths of a step at h.
  * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
