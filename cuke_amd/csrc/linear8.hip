@@ -185,6 +185,10 @@ static void launch_tiles(TileArgs &t, hipStream_t st)
     else if constexpr (!BOTH) hipLaunchKernelGGL((linear8_forward_kernel<T, S>), dim3((unsigned)blocks), dim3(S::kThreads), 0, st, t);
 }
 
+// Whether both sides' rows are near enough for the shapes with grouped_scales(), and whether a launch of another shape takes so many tiles.
+static bool near_rows(const Rows8 &a, const Rows8 &b) { return a.q_stride < (int64_t)1 << 24 && b.q_stride < (int64_t)1 << 24; }
+static bool far_launchable(int64_t a, int64_t b) { return tiles_launchable<TallB>(a, b) || tiles_launchable<LoneB>(a, b) || tiles_launchable<SmallB>(a, b); }
+
 // By forward_cost(); terms of both sides in 8 bits count in pairs.  The shape chosen takes 1.1 % longer than the best one on average over seventeen sizes with a 16-bit weight,
 // 1.4 % over as many with one in 8 bits.  Some of them (us; Large, Middle, Tall, Lone, Small; what is chosen in brackets), with a 16-bit weight:
 //   32768 x 2048 -> 2048, gelu, drop, act' kept  [329] 370 405 435 474       65536 x 512 -> 400, fp32 residual  79 [76] 76  82 88
@@ -199,7 +203,7 @@ static void launch_forward8(TileArgs &t, bool both, hipStream_t st)
     const int64_t moved = (t.e.out_f32 ? 4 : 2) * (t.e.residual ? 2 : 1) + (t.e.slope ? 1 : 0);
     int64_t epilogue = 64 * moved + (t.e.act > KGE_ACT_RELU ? 192 : 0) + (t.e.drop.cut ? 192 : 0);
     if (both) epilogue = epilogue * 13 / 10;
-    const bool near = !both || (t.a8.q_stride < (int64_t)1 << 24 && t.b8.q_stride < (int64_t)1 << 24);  // (grouped_scales())
+    const bool near = !both || near_rows(t.a8, t.b8);
     const double large = near ? forward_cost<LargeB>(t, epilogue + (t.e.residual ? 256 : 0), 1, 1.0, 1.0) : INFINITY;
     const double middle = near ? forward_cost<MiddleB>(t, epilogue, 2, both ? 0.7 : 0.73, both ? 3.5 : 2.5) : INFINITY, tall = forward_cost<TallB>(t, epilogue, 3, both ? 0.45 : 0.5, 2.3);
     const double small = forward_cost<SmallB>(t, epilogue, 3, both ? 0.4 : 0.45, 0.9), lone = forward_cost<LoneB>(t, epilogue, 1, both ? 0.35 : 0.4, 0.9);
@@ -392,6 +396,7 @@ int kge_linear8_fwd(const kge_linear *lin, const kge_rows8 *x8, const kge_rows8 
     if (!y) return KGE_EINVAL;
     if (y_stride < lin->out) return KGE_ESHAPE;
     const Plan8 p = plan8_of(lin, weight8 != nullptr);
+    if (weight8 && !p.pack_w && !p.few && !near_rows(rows8_of(x8), rows8_of(weight8)) && !far_launchable(lin->out, lin->rows)) return KGE_ESHAPE;
     const size_t need_saved = for_backward ? p.slope + p.w : 0, need = for_backward || p.few ? 0 : p.w;
     if (need_saved && (!saved || saved_bytes < need_saved || !aligned16(saved))) return KGE_EWORKSPACE;
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) return KGE_EWORKSPACE;

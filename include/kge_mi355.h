@@ -711,7 +711,8 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
  * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients; a value of x8 or weight8 that KGE_F16 cannot hold is infinite.
  * Products are exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for
  * answering: for_backward is 0 then (KGE_EINVAL).  Where all of x8, weight8 and a KGE_BF16 y meet, the matrix cores' product of 8-bit sides may be taken, which drops
- * from each sum of eight neighbouring terms what lies below 2^-13 of the largest one's power.
+ * from each sum of eight neighbouring terms what lies below 2^-13 of the largest one's power (rows 2^24 bytes apart and more: KGE_ESHAPE where rows or columns are so many that
+ * only tiles of 256 x 256 fit a launch).
  * The backward pass reads x8 where the forward pass did, so that it is all that is kept of the layer's input (its rows less than 2^26 bytes apart: KGE_ESHAPE);
  * act'(z) is kept in 8 bits too (steps of 1/200 from -0.135 up: within 0.0025).  dx is the gradient at the values that x8 stands for.  Otherwise as kge_linear_fwd and
  * kge_linear_bwd.
