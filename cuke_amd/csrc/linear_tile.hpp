@@ -5,7 +5,8 @@
 // memory.  A tile that lies across is turned by the transposing LDS reads on its way to the matrix cores.  16-bit tiles go to LDS 16 bytes a lane
 // without passing through registers; fp32 ones are taken through registers, where every value becomes three bf16 parts (mfma_split.hpp), of
 // whose nine products six are formed.  Rows in 8 bits go through registers too, where they become 16-bit ones (every e4m3 number times a power of two is
-// one), or, where both sides are in 8 bits, to LDS as they lie: the matrix cores take them with their powers.
+// one: of bf16 from 2^-130 up, of fp16 from 2^-21 to 65520; smaller ones are rounded), or, where both sides are in 8 bits, to LDS as they lie: the matrix cores take them with
+// their powers.
 #pragma once
 
 #include <type_traits>

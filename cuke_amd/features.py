@@ -256,7 +256,8 @@ def linear(x, weight, bias=None, *, act="none", residual=None, out_dtype=None, d
     because the residual is); 16-bit products are summed in fp32 and nothing is rounded before the end.
 
     x may be :class:`Rows8`, with a weight in bfloat16 or float16, whose type the layer has, or in 8 bits too: then dtype is the layer's (that of the bias, or
-    bfloat16, unless said otherwise)."""
+    bfloat16, unless said otherwise).  What is in 8 bits is multiplied as numbers of that type: float16 rounds those below 2^-21 and makes infinity of those from
+    65520 up, bfloat16 takes all as they are."""
     if isinstance(x, Rows8):
         y = _host8(x, weight, bias, act, residual, out_dtype, dtype, drop, seed, step, False)
         if y is not None:
@@ -472,7 +473,8 @@ def pack8(x) -> Rows8:
 
 
 def unpack8(rows8, dtype=torch.bfloat16) -> torch.Tensor:
-    """What rows in 8 bits stand for, as bfloat16, float16 or float32 (exact, but for what float16 cannot hold)."""
+    """What rows in 8 bits stand for, as bfloat16, float16 or float32 (exact, but for what float16 cannot hold: it rounds below 2^-21
+    and has no number from 65520 up)."""
     if isinstance(rows8, Rows8):
         y = _lib.host().unpack8(rows8.q, rows8.scale, rows8.cols, dtype)
         if y is not None:

@@ -667,8 +667,8 @@ typedef struct kge_rows8 {
 } kge_rows8;
 #define KGE_E4M3 3 /* beside kge_type_t, where a call says so: rows in 8 bits */
 
-/* x [rows, cols] of kge_type_t `type` to 8 bits, and back.  Unpacking is exact but for what `type` cannot hold (fp16: from 65520 on
-   infinite; else a value that was rounded up to 2^128). */
+/* x [rows, cols] of kge_type_t `type` to 8 bits, and back.  Unpacking is exact but for what `type` cannot hold (fp16: infinite from
+   65520 up, rounded to multiples of 2^-24 below 2^-21; bf16: to multiples of 2^-133 below 2^-130; bf16 and fp32: infinite what was rounded up to 2^128). */
 int kge_pack8(int32_t type, const void *x, int64_t x_stride, int64_t rows, int64_t cols, const kge_rows8 *out, void *stream);
 int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type, void *y, int64_t y_stride, void *stream);
 
@@ -708,8 +708,9 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
 
 /*
  * Linear layers (kge_linear, whose x and x_stride are not looked at) on rows in 8 bits, x8 [rows, in]:  y = drop(act(x8 weight^T + bias)) + residual.
- * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients; a value of x8 or weight8 that KGE_F16 cannot hold is infinite.
- * Products are exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for
+ * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients.  Values of x8 and weight8 enter the products as numbers of that
+ * type: of KGE_BF16 as they are (below 2^-130 rounded to multiples of 2^-133), of KGE_F16 as they are from 2^-21 up, rounded to multiples of
+ * 2^-24 below, infinite from 65520 up: rows of small numbers belong into a KGE_BF16 layer.  The products of these numbers are exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for
  * answering: for_backward is 0 then (KGE_EINVAL).  Where all of x8, weight8 and a KGE_BF16 y meet, the matrix cores' product of 8-bit sides may be taken, which drops
  * from each sum of eight neighbouring terms what lies below 2^-13 of the largest one's power (rows 2^24 bytes apart and more: KGE_ESHAPE where rows or columns are so many that
  * only tiles of 256 x 256 fit a launch).
