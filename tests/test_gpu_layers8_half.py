@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from test_gpu_features import DEV
+from test_gpu_features import DEV, act64
 from test_gpu_layers8 import values
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +82,19 @@ def test_the_smallest_bf16_numbers(rows, out, eight):
     y = features.linear(r, features.pack8(w) if eight else w.bfloat16(), out_dtype=torch.float32, dtype=torch.bfloat16).double()
     assert torch.equal(y[:, 1], number * 2.0 ** 20) and bool((y[:, 0] == 0).all())
     assert torch.equal(features.unpack8(r, torch.bfloat16).double(), values(r))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_what_a_derivative_in_8_bits_is_off_by(act, dtype):
+    """A step is 0.005: 0.0025 at most, 0.005 / sqrt(12) = 0.00144 in the mean square (of 65536 values within 1 %), and the gradient's own rounding."""
+    from cuke_amd import features
+    b = torch.randn(65536, generator=torch.Generator().manual_seed(1)).to(DEV).to(dtype)
+    w = torch.zeros((65536, 8), dtype=dtype, device=DEV)
+    fw = features.linear_forward(features.pack8(torch.zeros((1, 8), device=DEV)), w, b, act=act)
+    got = features.linear_backward(fw, torch.ones_like(fw.y), need_x=False, need_weight=False).bias.double()
+    want = act64(b.double(), act)[1]
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((got - want).abs() <= 0.0025 + half * want.abs() * 1.01 + 1e-6).all())
+    kept = (got - want).square().mean().sqrt().item()
+    assert 0.0013 <= kept <= (0.00146 ** 2 + (half * want.abs().max().item()) ** 2) ** 0.5
