@@ -1,6 +1,5 @@
 // Gradients of the root-mean-square norm (kge_rms_norm_bwd).  With n = h r and g = dy weight:
 //   dx = r (g - n mean(g n)) + dh,   dweight = sum over rows of dy n
-#include <algorithm>
 #include <type_traits>
 
 #include "linear_tile.hpp"
@@ -176,7 +175,61 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
     }
 }
 
-// Rows that registers do not hold, and those of two to seven columns: dx by a workgroup that goes over a row twice.
+// Rows of one to seven columns: a thread a row, dweight's sums in registers until the range's end.  Of one column g - n mean(g n) = g (1 - n^2) = g eps r^2: the difference of two
+// nearly equal numbers (eps 1e-6: one or two of fp32's digits are left), the product of what is known.  Bound by launches: 65536 bf16 rows of 1, 4
+// and 7 columns 8.3, 8.4 and 8.5 us with the joining of the sums (61, 202 and 294 with a workgroup a row, as longer rows have; the plain formula in torch some 100).
+template <class T, class D>
+__global__ __launch_bounds__(256) void rms_norm_grad_few_kernel(NormGradArgs a)
+{
+    __shared__ float part[4][8];
+    const int64_t first = (int64_t)blockIdx.x * a.rows_each, last = first + a.rows_each < a.rows ? first + a.rows_each : a.rows;
+    const int cols = (int)a.cols;
+    const float share = 1.0f / (float)cols;
+    float w[8], sum[8] = {};
+    if (a.weight) load8(static_cast<const T *>(a.weight), cols, w);
+    for (int64_t row = first + threadIdx.x; row < last; row += 256) {
+        const float kept = a.rstd[row], r = fabsf(kept);
+        float n[8], g[8], d[8] = {};
+        load8(static_cast<const T *>(a.h) + row * a.h_stride, cols, n);
+        load8(static_cast<const D *>(a.dy) + row * a.dy_stride, cols, g);
+        if (a.dh) load8(static_cast<const T *>(a.dh) + row * a.dh_stride, cols, d);
+        if constexpr (sizeof(T) == 2)
+            if (a.rest) add_rest<T>(n, a.rest[row]);
+        to_reach(kept, n);
+        float dot = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            n[e] *= r;
+            sum[e] = fmaf(g[e], n[e], sum[e]);
+            if (a.weight) g[e] *= w[e];
+            dot = fmaf(g[e], n[e], dot);
+        }
+        if (!a.dx) continue;
+        if (cols == 1) {
+            const double whole = kept < 0.0f ? r * 0x1p64 : r;
+            d[0] = (float)(a.eps * whole * whole * whole * g[0] + 0.0 * n[0] + d[0]);  // (of what is not finite NaN, as the difference would be)
+        } else {
+            const float mean = dot * share;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) g[e] -= n[e] * mean;
+            to_reach(kept, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d[e] = fmaf(r, g[e], d[e]);
+        }
+        store8(static_cast<T *>(a.dx) + row * a.dx_stride, d, cols);
+    }
+    if (!a.sums) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float all = lanes_sum(sum[e], 64);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][e] = all;
+    }
+    __syncthreads();
+    const int e = threadIdx.x;
+    if (e < 4 * (int)a.quads) a.sums[(int64_t)blockIdx.x * a.quads * 4 + e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
+}
+
+// Rows that registers do not hold: dx by a workgroup that goes over a row twice.
 template <class T, class D>
 __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
 {
@@ -222,20 +275,6 @@ __global__ __launch_bounds__(256) void rms_norm_grad_long_kernel(NormGradArgs a)
         }
     }
 }
-// dx of rows of one column, where g - n mean(g n) = g (1 - n^2) = g eps r^2: the difference of two nearly equal numbers (eps 1e-6: of fp32's digits one or two are left), the
-// product of what is known.  A thread a row.
-template <class T, class D>
-__global__ __launch_bounds__(256) void rms_norm_grad_one_kernel(NormGradArgs a)
-{
-    const double w = a.weight ? (double)(float)*static_cast<const T *>(a.weight) : 1.0;
-    for (int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x; row < a.rows; row += (int64_t)gridDim.x * 256) {
-        const double h = (double)(float)static_cast<const T *>(a.h)[row * a.h_stride], r = (double)a.rstd[row] * (a.rstd[row] < 0.0f ? -0x1p64 : 1.0);
-        double d = a.eps * r * r * r * w * (double)(float)static_cast<const D *>(a.dy)[row * a.dy_stride];
-        d += 0.0 * h;  // (of what is not finite NaN, as the difference would be)
-        if (a.dh) d += (double)(float)static_cast<const T *>(a.dh)[row * a.dh_stride];
-        static_cast<T *>(a.dx)[row * a.dx_stride] = (T)(float)d;
-    }
-}
 // dweight's sums over ranges of rows, of such rows: eight columns a thread
 template <class T, class D>
 __global__ __launch_bounds__(256) void rms_norm_long_sums_kernel(NormGradArgs a)
@@ -271,7 +310,7 @@ __global__ __launch_bounds__(256) void norm_join_kernel(SumArgs j)
 // ---- launches --------------------------------------------------------------------------------------
 static Hold grad_hold(int64_t rows, int64_t cols)
 {
-    return cols < 8 ? Hold{0, 256} : hold_of(rows, cols, 4096);
+    return cols < 8 ? Hold{0, 1} : hold_of(rows, cols, 4096);  // (rms_norm_grad_few_kernel)
 }
 
 // Ranges of rows, one a workgroup, that dweight is summed over: 512 of them (us with 512, 1024 and 2048: 65536 x 2048 bf16 211, 219, 221; 4096 x 1024 12.7, 15.2, 15.0;
@@ -283,8 +322,8 @@ struct Ranges {
 static Ranges ranges_of(int64_t rows, int64_t cols)
 {
     const Hold hold = grad_hold(rows, cols);
-    const int64_t turn = hold.pieces ? 256 / hold.lanes : 8, turns = ceil_div(rows, turn);
-    const int64_t across = hold.pieces ? 1 : ceil_div(cols, 2048), most = 512, want = across < most ? most / across : 1;
+    const int64_t turn = hold.pieces || hold.lanes == 1 ? 256 / hold.lanes : 8, turns = ceil_div(rows, turn);
+    const int64_t across = hold.pieces || hold.lanes == 1 ? 1 : ceil_div(cols, 2048), most = 512, want = across < most ? most / across : 1;
     const int64_t each = turn * ceil_div(turns, want);
     return Ranges{each > 0 ? each : 1, (int)ceil_div(rows, each > 0 ? each : 1)};
 }
@@ -296,11 +335,12 @@ static void launch_grads(const NormGradArgs &args, const Ranges &ranges, void *d
     const Hold hold = grad_hold(a.rows, a.cols);
     a.lanes = hold.lanes;
     const dim3 grid((unsigned)ranges.count), block(256);
-    if (hold.pieces == 0) {
+    if (hold.lanes == 1) {
+        hipLaunchKernelGGL((rms_norm_grad_few_kernel<T, D>), grid, block, 0, st, a);
+    } else if (hold.pieces == 0) {
         // (the sums first: dx may take the place of dy)
         if (a.sums) hipLaunchKernelGGL((rms_norm_long_sums_kernel<T, D>), dim3((unsigned)ceil_div(a.cols, 2048), (unsigned)ranges.count), block, 0, st, a);
-        if (a.dx && a.cols == 1) hipLaunchKernelGGL((rms_norm_grad_one_kernel<T, D>), dim3((unsigned)std::min<int64_t>(ceil_div(a.rows, 256), 1 << 20)), block, 0, st, a);
-        else if (a.dx) hipLaunchKernelGGL((rms_norm_grad_long_kernel<T, D>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), block, 0, st, a);
+        if (a.dx) hipLaunchKernelGGL((rms_norm_grad_long_kernel<T, D>), dim3((unsigned)(a.rows < (1 << 20) ? a.rows : (1 << 20))), block, 0, st, a);
     } else {
         with_hold(hold, [&](auto pieces, auto waves) {
             constexpr int kPieces = decltype(pieces)::value;

@@ -103,3 +103,63 @@ def test_one_column_by_the_c_call():
                                       wide[place].data_ptr(), 4, dw.data_ptr(), ws.data_ptr(), n, st) == 0
             assert torch.equal(wide[place][:300, :1], want.x) and torch.equal(dw, want.weight), (dtype, place)
             assert all(bool((t[300:] == 7).all()) and bool((t[:, 1:] == 7).all()) for t in wide.values())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [1, 2, 3, 4, 5, 6, 7])
+def test_few_columns_and_many_rows(cols, dtype):
+    """Ranges of rows that end inside a workgroup's turn, one and several turns a range; the same call gives the same bits."""
+    from cuke_amd import features
+    for i, rows in enumerate((255, 256, 257, 70001, 300000)):
+        print("few columns", rows, cols, dtype, flush=True)
+        c = Norm(rows, cols, dtype, residual=i % 2 == 0, weight=i != 1, layout=("plain", "apart")[i % 2])
+        fw = c.forward()
+        for dy in TYPES:
+            c.dy = c.dy.to(dy)
+            g = features.rms_norm_backward(fw, c.dy, c.dh)
+            c.check_backward(fw, g, (rows, cols))
+            again = features.rms_norm_backward(fw, c.dy, c.dh)
+            assert torch.equal(g.x, again.x) and (g.weight is None or torch.equal(g.weight, again.weight))
+            alone = features.rms_norm_backward(fw, c.dy, c.dh, need_weight=False)
+            assert torch.equal(alone.x, g.x) and alone.weight is None
+        if c.w is not None:
+            assert torch.equal(features.rms_norm_backward(fw, c.dy, need_x=False).weight, g.weight)
+
+
+def test_few_columns_by_the_c_call():
+    """dx in the place of dy and of dh; nothing is written beside rows, behind the last one or behind the workspace."""
+    from cuke_amd import _lib, features
+    L, st = _lib.lib(), torch.cuda.current_stream().cuda_stream
+    for dtype in TYPES:
+        for cols in (2, 5, 7):
+            c = Norm(777, cols, dtype)
+            fw = c.forward()
+            want = features.rms_norm_backward(fw, c.dy, c.dh)
+            d = _lib.RmsNorm(CODE[dtype], CODE[dtype], 777, cols, None, 0, None, 0, c.w.data_ptr(), c.eps)
+            n = L.kge_rms_norm_bwd_workspace(C.byref(d))
+            for place in ("dy", "dh", "apart"):
+                wide = {k: torch.full((780, cols + 3), 7.0, dtype=dtype, device=DEV) for k in ("dy", "dh", "apart")}
+                wide["dy"][:777, :cols], wide["dh"][:777, :cols] = c.dy, c.dh
+                dw, ws = torch.full((cols + 4,), 7.0, dtype=dtype, device=DEV), torch.full((n + 64,), 0x5A, dtype=torch.uint8, device=DEV)
+                rest = fw.rest.data_ptr() if fw.rest is not None else None
+                assert L.kge_rms_norm_bwd(C.byref(d), fw.h.data_ptr(), cols, fw.rstd.data_ptr(), rest, CODE[dtype], wide["dy"].data_ptr(), cols + 3, wide["dh"].data_ptr(),
+                                          cols + 3, wide[place].data_ptr(), cols + 3, dw.data_ptr(), ws.data_ptr(), n, st) == 0
+                assert torch.equal(wide[place][:777, :cols], want.x) and torch.equal(dw[:cols], want.weight), (dtype, cols, place)
+                assert all(bool((t[777:] == 7).all()) and bool((t[:, cols:] == 7).all()) for t in wide.values())
+                assert bool((dw[cols:] == 7).all()) and bool((ws[n:] == 0x5A).all())
+
+
+def test_few_columns_in_a_graph():
+    from cuke_amd import features
+    c = Norm(3000, 3, torch.bfloat16)
+    fw = c.forward()
+    features.rms_norm_backward(fw, c.dy, c.dh)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g = features.rms_norm_backward(fw, c.dy, c.dh)
+    for _ in range(3):
+        c.dy.mul_(0.7)
+        eager = features.rms_norm_backward(fw, c.dy, c.dh)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g.x, eager.x) and torch.equal(g.weight, eager.weight)
