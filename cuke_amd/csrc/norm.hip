@@ -119,7 +119,8 @@ __device__ __forceinline__ void finish_scales(const NormArgs &a, int64_t row, in
 
 // A row is held in registers, C pieces of eight columns a lane, by `lanes` lanes (WAVES: by two or four waves).  FULL: rows are whole pieces.
 // Bound by memory where rows are many: 65536 x 2048 bf16 with a residual and rest (1.14 GB) 185 us, 6.2 TB/s; a copy of 2 GB reaches 5.0.  Of few rows by what a wave
-// has to do for its share of one: 4096 x 1024 to 8 bits (29 MB) 9.4 us, to bf16 7.7, of which a launch and a row's two dependent reads are 4.
+// has to do for its share of one: 4096 x 1024 to 8 bits (29 MB) 9.4 us, to bf16 7.7, of which a launch, a row's read and, requested behind its sum, the
+// weight's are 4.
 template <class T, class O, int C, bool WAVES, bool FULL>
 __global__ __launch_bounds__(256) void rms_norm_kernel(NormArgs a)
 {

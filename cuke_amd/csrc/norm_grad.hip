@@ -35,7 +35,8 @@ struct Held {
 
 // A workgroup takes a range of rows, each held by `lanes` lanes (WAVES: by two or four waves); what the next row needs is requested while the present one is worked on.  A lane's
 // columns are the same in all rows, so dweight's sums wait in registers until the range's end.
-// Bound by memory: 65536 x 2048 bf16 with dh and rest (1.14 GB) 230 us, 5.0 TB/s; 4096 x 1024 (36 MB, in the caches) 8, and 2.4 for the joining of dweight's sums.
+// 65536 x 2048 bf16 with dh and rest (1.14 GB) 226 us, without 161 (0.81 GB): 5.0 TB/s, what a large copy reaches, but not the forward pass's 6.2; more or fewer ranges, two rows
+// requested ahead and dx alone (220) change little.  4096 x 1024 (36 MB, in the caches) 8, and 2.4 for the joining of dweight's sums.
 template <class T, class D, int C, bool WAVES, bool DH, bool REST>
 __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 {
@@ -177,7 +178,7 @@ __global__ __launch_bounds__(256) void rms_norm_grad_kernel(NormGradArgs a)
 
 // Rows of one to seven columns: a thread a row, dweight's sums in registers until the range's end.  Of one column g - n mean(g n) = g (1 - n^2) = g eps r^2: the difference of two
 // nearly equal numbers (eps 1e-6: one or two of fp32's digits are left), the product of what is known.  Bound by launches: 65536 bf16 rows of 1, 4
-// and 7 columns 8.3, 8.4 and 8.5 us with the joining of the sums (61, 202 and 294 with a workgroup a row, as longer rows have; the plain formula in torch some 100).
+// and 7 columns 8.3, 8.4 and 8.5 us with the joining of the sums (61, 202 and 294 with a workgroup a row, as the longest rows have).
 template <class T, class D>
 __global__ __launch_bounds__(256) void rms_norm_grad_few_kernel(NormGradArgs a)
 {
@@ -313,8 +314,8 @@ static Hold grad_hold(int64_t rows, int64_t cols)
     return cols < 8 ? Hold{0, 1} : hold_of(rows, cols, 4096);  // (rms_norm_grad_few_kernel)
 }
 
-// Ranges of rows, one a workgroup, that dweight is summed over: 512 of them (us with 512, 1024 and 2048: 65536 x 2048 bf16 211, 219, 221; 4096 x 1024 12.7, 15.2, 15.0;
-// 30000 x 300 20.6, 22.2, 24.6).
+// Ranges of rows, one a workgroup, that dweight is summed over: 512 of them (us with 256, 512, 1024 and 2048: 65536 x 2048 bf16 with dh and rest 220, 226, 228, 235, without
+// 158, 161, 172, 171; 4096 x 1024 11.8, 12.1, 15.0, 15.0; 30000 x 300 22.3, 20.9, 23.4, 27.9).
 struct Ranges {
     int64_t rows_each;
     int count;
