@@ -675,12 +675,12 @@ int kge_unpack8(const kge_rows8 *rows8, int64_t rows, int64_t cols, int32_t type
 /*
  * Root-mean-square norm of rows, a residual added in front of it:
  *   h = x + residual,   r[i] = (mean_j h[i][j]^2 + eps)^-1/2,   y[i][j] = h[i][j] r[i] weight[j]            (residual, weight NULL: 0, 1)
- * x, residual, weight and h have the type `type`; y any kge_type_t, or KGE_E4M3: rows in 8 bits (`y8`; else y, y_stride).  h (NULL: not wanted) is the sum
- * rounded to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32, or, of rows whose r is
- * 2^128 or more (a root mean square below 2^-128, with an eps below 2^-256), -r 2^-64.  Squares are summed in 64 bits, so that no value of a type
- * overflows; a value in 8 bits is the one nearest to the 64-bit result (of numbers 2^126 times smaller than their row's root mean square h r is a multiple of 2^-149 first).  rest (NULL: not wanted; KGE_F32: not looked at): 4 ceil(cols / 8) bytes a row, 4-byte
- * aligned, what rounding took from h, four bits an element, from -8 to 7: KGE_BF16: the fp32 bits of the sum less those of h, in units of 2^12; KGE_F16: in
- * 16ths of a step at h.
+ * x, residual, weight and h have the type `type`; y any kge_type_t, or KGE_E4M3: rows in 8 bits (`y8`; else y, y_stride).  h (NULL: not wanted) is the sum rounded
+ * to `type`; y is made of the sum itself.  rstd [rows] (NULL: not wanted) is r in fp32, or, of rows whose r is 2^128 or more (a root mean square below 2^-128, with
+ * an eps below 2^-256), -r 2^-64.  Squares are summed in 64 bits, so that no value of a type overflows; a value in 8 bits is the one nearest to the 64-bit result
+ * (with the r of sums as fp32 holds them; of numbers 2^126 times smaller than their row's root mean square h r is a multiple of 2^-149 first).  rest (NULL: not wanted; KGE_F32: not looked at): 4
+ * ceil(cols / 8) bytes a row, 4-byte aligned, what rounding took from h, four bits an element, from -8 to 7: KGE_BF16: the fp32 bits of the sum less those of h, in
+ * units of 2^12; KGE_F16: in 16ths of a step at h.
  * Gradients, from those of y (dy, of any kge_type_t dy_type) and of h where it went on by itself (dh, of type `type`, or NULL):
  *   g = dy weight,   dx = dresidual = r (g - h r^2 mean_j(g h)) + dh,   dweight[j] = sum_i dy[i][j] h[i][j] r[i]
  * h: what the forward call wrote there (x where there was no residual), rstd and rest too (NULL: the gradients are those of h as it was rounded).  dx [rows, cols]
@@ -708,15 +708,15 @@ int kge_rms_norm_bwd(const kge_rms_norm *norm, const void *h, int64_t h_stride, 
 
 /*
  * Linear layers (kge_linear, whose x and x_stride are not looked at) on rows in 8 bits, x8 [rows, in]:  y = drop(act(x8 weight^T + bias)) + residual.
- * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients.  Values of x8 and weight8 enter the products as numbers of that
- * type: of KGE_BF16 as they are (below 2^-130 rounded to multiples of 2^-133), of KGE_F16 as they are from 2^-21 up, rounded to multiples of
- * 2^-24 below, infinite from 65520 up: rows of small numbers belong into a KGE_BF16 layer.  The products of these numbers are exact and summed in fp32 on the matrix cores.  weight8 (NULL: none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for
- * answering: for_backward is 0 then (KGE_EINVAL).  Where all of x8, weight8 and a KGE_BF16 y meet, the matrix cores' product of 8-bit sides may be taken, which drops
- * from each sum of eight neighbouring terms what lies below 2^-13 of the largest one's power (rows 2^24 bytes apart and more: KGE_ESHAPE where rows or columns are so many that
- * only tiles of 256 x 256 fit a launch).
+ * type: KGE_BF16 or KGE_F16 (KGE_EINVAL for KGE_F32), that of weight, bias and the gradients.  Values of x8 and weight8 enter the products as numbers of that type:
+ * of KGE_BF16 as they are (below 2^-130 rounded to multiples of 2^-133), of KGE_F16 as they are from 2^-21 up, rounded to multiples of 2^-24 below, infinite from
+ * 65520 up: rows of small numbers belong into a KGE_BF16 layer.  The products of these numbers are exact and summed in fp32 on the matrix cores.  weight8 (NULL:
+ * none): the weight as rows in 8 bits, [out, in], in place of kge_linear.weight, for answering: for_backward is 0 then (KGE_EINVAL).  Where all of x8, weight8 and a
+ * KGE_BF16 y meet, the matrix cores' product of 8-bit sides may be taken, which drops from each sum of eight neighbouring terms what lies below 2^-13 of the largest
+ * one's power (rows 2^24 bytes apart and more: KGE_ESHAPE where rows or columns are so many that only tiles of 256 x 256 fit a launch).
  * The backward pass reads x8 where the forward pass did, so that it is all that is kept of the layer's input (its rows less than 2^26 bytes apart: KGE_ESHAPE);
- * act'(z) is kept in 8 bits too (steps of 1/200 from -0.135 up: within 0.0025, 0.0014 in the mean square, some 0.0022 of the gradients, of KGE_F16 too).  dx is the gradient at the values that x8 stands for.  Otherwise as kge_linear_fwd and
- * kge_linear_bwd.
+ * act'(z) is kept in 8 bits too (steps of 1/200 from -0.135 up: within 0.0025, 0.0014 in the mean square, some 0.0022 of the gradients, of KGE_F16 too).  dx is the
+ * gradient at the values that x8 stands for.  Otherwise as kge_linear_fwd and kge_linear_bwd.
  */
 size_t kge_linear8_saved_bytes(const kge_linear *lin);
 size_t kge_linear8_fwd_workspace(const kge_linear *lin, const kge_rows8 *weight8, int for_backward);
